@@ -156,9 +156,10 @@ def _quantise(x, fmt):
     ok = torch.isfinite(amax)
     live = ok & (amax >= TINY)
     safe = torch.where(live, amax, torch.ones_like(amax))
-    y = torch.where(live[..., None], xf * (QMAX[fmt] / safe)[..., None], torch.zeros_like(xf))
+    top = torch.full_like(amax, QMAX[fmt])  # (torch would multiply by the reciprocal of a plain number)
+    y = torch.where(live[..., None], xf * (top / safe)[..., None], torch.zeros_like(xf))
     q = y.round().to(torch.int8) if fmt == "int8" else y.to(torch.float8_e4m3fn)
-    scale = torch.where(live, amax / QMAX[fmt], torch.zeros_like(amax))
+    scale = torch.where(live, amax / top, torch.zeros_like(amax))
     return q, torch.where(ok, scale, torch.full_like(scale, math.nan))
 
 
