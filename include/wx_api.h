@@ -629,6 +629,95 @@ int wx_refine_text(wx_ctx* ctx, const wx_dit_config* cfg, const wx_qweight* cond
                    const wx_lora_pack* condition_lora, const wx_block_weights* blocks, int n_blocks,
                    const void* final_norm, const void* text, int64_t L, int64_t text_dim, void* out, void* scratch);
 
+/* ------------------------------------------- text side: rotary positions */
+/* The text model whose hidden states condition the video (the reference runs it once per
+ * generation, H3TextEncoder.swift) is decoder-only with grouped heads: the entry points of
+ * this and the next three sections are what its layers need between their linears.
+ * Head dimension 128 or 64 throughout; strides are in elements. */
+enum wx_rope_scaling {
+  WX_ROPE_PLAIN = 0,
+  WX_ROPE_LINEAR = 1,   /* every frequency / factor */
+  WX_ROPE_BY_PARTS = 2, /* by its turns over original_positions: <= low / factor, >= high kept, linear between */
+};
+/* host: inv_freq[i] = base^(-2i/rot) scaled for a longer context, i < rot/2, rot <= 128 */
+int wx_rope_inv_freq(int rot, double base, int scaling, double factor, double original_positions, double low,
+                     double high, double* inv_freq);
+/* cos_t / sin_t [positions, nf] fp32 on the device = magnitude * cos / sin(p * inv_freq[f]);
+ * inv_freq on the host; angles and functions in 64 bits, rounded once */
+int wx_rope_table(wx_ctx* ctx, const double* inv_freq, int nf, int64_t positions, double magnitude, float* cos_t,
+                  float* sin_t);
+typedef struct wx_rope {
+  const float* cos_t; /* [positions, rot/2] */
+  const float* sin_t;
+  int64_t positions;
+  int32_t rot;         /* leading columns of a head that turn; multiple of 8, <= head_dim */
+  int32_t interleaved; /* pairs (2i, 2i+1) instead of (i, i + rot/2) */
+} wx_rope;
+/* y[t, h] = x[t, h] with its first rot columns turned by positions[t] (device); the others
+ * are copied. y may be x. A position outside the table leaves the token's rows unwritten and
+ * sets the device error word (WX_ERR_DEVICE from wx_ctx_check_device). */
+int wx_rope_apply(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, const void* x, int64_t row_stride,
+                  int64_t tokens, int heads, int head_dim, void* y, int64_t y_stride);
+
+/* ------------------------------------------- text side: paged K/V cache */
+enum wx_kv_format { WX_KV_BF16 = 0, WX_KV_INT8 = 1, WX_KV_E4M3 = 2 };
+typedef struct wx_kv_cache {
+  void* k; /* [pages, kv_heads, page_size, head_dim] in `format` */
+  void* v;
+  float* k_scale; /* [pages, kv_heads, page_size]; NULL for WX_KV_BF16 */
+  float* v_scale;
+  int64_t pages;
+  int32_t page_size; /* 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t format;
+} wx_kv_cache;
+/* Writes k and v rows [tokens, kv_heads, head_dim] (bf16) to slots[t] = page * page_size +
+ * offset (device; < 0 skips the token). 8-bit formats: scale = amax / 127 (int8) or
+ * amax / 448 (e4m3) of the row, value = x * (127 | 448) / amax to nearest even; a row with
+ * infinity or NaN gets scale NaN (it reads back as NaN), one below 2^-100 throughout zeros.
+ * A slot beyond the cache is skipped and sets the device error word. */
+int wx_kv_append(wx_ctx* ctx, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
+                 int64_t v_stride, int64_t tokens, const int64_t* slots);
+/* wx_rope_apply of q into q_out and of k, and wx_kv_append, in one launch: the turned k is
+ * quantised from its fp32 values (not rounded to bf16 first) and not written elsewhere. */
+int wx_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, const void* q, int64_t q_stride,
+                      int q_heads, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
+                      int64_t v_stride, int64_t tokens, const int64_t* slots, void* q_out, int64_t q_out_stride);
+/* k_out / v_out [tokens, kv_heads, head_dim] = bf16(value * scale) of the slots; < 0 reads zeros */
+int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,
+               int64_t out_stride);
+
+/* ------------------------------------------- text side: attention */
+/* Query head h reads K/V head h / (q_heads / kv_heads). Row i of a sequence with Lq query and
+ * Lk key rows stands at key i + Lk - Lq: causal lets it see keys up to there, window > 0 only
+ * the last `window` keys up to there. out = softmax(scale q k^T) v; lse (optional, [total_q,
+ * q_heads] fp32) = log of the softmax's denominator. A row that sees no key gets out 0 and
+ * lse -inf. Keys that a row does not see do not influence it, whatever they hold. */
+typedef struct wx_attn_dims {
+  int64_t total_q; /* query rows of all sequences */
+  int32_t batch;   /* sequences */
+  int32_t max_q;   /* longest Lq: chooses the kernel; results do not depend on it */
+  int32_t q_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t causal;
+  int32_t window; /* 0: none; needs causal */
+  float scale;    /* > 0 */
+} wx_attn_dims;
+/* Whole prompts, packed: sequence b has query rows cu_q[b]..cu_q[b+1] of q [total_q, q_heads,
+ * head_dim] and key rows cu_k[b]..cu_k[b+1] of k, v [total_k, kv_heads, head_dim] (cu arrays on
+ * the device; cu_k NULL = cu_q). */
+int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, int64_t total_k, const int32_t* cu_q,
+                        const int32_t* cu_k, void* out, int64_t out_stride, float* lse);
+/* New tokens (1 per sequence when decoding, a chunk of a prompt otherwise) over the paged cache
+ * that holds them already: sequence b has kv_lens[b] cached tokens in pages block_table[b,
+ * 0..], its queries being the last ones. Block entries beyond the length are not read. */
+int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
+                       const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
+                       const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride, float* lse);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,8 @@ WX_ERR_UNSUPPORTED = -5
 EPI_NONE, EPI_GELU, EPI_GATE_RESID, EPI_SWIGLU = 0, 1, 2, 3
 SPARSE_DENSE, SPARSE_SOL, SPARSE_TOPK = 0, 1, 2
 MLP_GELU, MLP_SWIGLU = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BY_PARTS = 0, 1, 2
+KV_BF16, KV_INT8, KV_E4M3 = 0, 1, 2
 
 
 class WxError(RuntimeError):
@@ -108,6 +110,23 @@ class Guidance(C.Structure):
 
 class DenseBf16(C.Structure):
     _fields_ = [("w", C.c_void_p), ("bias", C.c_void_p), ("k", C.c_int64), ("n", C.c_int64)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("cos_t", C.c_void_p), ("sin_t", C.c_void_p), ("positions", C.c_int64), ("rot", C.c_int32),
+                ("interleaved", C.c_int32)]
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("pages", C.c_int64), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("format", C.c_int32)]
+
+
+class AttnDims(C.Structure):
+    _fields_ = [("total_q", C.c_int64), ("batch", C.c_int32), ("max_q", C.c_int32), ("q_heads", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32),
+                ("scale", C.c_float)]
 
 
 _vp, _i64, _i32, _f32, _f64, _u32 = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_double, C.c_uint32
@@ -216,6 +235,17 @@ _SIGS = {
     "wx_refine_text_scratch_bytes": (_i64, [C.POINTER(DitConfig), _i64, _i64]),
     "wx_refine_text": (_i32, [_vp, C.POINTER(DitConfig), C.POINTER(QWeight), C.POINTER(LoraPack),
                               C.POINTER(BlockWeights), _i32, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "wx_rope_inv_freq": (_i32, [_i32, _f64, _i32, _f64, _f64, _f64, _f64, _vp]),
+    "wx_rope_table": (_i32, [_vp, _vp, _i32, _i64, _f64, _vp, _vp]),
+    "wx_rope_apply": (_i32, [_vp, C.POINTER(Rope), _vp, _vp, _i64, _i64, _i32, _i32, _vp, _i64]),
+    "wx_kv_append": (_i32, [_vp, C.POINTER(KvCache), _vp, _i64, _vp, _i64, _i64, _vp]),
+    "wx_rope_kv_append": (_i32, [_vp, C.POINTER(Rope), _vp, _vp, _i64, _i32, C.POINTER(KvCache), _vp, _i64, _vp, _i64,
+                                 _i64, _vp, _vp, _i64]),
+    "wx_kv_read": (_i32, [_vp, C.POINTER(KvCache), _vp, _i64, _vp, _vp, _i64]),
+    "wx_prompt_attention": (_i32, [_vp, C.POINTER(AttnDims), _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
+                                   _i64, _vp]),
+    "wx_paged_attention": (_i32, [_vp, C.POINTER(AttnDims), _vp, _i64, C.POINTER(KvCache), _vp, _vp, _vp, _i64, _vp,
+                                  _i64, _vp]),
 }
 
 _lib = None

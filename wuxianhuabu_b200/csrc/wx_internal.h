@@ -54,6 +54,9 @@ struct wx_ctx {
   void* p2p_peer[8] = {};
   int* p2p_counters = nullptr;
   uint32_t p2p_epoch = 0;
+  // arrival counters of kernels whose CTAs join partial results (arrival_counters)
+  int* arrivals = nullptr;
+  int64_t n_arrivals = 0;
   // limit of the cross-GPU flag waits (sequence-parallel exchange, wx_ctx_wait_flags)
   uint64_t peer_wait_ns = 10000000000ull;
 };
@@ -98,6 +101,15 @@ int make_tmap_bf16_2d(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t 
 // box `box_cols` x `box_rows`, zero fill out of bounds.
 int make_tmap_u32_2d(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                      uint32_t box_cols, uint32_t box_rows);
+
+// 2-D byte tensor map of contiguous rows of `cols` (64 or 128) bytes, box `box_rows` whole rows,
+// swizzled over the row's width, zero fill out of bounds.
+int make_tmap_u8_rows(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t rows, uint32_t cols,
+                      uint32_t box_rows);
+
+// `n` counters on the device, zero between launches: a kernel that counts arrivals on them sets
+// each back to zero with the last arrival (every CTA arrives, whatever happened to its work).
+int* arrival_counters(wx_ctx* ctx, int64_t n, int* status);
 
 // releases the NCCL communicator of a context (no-op without one)
 void sp_destroy_comm(wx_ctx* ctx);

@@ -61,10 +61,17 @@ class Context:
         if st != 0:
             raise WxError(st, f"wx_ctx_create(device={device}) failed")
         self.h = h
+        self._stream: Optional[torch.cuda.Stream] = None
 
     def sync_stream(self) -> None:
-        s = torch.cuda.current_stream(self.device).cuda_stream
-        check(self.lib.wx_ctx_set_stream(self.h, C.c_void_p(s)), self.h)
+        s = torch.cuda.current_stream(self.device)
+        if s != self._stream:
+            # the context's workspace is shared: a call on another stream waits for the calls
+            # queued on the last one (a capture orders its own work and must not reach outside)
+            if self._stream is not None and not torch.cuda.is_current_stream_capturing():
+                s.wait_stream(self._stream)
+            self._stream = s
+        check(self.lib.wx_ctx_set_stream(self.h, C.c_void_p(s.cuda_stream)), self.h)
 
     def check_device(self) -> None:
         check(self.lib.wx_ctx_check_device(self.h), self.h)
