@@ -9,135 +9,15 @@
 
 #include <algorithm>
 
-#include "wx_ptx.cuh"
-#include "wx_text.h"
+#include "wx_text_dev.cuh"
 
 namespace wx {
-
-struct TextAttnParams {
-  const __nv_bfloat16* q;
-  int64_t q_stride;
-  __nv_bfloat16* out;
-  int64_t out_stride;
-  float* lse;
-  const int32_t* cu_q;
-  const int32_t* cu_k;      // contiguous K/V (block_table == nullptr)
-  const int32_t* kv_lens;   // paged K/V
-  const int32_t* block_table;
-  int64_t blocks_per_seq;
-  const float *ks, *vs;     // scales of an 8-bit cache
-  int64_t pages;
-  int page_shift;
-  int batch, hq, hkv, group;
-  int64_t total_q, total_k;
-  int causal, window;
-  float sl2;  // scale * log2(e): scores and maxima are kept in base 2
-  float* part;              // split items: [2 * gridDim][16][hd] sums, then [..][16] maxima and denominators
-  float* part_ml;
-  int* counters;            // per item: pieces that have arrived (0 between launches)
-  int64_t n_items;          // of them
-  int* err;
-};
-
-// One sequence as the kernels see it; lengths and offsets from the device are clamped to the
-// buffers, so that wrong ones give wrong rows and an error word but no access outside.
-struct Seq {
-  int64_t q0, k0;
-  int lq, lk;
-};
-
-__device__ __forceinline__ Seq load_seq(const TextAttnParams& p, int b) {
-  Seq s;
-  const int64_t a = p.cu_q[b], e = p.cu_q[b + 1];
-  s.q0 = min64(max64(a, 0), p.total_q);
-  const int64_t q1 = min64(max64(e, s.q0), p.total_q);
-  s.lq = (int)(q1 - s.q0);
-  bool bad = s.q0 != a || q1 != e;
-  if (p.block_table) {
-    const int64_t n = p.kv_lens[b], cap = p.blocks_per_seq << p.page_shift;
-    s.k0 = 0;
-    s.lk = (int)min64(max64(n, 0), cap);
-    bad |= s.lk != n;
-  } else {
-    const int64_t c = p.cu_k[b], d = p.cu_k[b + 1];
-    s.k0 = min64(max64(c, 0), p.total_k);
-    const int64_t k1 = min64(max64(d, s.k0), p.total_k);
-    s.lk = (int)(k1 - s.k0);
-    bad |= s.k0 != c || k1 != d;
-  }
-  if (bad) set_dev_error(p.err, kDevBadArgs);
-  return s;
-}
-
-// keys [lo, hi) that query token `tok` of a sequence sees
-__device__ __forceinline__ int key_hi(const TextAttnParams& p, const Seq& s, int tok) {
-  return p.causal ? max(0, min(s.lk, tok + s.lk - s.lq + 1)) : s.lk;
-}
-__device__ __forceinline__ int key_lo(const TextAttnParams& p, const Seq& s, int tok) {
-  return p.window > 0 ? max(0, tok + s.lk - s.lq - p.window + 1) : 0;
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// ------------------------------------------------------------------ 8-bit -> bf16
-// Two stored bytes -> a bf16 pair, exactly. int8: 128 + low 7 bits and 128 or 256 (sign bit)
-// are both bf16 numbers whose difference is the value. e4m3: its 7 low bits are the top of a
-// bf16 with the exponent off by 120 (a bf16 product by 2^120 also sets subnormals right).
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-// byte `lo` of {b:a} to the low half, byte `hi` to the high half
-template <int FMT>
-__device__ __forceinline__ uint32_t bytes_to_bf16x2(uint32_t a, uint32_t b, int lo, int hi) {
-  if constexpr (FMT == kKvInt8) {
-    const uint32_t w = __byte_perm(a, b, (uint32_t)(lo | hi << 8));
-    return sub_bf16x2((w & 0x007f007fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u);
-  } else {
-    const uint32_t w = __byte_perm(a, b, (uint32_t)(lo << 4 | hi << 12));
-    return mul_bf16x2((w & 0x80008000u) | ((w >> 4) & 0x07f007f0u), 0x7b807b80u);  // 2^120
-  }
-}
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ float lds_f32(uint32_t a) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
 }
 
 // ------------------------------------------------- few query rows: text_rows_attn_kernel
@@ -759,11 +639,19 @@ static void fill_params(wx_ctx* ctx, const wx_attn_dims* d, const void* q, int64
 }
 
 template <int FMT, int HD>
-static int launch_rows_attn(wx_ctx* ctx, const CUtensorMap& tk, const CUtensorMap& tv, TextAttnParams& p) {
+static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   using G = RowsGeom<FMT, HD>;
   const int grid = ctx->num_sms;
   const int64_t items = (int64_t)p.hkv * (p.total_q * p.group / 16 + p.batch);
+  CUtensorMap tk, tv;
   int st;
+  if (FMT == kKvBf16) {
+    if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, 16))) return st;
+    if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, 16))) return st;
+  } else {
+    if ((st = make_tmap_u8_rows(ctx, &tk, kv.k, kv.rows, (uint32_t)kv.cols, 16))) return st;
+    if ((st = make_tmap_u8_rows(ctx, &tv, kv.v, kv.rows, (uint32_t)kv.cols, 16))) return st;
+  }
   Carve c;
   const size_t o_part = c.take((size_t)grid * 2 * 16 * HD * 4), o_ml = c.take((size_t)grid * 2 * 16 * 8);
   uint8_t* ws = static_cast<uint8_t*>(workspace(ctx, c.off, &st));
@@ -779,14 +667,16 @@ static int launch_rows_attn(wx_ctx* ctx, const CUtensorMap& tk, const CUtensorMa
   return launch_status(ctx, "text_rows_attn");
 }
 
-static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, int fmt, const CUtensorMap& tk, const CUtensorMap& tv,
-                         TextAttnParams& p) {
+// Up to 16 flattened rows a sequence (a decoding step, a few drafted tokens) fill one tile of the
+// rows kernel, which is bound by the K/V bytes; more rows go to the tcgen05 kernel.
+static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParams& p, const KvSource& kv) {
   const bool big = d->head_dim == 128;
-  if (fmt == kKvInt8)
-    return big ? launch_rows_attn<kKvInt8, 128>(ctx, tk, tv, p) : launch_rows_attn<kKvInt8, 64>(ctx, tk, tv, p);
-  if (fmt == kKvE4m3)
-    return big ? launch_rows_attn<kKvE4m3, 128>(ctx, tk, tv, p) : launch_rows_attn<kKvE4m3, 64>(ctx, tk, tv, p);
-  return big ? launch_rows_attn<kKvBf16, 128>(ctx, tk, tv, p) : launch_rows_attn<kKvBf16, 64>(ctx, tk, tv, p);
+  if (kv.format == kKvBf16 && (int64_t)d->max_q * p.group > 16) return text_flash(ctx, p, d->head_dim, kv);
+  if (kv.format == kKvInt8)
+    return big ? launch_rows_attn<kKvInt8, 128>(ctx, p, kv) : launch_rows_attn<kKvInt8, 64>(ctx, p, kv);
+  if (kv.format == kKvE4m3)
+    return big ? launch_rows_attn<kKvE4m3, 128>(ctx, p, kv) : launch_rows_attn<kKvE4m3, 64>(ctx, p, kv);
+  return big ? launch_rows_attn<kKvBf16, 128>(ctx, p, kv) : launch_rows_attn<kKvBf16, 64>(ctx, p, kv);
 }
 
 }  // namespace wx
@@ -808,11 +698,10 @@ int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, in
   fill_params(ctx, dims, q, q_stride, cu_q, out, out_stride, lse, p);
   p.cu_k = cu_k ? cu_k : cu_q;
   p.total_k = total_k;
-  CUtensorMap tk, tv;  // (with no keys at all the maps are never read: any valid address serves)
-  const uint64_t rows = (uint64_t)std::max<int64_t>(total_k, 1);
-  if ((st = make_tmap_bf16_2d(ctx, &tk, total_k ? k : q, rows, (uint64_t)cols, (uint64_t)k_stride, 64, 16))) return st;
-  if ((st = make_tmap_bf16_2d(ctx, &tv, total_k ? v : q, rows, (uint64_t)cols, (uint64_t)v_stride, 64, 16))) return st;
-  return dispatch_attn(ctx, dims, kKvBf16, tk, tv, p);
+  // (with no keys at all nothing is read: any valid address serves the tensor maps)
+  const KvSource kv{total_k ? k : q, total_k ? v : q, (uint64_t)std::max<int64_t>(total_k, 1), (uint64_t)cols,
+                    (uint64_t)k_stride, (uint64_t)v_stride, kKvBf16};
+  return dispatch_attn(ctx, dims, p, kv);
 }
 
 int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
@@ -835,16 +724,9 @@ int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int
   p.vs = cache->v_scale;
   p.pages = cache->pages;
   p.page_shift = __builtin_ctz((unsigned)cache->page_size);
-  const uint64_t rows = (uint64_t)cache->pages * cache->kv_heads * cache->page_size;
-  CUtensorMap tk, tv;
-  if (cache->format == WX_KV_BF16) {
-    if ((st = make_tmap_bf16_2d(ctx, &tk, cache->k, rows, cache->head_dim, cache->head_dim, 64, 16))) return st;
-    if ((st = make_tmap_bf16_2d(ctx, &tv, cache->v, rows, cache->head_dim, cache->head_dim, 64, 16))) return st;
-  } else {
-    if ((st = make_tmap_u8_rows(ctx, &tk, cache->k, rows, cache->head_dim, 16))) return st;
-    if ((st = make_tmap_u8_rows(ctx, &tv, cache->v, rows, cache->head_dim, 16))) return st;
-  }
-  return dispatch_attn(ctx, dims, cache->format, tk, tv, p);
+  const KvSource kv{cache->k, cache->v, (uint64_t)cache->pages * cache->kv_heads * cache->page_size,
+                    (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, cache->format};
+  return dispatch_attn(ctx, dims, p, kv);
 }
 
 }  // extern "C"

@@ -1,0 +1,140 @@
+// wx_text_dev.cuh — device pieces shared by the text side's attention kernels (wx_text_attn.cu,
+// wx_text_flash.cu): launch parameters, a sequence's bounds, 8-bit -> bf16.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "wx_ptx.cuh"
+#include "wx_text.h"
+
+namespace wx {
+
+struct TextAttnParams {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  float* lse;
+  const int32_t* cu_q;
+  const int32_t* cu_k;      // contiguous K/V (block_table == nullptr)
+  const int32_t* kv_lens;   // paged K/V
+  const int32_t* block_table;
+  int64_t blocks_per_seq;
+  const float *ks, *vs;     // scales of an 8-bit cache
+  int64_t pages;
+  int page_shift;
+  int batch, hq, hkv, group;
+  int64_t total_q, total_k;
+  int causal, window;
+  float sl2;  // scale * log2(e): scores and maxima are kept in base 2
+  float* part;              // split items: [2 * gridDim][16][hd] sums, then [..][16] maxima and denominators
+  float* part_ml;
+  int* counters;            // per item: pieces that have arrived (0 between launches)
+  int64_t n_items;          // of them
+  int* err;
+};
+
+// where K and V rows lie: `rows` rows of `cols` elements (strides in elements)
+struct KvSource {
+  const void *k, *v;
+  uint64_t rows, cols, k_stride, v_stride;
+  int format;
+};
+
+// attention for many query rows (wx_text_flash.cu)
+int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv);
+
+// One sequence as the kernels see it; lengths and offsets from the device are clamped to the
+// buffers, so that wrong ones give wrong rows and an error word but no access outside.
+struct Seq {
+  int64_t q0, k0;
+  int lq, lk;
+};
+
+__device__ __forceinline__ Seq load_seq(const TextAttnParams& p, int b) {
+  Seq s;
+  const int64_t a = p.cu_q[b], e = p.cu_q[b + 1];
+  s.q0 = min64(max64(a, 0), p.total_q);
+  const int64_t q1 = min64(max64(e, s.q0), p.total_q);
+  s.lq = (int)(q1 - s.q0);
+  bool bad = s.q0 != a || q1 != e;
+  if (p.block_table) {
+    const int64_t n = p.kv_lens[b], cap = p.blocks_per_seq << p.page_shift;
+    s.k0 = 0;
+    s.lk = (int)min64(max64(n, 0), cap);
+    bad |= s.lk != n;
+  } else {
+    const int64_t c = p.cu_k[b], d = p.cu_k[b + 1];
+    s.k0 = min64(max64(c, 0), p.total_k);
+    const int64_t k1 = min64(max64(d, s.k0), p.total_k);
+    s.lk = (int)(k1 - s.k0);
+    bad |= s.k0 != c || k1 != d;
+  }
+  if (bad) set_dev_error(p.err, kDevBadArgs);
+  return s;
+}
+
+// keys [lo, hi) that query token `tok` of a sequence sees
+__device__ __forceinline__ int key_hi(const TextAttnParams& p, const Seq& s, int tok) {
+  return p.causal ? max(0, min(s.lk, tok + s.lk - s.lq + 1)) : s.lk;
+}
+__device__ __forceinline__ int key_lo(const TextAttnParams& p, const Seq& s, int tok) {
+  return p.window > 0 ? max(0, tok + s.lk - s.lq - p.window + 1) : 0;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ------------------------------------------------------------------ 8-bit -> bf16
+// Two stored bytes -> a bf16 pair, exactly. int8: 128 + low 7 bits and 128 or 256 (sign bit)
+// are both bf16 numbers whose difference is the value. e4m3: its 7 low bits are the top of a
+// bf16 with the exponent off by 120 (a bf16 product by 2^120 also sets subnormals right).
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// byte `lo` of {b:a} to the low half, byte `hi` to the high half
+template <int FMT>
+__device__ __forceinline__ uint32_t bytes_to_bf16x2(uint32_t a, uint32_t b, int lo, int hi) {
+  if constexpr (FMT == kKvInt8) {
+    const uint32_t w = __byte_perm(a, b, (uint32_t)(lo | hi << 8));
+    return sub_bf16x2((w & 0x007f007fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u);
+  } else {
+    const uint32_t w = __byte_perm(a, b, (uint32_t)(lo << 4 | hi << 12));
+    return mul_bf16x2((w & 0x80008000u) | ((w >> 4) & 0x07f007f0u), 0x7b807b80u);  // 2^120
+  }
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+}  // namespace wx
