@@ -28,7 +28,7 @@ constexpr int kTfThreads = 384;
 constexpr int kTfRegsLow = 72, kTfRegsHigh = 216;
 static_assert(kTfRegsLow * 128 + kTfRegsHigh * 256 <= 168 * kTfThreads, "register split exceeds the launch");
 constexpr int kTfKStages = 3, kTfVStages = 2;
-constexpr int kTfItems = 4;     // items announced ahead
+constexpr int kTfItems = 2;     // item slots: the one at work and the next
 constexpr int kTfChunk = 128 * 128;  // one 64-column SW128 chunk of a 128-row tile
 constexpr int kTfBadRows = 1024;     // V rows with non-finite values remembered per item
 constexpr int kTfBadWords = 5;       // key, 128-bit column mask
@@ -93,6 +93,7 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 struct TfParams {
   TextAttnParams a;
   int box;             // rows of a K/V box: 128, or a page where pages are smaller
+  int* next;           // [2] items handed out, CTAs that have finished (0, 0 between launches)
   uint32_t* bad_rows;  // [CTA][kTfItems][kTfBadRows][kTfBadWords]
 };
 
@@ -377,10 +378,16 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     uint32_t nv = 0;                 // V tiles of the items before
     uint32_t raw[kTfVStages] = {};   // masked tiles mended per stage
     TfItem cur, next;
-    find(blockIdx.x, next);
+    // Items are handed out on demand: their costs differ by the length of their key range, and
+    // dealt out in turn the CTA that gets a head's first item would get every head's first.
+    auto hand_out = [&]() {
+      int i = 0;
+      if (lane == 0) i = atomicAdd(tp.next, 1);
+      return (int64_t)__shfl_sync(0xffffffffu, i, 0);
+    };
+    find(hand_out(), next);
     bool ok = true;
     for (int n = 0;; ++n) {
-      // announce item n, then item n + 1 is known when item n's tiles are mended
       if (n >= kTfItems &&
           !mbar_wait(bar(kBTfItemEmpty + n % kTfItems), ((n / kTfItems) & 1) ^ 1u, p.err, kDevTimeoutOther, abort_flag))
         ok = false;
@@ -392,7 +399,6 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       __syncwarp();
       cur = next;
       if (!cur.valid) break;
-      find((int64_t)blockIdx.x + (int64_t)(n + 1) * gridDim.x, next);
       uint32_t* list =
           tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
       const int t0 = cur.first(), t1 = cur.last();
@@ -460,6 +466,12 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         if (lane == 0) mbar_arrive(bar(kBTfVFull + s));
       }
       nv += (uint32_t)(t1 - t0);
+      if (ok) find(hand_out(), next);
+    }
+    if (lane == 0 && atomicAdd(tp.next + 1, 1) == (int)gridDim.x - 1) {
+      tp.next[0] = 0;  // nobody asks any more: ready for the next launch
+      tp.next[1] = 0;
+      __threadfence();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTfRegsHigh));
@@ -674,6 +686,7 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tk, const CUtensorMap& t
   void* ws = workspace(ctx, (size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4, &st);
   if (!ws) return st;
   tp.bad_rows = static_cast<uint32_t*>(ws);
+  if (!(tp.next = arrival_counters(ctx, 2, &st))) return st;
   ProfScope prof(ctx, kProfAttn);
   fn<<<grid, kTfThreads, TfGeom<HD>::kSmem, ctx->stream>>>(tk, tv, tp);
   return launch_status(ctx, "text_flash");
