@@ -107,6 +107,25 @@ int make_tmap_u32_2d(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t r
   return WX_OK;
 }
 
+int make_tmap_bf16_3d(wx_ctx* ctx, CUtensorMap* map, const void* base, const uint64_t (&dims)[3],
+                      const uint64_t (&ld)[2], const uint32_t (&box)[3]) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return set_error(ctx, WX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  if (!aligned16(base) || (ld[0] * 2) % 16 != 0 || (ld[1] * 2) % 16 != 0)
+    return set_error(ctx, WX_ERR_INVALID, "TMA operand needs 16-byte aligned base and strides");
+  cuuint64_t gdim[3] = {dims[0], dims[1], dims[2]};
+  cuuint64_t gstride[2] = {ld[0] * 2, ld[1] * 2};
+  cuuint32_t b[3] = {box[0], box[1], box[2]};
+  cuuint32_t estride[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), gdim, gstride, b, estride,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(ctx, WX_ERR_CUDA, "cuTensorMapEncodeTiled (3-D) failed (%d): %llu x %llu x %llu", (int)r,
+                     (unsigned long long)dims[2], (unsigned long long)dims[1], (unsigned long long)dims[0]);
+  return WX_OK;
+}
+
 int make_tmap_u8_rows(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t rows, uint32_t cols,
                       uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();

@@ -102,6 +102,11 @@ int make_tmap_bf16_2d(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t 
 int make_tmap_u32_2d(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                      uint32_t box_cols, uint32_t box_rows);
 
+// 3-D bf16 tensor map, innermost dimension first; `ld` the element strides of the outer two,
+// 128-byte swizzle, zero fill out of bounds.
+int make_tmap_bf16_3d(wx_ctx* ctx, CUtensorMap* map, const void* base, const uint64_t (&dims)[3],
+                      const uint64_t (&ld)[2], const uint32_t (&box)[3]);
+
 // 2-D byte tensor map of contiguous rows of `cols` (64 or 128) bytes, box `box_rows` whole rows,
 // swizzled over the row's width, zero fill out of bounds.
 int make_tmap_u8_rows(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t rows, uint32_t cols,

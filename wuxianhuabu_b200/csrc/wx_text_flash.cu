@@ -1,8 +1,8 @@
 // wx_text_flash.cu — attention of the text side for many query rows: whole packed prompts, and
 // chunks of new tokens over the paged cache.
 //
-// Mathematics: the query rows of one K/V head are flattened to r = token * G + g, so 256 rows
-// (256 / G tokens) share one walk over the keys they may see; each row keeps a running maximum
+// Mathematics: the query rows of one K/V head are flattened to r = token * G + g, so the rows of
+// 2 * floor(128 / G) tokens share one walk over the keys they may see; each row keeps a running maximum
 // and denominator, o = sum 2^(s - m) v is rescaled only when the maximum has grown by more than
 // 2^8, and the weights are rounded to bf16 for the second product (the denominator is not).
 //
@@ -14,7 +14,7 @@
 //   P overwrites the first half of its S as packed bf16.
 //   Warp 0: TMA producer of K and V. Warps 1 / 2: MMA issuer of slot A / B. Warp 3: finds the
 //   items and mends masked V tiles. Warps 4-7 / 8-11: softmax and epilogue of slot A / B (thread
-//   r owns row r); they also bring the next item's Q into shared memory before their epilogue.
+//   r owns row r); one of their threads fetches the next item's Q as soon as the last S is done.
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -42,10 +42,10 @@ struct TfGeom {
   static constexpr int kSmem = kItemOff + kTfItems * 128 + 1024;
 };
 
-// One item: 256 flattened rows of one K/V head of one sequence
+// One item: the query heads of one K/V head for 2 * TT tokens of one sequence
 struct TfItem {
   int valid;
-  int b, h, row0;  // first flattened row
+  int b, h, tok0;  // tok0: first token
   int lq, lk, q0, k0;
   int a0, a1, b0, b1;    // key tiles [a0, a1) of slot A, [b0, b1) of slot B
   int free_hi, free_lo;  // tiles inside [free_lo, free_hi) are unmasked for every row
@@ -60,7 +60,7 @@ struct TfItem {
 enum : int {
   kBTfItemFull = 0,                       // [items]
   kBTfItemEmpty = kBTfItemFull + kTfItems,  // [items] count 11: every other warp has read it
-  kBTfQFull = kBTfItemEmpty + kTfItems,   // [2] count 4
+  kBTfQFull = kBTfItemEmpty + kTfItems,   // [2]
   kBTfKFull = kBTfQFull + 2,              // [K stages]
   kBTfKEmpty = kBTfKFull + kTfKStages,    // count 2: both slots
   kBTfVRaw = kBTfKEmpty + kTfKStages,     // [V stages] a masked tile has landed
@@ -92,6 +92,7 @@ __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
 
 struct TfParams {
   TextAttnParams a;
+  int tt;              // tokens of a slot: floor(128 / G)
   int box;             // rows of a K/V box: 128, or a page where pages are smaller
   int* next;           // [2] items handed out, CTAs that have finished (0, 0 between launches)
   uint32_t* bad_rows;  // [CTA][kTfItems][kTfBadRows][kTfBadWords]
@@ -99,7 +100,8 @@ struct TfParams {
 
 template <int HD>
 __global__ void __launch_bounds__(kTfThreads, 1)
-    text_flash_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, TfParams tp) {
+    text_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                      const __grid_constant__ CUtensorMap tmV, TfParams tp) {
   using G = TfGeom<HD>;
   constexpr int kTile = G::kTile;
   const TextAttnParams& p = tp.a;
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       uint32_t c = 1;
       if (i >= kBTfItemEmpty && i < kBTfItemEmpty + kTfItems) c = 11;
       if ((i >= kBTfKEmpty && i < kBTfKEmpty + kTfKStages) || (i >= kBTfVFull && i < kBTfVEmpty + kTfVStages)) c = 2;
-      if ((i >= kBTfQFull && i < kBTfQFull + 2) || (i >= kBTfPFull && i < kBTfPFull + 8) ||
+      if ((i >= kBTfPFull && i < kBTfPFull + 8) ||
           (i >= kBTfOEmpty && i < kBTfOEmpty + 2))
         c = 4;
       mbar_init(bar(i), c);
@@ -159,6 +161,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTfRegsLow));
     // ------------------------------------------------------------ producer
     if (lane == 0) {
+      prefetch_tmap(&tmQ);
       prefetch_tmap(&tmK);
       prefetch_tmap(&tmV);
     }
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     auto seq_items = [&](int b) -> int64_t {
       if (b >= p.batch) return 0;
       const Seq s = load_seq(p, b);
-      return (((int64_t)s.lq * p.group + 255) / 256) * p.hkv;
+      return (int64_t)((s.lq + 2 * tp.tt - 1) / (2 * tp.tt)) * p.hkv;
     };
     int wb = 0;
     int64_t wi = 0;  // items of the sequences before wb
@@ -346,29 +349,28 @@ __global__ void __launch_bounds__(kTfThreads, 1)
           const int src = __ffs(__ballot_sync(0xffffffffu, at < wi + nc)) - 1;
           const int in_b = (int)(at - wi - __shfl_sync(0xffffffffu, nc - n, src));
           const Seq s = load_seq(p, wb + src);
-          const int64_t rows = (int64_t)s.lq * p.group;
-          const int tiles = (int)((rows + 255) / 256);
+          const int tiles = (s.lq + 2 * tp.tt - 1) / (2 * tp.tt);
           c.valid = 1;
           c.b = wb + src;
           c.h = in_b / tiles;
-          c.row0 = (tiles - 1 - in_b % tiles) * 256;
+          c.tok0 = (tiles - 1 - in_b % tiles) * 2 * tp.tt;
           c.lq = s.lq;
           c.lk = s.lk;
           c.q0 = (int)s.q0;
           c.k0 = (int)s.k0;
-          auto tiles_of = [&](int64_t r0, int& x0, int& x1) {
-            const int64_t r1 = min64(rows, r0 + 128);
+          auto tiles_of = [&](int k0, int& x0, int& x1) {
+            const int k1 = min(s.lq, k0 + tp.tt);  // tokens [k0, k1)
             x0 = x1 = 0;
-            if (r0 >= r1) return;
-            const int hi = key_hi(p, s, (int)((r1 - 1) / p.group)), lo = key_lo(p, s, (int)(r0 / p.group));
+            if (k0 >= k1) return;
+            const int hi = key_hi(p, s, k1 - 1), lo = key_lo(p, s, k0);
             if (hi <= lo) return;
             x0 = lo >> 7;
             x1 = (hi + 127) >> 7;
           };
-          tiles_of(c.row0, c.a0, c.a1);
-          tiles_of(c.row0 + 128, c.b0, c.b1);
-          c.free_hi = key_hi(p, s, c.row0 / p.group);
-          c.free_lo = key_lo(p, s, (int)((min64(rows, c.row0 + 256) - 1) / p.group));
+          tiles_of(c.tok0, c.a0, c.a1);
+          tiles_of(c.tok0 + tp.tt, c.b0, c.b1);
+          c.free_hi = key_hi(p, s, c.tok0);
+          c.free_lo = key_lo(p, s, min(s.lq, c.tok0 + 2 * tp.tt) - 1);
           return;
         }
         wi += all;
@@ -377,7 +379,6 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     };
     uint32_t nv = 0;                 // V tiles of the items before
     uint32_t raw[kTfVStages] = {};   // masked tiles mended per stage
-    TfItem cur, next;
     // Items are handed out on demand: their costs differ by the length of their key range, and
     // dealt out in turn the CTA that gets a head's first item would get every head's first.
     auto hand_out = [&]() {
@@ -385,20 +386,27 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       if (lane == 0) i = atomicAdd(tp.next, 1);
       return (int64_t)__shfl_sync(0xffffffffu, i, 0);
     };
-    find(hand_out(), next);
     bool ok = true;
-    for (int n = 0;; ++n) {
-      if (n >= kTfItems &&
+    auto announce = [&](int n, TfItem& c) {
+      if (n >= kTfItems && ok &&
           !mbar_wait(bar(kBTfItemEmpty + n % kTfItems), ((n / kTfItems) & 1) ^ 1u, p.err, kDevTimeoutOther, abort_flag))
         ok = false;
-      if (!ok) next.valid = 0;
+      if (!ok) c.valid = 0;
       if (lane == 0) {
-        items[n % kTfItems] = next;
+        items[n % kTfItems] = c;
         mbar_arrive(bar(kBTfItemFull + n % kTfItems));
       }
       __syncwarp();
+    };
+    TfItem cur, next;
+    find(hand_out(), next);
+    announce(0, next);
+    for (int n = 0; next.valid; ++n) {
       cur = next;
-      if (!cur.valid) break;
+      // the next item is announced while this one is at work (as soon as the last one's slot is
+      // free), so that its loads and first products follow on without a gap
+      find(hand_out(), next);
+      announce(n + 1, next);
       uint32_t* list =
           tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
       const int t0 = cur.first(), t1 = cur.last();
@@ -466,7 +474,6 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         if (lane == 0) mbar_arrive(bar(kBTfVFull + s));
       }
       nv += (uint32_t)(t1 - t0);
-      if (ok) find(hand_out(), next);
     }
     if (lane == 0 && atomicAdd(tp.next + 1, 1) == (int)gridDim.x - 1) {
       tp.next[0] = 0;  // nobody asks any more: ready for the next launch
@@ -485,38 +492,28 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     uint32_t base_a = 0, base_b = 0;  // tiles of slot A / B in the items before
     uint32_t n_o = 0;           // items of this slot that had tiles
 
-    // Q rows of the item into shared memory: 16 lanes per row (HD 128), rows past the end zero
+    // The item's Q by TMA: G heads of TT tokens are the slot's rows in order (rows of other
+    // sequences or past the end may come along: their results are not written).
+    const uint32_t q_bytes = (uint32_t)(tp.tt * p.group * HD * 2);
     auto load_q = [&](const TfItem& c) {
-      if (c.hi(X) <= c.lo(X)) return;
-      constexpr int kLanes = HD / 8, kRows = 32 / kLanes;
-      const int64_t rows = (int64_t)c.lq * p.group;
-      const int ch = lane % kLanes;
-#pragma unroll 4
-      for (int i = 0; i < 32 / kRows; ++i) {
-        const int rr = quarter * 32 + i * kRows + lane / kLanes;
-        const int64_t fr = (int64_t)c.row0 + X * 128 + rr;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (fr < rows) {
-          const int tok = (int)fr / p.group, head = c.h * p.group + (int)fr % p.group;
-          w = __ldg(reinterpret_cast<const uint4*>(p.q + ((int64_t)c.q0 + tok) * p.q_stride + (int64_t)head * HD + ch * 8));
-        }
-        sts128(sQ(X) + (uint32_t)((ch >> 3) * kTfChunk + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)), w);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kBTfQFull + X));
+      if (c.hi(X) <= c.lo(X) || quarter != 0 || lane != 0) return;
+      mbar_arrive_expect_tx(bar(kBTfQFull + X), q_bytes);
+#pragma unroll
+      for (int ch = 0; ch < G::kChunks; ++ch)
+        tma_load_3d(sQ(X) + ch * kTfChunk, &tmQ, bar(kBTfQFull + X), ch * 64, c.h * p.group, c.q0 + c.tok0 + X * tp.tt);
     };
 
+    const int my_tok = r / p.group, my_g = r % p.group;  // (rows past TT * G are not live)
     TfItem it, nx;
     bool ok = true;
     bool have = take_item(0, it);
     if (have) load_q(it);
     for (int n = 0; have; ++n) {
       const int a0 = it.lo(X), a1 = it.hi(X);
-      const int64_t fr = (int64_t)it.row0 + X * 128 + r;
-      const bool live = fr < (int64_t)it.lq * p.group;
-      const int tok = live ? (int)fr / p.group : 0;
-      const int head = it.h * p.group + (live ? (int)fr % p.group : 0);
+      const bool live = r < tp.tt * p.group && it.tok0 + X * tp.tt + my_tok < it.lq;
+      const int tok = live ? it.tok0 + X * tp.tt + my_tok : 0;
+      const int head = it.h * p.group + my_g;
+      bool q_sent = false;
       const int hi = live ? (p.causal ? max(0, min(it.lk, tok + it.lk - it.lq + 1)) : it.lk) : 0;
       const int lo = p.window > 0 ? max(0, tok + it.lk - it.lq - p.window + 1) : 0;
       float m = -INFINITY, l = 0.f;
@@ -526,6 +523,12 @@ __global__ void __launch_bounds__(kTfThreads, 1)
           break;
         }
         tc_fence_after();
+        // the slot's last S is done: its Q may be replaced, if the next item is known yet
+        if (t == a1 - 1 && quarter == 0 && mbar_try_wait(bar(kBTfItemFull + (n + 1) % kTfItems), ((n + 1) / kTfItems) & 1)) {
+          const TfItem& c = items[(n + 1) % kTfItems];
+          if (c.valid) load_q(c);
+          q_sent = true;
+        }
         float v[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(v + c * 32));
@@ -606,10 +609,9 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       }
       base_a += (uint32_t)max(0, it.a1 - it.a0);
       base_b += (uint32_t)max(0, it.b1 - it.b0);
-      // the next item's Q goes in first (the last S of this slot has completed): its products
-      // then run while this item's rows are written
+      // the next item's Q goes in first: its products then run while this item's rows are written
       have = ok && take_item(n + 1, nx);
-      if (have) load_q(nx);
+      if (have && !q_sent) load_q(nx);
       const bool any = a1 > a0;
       if (ok && any) ok = mbar_wait(bar(kBTfOFull + X), n_o & 1, p.err, kDevTimeoutSoftmax, abort_flag);
       n_o += any ? 1 : 0;
@@ -669,7 +671,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
 }
 
 template <int HD>
-static int launch_flash(wx_ctx* ctx, const CUtensorMap& tk, const CUtensorMap& tv, TfParams& tp) {
+static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, TfParams& tp) {
   auto fn = text_flash_kernel<HD>;
   int st = ensure_smem_attr(ctx, (const void*)fn, TfGeom<HD>::kSmem, "text_flash");
   if (st) return st;
@@ -681,14 +683,14 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tk, const CUtensorMap& t
   }();
   if (!regs_ok) return set_error(ctx, WX_ERR_CUDA, "text_flash: register split does not fit");
   const TextAttnParams& p = tp.a;
-  const int64_t items = (int64_t)p.hkv * (p.total_q * p.group / 256 + p.batch);
+  const int64_t items = (int64_t)p.hkv * (p.total_q / (2 * tp.tt) + p.batch);
   const int grid = (int)std::min<int64_t>(ctx->num_sms, items);
   void* ws = workspace(ctx, (size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4, &st);
   if (!ws) return st;
   tp.bad_rows = static_cast<uint32_t*>(ws);
   if (!(tp.next = arrival_counters(ctx, 2, &st))) return st;
   ProfScope prof(ctx, kProfAttn);
-  fn<<<grid, kTfThreads, TfGeom<HD>::kSmem, ctx->stream>>>(tk, tv, tp);
+  fn<<<grid, kTfThreads, TfGeom<HD>::kSmem, ctx->stream>>>(tq, tk, tv, tp);
   return launch_status(ctx, "text_flash");
 }
 
@@ -696,11 +698,16 @@ int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSourc
   TfParams tp{};
   tp.a = p;
   tp.box = p.block_table ? std::min(128, 1 << p.page_shift) : 128;
-  CUtensorMap tk, tv;
+  tp.tt = 128 / p.group;
+  CUtensorMap tq, tk, tv;
   int st;
+  const uint64_t dims[3] = {(uint64_t)head_dim, (uint64_t)p.hq, (uint64_t)p.total_q};
+  const uint64_t ld[2] = {(uint64_t)head_dim, (uint64_t)p.q_stride};
+  const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tp.tt};
+  if ((st = make_tmap_bf16_3d(ctx, &tq, p.q, dims, ld, box))) return st;
   if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, tp.box))) return st;
   if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, tp.box))) return st;
-  return head_dim == 128 ? launch_flash<128>(ctx, tk, tv, tp) : launch_flash<64>(ctx, tk, tv, tp);
+  return head_dim == 128 ? launch_flash<128>(ctx, tq, tk, tv, tp) : launch_flash<64>(ctx, tq, tk, tv, tp);
 }
 
 }  // namespace wx
