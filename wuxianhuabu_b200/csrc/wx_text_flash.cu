@@ -30,6 +30,7 @@ static_assert(kTfRegsLow * 128 + kTfRegsHigh * 256 <= 168 * kTfThreads, "registe
 constexpr int kTfKStages = 3, kTfVStages = 2;
 constexpr int kTfItems = 2;     // item slots: the one at work and the next
 constexpr int kTfChunk = 128 * 128;  // one 64-column SW128 chunk of a 128-row tile
+constexpr int64_t kTfL2 = int64_t(48) << 20;
 constexpr int kTfBadRows = 1024;     // V rows with non-finite values remembered per item
 constexpr int kTfBadWords = 5;       // key, 128-bit column mask
 
@@ -59,7 +60,7 @@ struct TfItem {
 
 enum : int {
   kBTfItemFull = 0,                       // [items]
-  kBTfItemEmpty = kBTfItemFull + kTfItems,  // [items] count 11: every other warp has read it
+  kBTfItemEmpty = kBTfItemFull + kTfItems,  // [items] count 11: every other warp is done with it
   kBTfQFull = kBTfItemEmpty + kTfItems,   // [2]
   kBTfKFull = kBTfQFull + 2,              // [K stages]
   kBTfKEmpty = kBTfKFull + kTfKStages,    // count 2: both slots
@@ -70,7 +71,8 @@ enum : int {
   kBTfPFull = kBTfSFull + 2,              // [2][4] count 4
   kBTfOFull = kBTfPFull + 8,              // [2]
   kBTfOEmpty = kBTfOFull + 2,             // [2] count 4: the epilogue has read O
-  kBTfDrain = kBTfOEmpty + 2,             // [2]
+  kBTfTurn = kBTfOEmpty + 2,              // [2] count 4: a slot's exponentials of a tile are issued
+  kBTfDrain = kBTfTurn + 2,               // [2]
   kBTfCount = kBTfDrain + 2
 };
 static_assert(kBTfCount * 8 + 32 <= 512, "barriers overlap the items");
@@ -88,6 +90,37 @@ __device__ __forceinline__ uint64_t fresh64(uint64_t v) {
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// 32 lanes x 16 columns of 32-bit: thread i of the warp gets lane (base + i), 16 columns
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Zeroes the non-finite values of row r of a V tile and notes their columns in `entry`.
+template <int HD>
+__device__ __noinline__ void remember_row(uint32_t row, int r, int key, uint32_t* entry) {
+  uint32_t mask[4] = {0, 0, 0, 0};
+#pragma unroll 1
+  for (int d = 0; d < HD; ++d) {
+    const uint32_t at = row + (d >> 6) * kTfChunk + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2;
+    if ((lds_u16(at) & 0x7f80u) != 0x7f80u) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mask[e] |= (d >> 5) == e ? 1u << (d & 31) : 0u;
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((uint16_t)0) : "memory");
+  }
+  if (!entry) return;
+  entry[0] = (uint32_t)key;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) entry[1 + e] = mask[e];
 }
 
 struct TfParams {
@@ -115,7 +148,6 @@ __global__ void __launch_bounds__(kTfThreads, 1)
   auto bar = [&](int i) { return smem_u32(bars + i); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBTfCount);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* turns = reinterpret_cast<int*>(tmem_slot + 2);  // [2] warps x tiles whose exponentials are done
   TfItem* items = reinterpret_cast<TfItem*>(smem + G::kItemOff);
   static_assert(sizeof(TfItem) <= 128, "item slots");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -126,12 +158,11 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       if (i >= kBTfItemEmpty && i < kBTfItemEmpty + kTfItems) c = 11;
       if ((i >= kBTfKEmpty && i < kBTfKEmpty + kTfKStages) || (i >= kBTfVFull && i < kBTfVEmpty + kTfVStages)) c = 2;
       if ((i >= kBTfPFull && i < kBTfPFull + 8) ||
-          (i >= kBTfOEmpty && i < kBTfOEmpty + 2))
+          (i >= kBTfOEmpty && i < kBTfTurn + 2))
         c = 4;
       mbar_init(bar(i), c);
     }
     *abort_flag = 0;
-    turns[0] = turns[1] = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -143,14 +174,12 @@ __global__ void __launch_bounds__(kTfThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // item n as this warp sees it; its slot goes back when the warp is done with it
-  auto take_item = [&](int n, TfItem& it) -> bool {
-    if (!mbar_wait(bar(kBTfItemFull + n % kTfItems), (n / kTfItems) & 1, p.err, kDevTimeoutOther, abort_flag)) {
-      it.valid = 0;
-      return false;
-    }
-    it = items[n % kTfItems];
-    return it.valid != 0;
+  // item n, in shared memory until this warp drops it (nullptr: no more items, or a wait ran out)
+  auto take_item = [&](int n) -> const TfItem* {
+    if (!mbar_wait(bar(kBTfItemFull + n % kTfItems), (n / kTfItems) & 1, p.err, kDevTimeoutOther, abort_flag))
+      return nullptr;
+    const TfItem* it = items + n % kTfItems;
+    return it->valid ? it : nullptr;
   };
   auto drop_item = [&](int n) {
     __syncwarp();
@@ -167,9 +196,11 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     }
     uint32_t nk = 0, nv = 0;  // tiles loaded
     const int boxes = 128 / tp.box;
-    TfItem it;
     bool ok = true;
-    for (int n = 0; ok && take_item(n, it); ++n) {
+    for (int n = 0; ok; ++n) {
+      const TfItem* at = take_item(n);
+      if (!at) break;
+      const TfItem& it = *at;
       const int t0 = it.first(), t1 = it.last();
       int ids = 0, ids_from = -1;  // block entries of 32 consecutive boxes, one per lane
       auto load = [&](bool is_k, int t) -> bool {
@@ -215,10 +246,13 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         if (is_k) ++nk; else ++nv;
         return true;
       };
-      ok = t1 <= t0 || (load(true, t0) && (t0 + 1 >= t1 || load(true, t0 + 1)));
-      for (int t = t0; t < t1 && ok; ++t) {
-        ok = load(false, t);
-        if (ok && t + 2 < t1) ok = load(true, t + 2);
+      // K two tiles ahead of V: K0 K1 V0 K2 V1 ...
+#pragma unroll 1
+      for (int i = 0; i < 2 * (t1 - t0) && ok; ++i) {
+        const int tiles = t1 - t0;
+        const bool tail = i >= 2 * tiles - 1;  // (the last two are both V; a single tile is K0 V0)
+        const bool is_k = i < 2 ? (i == 0 || tiles > 1) : !tail && (i & 1);
+        ok = load(is_k, t0 + (is_k ? (i < 2 ? i : (i + 1) / 2) : tail ? tiles - 1 : (i - 1) / 2));
       }
       drop_item(n);
     }
@@ -243,73 +277,67 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     uint32_t mine = 0;  // tiles of this slot so far
     uint32_t n_o = 0;   // items in which this slot had tiles
     bool ok = true, issued = false;
-    TfItem it;
-    for (int n = 0; ok && take_item(n, it); ++n) {
+    for (int n = 0; ok; ++n) {
+      const TfItem* at = take_item(n);
+      if (!at) break;
+      const TfItem& it = *at;
       const int t0 = it.first(), t1 = it.last();
       const bool any = it.hi(X) > it.lo(X);
       const int a0 = any ? it.lo(X) : t1, a1 = any ? it.hi(X) : t1;
       if (lane == 0) {
-        auto wait_k = [&](int t) {
-          const uint32_t c = kv + (uint32_t)(t - t0);
-          return mbar_wait(bar(kBTfKFull + c % kTfKStages), (c / kTfKStages) & 1, p.err, kDevTimeoutFull, abort_flag);
-        };
-        auto wait_v = [&](int t) {
-          const uint32_t c = kv + (uint32_t)(t - t0);
-          return mbar_wait(bar(kBTfVFull + c % kTfVStages), (c / kTfVStages) & 1, p.err, kDevTimeoutFull, abort_flag);
-        };
-        auto kbar = [&](int t) { return bar(kBTfKEmpty + (kv + (uint32_t)(t - t0)) % kTfKStages); };
-        auto vbar = [&](int t) { return bar(kBTfVEmpty + (kv + (uint32_t)(t - t0)) % kTfVStages); };
-        auto skip = [&](int t) {  // a tile only the other slot works on
-          if (!wait_k(t)) return false;
-          mbar_arrive(kbar(t));
-          if (!wait_v(t)) return false;
-          mbar_arrive(vbar(t));
-          return true;
-        };
-        auto issue_s = [&](int t) {
-          tc_fence_after();
-          const uint64_t dk = fresh64(smem_desc_sw128(sK((kv + (uint32_t)(t - t0)) % kTfKStages), 16, 1024));
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = ((kk >> 2) * kTfChunk + (kk & 3) * 32) >> 4;
-            umma_bf16(tS, dq + off, dk + off, idesc_s, kk > 0 ? 1u : 0u);
-          }
-          issued = true;
-          umma_commit(bar(kBTfSFull + X));
-          umma_commit(kbar(t));
-        };
         if (any) ok = mbar_wait(bar(kBTfQFull + X), n_o & 1, p.err, kDevTimeoutSoftmax, abort_flag);
-        for (int t = t0; ok && t < a0; ++t) ok = skip(t);
-        if (ok && a0 < a1 && (ok = wait_k(a0))) issue_s(a0);
-        for (int t = a0; ok && t < a1; ++t) {
+        // step t: O += P(t) V(t), then S(t + 1); a tile that only the other slot works on is
+        // just given back
+#pragma unroll 1
+        for (int t = t0 - 1; t < t1 && ok; ++t) {
           // V(t) and K(t+1) are waited for before P(t): PV(t) and S(t+1) then go out back to back
-          ok = wait_v(t) && (t + 1 >= a1 || wait_k(t + 1));
+          const uint32_t cv = kv + (uint32_t)(t - t0), ck = cv + 1;
+          const uint32_t sv = cv % kTfVStages, sk = ck % kTfKStages;
+          if (t >= t0)
+            ok = mbar_wait(bar(kBTfVFull + sv), (cv / kTfVStages) & 1, p.err, kDevTimeoutFull, abort_flag);
+          if (ok && t + 1 < t1)
+            ok = mbar_wait(bar(kBTfKFull + sk), (ck / kTfKStages) & 1, p.err, kDevTimeoutFull, abort_flag);
           // the first product of an item overwrites O: the last epilogue must have read it
           if (ok && t == a0 && n_o > 0)
             ok = mbar_wait(bar(kBTfOEmpty + X), (n_o - 1) & 1, p.err, kDevTimeoutSoftmax, abort_flag);
           if (!ok) break;
-          const uint64_t dv =
-              fresh64(smem_desc_sw128(sV((kv + (uint32_t)(t - t0)) % kTfVStages), kTfChunk, 1024));
+          if (t >= a0 && t < a1) {
+            const uint64_t dv = fresh64(smem_desc_sw128(sV(sv), kTfChunk, 1024));
 #pragma unroll
-          for (int part = 0; part < 4 && ok; ++part) {
-            if (!mbar_wait(bar(kBTfPFull + X * 4 + part), (mine + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax,
-                           abort_flag)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
+            for (int part = 0; part < 4; ++part) {
+              if (!mbar_wait(bar(kBTfPFull + X * 4 + part), (mine + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax,
+                             abort_flag)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-              const int kk = part * 2 + k2;
-              umma_bf16_ts(tO, tS + kk * 8, dv + (uint64_t)(kk * (2048 >> 4)), idesc_o, (t > a0 || kk > 0) ? 1u : 0u);
+              for (int k2 = 0; k2 < 2; ++k2) {
+                const int kk = part * 2 + k2;
+                umma_bf16_ts(tO, tS + kk * 8, dv + (uint64_t)(kk * (2048 >> 4)), idesc_o, (t > a0 || kk > 0) ? 1u : 0u);
+              }
             }
+            if (!ok) break;
+            umma_commit(bar(kBTfVEmpty + sv));
+            if (t == a1 - 1) umma_commit(bar(kBTfOFull + X));
+          } else if (t >= t0) {
+            mbar_arrive(bar(kBTfVEmpty + sv));
           }
-          if (!ok) break;
-          umma_commit(vbar(t));
-          if (t + 1 < a1) issue_s(t + 1);
+          if (t + 1 >= a0 && t + 1 < a1) {
+            tc_fence_after();
+            const uint64_t dk = fresh64(smem_desc_sw128(sK(sk), 16, 1024));
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * kTfChunk + (kk & 3) * 32) >> 4;
+              umma_bf16(tS, dq + off, dk + off, idesc_s, kk > 0 ? 1u : 0u);
+            }
+            issued = true;
+            umma_commit(bar(kBTfSFull + X));
+            umma_commit(bar(kBTfKEmpty + sk));
+          } else if (t + 1 < t1) {
+            mbar_arrive(bar(kBTfKEmpty + sk));
+          }
         }
-        if (ok && a0 < a1) umma_commit(bar(kBTfOFull + X));
-        for (int t = max(a1, t0); ok && t < t1; ++t) ok = skip(t);
         mine += (uint32_t)(a1 - a0);
         kv += (uint32_t)(t1 - t0);
         n_o += any ? 1 : 0;
@@ -324,58 +352,70 @@ __global__ void __launch_bounds__(kTfThreads, 1)
   } else if (warp == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTfRegsLow));
     // ------------------------------------------------------------ items, and masked V tiles
-    // Items in the order (sequence, K/V head, rows from the last): CTAs that run at the same
-    // time share a head's keys in L2, and the long causal rows of a head go first.
-    auto seq_items = [&](int b) -> int64_t {
+    // Items in the order (sequence, chunk of K/V heads, rows from the last, head): the long causal
+    // rows go first, so that the short ones level the CTAs out at the end, and a chunk holds as
+    // many heads as keep their keys and values (kTfL2 bytes) in L2 together.
+    auto seq_items = [&](int b) -> int {
       if (b >= p.batch) return 0;
       const Seq s = load_seq(p, b);
-      return (int64_t)((s.lq + 2 * tp.tt - 1) / (2 * tp.tt)) * p.hkv;
+      return (int)((unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt)) * p.hkv;
     };
     int wb = 0;
-    int64_t wi = 0;  // items of the sequences before wb
-    auto find = [&](int64_t at, TfItem& c) {
-      c.valid = 0;
-      c.bad = 0;
+    int wi = 0;  // items of the sequences before wb
+    // item number `at` into its slot (every lane works it out, lane 0 writes); false: no such item
+    auto find = [&](int at, TfItem* dst) -> bool {
       while (wb < p.batch) {
-        const int64_t n = seq_items(wb + lane);
-        int64_t nc = n;
+        const int n = seq_items(wb + lane);
+        int nc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int64_t a = __shfl_up_sync(0xffffffffu, nc, o);
+          const int a = __shfl_up_sync(0xffffffffu, nc, o);
           if (lane >= o) nc += a;
         }
-        const int64_t all = __shfl_sync(0xffffffffu, nc, 31);
+        const int all = __shfl_sync(0xffffffffu, nc, 31);
         if (at < wi + all) {
           const int src = __ffs(__ballot_sync(0xffffffffu, at < wi + nc)) - 1;
-          const int in_b = (int)(at - wi - __shfl_sync(0xffffffffu, nc - n, src));
-          const Seq s = load_seq(p, wb + src);
-          const int tiles = (s.lq + 2 * tp.tt - 1) / (2 * tp.tt);
-          c.valid = 1;
-          c.b = wb + src;
-          c.h = in_b / tiles;
-          c.tok0 = (tiles - 1 - in_b % tiles) * 2 * tp.tt;
-          c.lq = s.lq;
-          c.lk = s.lk;
-          c.q0 = (int)s.q0;
-          c.k0 = (int)s.k0;
-          auto tiles_of = [&](int k0, int& x0, int& x1) {
-            const int k1 = min(s.lq, k0 + tp.tt);  // tokens [k0, k1)
-            x0 = x1 = 0;
-            if (k0 >= k1) return;
-            const int hi = key_hi(p, s, k1 - 1), lo = key_lo(p, s, k0);
-            if (hi <= lo) return;
-            x0 = lo >> 7;
-            x1 = (hi + 127) >> 7;
-          };
-          tiles_of(c.tok0, c.a0, c.a1);
-          tiles_of(c.tok0 + tp.tt, c.b0, c.b1);
-          c.free_hi = key_hi(p, s, c.tok0);
-          c.free_lo = key_lo(p, s, min(s.lq, c.tok0 + 2 * tp.tt) - 1);
-          return;
+          const unsigned in_b = (unsigned)(at - wi - __shfl_sync(0xffffffffu, nc - n, src));
+          if (lane == 0) {
+            const Seq s = load_seq(p, wb + src);
+            const unsigned tiles = (unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt);
+            const unsigned fit = (unsigned)(kTfL2 / (HD * 4)) / (unsigned)max(1, s.lk);
+            const unsigned heads = max(1u, min((unsigned)p.hkv, fit));
+            const unsigned chunk = in_b / (tiles * heads), rest = in_b - chunk * tiles * heads;
+            const unsigned mine = min(heads, p.hkv - chunk * heads);
+            const int tok0 = (int)((tiles - 1 - rest / mine) * 2) * tp.tt;
+            dst->valid = 1;
+            dst->bad = 0;
+            dst->b = wb + src;
+            dst->h = (int)(chunk * heads + rest % mine);
+            dst->tok0 = tok0;
+            dst->lq = s.lq;
+            dst->lk = s.lk;
+            dst->q0 = (int)s.q0;
+            dst->k0 = (int)s.k0;
+#pragma unroll 1
+            for (int X = 0; X < 2; ++X) {
+              const int k0 = tok0 + X * tp.tt, k1 = min(s.lq, k0 + tp.tt);  // tokens [k0, k1)
+              int x0 = 0, x1 = 0;
+              if (k0 < k1) {
+                const int hi = key_hi(p, s, k1 - 1), lo = key_lo(p, s, k0);
+                if (hi > lo) {
+                  x0 = lo >> 7;
+                  x1 = (hi + 127) >> 7;
+                }
+              }
+              (X ? dst->b0 : dst->a0) = x0;
+              (X ? dst->b1 : dst->a1) = x1;
+            }
+            dst->free_hi = key_hi(p, s, tok0);
+            dst->free_lo = key_lo(p, s, min(s.lq, tok0 + 2 * tp.tt) - 1);
+          }
+          return true;
         }
         wi += all;
         wb += 32;
       }
+      return false;
     };
     uint32_t nv = 0;                 // V tiles of the items before
     uint32_t raw[kTfVStages] = {};   // masked tiles mended per stage
@@ -384,29 +424,31 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     auto hand_out = [&]() {
       int i = 0;
       if (lane == 0) i = atomicAdd(tp.next, 1);
-      return (int64_t)__shfl_sync(0xffffffffu, i, 0);
+      return __shfl_sync(0xffffffffu, i, 0);
     };
     bool ok = true;
-    auto announce = [&](int n, TfItem& c) {
+    // finds the item that comes n-th on this CTA and announces it, once its slot is free
+    auto announce = [&](int n) -> bool {
+      const int at = hand_out();
       if (n >= kTfItems && ok &&
           !mbar_wait(bar(kBTfItemEmpty + n % kTfItems), ((n / kTfItems) & 1) ^ 1u, p.err, kDevTimeoutOther, abort_flag))
         ok = false;
-      if (!ok) c.valid = 0;
-      if (lane == 0) {
-        items[n % kTfItems] = c;
-        mbar_arrive(bar(kBTfItemFull + n % kTfItems));
-      }
+      const bool more = ok && find(at, items + n % kTfItems);
+      if (!more && lane == 0) items[n % kTfItems].valid = 0;
       __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kBTfItemFull + n % kTfItems));
+      __syncwarp();
+      return more;
     };
-    TfItem cur, next;
-    find(hand_out(), next);
-    announce(0, next);
-    for (int n = 0; next.valid; ++n) {
-      cur = next;
-      // the next item is announced while this one is at work (as soon as the last one's slot is
-      // free), so that its loads and first products follow on without a gap
-      find(hand_out(), next);
-      announce(n + 1, next);
+    // Item n is announced while item n - 1 is at work (as soon as the slot of the one before is
+    // free), so that its loads and first products follow on without a gap; then the masked V
+    // tiles of item n - 1 are mended as they land.
+    bool more = true;
+    for (int next = 0; more; ++next) {
+      more = announce(next);
+      const int n = next - 1;
+      if (n < 0) continue;
+      const TfItem& cur = items[n % kTfItems];
       uint32_t* list =
           tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
       const int t0 = cur.first(), t1 = cur.last();
@@ -428,7 +470,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
           const bool past = t * 128 + r >= cur.lk;
           __nv_bfloat162 probe = __floats2bfloat162_rn(0.f, 0.f);
           const __nv_bfloat162 zero = probe;
-#pragma unroll
+#pragma unroll 4
           for (int c = 0; c < HD / 8; ++c) {
             const uint4 w = lds128(row + (c >> 3) * kTfChunk + (((c & 7) ^ (r & 7)) << 4));
             const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
@@ -437,32 +479,13 @@ __global__ void __launch_bounds__(kTfThreads, 1)
           }
           const bool odd = !past && (__hisnan(probe.x) || __hisnan(probe.y));
           if (past) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < HD / 8; ++c) sts128(row + (c >> 3) * kTfChunk + (c << 4 & 127), make_uint4(0, 0, 0, 0));
           }
           const uint32_t who = __ballot_sync(0xffffffffu, odd);
           if (odd) {
-            uint32_t mask[4] = {0, 0, 0, 0};
-#pragma unroll 1
-            for (int c = 0; c < HD / 8; ++c) {
-              const uint32_t at = row + (c >> 3) * kTfChunk + (((c & 7) ^ (r & 7)) << 4);
-#pragma unroll 1
-              for (int e = 0; e < 8; ++e)
-                if ((lds_u16(at + 2 * e) & 0x7f80u) == 0x7f80u) {
-                  const int d = c * 8 + e;
-                  mask[0] |= d < 32 ? 1u << (d & 31) : 0u;
-                  mask[1] |= (d >> 5) == 1 ? 1u << (d & 31) : 0u;
-                  mask[2] |= (d >> 5) == 2 ? 1u << (d & 31) : 0u;
-                  mask[3] |= (d >> 5) == 3 ? 1u << (d & 31) : 0u;
-                  asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + 2 * e), "h"((uint16_t)0) : "memory");
-                }
-            }
             const int slot = bad + __popc(who & ((1u << lane) - 1u));
-            if (slot < kTfBadRows) {
-              list[slot * kTfBadWords] = (uint32_t)(t * 128 + r);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) list[slot * kTfBadWords + 1 + e] = mask[e];
-            }
+            remember_row<HD>(row, r, t * 128 + r, slot < kTfBadRows ? list + slot * kTfBadWords : nullptr);
           }
           bad += __popc(who);
           __syncwarp();
@@ -489,8 +512,9 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + lane_addr + (uint32_t)(X * 128);
     const uint32_t tO = tmem + lane_addr + 256 + (uint32_t)(X * 128);
-    uint32_t base_a = 0, base_b = 0;  // tiles of slot A / B in the items before
-    uint32_t n_o = 0;           // items of this slot that had tiles
+    uint32_t mine = 0;   // tiles of this slot so far
+    uint32_t both = 0;   // key tiles of all items before this one
+    uint32_t n_o = 0;    // items in which this slot had tiles
 
     // The item's Q by TMA: G heads of TT tokens are the slot's rows in order (rows of other
     // sequences or past the end may come along: their results are not written).
@@ -504,21 +528,43 @@ __global__ void __launch_bounds__(kTfThreads, 1)
     };
 
     const int my_tok = r / p.group, my_g = r % p.group;  // (rows past TT * G are not live)
-    TfItem it, nx;
+    // The exponentials of the two slots take turns, A before B in each tile: together they would
+    // share the MUFU pipe while the tensor pipe idles. Every tile of an item counts for both
+    // slots, so that neither is ever more than one turn ahead.
+    auto my_turn = [&](uint32_t g) {
+      if (X == 0)
+        return g == 0 || mbar_wait(bar(kBTfTurn + 1), (g - 1) & 1, p.err, kDevTimeoutSoftmax, abort_flag);
+      return mbar_wait(bar(kBTfTurn), g & 1, p.err, kDevTimeoutSoftmax, abort_flag);
+    };
+    auto pass_turn = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kBTfTurn + X));
+    };
     bool ok = true;
-    bool have = take_item(0, it);
-    if (have) load_q(it);
-    for (int n = 0; have; ++n) {
-      const int a0 = it.lo(X), a1 = it.hi(X);
-      const bool live = r < tp.tt * p.group && it.tok0 + X * tp.tt + my_tok < it.lq;
-      const int tok = live ? it.tok0 + X * tp.tt + my_tok : 0;
-      const int head = it.h * p.group + my_g;
+    const TfItem* at = take_item(0);
+    if (at) load_q(*at);
+    for (int n = 0; at; ++n) {
+      const TfItem& it = *at;
+      const int t0 = it.first(), t1 = it.last();
+      const bool any = it.hi(X) > it.lo(X);
+      const int a0 = any ? it.lo(X) : t1, a1 = any ? it.hi(X) : t1;
+      const int tok = it.tok0 + X * tp.tt + my_tok;
+      const bool live = r < tp.tt * p.group && tok < it.lq;
+      int hi = 0, lo = 0;
+      if (live) {
+        const Seq s{it.q0, it.k0, it.lq, it.lk};
+        hi = key_hi(p, s, tok);
+        lo = key_lo(p, s, tok);
+      }
       bool q_sent = false;
-      const int hi = live ? (p.causal ? max(0, min(it.lk, tok + it.lk - it.lq + 1)) : it.lk) : 0;
-      const int lo = p.window > 0 ? max(0, tok + it.lk - it.lq - p.window + 1) : 0;
       float m = -INFINITY, l = 0.f;
-      for (int t = a0; t < a1; ++t) {
-        if (!mbar_wait(bar(kBTfSFull + X), ((X ? base_b : base_a) + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax, abort_flag)) {
+      for (int t = t0; t < t1; ++t) {
+        if (t < a0 || t >= a1) {  // the other slot's alone
+          if (!(ok = my_turn(both + (uint32_t)(t - t0)))) break;
+          pass_turn();
+          continue;
+        }
+        if (!mbar_wait(bar(kBTfSFull + X), (mine + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax, abort_flag)) {
           ok = false;
           break;
         }
@@ -529,16 +575,28 @@ __global__ void __launch_bounds__(kTfThreads, 1)
           if (c.valid) load_q(c);
           q_sent = true;
         }
+        if (it.masked(t)) {
+          // a short loop over S in TMEM: few tiles are masked, and unrolled over 128 registers this
+          // code left the instruction cache between two of them (2 to 4 us a tile instead of 0.5)
+          const int lim = hi - t * 128, from = lo - t * 128;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float x[32];
+            tmem_ld32(tS + c * 32, x);
+            const int a = min(32, max(0, lim - c * 32)), b = min(32, max(0, from - c * 32));
+            const uint32_t keep = (a == 32 ? ~0u : (1u << a) - 1u) & ~(b == 32 ? ~0u : (1u << b) - 1u);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(keep >> i & 1u)) x[i] = -INFINITY;
+            tmem_st32(tS + c * 32, x);
+          }
+          tmem_wait_st();
+        }
         float v[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(v + c * 32));
         tmem_wait_ld();
-        if (it.masked(t)) {
-          const int lim = hi - t * 128, from = lo - t * 128;
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= lim || i < from) v[i] = -INFINITY;
-        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 128; i += 8) {
@@ -569,15 +627,9 @@ __global__ void __launch_bounds__(kTfThreads, 1)
             tmem_st32(tO + c * 32, o);
           }
         }
-        // The exponentials of the two slots take turns: together they would share the MUFU pipe
-        // while the tensor pipe idles. A tile the other slot does not have is not waited for.
-        // (Only a matter of speed: the wait is bounded and needs no order.)
-        {
-          const int to = X == 0 ? t - 1 : t;  // the other slot's tile that goes before
-          if (to >= it.lo(X ^ 1) && to < it.hi(X ^ 1)) {
-            const int want = 4 * ((int)(X ? base_a : base_b) + to - it.lo(X ^ 1) + 1);
-            for (int i = 0; i < 512 && *reinterpret_cast<volatile int*>(turns + (X ^ 1)) - want < 0; ++i) {}
-          }
+        if (!my_turn(both + (uint32_t)(t - t0))) {
+          ok = false;
+          break;
         }
         const float mu = m == -INFINITY ? 0.f : m * p.sl2;
         const float2 sl2x2 = make_float2(p.sl2, p.sl2), nmu2 = make_float2(-mu, -mu);
@@ -595,10 +647,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
             pk[i] = pack_bf16x2(e.x, e.y);
           }
           tmem_st16(tS + c * 16, pk);
-          if (c == 3) {
-            __syncwarp();
-            if (lane == 0) atomicAdd(turns + X, 1);
-          }
+          if (c == 3) pass_turn();
           tmem_wait_st();  // this quarter of P is in TMEM: its products may start
           tc_fence_before();
           __syncwarp();
@@ -607,58 +656,71 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         const float2 u = __fadd2_rn(__fadd2_rn(rs[0], rs[1]), __fadd2_rn(rs[2], rs[3]));
         l = l * alpha + (u.x + u.y);
       }
-      base_a += (uint32_t)max(0, it.a1 - it.a0);
-      base_b += (uint32_t)max(0, it.b1 - it.b0);
+      mine += (uint32_t)(a1 - a0);
+      both += (uint32_t)(t1 - t0);
       // the next item's Q goes in first: its products then run while this item's rows are written
-      have = ok && take_item(n + 1, nx);
-      if (have && !q_sent) load_q(nx);
-      const bool any = a1 > a0;
+      const TfItem* next = ok ? take_item(n + 1) : nullptr;
+      if (next && !q_sent) load_q(*next);
       if (ok && any) ok = mbar_wait(bar(kBTfOFull + X), n_o & 1, p.err, kDevTimeoutSoftmax, abort_flag);
       n_o += any ? 1 : 0;
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      const int bad = any ? *reinterpret_cast<volatile int*>(&items[n % kTfItems].bad) : 0;
-      __nv_bfloat16* orow = p.out + ((int64_t)it.q0 + tok) * p.out_stride + (int64_t)head * HD;
-      const uint32_t* list =
-          tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
+      const float inv = l == 0.f ? 0.f : __fdividef(1.0f, l);
+      const int bad = any ? *reinterpret_cast<const volatile int*>(&it.bad) : 0;
+      __nv_bfloat16* row = p.out + ((int64_t)it.q0 + tok) * p.out_stride + (int64_t)(it.h * p.group + my_g) * HD;
+      if (!ok || !live || !WX_IN_BOUNDS(p.err, it.q0 + tok < p.total_q)) row = nullptr;
+      // 16-byte units are exchanged between two neighbouring lanes, so that a store covers 32
+      // bytes (a whole sector) of each row: `even` is the row of the lower lane, `odd` the other's
+      const auto other = reinterpret_cast<__nv_bfloat16*>(
+          __shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), 1));
+      __nv_bfloat16 *even = lane & 1 ? other : row, *odd = lane & 1 ? row : other;
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
-        float o[32];
+      for (int c = 0; c < HD / 16; ++c) {
+        float o[16];
         if (any) {
-          tmem_ld32(tO + c * 32, o);
+          tmem_ld16(tO + c * 16, o);
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          for (int i = 0; i < 16; ++i) o[i] = 0.f;
         }
         if (bad) {  // non-finite values of V that this row does see
-          uint32_t hit = 0;
+          const int col = c * 16;
+          uint32_t hit = bad > kTfBadRows ? ~0u : 0u;
+          const uint32_t* list =
+              tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
 #pragma unroll 1
           for (int e = 0; e < min(bad, kTfBadRows); ++e) {
             const int key = (int)__ldcg(list + e * kTfBadWords);
-            if (key >= lo && key < hi) hit |= __ldcg(list + e * kTfBadWords + 1 + c);
+            if (key >= lo && key < hi) hit |= __ldcg(list + e * kTfBadWords + 1 + (col >> 5)) >> (col & 31);
           }
-          if (bad > kTfBadRows) hit = 0xffffffffu;
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
+          for (int i = 0; i < 16; ++i)
             if (hit >> i & 1u) o[i] = __int_as_float(0x7fc00000);
         }
-        if (ok && live && WX_IN_BOUNDS(p.err, it.q0 + tok < p.total_q)) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8)
-            *reinterpret_cast<uint4*>(orow + c * 32 + i) =
-                make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
-                           pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv), pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
-        }
+        uint4 w0 = make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+                              pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
+        uint4 w1 = make_uint4(pack_bf16x2(o[8] * inv, o[9] * inv), pack_bf16x2(o[10] * inv, o[11] * inv),
+                              pack_bf16x2(o[12] * inv, o[13] * inv), pack_bf16x2(o[14] * inv, o[15] * inv));
+        // lower lane: both first units, upper lane: both second units
+        uint4 give = lane & 1 ? w0 : w1;
+        give.x = __shfl_xor_sync(0xffffffffu, give.x, 1);
+        give.y = __shfl_xor_sync(0xffffffffu, give.y, 1);
+        give.z = __shfl_xor_sync(0xffffffffu, give.z, 1);
+        give.w = __shfl_xor_sync(0xffffffffu, give.w, 1);
+        if (lane & 1) w0 = give;
+        else w1 = give;
+        const int at_col = c * 16 + (lane & 1) * 8;
+        if (even) *reinterpret_cast<uint4*>(even + at_col) = w0;
+        if (odd) *reinterpret_cast<uint4*>(odd + at_col) = w1;
       }
-      if (ok && live && p.lse)
-        p.lse[((int64_t)it.q0 + tok) * p.hq + head] =
-            l == 0.f ? -INFINITY : (m * p.sl2 + log2f(l)) * 0.69314718055994531f;
       tc_fence_before();
       __syncwarp();
       if (lane == 0 && any) mbar_arrive(bar(kBTfOEmpty + X));
+      if (ok && live && p.lse)
+        p.lse[((int64_t)it.q0 + tok) * p.hq + it.h * p.group + my_g] =
+            l == 0.f ? -INFINITY : (m * p.sl2 + __log2f(l)) * 0.69314718055994531f;
       drop_item(n);
-      it = nx;
+      at = next;
     }
   }
 
