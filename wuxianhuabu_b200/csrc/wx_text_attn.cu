@@ -671,7 +671,7 @@ static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
 // rows kernel, which is bound by the K/V bytes; more rows go to the tcgen05 kernel.
 static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParams& p, const KvSource& kv) {
   const bool big = d->head_dim == 128;
-  if (kv.format == kKvBf16 && (int64_t)d->max_q * p.group > 16) return text_flash(ctx, p, d->head_dim, kv);
+  if ((int64_t)d->max_q * p.group > 16) return text_flash(ctx, p, d->head_dim, kv);
   if (kv.format == kKvInt8)
     return big ? launch_rows_attn<kKvInt8, 128>(ctx, p, kv) : launch_rows_attn<kKvInt8, 64>(ctx, p, kv);
   if (kv.format == kKvE4m3)

@@ -15,6 +15,8 @@
 //   Warp 0: TMA producer of K and V. Warps 1 / 2: MMA issuer of slot A / B. Warp 3: finds the
 //   items and mends masked V tiles. Warps 4-7 / 8-11: softmax and epilogue of slot A / B (thread
 //   r owns row r); one of their threads fetches the next item's Q as soon as the last S is done.
+//   8-bit cache: warp 0 brings raw rows and scales, warps 12-15 turn them into bf16 tiles (exact:
+//   the key's scale multiplies its scores, the value's scale its weights, both in fp32).
 #include <cuda_runtime.h>
 #include <math.h>
 
@@ -24,21 +26,30 @@
 
 namespace wx {
 
-constexpr int kTfThreads = 384;
-constexpr int kTfRegsLow = 72, kTfRegsHigh = 216;
-static_assert(kTfRegsLow * 128 + kTfRegsHigh * 256 <= 168 * kTfThreads, "register split exceeds the launch");
-constexpr int kTfKStages = 3, kTfVStages = 2;
+constexpr int kTfVStages = 2;
+constexpr int kTfRaw = 3;       // 8-bit: raw half tiles (64 keys) in flight
+constexpr int kTfScales = 4;    // 8-bit: tiles of scales kept
 constexpr int kTfItems = 2;     // item slots: the one at work and the next
 constexpr int kTfChunk = 128 * 128;  // one 64-column SW128 chunk of a 128-row tile
 constexpr int64_t kTfL2 = int64_t(48) << 20;
 constexpr int kTfBadRows = 1024;     // V rows with non-finite values remembered per item
 constexpr int kTfBadWords = 5;       // key, 128-bit column mask
 
-template <int HD>
+template <int FMT, int HD>
 struct TfGeom {
+  static constexpr bool kWide = FMT != kKvBf16;
+  static constexpr int kThreads = kWide ? 512 : 384;
+  static constexpr int kKStages = kWide ? 2 : 3;
+  // registers of the control (and conversion) warps and of the softmax warps after setmaxnreg
+  static constexpr int kRegsLow = kWide ? 56 : 72, kRegsHigh = kWide ? 200 : 216;
+  static constexpr int kRegsUsed = kRegsLow * (kThreads - 256) + kRegsHigh * 256;
+  static_assert(kRegsUsed <= 65536 / kThreads / 8 * 8 * kThreads, "register split exceeds the launch");
   static constexpr int kTile = 128 * HD * 2;
   static constexpr int kChunks = HD / 64;
-  static constexpr int kBarOff = (2 + kTfKStages + kTfVStages) * kTile;
+  static constexpr int kRawBytes = 64 * HD;
+  static constexpr int kRawOff = (2 + kKStages + kTfVStages) * kTile;
+  static constexpr int kScaleOff = kRawOff + (kWide ? kTfRaw * kRawBytes : 0);  // [tile][k, v][key]
+  static constexpr int kBarOff = kScaleOff + (kWide ? kTfScales * 1024 : 0);
   static constexpr int kItemOff = kBarOff + 512;
   static constexpr int kSmem = kItemOff + kTfItems * 128 + 1024;
 };
@@ -60,12 +71,12 @@ struct TfItem {
 
 enum : int {
   kBTfItemFull = 0,                       // [items]
-  kBTfItemEmpty = kBTfItemFull + kTfItems,  // [items] count 11: every other warp is done with it
+  kBTfItemEmpty = kBTfItemFull + kTfItems,  // [items] count 11 (8-bit: 15): every other warp is done with it
   kBTfQFull = kBTfItemEmpty + kTfItems,   // [2]
-  kBTfKFull = kBTfQFull + 2,              // [K stages]
-  kBTfKEmpty = kBTfKFull + kTfKStages,    // count 2: both slots
-  kBTfVRaw = kBTfKEmpty + kTfKStages,     // [V stages] a masked tile has landed
-  kBTfVFull = kBTfVRaw + kTfVStages,      // [V stages] count 2: landed, and mended where masked
+  kBTfKFull = kBTfQFull + 2,              // [3] (8-bit: count 4, the conversion warps)
+  kBTfKEmpty = kBTfKFull + 3,             // [3] count 2: both slots
+  kBTfVRaw = kBTfKEmpty + 3,              // [V stages] a masked tile has landed
+  kBTfVFull = kBTfVRaw + kTfVStages,      // [V stages] count 2: landed, and mended where masked (8-bit: 4)
   kBTfVEmpty = kBTfVFull + kTfVStages,    // count 2
   kBTfSFull = kBTfVEmpty + kTfVStages,    // [2]
   kBTfPFull = kBTfSFull + 2,              // [2][4] count 4
@@ -73,7 +84,10 @@ enum : int {
   kBTfOEmpty = kBTfOFull + 2,             // [2] count 4: the epilogue has read O
   kBTfTurn = kBTfOEmpty + 2,              // [2] count 4: a slot's exponentials of a tile are issued
   kBTfDrain = kBTfTurn + 2,               // [2]
-  kBTfCount = kBTfDrain + 2
+  kBTfRawFull = kBTfDrain + 2,            // [raw] 8-bit rows have landed
+  kBTfRawEmpty = kBTfRawFull + kTfRaw,    // [raw] count 4
+  kBTfScale = kBTfRawEmpty + kTfRaw,      // [scales] a tile's scales have landed
+  kBTfCount = kBTfScale + kTfScales
 };
 static_assert(kBTfCount * 8 + 32 <= 512, "barriers overlap the items");
 
@@ -123,27 +137,40 @@ __device__ __noinline__ void remember_row(uint32_t row, int r, int key, uint32_t
   for (int e = 0; e < 4; ++e) entry[1 + e] = mask[e];
 }
 
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+
 struct TfParams {
   TextAttnParams a;
   int tt;              // tokens of a slot: floor(128 / G)
   int box;             // rows of a K/V box: 128, or a page where pages are smaller
   int* next;           // [2] items handed out, CTAs that have finished (0, 0 between launches)
   uint32_t* bad_rows;  // [CTA][kTfItems][kTfBadRows][kTfBadWords]
+  const uint8_t *k8, *v8;  // rows of an 8-bit cache
 };
 
-template <int HD>
-__global__ void __launch_bounds__(kTfThreads, 1)
+template <int FMT, int HD>
+__global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     text_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, TfParams tp) {
-  using G = TfGeom<HD>;
-  constexpr int kTile = G::kTile;
+  using G = TfGeom<FMT, HD>;
+  constexpr bool kW = G::kWide;
+  constexpr int kTile = G::kTile, kKStages = G::kKStages;
   const TextAttnParams& p = tp.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   auto sQ = [&](int X) { return sbase + (uint32_t)X * kTile; };
   auto sK = [&](int s) { return sbase + (uint32_t)(2 + s) * kTile; };
-  auto sV = [&](int s) { return sbase + (uint32_t)(2 + kTfKStages + s) * kTile; };
+  auto sV = [&](int s) { return sbase + (uint32_t)(2 + kKStages + s) * kTile; };
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kBarOff);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBTfCount);
@@ -155,11 +182,13 @@ __global__ void __launch_bounds__(kTfThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBTfCount; ++i) {
       uint32_t c = 1;
-      if (i >= kBTfItemEmpty && i < kBTfItemEmpty + kTfItems) c = 11;
-      if ((i >= kBTfKEmpty && i < kBTfKEmpty + kTfKStages) || (i >= kBTfVFull && i < kBTfVEmpty + kTfVStages)) c = 2;
-      if ((i >= kBTfPFull && i < kBTfPFull + 8) ||
-          (i >= kBTfOEmpty && i < kBTfTurn + 2))
-        c = 4;
+      if (i >= kBTfItemEmpty && i < kBTfItemEmpty + kTfItems) c = kW ? 15 : 11;
+      if (i >= kBTfKFull && i < kBTfKEmpty && kW) c = 4;
+      if (i >= kBTfKEmpty && i < kBTfVRaw) c = 2;
+      if (i >= kBTfVFull && i < kBTfVEmpty) c = kW ? 4 : 2;
+      if (i >= kBTfVEmpty && i < kBTfSFull) c = 2;
+      if ((i >= kBTfPFull && i < kBTfOFull) || (i >= kBTfOEmpty && i < kBTfDrain)) c = 4;
+      if (i >= kBTfRawEmpty && i < kBTfScale) c = 4;
       mbar_init(bar(i), c);
     }
     *abort_flag = 0;
@@ -187,7 +216,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
   };
 
   if (warp == 0) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTfRegsLow));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLow));
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       prefetch_tmap(&tmQ);
@@ -203,9 +232,60 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       const TfItem& it = *at;
       const int t0 = it.first(), t1 = it.last();
       int ids = 0, ids_from = -1;  // block entries of 32 consecutive boxes, one per lane
+      // block entry of box b of the sequence (b0: the tile's first box)
+      auto page_of = [&](int b0, int bx) -> int {
+        if (ids_from < 0 || b0 < ids_from || b0 + boxes > ids_from + 32) {
+          ids_from = b0;
+          const int64_t j = (int64_t)(b0 + lane) * tp.box;
+          ids = 0;
+          if (j < it.lk) {
+            ids = p.block_table[it.b * p.blocks_per_seq + (j >> p.page_shift)];
+            if (ids < 0 || ids >= p.pages) {
+              set_dev_error(p.err, kDevBadArgs);
+              ids = 0;
+            }
+          }
+        }
+        return __shfl_sync(0xffffffffu, ids, (b0 - ids_from + bx) & 31);
+      };
+      auto cache_row = [&](int page, int j) -> int64_t {
+        return (((int64_t)page * p.hkv + it.h) << p.page_shift) | (j & ((1 << p.page_shift) - 1));
+      };
+      // 8-bit: a tile in two halves of 64 raw rows, its scales with the keys; rows past the
+      // sequence's last key are not loaded (what stands there is finite, and masked)
+      auto load_raw = [&](bool is_k, int t) -> bool {
+        const int per_half = 64 / tp.box;
+        const int page = page_of(t * boxes, lane % boxes);
+        const int nb = min(boxes, (it.lk - t * 128 + tp.box - 1) / tp.box);
+        const int64_t row = cache_row(page, t * 128 + (lane % boxes) * tp.box);
+        if (is_k) {
+          const uint32_t sc = nk % kTfScales, full = bar(kBTfScale + sc);
+          const uint32_t dst = sbase + G::kScaleOff + sc * 1024 + (uint32_t)lane * tp.box * 4;
+          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(nb * tp.box * 8));
+          __syncwarp();
+          if (lane < nb) {
+            bulk_load(dst, p.ks + row, (uint32_t)tp.box * 4, full);
+            bulk_load(dst + 512, p.vs + row, (uint32_t)tp.box * 4, full);
+          }
+          ++nk;
+        }
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, ++nv) {  // (nv counts raw halves here)
+          const uint32_t s = nv % kTfRaw;
+          if (!mbar_wait(bar(kBTfRawEmpty + s), ((nv / kTfRaw) & 1) ^ 1u, p.err, kDevTimeoutEmpty, abort_flag)) return false;
+          const int n = max(0, min(per_half, nb - half * per_half)), bx = lane - half * per_half;
+          if (lane == 0) mbar_arrive_expect_tx(bar(kBTfRawFull + s), (uint32_t)(n * tp.box * HD));
+          __syncwarp();
+          if (bx >= 0 && bx < n)
+            bulk_load(sbase + G::kRawOff + s * G::kRawBytes + (uint32_t)(bx * tp.box * HD),
+                      (is_k ? tp.k8 : tp.v8) + row * HD, (uint32_t)(tp.box * HD), bar(kBTfRawFull + s));
+        }
+        return true;
+      };
       auto load = [&](bool is_k, int t) -> bool {
+        if constexpr (kW) return load_raw(is_k, t);
         const uint32_t cnt = is_k ? nk : nv;
-        const int ns = is_k ? kTfKStages : kTfVStages;
+        const int ns = is_k ? kKStages : kTfVStages;
         const uint32_t s = cnt % ns, par = ((cnt / ns) & 1) ^ 1u;
         if (!mbar_wait(bar((is_k ? kBTfKEmpty : kBTfVEmpty) + s), par, p.err, kDevTimeoutEmpty, abort_flag)) return false;
         const bool mend = !is_k && it.masked(t);
@@ -222,24 +302,10 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         if (!p.block_table) {
           if (lane < G::kChunks) tma_load_2d(dst + lane * kTfChunk, tm, full, it.h * HD + lane * 64, it.k0 + t * 128);
         } else {
-          const int b0 = t * boxes;
-          if (ids_from < 0 || b0 < ids_from || b0 + boxes > ids_from + 32) {
-            ids_from = b0;
-            const int64_t j = (int64_t)(b0 + lane) * tp.box;
-            ids = 0;
-            if (j < it.lk) {
-              ids = p.block_table[it.b * p.blocks_per_seq + (j >> p.page_shift)];
-              if (ids < 0 || ids >= p.pages) {
-                set_dev_error(p.err, kDevBadArgs);
-                ids = 0;
-              }
-            }
-          }
           const int bx = lane / G::kChunks, ch = lane % G::kChunks;
-          const int page = __shfl_sync(0xffffffffu, ids, (b0 - ids_from + bx) & 31);
+          const int page = page_of(t * boxes, bx);
           if (bx < nb) {
-            const int j = t * 128 + bx * tp.box;
-            const int row = (int)((((int64_t)page * p.hkv + it.h) << p.page_shift) | (j & ((1 << p.page_shift) - 1)));
+            const int row = (int)cache_row(page, t * 128 + bx * tp.box);
             tma_load_2d(dst + ch * kTfChunk + bx * tp.box * 128, tm, full, ch * 64, row);
           }
         }
@@ -265,7 +331,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       }
     }
   } else if (warp == 1 || warp == 2) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTfRegsLow));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLow));
     // ------------------------------------------------------------ MMA issuer of slot X
     const int X = warp - 1;
     constexpr uint32_t idesc_s = idesc_bf16_f32(128, 128, false, false);
@@ -292,11 +358,11 @@ __global__ void __launch_bounds__(kTfThreads, 1)
         for (int t = t0 - 1; t < t1 && ok; ++t) {
           // V(t) and K(t+1) are waited for before P(t): PV(t) and S(t+1) then go out back to back
           const uint32_t cv = kv + (uint32_t)(t - t0), ck = cv + 1;
-          const uint32_t sv = cv % kTfVStages, sk = ck % kTfKStages;
+          const uint32_t sv = cv % kTfVStages, sk = ck % kKStages;
           if (t >= t0)
             ok = mbar_wait(bar(kBTfVFull + sv), (cv / kTfVStages) & 1, p.err, kDevTimeoutFull, abort_flag);
           if (ok && t + 1 < t1)
-            ok = mbar_wait(bar(kBTfKFull + sk), (ck / kTfKStages) & 1, p.err, kDevTimeoutFull, abort_flag);
+            ok = mbar_wait(bar(kBTfKFull + sk), (ck / kKStages) & 1, p.err, kDevTimeoutFull, abort_flag);
           // the first product of an item overwrites O: the last epilogue must have read it
           if (ok && t == a0 && n_o > 0)
             ok = mbar_wait(bar(kBTfOEmpty + X), (n_o - 1) & 1, p.err, kDevTimeoutSoftmax, abort_flag);
@@ -350,7 +416,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       mbar_drain(bar(kBTfDrain + X), 0);
     }
   } else if (warp == 3) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kTfRegsLow));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLow));
     // ------------------------------------------------------------ items, and masked V tiles
     // Items in the order (sequence, chunk of K/V heads, rows from the last, head): the long causal
     // rows go first, so that the short ones level the CTAs out at the end, and a chunk holds as
@@ -454,7 +520,7 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       const int t0 = cur.first(), t1 = cur.last();
       int bad = 0;
       for (int t = t0; t < t1 && ok; ++t) {
-        if (!cur.masked(t)) continue;
+        if (kW || !cur.masked(t)) continue;
         const uint32_t s = (nv + (uint32_t)(t - t0)) % kTfVStages;
         uint32_t& done = s == 0 ? raw[0] : raw[1];
         if (!mbar_wait(bar(kBTfVRaw + s), done & 1, p.err, kDevTimeoutFull, abort_flag)) {
@@ -503,8 +569,60 @@ __global__ void __launch_bounds__(kTfThreads, 1)
       tp.next[1] = 0;
       __threadfence();
     }
+  } else if (kW && warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLow));
+    // ------------------------------------------------ 8-bit rows -> bf16 tiles (128 threads)
+    const int tid = (int)threadIdx.x - 384;
+    uint32_t nk = 0, nv = 0, nr = 0;  // K tiles, V tiles, raw halves so far
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const TfItem* at = take_item(n);
+      if (!at) break;
+      const int t0 = at->first(), tiles = at->last() - t0;
+#pragma unroll 1
+      for (int i = 0; i < 2 * tiles && ok; ++i) {  // in the producer's order
+        const bool tail = i >= 2 * tiles - 1;
+        const bool is_k = i < 2 ? (i == 0 || tiles > 1) : !tail && (i & 1);
+        const uint32_t cnt = is_k ? nk : nv;
+        const uint32_t s = cnt % 2;
+        static_assert(kTfVStages == 2, "two K and two V stages");
+        if (!mbar_wait(bar((is_k ? kBTfKEmpty : kBTfVEmpty) + s), ((cnt / 2) & 1) ^ 1u, p.err, kDevTimeoutEmpty, abort_flag)) {
+          ok = false;
+          break;
+        }
+        const uint32_t dst = is_k ? sK(s) : sV(s);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, ++nr) {
+          const uint32_t rs = nr % kTfRaw;
+          if (ok && !mbar_wait(bar(kBTfRawFull + rs), (nr / kTfRaw) & 1, p.err, kDevTimeoutFull, abort_flag)) ok = false;
+          if (!ok) break;
+          const uint32_t raw = sbase + G::kRawOff + rs * G::kRawBytes;
+#pragma unroll
+          for (int j = 0; j < 64 * HD / 16 / 128; ++j) {
+            const int u = j * 128 + tid, row = half * 64 + u / (HD / 16), c = u % (HD / 16);
+            const uint4 w = lds128(raw + (uint32_t)u * 16);
+            const uint4 x0 = make_uint4(bytes_to_bf16x2<FMT>(w.x, 0, 0, 1), bytes_to_bf16x2<FMT>(w.x, 0, 2, 3),
+                                        bytes_to_bf16x2<FMT>(w.y, 0, 0, 1), bytes_to_bf16x2<FMT>(w.y, 0, 2, 3));
+            const uint4 x1 = make_uint4(bytes_to_bf16x2<FMT>(w.z, 0, 0, 1), bytes_to_bf16x2<FMT>(w.z, 0, 2, 3),
+                                        bytes_to_bf16x2<FMT>(w.w, 0, 0, 1), bytes_to_bf16x2<FMT>(w.w, 0, 2, 3));
+            const uint32_t at_row = dst + (uint32_t)((c >> 2) * kTfChunk + row * 128);
+            // (the upper half of a 128-byte row stores its second unit first: no bank conflicts)
+            const int first = (c >> 2) & 1;
+            sts128(at_row + (((((c & 3) << 1) + first) ^ (row & 7)) << 4), first ? x1 : x0);
+            sts128(at_row + (((((c & 3) << 1) + (first ^ 1)) ^ (row & 7)) << 4), first ? x0 : x1);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kBTfRawEmpty + rs));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && ok) mbar_arrive(bar((is_k ? kBTfKFull : kBTfVFull) + s));
+        if (is_k) ++nk; else ++nv;
+      }
+      drop_item(n);
+    }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kTfRegsHigh));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kRegsHigh));
     // ------------------------------------------------ softmax + epilogue of slot X
     const int X = (warp - 4) >> 2;
     const int quarter = warp & 3;
@@ -575,16 +693,21 @@ __global__ void __launch_bounds__(kTfThreads, 1)
           if (c.valid) load_q(c);
           q_sent = true;
         }
-        if (it.masked(t)) {
+        const bool masked = it.masked(t);
+        const int lim = hi - t * 128, from = lo - t * 128;
+        // bits of the keys 32 c .. 32 c + 31 that this row sees
+        auto keep_bits = [&](int c) -> uint32_t {
+          const int a = min(32, max(0, lim - c * 32)), b = min(32, max(0, from - c * 32));
+          return (a == 32 ? ~0u : (1u << a) - 1u) & ~(b == 32 ? ~0u : (1u << b) - 1u);
+        };
+        if (!kW && masked) {
           // a short loop over S in TMEM: few tiles are masked, and unrolled over 128 registers this
           // code left the instruction cache between two of them (2 to 4 us a tile instead of 0.5)
-          const int lim = hi - t * 128, from = lo - t * 128;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float x[32];
             tmem_ld32(tS + c * 32, x);
-            const int a = min(32, max(0, lim - c * 32)), b = min(32, max(0, from - c * 32));
-            const uint32_t keep = (a == 32 ? ~0u : (1u << a) - 1u) & ~(b == 32 ? ~0u : (1u << b) - 1u);
+            const uint32_t keep = keep_bits(c);
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -597,6 +720,32 @@ __global__ void __launch_bounds__(kTfThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(v + c * 32));
         tmem_wait_ld();
+        uint32_t scales = 0;
+        if constexpr (kW) {
+          const uint32_t g = both + (uint32_t)(t - t0);
+          scales = sbase + G::kScaleOff + (g % kTfScales) * 1024;
+          if (!mbar_wait(bar(kBTfScale + g % kTfScales), (g / kTfScales) & 1, p.err, kDevTimeoutFull, abort_flag)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int i = 0; i < 128; i += 4) {
+            const float4 f = lds_f4(scales + i * 4);
+            v[i] *= f.x;
+            v[i + 1] *= f.y;
+            v[i + 2] *= f.z;
+            v[i + 3] *= f.w;
+          }
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t keep = keep_bits(c);
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(keep >> i & 1u)) v[c * 32 + i] = -INFINITY;
+            }
+          }
+        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 128; i += 8) {
@@ -644,7 +793,18 @@ __global__ void __launch_bounds__(kTfThreads, 1)
             const float2 a = __ffma2_rn(make_float2(v[32 * c + 2 * i], v[32 * c + 2 * i + 1]), sl2x2, nmu2);
             const float2 e = make_float2(exp2_approx(a.x), exp2_approx(a.y));
             rs[i & 3] = __fadd2_rn(rs[i & 3], e);
-            pk[i] = pack_bf16x2(e.x, e.y);
+            if constexpr (kW) {
+              const float2 f = lds_f2(scales + 512 + (32 * c + 2 * i) * 4);
+              pk[i] = pack_bf16x2(e.x * f.x, e.y * f.y);
+            } else {
+              pk[i] = pack_bf16x2(e.x, e.y);
+            }
+          }
+          if (kW && masked) {  // an unseen key's scale may be anything: its weight is 0, not 0 * scale
+            const uint32_t keep = keep_bits(c);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              pk[i] &= (keep >> (2 * i) & 1u ? 0xffffu : 0u) | (keep >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
           }
           tmem_st16(tS + c * 16, pk);
           if (c == 3) pass_turn();
@@ -732,16 +892,17 @@ __global__ void __launch_bounds__(kTfThreads, 1)
   }
 }
 
-template <int HD>
+template <int FMT, int HD>
 static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, TfParams& tp) {
-  auto fn = text_flash_kernel<HD>;
-  int st = ensure_smem_attr(ctx, (const void*)fn, TfGeom<HD>::kSmem, "text_flash");
+  using G = TfGeom<FMT, HD>;
+  auto fn = text_flash_kernel<FMT, HD>;
+  int st = ensure_smem_attr(ctx, (const void*)fn, G::kSmem, "text_flash");
   if (st) return st;
   // setmaxnreg moves registers within what the launch reserved
   static const bool regs_ok = [] {
     cudaFuncAttributes fa{};
-    return cudaFuncGetAttributes(&fa, (const void*)text_flash_kernel<HD>) == cudaSuccess &&
-           fa.numRegs * kTfThreads >= kTfRegsLow * 128 + kTfRegsHigh * 256;
+    return cudaFuncGetAttributes(&fa, (const void*)text_flash_kernel<FMT, HD>) == cudaSuccess &&
+           fa.numRegs * G::kThreads >= G::kRegsUsed;
   }();
   if (!regs_ok) return set_error(ctx, WX_ERR_CUDA, "text_flash: register split does not fit");
   const TextAttnParams& p = tp.a;
@@ -752,7 +913,7 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   tp.bad_rows = static_cast<uint32_t*>(ws);
   if (!(tp.next = arrival_counters(ctx, 2, &st))) return st;
   ProfScope prof(ctx, kProfAttn);
-  fn<<<grid, kTfThreads, TfGeom<HD>::kSmem, ctx->stream>>>(tq, tk, tv, tp);
+  fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(tq, tk, tv, tp);
   return launch_status(ctx, "text_flash");
 }
 
@@ -767,9 +928,18 @@ int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSourc
   const uint64_t ld[2] = {(uint64_t)head_dim, (uint64_t)p.q_stride};
   const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tp.tt};
   if ((st = make_tmap_bf16_3d(ctx, &tq, p.q, dims, ld, box))) return st;
+  const bool big = head_dim == 128;
+  if (kv.format != kKvBf16) {  // raw rows by untiled copies: the maps of K and V are not used
+    tp.box = std::min(64, 1 << p.page_shift);
+    tp.k8 = static_cast<const uint8_t*>(kv.k);
+    tp.v8 = static_cast<const uint8_t*>(kv.v);
+    if (kv.format == kKvInt8)
+      return big ? launch_flash<kKvInt8, 128>(ctx, tq, tq, tq, tp) : launch_flash<kKvInt8, 64>(ctx, tq, tq, tq, tp);
+    return big ? launch_flash<kKvE4m3, 128>(ctx, tq, tq, tq, tp) : launch_flash<kKvE4m3, 64>(ctx, tq, tq, tq, tp);
+  }
   if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, tp.box))) return st;
   if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, tp.box))) return st;
-  return head_dim == 128 ? launch_flash<128>(ctx, tq, tk, tv, tp) : launch_flash<64>(ctx, tq, tk, tv, tp);
+  return big ? launch_flash<kKvBf16, 128>(ctx, tq, tk, tv, tp) : launch_flash<kKvBf16, 64>(ctx, tq, tk, tv, tp);
 }
 
 }  // namespace wx
