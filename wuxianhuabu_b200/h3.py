@@ -47,6 +47,12 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
+# the current stream's handle without the Stream object around it (a few calls of the text side
+# take about as long on the device as that object takes to make)
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
 class Context:
     """One libwx context per CUDA device; calls are ordered on torch's current stream."""
 
@@ -62,16 +68,19 @@ class Context:
             raise WxError(st, f"wx_ctx_create(device={device}) failed")
         self.h = h
         self._stream: Optional[torch.cuda.Stream] = None
+        self._raw_stream: Optional[int] = None  # the context's stream, as set last
 
     def sync_stream(self) -> None:
+        raw = _current_raw_stream(self.device)
+        if raw == self._raw_stream:
+            return
         s = torch.cuda.current_stream(self.device)
-        if s != self._stream:
-            # the context's workspace is shared: a call on another stream waits for the calls
-            # queued on the last one (a capture orders its own work and must not reach outside)
-            if self._stream is not None and not torch.cuda.is_current_stream_capturing():
-                s.wait_stream(self._stream)
-            self._stream = s
+        # the context's workspace is shared: a call on another stream waits for the calls queued on
+        # the last one (a capture orders its own work and must not reach outside)
+        if self._stream is not None and not torch.cuda.is_current_stream_capturing():
+            s.wait_stream(self._stream)
         check(self.lib.wx_ctx_set_stream(self.h, C.c_void_p(s.cuda_stream)), self.h)
+        self._stream, self._raw_stream = s, raw
 
     def check_device(self) -> None:
         check(self.lib.wx_ctx_check_device(self.h), self.h)
@@ -83,7 +92,9 @@ class Context:
 
     def call(self, name: str, *args) -> None:
         self.sync_stream()
-        check(getattr(self.lib, name)(self.h, *args), self.h)
+        st = getattr(self.lib, name)(self.h, *args)
+        if st:
+            check(st, self.h)
 
     TRACE_PHASES = ("norm1", "qkv", "rope", "attn", "out", "mlp")
     TRACE_MODES = ("dense", "sparse", "reuse")

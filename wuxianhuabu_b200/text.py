@@ -17,7 +17,6 @@ block entries) are caught by the kernels and raise at the next ``Context.check_d
 from __future__ import annotations
 
 import ctypes as C
-import math
 from dataclasses import dataclass
 from typing import Optional
 
@@ -39,31 +38,43 @@ def _invalid(msg: str) -> WxError:
     return WxError(_lib.WX_ERR_INVALID, msg)
 
 
-def _need_ints(dtype: torch.dtype, n: Optional[int], what: str, t: torch.Tensor) -> torch.Tensor:
+def _need_ints(dtype: torch.dtype, n: Optional[int], what: str, t: torch.Tensor) -> int:
+    """The device pointer of a contiguous integer tensor of n entries."""
     if not t.is_cuda or t.dtype != dtype or not t.is_contiguous():
         raise _invalid(f"{what} must be a contiguous CUDA {dtype} tensor, got {t.dtype} on {t.device}")
     if n is not None and t.numel() != n:
         raise _invalid(f"{what} must have {n} entries, got {t.numel()}")
-    return t
+    return t.data_ptr()
 
 
 def _rows(t: torch.Tensor, what: str) -> tuple[int, int, int, int]:
     """tokens, heads, head_dim and the token stride of a [tokens, heads, head_dim] tensor."""
-    _need_bf16_cuda(t)
+    if t.dtype != torch.bfloat16 or not t.is_cuda:
+        _need_bf16_cuda(t)
     if t.dim() != 3:
         raise _invalid(f"{what} must be [tokens, heads, head_dim]")
     n, h, d = t.shape
-    if n and (t.stride(2) != 1 or (h > 1 and t.stride(1) != d)):
+    s0, s1, s2 = t.stride()
+    if n and (s2 != 1 or (h > 1 and s1 != d)):
         raise _invalid(f"{what} must have contiguous heads")
-    return n, h, d, t.stride(0) if n > 1 else max(t.stride(0), h * d)
+    return n, h, d, s0 if n > 1 else max(s0, h * d)
 
 
 def _same_device(*ts: torch.Tensor) -> int:
-    dev = ts[0].device
-    for t in ts[1:]:
-        if t.device != dev:
-            raise _invalid(f"tensors on {dev} and {t.device}")
-    return dev.index
+    dev = ts[0].get_device()
+    for t in ts:
+        if t.get_device() != dev:
+            raise _invalid(f"tensors on {ts[0].device} and {t.device}")
+    return dev
+
+
+def _out_rows(like: torch.Tensor, n: int, h: int, d: int, out: Optional[torch.Tensor], msg: str):
+    """The output tensor (a new one without ``out``) and its token stride."""
+    if out is None:
+        return like.new_empty((n, h, d)), h * d
+    if out.shape != like.shape:
+        raise _invalid(msg)
+    return out, _rows(out, "out")[3]
 
 
 @dataclass
@@ -99,6 +110,7 @@ class RopeTable:
         self.interleaved = interleaved
         self.cos = torch.empty((positions, rot // 2), dtype=torch.float32, device=dev)
         self.sin = torch.empty_like(self.cos)
+        self._desc = self._describe()
         ctx.call("wx_rope_table", inv.ctypes.data, rot // 2, positions, float(s.magnitude), _p(self.cos), _p(self.sin))
 
     @classmethod
@@ -112,23 +124,20 @@ class RopeTable:
         _same_device(cos, sin)
         self = cls.__new__(cls)
         self.cos, self.sin, self.interleaved, self.inv_freq = cos, sin, interleaved, None
+        self._desc = self._describe()
         return self
 
-    def _desc(self) -> Rope:
+    def _describe(self):
         n, half = self.cos.shape
-        return Rope(_p(self.cos), _p(self.sin), n, 2 * half, int(self.interleaved))
+        return C.byref(Rope(_p(self.cos), _p(self.sin), n, 2 * half, int(self.interleaved)))
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [tokens, heads, head_dim] with token t turned by positions[t] (int32); ``out`` may be x."""
         n, h, d, stride = _rows(x, "x")
-        _need_ints(torch.int32, n, "positions", positions)
-        o = torch.empty((n, h, d), dtype=torch.bfloat16, device=x.device) if out is None else out
-        if o.shape != x.shape:
-            raise _invalid("out must have x's shape")
-        dev = _same_device(x, positions, o, self.cos)
-        r = self._desc()
-        context(dev).call("wx_rope_apply", C.byref(r), _p(positions), _p(x), stride, n, h, d, _p(o),
-                          _rows(o, "out")[3])
+        at = _need_ints(torch.int32, n, "positions", positions)
+        o, ostride = _out_rows(x, n, h, d, out, "out must have x's shape")
+        context(_same_device(x, positions, o, self.cos)).call(
+            "wx_rope_apply", self._desc, at, x.data_ptr(), stride, n, h, d, o.data_ptr(), ostride)
         return o
 
 
@@ -152,6 +161,7 @@ class PagedKVCache:
         if fmt != "bf16":
             self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=dev)
             self.v_scale = torch.zeros_like(self.k_scale)
+        self._describe()
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
@@ -171,80 +181,68 @@ class PagedKVCache:
         self = cls.__new__(cls)
         self.fmt, self.k, self.v = fmt, k, v
         self.k_scale, self.v_scale = (k_scale, v_scale) if fmt != "bf16" else (None, None)
+        self._describe()
         return self
 
-    @property
-    def pages(self) -> int:
-        return self.k.shape[0]
-
-    @property
-    def kv_heads(self) -> int:
-        return self.k.shape[1]
-
-    @property
-    def page_size(self) -> int:
-        return self.k.shape[2]
-
-    @property
-    def head_dim(self) -> int:
-        return self.k.shape[3]
-
-    def _desc(self) -> KvCache:
-        pages, heads, page, d = self.k.shape
-        return KvCache(_p(self.k), _p(self.v), _p(self.k_scale), _p(self.v_scale), pages, page, heads, d,
-                       _FORMATS[self.fmt][0])
+    def _describe(self) -> None:
+        self.pages, self.kv_heads, self.page_size, self.head_dim = self.k.shape
+        self._desc = C.byref(KvCache(_p(self.k), _p(self.v), _p(self.k_scale), _p(self.v_scale), self.pages,
+                                     self.page_size, self.kv_heads, self.head_dim, _FORMATS[self.fmt][0]))
 
     def _kv(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
         n, h, d, ks = _rows(k, "k")
         nv, hv, dv, vs = _rows(v, "v")
         if (n, h, d) != (nv, hv, dv) or (h, d) != (self.kv_heads, self.head_dim):
             raise _invalid("k and v must be [tokens, kv_heads, head_dim] of the cache")
-        _need_ints(torch.int64, n, "slots", slots)
-        return n, ks, vs
+        return n, ks, vs, _need_ints(torch.int64, n, "slots", slots)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Write k and v of each token to its slot (< 0: skipped), quantised to the format."""
-        n, ks, vs = self._kv(k, v, slots)
-        dev = _same_device(self.k, k, v, slots)
-        d = self._desc()
-        context(dev).call("wx_kv_append", C.byref(d), _p(k), ks, _p(v), vs, n, _p(slots))
+        n, ks, vs, at = self._kv(k, v, slots)
+        context(_same_device(self.k, k, v, slots)).call("wx_kv_append", self._desc, k.data_ptr(), ks, v.data_ptr(), vs,
+                                                        n, at)
 
     def append_roped(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rope: RopeTable,
                      positions: torch.Tensor, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """``rope.apply`` of q (returned) and k, and ``append`` of k and v, in one launch."""
-        n, ks, vs = self._kv(k, v, slots)
+        n, ks, vs, at = self._kv(k, v, slots)
         nq, hq, dq, qs = _rows(q, "q")
         if (nq, dq) != (n, self.head_dim):
             raise _invalid("q must be [tokens, q_heads, head_dim] of k's tokens")
-        _need_ints(torch.int32, n, "positions", positions)
-        o = torch.empty((n, hq, dq), dtype=torch.bfloat16, device=q.device) if q_out is None else q_out
-        if o.shape != q.shape:
-            raise _invalid("q_out must have q's shape")
-        dev = _same_device(self.k, q, k, v, slots, positions, o, rope.cos)
-        d, r = self._desc(), rope._desc()
-        context(dev).call("wx_rope_kv_append", C.byref(r), _p(positions), _p(q), qs, hq, C.byref(d), _p(k), ks, _p(v),
-                          vs, n, _p(slots), _p(o), _rows(o, "q_out")[3])
+        pos = _need_ints(torch.int32, n, "positions", positions)
+        o, ostride = _out_rows(q, n, hq, dq, q_out, "q_out must have q's shape")
+        context(_same_device(self.k, q, k, v, slots, positions, o, rope.cos)).call(
+            "wx_rope_kv_append", rope._desc, pos, q.data_ptr(), qs, hq, self._desc, k.data_ptr(), ks, v.data_ptr(), vs,
+            n, at, o.data_ptr(), ostride)
         return o
 
     def read(self, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """k and v of the slots as bf16 [tokens, kv_heads, head_dim] (< 0: zeros)."""
-        _need_ints(torch.int64, None, "slots", slots)
-        n = slots.numel()
-        k = torch.empty((n, self.kv_heads, self.head_dim), dtype=torch.bfloat16, device=self.k.device)
+        at = _need_ints(torch.int64, None, "slots", slots)
+        n, h, d = slots.numel(), self.kv_heads, self.head_dim
+        k = torch.empty((n, h, d), dtype=torch.bfloat16, device=self.k.device)
         v = torch.empty_like(k)
-        dev = _same_device(self.k, slots)
-        d = self._desc()
-        context(dev).call("wx_kv_read", C.byref(d), _p(slots), n, _p(k), _p(v), self.kv_heads * self.head_dim)
+        context(_same_device(self.k, slots)).call("wx_kv_read", self._desc, at, n, k.data_ptr(), v.data_ptr(), h * d)
         return k, v
 
 
 def _attn_out(q: torch.Tensor, out: Optional[torch.Tensor], return_lse: bool):
     n, h, d, stride = _rows(q, "q")
-    o = torch.empty((n, h, d), dtype=torch.bfloat16, device=q.device) if out is None else out
-    if o.shape != q.shape:
-        raise _invalid("out must have q's shape")
+    o, ostride = _out_rows(q, n, h, d, out, "out must have q's shape")
     lse = torch.empty((n, h), dtype=torch.float32, device=q.device) if return_lse else None
-    return n, h, d, stride, o, _rows(o, "out")[3], lse
+    return n, h, d, stride, o, ostride, lse
+
+
+def _batch_of(cu_seqlens: torch.Tensor) -> int:
+    batch = cu_seqlens.numel() - 1
+    if batch < 0:
+        raise _invalid("cu_seqlens needs at least one entry")
+    return batch
+
+
+def _dims(n: int, batch: int, max_len: int, h: int, hk: int, d: int, causal: bool, window: int,
+          scale: Optional[float]):
+    return C.byref(AttnDims(n, batch, max_len, h, hk, d, causal, window, d ** -0.5 if scale is None else scale))
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_len: int,
@@ -261,17 +259,12 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     nv, hv, dv, vs = _rows(v, "v")
     if (nk, hk, dk) != (nv, hv, dv) or dk != d:
         raise _invalid("k and v must be [tokens, kv_heads, head_dim] of q's head_dim")
-    batch = cu_seqlens.numel() - 1
-    if batch < 0:
-        raise _invalid("cu_seqlens needs at least one entry")
-    _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
-    if cu_seqlens_k is not None:
-        _need_ints(torch.int32, batch + 1, "cu_seqlens_k", cu_seqlens_k)
-    dev = _same_device(q, k, v, cu_seqlens, o, *([] if cu_seqlens_k is None else [cu_seqlens_k]))
-    dims = AttnDims(n, batch, max_len, h, hk, d, int(causal), window,
-                    float(1.0 / math.sqrt(d) if scale is None else scale))
-    context(dev).call("wx_prompt_attention", C.byref(dims), _p(q), qs, _p(k), ks, _p(v), vs, nk, _p(cu_seqlens),
-                      _p(cu_seqlens_k), _p(o), os_, _p(lse))
+    batch = _batch_of(cu_seqlens)
+    cu = _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
+    cu_k = None if cu_seqlens_k is None else _need_ints(torch.int32, batch + 1, "cu_seqlens_k", cu_seqlens_k)
+    dev = _same_device(q, k, v, cu_seqlens, o, cu_seqlens if cu_k is None else cu_seqlens_k)
+    context(dev).call("wx_prompt_attention", _dims(n, batch, max_len, h, hk, d, causal, window, scale), q.data_ptr(), qs,
+                      k.data_ptr(), ks, v.data_ptr(), vs, nk, cu, cu_k, o.data_ptr(), os_, _p(lse))
     return (o, lse) if return_lse else o
 
 
@@ -282,20 +275,15 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
     are the last of the kv_lens[b] tokens cached in pages block_table[b] (int32, [batch, blocks];
     entries beyond the length are not read). ``max_len``: the longest query length."""
     n, h, d, qs, o, os_, lse = _attn_out(q, out, return_lse)
-    batch = cu_seqlens.numel() - 1
-    if batch < 0:
-        raise _invalid("cu_seqlens needs at least one entry")
-    _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
-    _need_ints(torch.int32, batch, "kv_lens", kv_lens)
-    _need_ints(torch.int32, None, "block_table", block_table)
+    batch = _batch_of(cu_seqlens)
+    cu = _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
+    lens = _need_ints(torch.int32, batch, "kv_lens", kv_lens)
+    table = _need_ints(torch.int32, None, "block_table", block_table)
     if block_table.dim() != 2 or block_table.shape[0] != batch:
         raise _invalid("block_table must be [batch, blocks]")
     if d != cache.head_dim:
         raise _invalid("q must have the cache's head_dim")
     dev = _same_device(q, cache.k, cu_seqlens, kv_lens, block_table, o)
-    dims = AttnDims(n, batch, max_len, h, cache.kv_heads, d, int(causal), window,
-                    float(1.0 / math.sqrt(d) if scale is None else scale))
-    c = cache._desc()
-    context(dev).call("wx_paged_attention", C.byref(dims), _p(q), qs, C.byref(c), _p(cu_seqlens), _p(kv_lens),
-                      _p(block_table), block_table.shape[1], _p(o), os_, _p(lse))
+    context(dev).call("wx_paged_attention", _dims(n, batch, max_len, h, cache.kv_heads, d, causal, window, scale),
+                      q.data_ptr(), qs, cache._desc, cu, lens, table, block_table.shape[1], o.data_ptr(), os_, _p(lse))
     return (o, lse) if return_lse else o
