@@ -12,8 +12,7 @@
 #include <algorithm>
 
 #include "wx_internal.h"
-#include "wx_ptx.cuh"
-#include "wx_text.h"
+#include "wx_text_dev.cuh"
 
 namespace wx {
 
@@ -36,14 +35,22 @@ __global__ void rope_table_kernel(RopeFreqs f, int nf, int64_t positions, double
 }
 
 // --------------------------------------------------------------- rows of a token
-// One launch serves rope alone, the cache write alone and both fused. A token's rows are
-// its q heads, then k heads, then v heads; HD/8 neighbouring lanes own a row, 8 values each.
+// One launch serves rope alone, the cache write alone and both fused. A token's rows are its q
+// heads, then k heads, then v heads. HD / (2 W) neighbouring lanes own a row; a lane holds two
+// groups of W columns, placed so that both halves of each pair it turns are its own (W = 8: 16-byte
+// accesses; W = 4 where rot is no multiple of 16).
+//
+// Bound by HBM: each value is read once and written once, the table row of a token (rot * 4 bytes)
+// is shared by its heads. A warp issues the loads of all its rows (up to kRowGroups groups) before
+// the first store: the outputs may alias the inputs, so the compiler could not.
+constexpr int kRowGroups = 4;
+
 struct RowsParams {
   const __nv_bfloat16 *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;  // elements between tokens
   int nq, nkv;                           // q rows, and k (= v) rows of a token (0 without a cache)
   int64_t tokens;
-  int rows_per_warp;
+  int rows_per_warp, chunks;             // a token's rows are dealt to `chunks` warps
   // rotation (rot = 0: none)
   const float *cos_t, *sin_t;
   const int32_t* pos;
@@ -60,77 +67,113 @@ struct RowsParams {
   int* err;
 };
 
-// 8 values of a row -> the stored format. The scale is amax / 127 or amax / 448 of the fp32
-// values (amax reduced over the row's lanes); the value stored is value * (127 | 448) / amax
-// rounded to nearest even. A row with infinity or NaN stores scale NaN and zeros, so that it
-// reads back as NaN; a row below 2^-100 everywhere (127 / amax could overflow) stores zeros.
-template <int FMT, int HD>
-__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float* scale) {
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[i]));
-  bool bad = false;  // fmaxf drops NaN
-#pragma unroll
-  for (int i = 0; i < 8; ++i) bad |= !(fabsf(x[i]) <= 3.402823466e38f);
-  if (bad) amax = INFINITY;
-#pragma unroll
-  for (int o = HD / 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  constexpr float kMax = FMT == kKvInt8 ? 127.f : 448.f;
-  const bool finite = amax <= 3.402823466e38f;
-  const bool live = finite && amax >= 0x1p-100f;
-  const float inv = live ? __fdiv_rn(kMax, amax) : 0.f;
-  *scale = finite ? (live ? __fdiv_rn(amax, kMax) : 0.f) : __int_as_float(0x7fc00000);
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float y[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = live ? __fmul_rn(x[4 * h + i], inv) : 0.f;
-    if constexpr (FMT == kKvInt8) {
-      uint32_t b = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b |= ((uint32_t)__float2int_rn(y[i]) & 0xffu) << (8 * i);
-      w[h] = b;
+template <int W>
+struct Cols {  // W bf16 columns in memory
+  uint32_t w[W / 2];
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    if constexpr (W == 8) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
     } else {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-      w[h] = lo | hi << 16;
+      const uint2 x = *reinterpret_cast<const uint2*>(p);
+      w[0] = x.x, w[1] = x.y;
     }
   }
-  return make_uint2(w[0], w[1]);
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const {
+    if constexpr (W == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+};
+
+// N values of a row (its other values in the neighbouring kLanes lanes) -> the stored format,
+// packed in words. The scale is amax / 127 or amax / 448 of the fp32 values; the value stored is
+// value * (127 | 448) / amax rounded to nearest even. A row with infinity or NaN stores scale NaN
+// and zeros, so that it reads back as NaN; a row below 2^-100 everywhere (127 / amax could
+// overflow) stores zeros.
+//
+// This kernel is issue-bound before it is HBM-bound, hence: the magnitudes are compared as bits
+// (NaN and infinity come out on top), int8 values are rounded by adding 1.5 * 2^23 (the low byte of
+// the sum is the integer), products are packed in pairs.
+template <int FMT, int N, int kLanes>
+__device__ __forceinline__ float quantise(const float (&x)[N], uint32_t (&w)[N / 4]) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) bits = max(bits, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+  constexpr float kMax = FMT == kKvInt8 ? 127.f : 448.f;
+  const float amax = __uint_as_float(bits);
+  const bool finite = bits < 0x7f800000u;
+  const bool live = finite && amax >= 0x1p-100f;
+  const float inv = live ? __fdiv_rn(kMax, amax) : 0.f;
+  const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+  for (int h = 0; h < N / 4; ++h) {
+    float2 lo = __fmul2_rn(make_float2(x[4 * h], x[4 * h + 1]), inv2);
+    float2 hi = __fmul2_rn(make_float2(x[4 * h + 2], x[4 * h + 3]), inv2);
+    if constexpr (FMT == kKvInt8) {
+      // (single sums: a packed one would be fused with the product before it, into one rounding)
+      auto byte = [](float y) { return __float_as_uint(__fadd_rn(y, 12582912.f)); };
+      const uint32_t a = __byte_perm(byte(lo.x), byte(lo.y), 0x0040);
+      const uint32_t b = __byte_perm(byte(hi.x), byte(hi.y), 0x0040);
+      w[h] = __byte_perm(a, b, 0x5410);
+    } else {
+      const uint32_t a = __nv_cvt_float2_to_fp8x2(lo, __NV_SATFINITE, __NV_E4M3);
+      const uint32_t b = __nv_cvt_float2_to_fp8x2(hi, __NV_SATFINITE, __NV_E4M3);
+      w[h] = a | b << 16;
+    }
+    if (!live) w[h] = 0;
+  }
+  return finite ? (live ? __fdiv_rn(amax, kMax) : 0.f) : __int_as_float(0x7fc00000);
 }
 
-template <int FMT, int HD>
-__global__ void __launch_bounds__(256) text_rows_kernel(RowsParams p) {
-  constexpr int kLanes = HD / 8;         // lanes of a row
-  constexpr int kRows = 32 / kLanes;     // rows of a warp at a time
+template <int FMT, int HD, int W, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 4) text_rows_kernel(RowsParams p) {
+  constexpr int kLanes = HD / (2 * W);  // lanes of a row
+  constexpr int kRows = 32 / kLanes;    // rows of a warp at a time
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes;
   const int per_token = p.nq + 2 * p.nkv;
-  const int chunks = (per_token + p.rows_per_warp - 1) / p.rows_per_warp;
   const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int64_t t = w / chunks;
+  const int64_t t = w / p.chunks;
   if (t >= p.tokens) return;
-  const int r0 = (int)(w % chunks) * p.rows_per_warp;
+  const int r0 = (int)(w % p.chunks) * p.rows_per_warp;
   const int r1 = min(per_token, r0 + p.rows_per_warp);
 
-  // columns of this lane: two groups of 4, so that both halves of a pair sit in one lane
-  const bool turn = j < p.rot / 8;
-  const int c0 = turn ? (p.interleaved ? 8 * j : 4 * j) : 8 * j;
-  const int c1 = turn ? (p.interleaved ? 8 * j + 4 : p.rot / 2 + 4 * j) : 8 * j + 4;
-  float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
-  bool pos_ok = true;
+  const bool turn = j < p.rot / (2 * W);
+  const bool apart = turn && !INTERLEAVED;  // pairs (i, i + rot / 2)
+  const int c0 = apart ? W * j : 2 * W * j;
+  const int c1 = apart ? p.rot / 2 + W * j : 2 * W * j + W;
+
+  Cols<W> a[kRowGroups], b[kRowGroups];
+#pragma unroll
+  for (int g = 0; g < kRowGroups; ++g) {
+    const int r = r0 + g * kRows + lane / kLanes;
+    if (r >= r1) continue;
+    const __nv_bfloat16* src = r < p.nq           ? p.q + t * p.q_stride + (int64_t)r * HD
+                               : r < p.nq + p.nkv ? p.k + t * p.k_stride + (int64_t)(r - p.nq) * HD
+                                                  : p.v + t * p.v_stride + (int64_t)(r - p.nq - p.nkv) * HD;
+    a[g].load(src + c0);
+    b[g].load(src + c1);
+  }
+
+  float cs[W], sn[W];
   if (p.rot) {
     const int64_t pos = p.pos[t];
-    pos_ok = pos >= 0 && pos < p.positions;
-    if (!pos_ok) {
+    if (pos < 0 || pos >= p.positions) {
       if (lane == 0) set_dev_error(p.err, kDevBadArgs);
-    } else if (turn) {
-      cs = *reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + 4 * j);
-      sn = *reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + 4 * j);
+      return;
+    }
+    if (turn) {
+#pragma unroll
+      for (int i = 0; i < W; i += 4) {
+        const float4 c = *reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + W * j + i);
+        const float4 s = *reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + W * j + i);
+        cs[i] = c.x, cs[i + 1] = c.y, cs[i + 2] = c.z, cs[i + 3] = c.w;
+        sn[i] = s.x, sn[i + 1] = s.y, sn[i + 2] = s.z, sn[i + 3] = s.w;
+      }
     }
   }
-  if (!pos_ok) return;
   int64_t slot = -1;
   if (p.nkv) {
     slot = p.slots[t];
@@ -140,129 +183,131 @@ __global__ void __launch_bounds__(256) text_rows_kernel(RowsParams p) {
     }
   }
 
-#pragma unroll 4
-  for (int rb = r0; rb < r1; rb += kRows) {
-    const int r = rb + lane / kLanes;
+#pragma unroll
+  for (int g = 0; g < kRowGroups; ++g) {
+    if (r0 + g * kRows >= r1) break;  // (the warp as a whole)
+    const int r = r0 + g * kRows + lane / kLanes;
     const bool live = r < r1;
     const bool is_q = r < p.nq, is_v = r >= p.nq + p.nkv;
     const int h = is_q ? r : is_v ? r - p.nq - p.nkv : r - p.nq;
-    const __nv_bfloat16* src = is_q   ? p.q + t * p.q_stride + (int64_t)h * HD
-                               : is_v ? p.v + t * p.v_stride + (int64_t)h * HD
-                                      : p.k + t * p.k_stride + (int64_t)h * HD;
-    uint2 a = make_uint2(0, 0), b = make_uint2(0, 0);
-    if (live) {
-      a = *reinterpret_cast<const uint2*>(src + c0);
-      b = *reinterpret_cast<const uint2*>(src + c1);
+    float x[2 * W];
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const uint32_t u = live ? a[g].w[i] : 0, v = live ? b[g].w[i] : 0;
+      x[2 * i] = bf16_lo(u), x[2 * i + 1] = bf16_hi(u);
+      x[W + 2 * i] = bf16_lo(v), x[W + 2 * i + 1] = bf16_hi(v);
     }
-    float x[8] = {bf16_lo(a.x), bf16_hi(a.x), bf16_lo(a.y), bf16_hi(a.y),
-                  bf16_lo(b.x), bf16_hi(b.x), bf16_lo(b.y), bf16_hi(b.y)};
     if (turn && !is_v) {
-      // (x1, x2) -> (x1 c - x2 s, x2 c + x1 s), each product rounded by itself: the same
-      // bits whichever path rotates (a contracted form would depend on the compiler)
-      const float c[4] = {cs.x, cs.y, cs.z, cs.w}, s[4] = {sn.x, sn.y, sn.z, sn.w};
-      float y[8];
+      // (x1, x2) -> (x1 c - x2 s, x2 c + x1 s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x1 = p.interleaved ? x[2 * i] : x[i], x2 = p.interleaved ? x[2 * i + 1] : x[i + 4];
-        y[i] = __fsub_rn(__fmul_rn(x1, c[i]), __fmul_rn(x2, s[i]));
-        y[i + 4] = __fadd_rn(__fmul_rn(x2, c[i]), __fmul_rn(x1, s[i]));
+      for (int i = 0; i < W; i += 2) {
+        float &a0 = x[INTERLEAVED ? 2 * i : i], &a1 = x[INTERLEAVED ? 2 * i + 2 : i + 1];
+        float &b0 = x[INTERLEAVED ? 2 * i + 1 : W + i], &b1 = x[INTERLEAVED ? 2 * i + 3 : W + i + 1];
+        const float2 x1 = make_float2(a0, a1), x2 = make_float2(b0, b1);
+        const float2 c = make_float2(cs[i], cs[i + 1]), s = make_float2(sn[i], sn[i + 1]);
+        const float2 ns = make_float2(-sn[i], -sn[i + 1]);
+        const float2 u = __ffma2_rn(x1, c, __fmul2_rn(x2, ns));
+        const float2 v = __ffma2_rn(x2, c, __fmul2_rn(x1, s));
+        a0 = u.x, a1 = u.y, b0 = v.x, b1 = v.y;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = p.interleaved ? y[(i >> 1) + 4 * (i & 1)] : y[i];
     }
-    if (is_q || FMT == kKvBf16) {
-      a = make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
-      b = make_uint2(pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-    }
-    const int64_t row = slot < 0 ? 0 : ((((slot >> p.page_shift) * p.nkv + h) << p.page_shift) |
-                                        (slot & ((1 << p.page_shift) - 1)));
-    uint2 qv = make_uint2(0, 0);
+    uint32_t qv[W / 2] = {};
     float scale = 0.f;
-    if constexpr (FMT != kKvBf16) qv = quantise8<FMT, HD>(x, &scale);  // (all lanes: it shuffles)
+    if constexpr (FMT != kKvBf16) scale = quantise<FMT, 2 * W, kLanes>(x, qv);  // (all lanes: it shuffles)
     if (!live) continue;
-    if (is_q) {
-      __nv_bfloat16* o = p.q_out + t * p.q_out_stride + (int64_t)h * HD;
-      *reinterpret_cast<uint2*>(o + c0) = a;
-      *reinterpret_cast<uint2*>(o + c1) = b;
-    } else if (slot >= 0) {
-      uint8_t* base = is_v ? p.vc : p.kc;
-      if constexpr (FMT == kKvBf16) {
-        __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(base) + row * HD;
-        *reinterpret_cast<uint2*>(o + c0) = a;
-        *reinterpret_cast<uint2*>(o + c1) = b;
-      } else {
-        *reinterpret_cast<uint32_t*>(base + row * HD + c0) = qv.x;
-        *reinterpret_cast<uint32_t*>(base + row * HD + c1) = qv.y;
-        if (j == 0) (is_v ? p.vs : p.ks)[row] = scale;
+    const int64_t row = ((((slot >> p.page_shift) * p.nkv + h) << p.page_shift) | (slot & ((1 << p.page_shift) - 1)));
+    if (is_q || FMT == kKvBf16) {
+      __nv_bfloat16* o = is_q ? p.q_out + t * p.q_out_stride + (int64_t)h * HD
+                              : reinterpret_cast<__nv_bfloat16*>(is_v ? p.vc : p.kc) + row * HD;
+      if (!is_q && slot < 0) continue;
+      Cols<W> lo, hi;
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) {
+        lo.w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        hi.w[i] = pack_bf16x2(x[W + 2 * i], x[W + 2 * i + 1]);
       }
+      lo.store(o + c0);
+      hi.store(o + c1);
+    } else if (slot >= 0) {
+      uint8_t* o = (is_v ? p.vc : p.kc) + row * HD;
+      if constexpr (W == 8) {
+        *reinterpret_cast<uint2*>(o + c0) = make_uint2(qv[0], qv[1]);
+        *reinterpret_cast<uint2*>(o + c1) = make_uint2(qv[2], qv[3]);
+      } else {
+        *reinterpret_cast<uint32_t*>(o + c0) = qv[0];
+        *reinterpret_cast<uint32_t*>(o + c1) = qv[1];
+      }
+      if (j == 0) (is_v ? p.vs : p.ks)[row] = scale;
     }
   }
 }
 
 // ------------------------------------------------------------------- reading back
-// value * scale, one rounding to bf16; a slot < 0 reads zeros
+// value * scale, one rounding to bf16; a slot < 0 reads zeros. A lane reads 16 values of a row,
+// HD / 16 lanes a row; a warp has up to kRowGroups groups of rows in flight, as above.
 struct ReadParams {
   const uint8_t *kc, *vc;
   const float *ks, *vs;
   const int64_t* slots;
   int64_t tokens, n_slots;
   int nkv, page_shift;
+  int rows_per_warp, chunks;
   __nv_bfloat16 *k, *v;
   int64_t out_stride;
   int* err;
 };
 
-__device__ __forceinline__ float int8_at(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
-__device__ __forceinline__ float2 e4m3x2(uint32_t w, int i) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
-  return __half22float2(__half2(h));
-}
-
 template <int FMT, int HD>
 __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p) {
-  constexpr int kLanes = HD / 8;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int j = (int)(i % kLanes);
-  const int64_t row_i = i / kLanes;
-  const int h2 = (int)(row_i % (2 * p.nkv));
-  const int64_t t = row_i / (2 * p.nkv);
+  constexpr int kLanes = HD / 16, kRows = 32 / kLanes;
+  constexpr int kVec = FMT == kKvBf16 ? 2 : 1;  // 16-byte units of 16 values
+  const int lane = threadIdx.x & 31;
+  const int j = lane % kLanes;
+  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int64_t t = w / p.chunks;
   if (t >= p.tokens) return;
-  const bool is_v = h2 >= p.nkv;
-  const int h = is_v ? h2 - p.nkv : h2;
+  const int r0 = (int)(w % p.chunks) * p.rows_per_warp;
+  const int r1 = min(2 * p.nkv, r0 + p.rows_per_warp);
   int64_t slot = p.slots[t];
   if (slot >= p.n_slots) {
-    if (j == 0) set_dev_error(p.err, kDevBadArgs);
+    if (lane == 0) set_dev_error(p.err, kDevBadArgs);
     slot = -1;
   }
-  uint4 o = make_uint4(0, 0, 0, 0);
-  if (slot >= 0) {
-    const int64_t row = (((slot >> p.page_shift) * p.nkv + h) << p.page_shift) | (slot & ((1 << p.page_shift) - 1));
-    const uint8_t* base = is_v ? p.vc : p.kc;
+  const int64_t page = slot >> p.page_shift, inside = slot & ((1 << p.page_shift) - 1);
+  uint4 x[kRowGroups][kVec];
+  float s[kRowGroups];
+#pragma unroll
+  for (int g = 0; g < kRowGroups; ++g) {
+    const int r = r0 + g * kRows + lane / kLanes;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[g][e] = make_uint4(0, 0, 0, 0);
+    s[g] = 0.f;
+    if (r >= r1 || slot < 0) continue;
+    const bool is_v = r >= p.nkv;
+    const int64_t row = ((page * p.nkv + (is_v ? r - p.nkv : r)) << p.page_shift) | inside;
+    const uint4* src = reinterpret_cast<const uint4*>(is_v ? p.vc : p.kc) + (row * HD / 16 + j) * kVec;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[g][e] = __ldg(src + e);
+    if constexpr (FMT != kKvBf16) s[g] = __ldg((is_v ? p.vs : p.ks) + row);
+  }
+#pragma unroll
+  for (int g = 0; g < kRowGroups; ++g) {
+    const int r = r0 + g * kRows + lane / kLanes;
+    if (r >= r1) continue;
+    const bool is_v = r >= p.nkv;
+    uint4* dst = reinterpret_cast<uint4*>((is_v ? p.v : p.k) + t * p.out_stride +
+                                          (int64_t)(is_v ? r - p.nkv : r) * HD) + 2 * j;
     if constexpr (FMT == kKvBf16) {
-      o = *reinterpret_cast<const uint4*>(base + (row * HD + 8 * j) * 2);
+      dst[0] = x[g][0];
+      dst[1] = x[g][1];
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(base + row * HD + 8 * j);
-      const float s = (is_v ? p.vs : p.ks)[row];
-      float x[8];
-      if constexpr (FMT == kKvInt8) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = int8_at(e < 4 ? w.x : w.y, e & 3);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = e4m3x2(e < 2 ? w.x : w.y, e & 1);
-          x[2 * e] = f.x;
-          x[2 * e + 1] = f.y;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= s;
-      o = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                     pack_bf16x2(x[6], x[7]));
+      const uint4 u = x[g][0];
+      dst[0] = make_uint4(bytes_times<FMT>(u.x, 0, s[g]), bytes_times<FMT>(u.x, 1, s[g]),
+                          bytes_times<FMT>(u.y, 0, s[g]), bytes_times<FMT>(u.y, 1, s[g]));
+      dst[1] = make_uint4(bytes_times<FMT>(u.z, 0, s[g]), bytes_times<FMT>(u.z, 1, s[g]),
+                          bytes_times<FMT>(u.w, 0, s[g]), bytes_times<FMT>(u.w, 1, s[g]));
     }
   }
-  __nv_bfloat16* dst = (is_v ? p.v : p.k) + t * p.out_stride + (int64_t)h * HD + 8 * j;
-  *reinterpret_cast<uint4*>(dst) = o;
 }
 
 // --------------------------------------------------------------------- host side
@@ -289,31 +334,43 @@ static int check_rope(wx_ctx* ctx, const wx_rope* r, int head_dim, const int32_t
   return WX_OK;
 }
 
+// How a token's rows are dealt to warps: as many as a warp keeps in flight, fewer where there are
+// too few tokens to give every SM 64 warps (a warp's rows follow one another).
+static int64_t deal_rows(wx_ctx* ctx, int64_t tokens, int per_token, int rows_at_once, int* rows_per_warp, int* chunks) {
+  *rows_per_warp = rows_at_once * kRowGroups;
+  while (*rows_per_warp > rows_at_once &&
+         tokens * ((per_token + *rows_per_warp - 1) / *rows_per_warp) < (int64_t)ctx->num_sms * 64)
+    *rows_per_warp /= 2;
+  *chunks = (per_token + *rows_per_warp - 1) / *rows_per_warp;
+  return (tokens * *chunks + 7) / 8;  // blocks of 8 warps
+}
+
+template <int FMT, int HD, int W>
+static void start_rows(unsigned g, cudaStream_t s, const RowsParams& p) {
+  if (p.interleaved) text_rows_kernel<FMT, HD, W, true><<<g, 256, 0, s>>>(p);
+  else text_rows_kernel<FMT, HD, W, false><<<g, 256, 0, s>>>(p);
+}
+
+template <int HD, int W>
+static void start_rows(int fmt, unsigned g, cudaStream_t s, const RowsParams& p) {
+  if (fmt == kKvInt8) start_rows<kKvInt8, HD, W>(g, s, p);
+  else if (fmt == kKvE4m3) start_rows<kKvE4m3, HD, W>(g, s, p);
+  else start_rows<kKvBf16, HD, W>(g, s, p);
+}
+
 static int launch_rows(wx_ctx* ctx, RowsParams& p, int fmt, int head_dim) {
   if (p.tokens == 0) return WX_OK;
-  const int per_token = p.nq + 2 * p.nkv;
-  const int rows = 256 / head_dim;  // rows of a warp at a time
-  // Eight rows a warp reuse the token's table row and keep 4 loads in flight per lane; with few
-  // tokens fewer rows a warp fill the SMs instead (a warp's rows follow one another).
-  p.rows_per_warp = 8;
-  while (p.rows_per_warp > rows &&
-         p.tokens * ((per_token + p.rows_per_warp - 1) / p.rows_per_warp) < (int64_t)ctx->num_sms * 32)
-    p.rows_per_warp /= 2;
-  const int64_t warps = p.tokens * ((per_token + p.rows_per_warp - 1) / p.rows_per_warp);
-  const int64_t blocks = (warps + 7) / 8;
+  const int W = p.rot % 16 == 0 ? 8 : 4;
+  const int64_t blocks =
+      deal_rows(ctx, p.tokens, p.nq + 2 * p.nkv, 32 / (head_dim / (2 * W)), &p.rows_per_warp, &p.chunks);
   if (blocks > INT32_MAX) return set_error(ctx, WX_ERR_UNSUPPORTED, "too many tokens in one call");
   p.err = ctx->dev_err;
   ProfScope prof(ctx, kProfRow);
   const unsigned g = (unsigned)blocks;
-  if (head_dim == 128) {
-    if (fmt == kKvInt8) text_rows_kernel<kKvInt8, 128><<<g, 256, 0, ctx->stream>>>(p);
-    else if (fmt == kKvE4m3) text_rows_kernel<kKvE4m3, 128><<<g, 256, 0, ctx->stream>>>(p);
-    else text_rows_kernel<kKvBf16, 128><<<g, 256, 0, ctx->stream>>>(p);
-  } else {
-    if (fmt == kKvInt8) text_rows_kernel<kKvInt8, 64><<<g, 256, 0, ctx->stream>>>(p);
-    else if (fmt == kKvE4m3) text_rows_kernel<kKvE4m3, 64><<<g, 256, 0, ctx->stream>>>(p);
-    else text_rows_kernel<kKvBf16, 64><<<g, 256, 0, ctx->stream>>>(p);
-  }
+  if (head_dim == 128)
+    W == 8 ? start_rows<128, 8>(fmt, g, ctx->stream, p) : start_rows<128, 4>(fmt, g, ctx->stream, p);
+  else
+    W == 8 ? start_rows<64, 8>(fmt, g, ctx->stream, p) : start_rows<64, 4>(fmt, g, ctx->stream, p);
   return launch_status(ctx, "text_rows");
 }
 
@@ -466,8 +523,8 @@ int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int6
   p.v = static_cast<__nv_bfloat16*>(v_out);
   p.out_stride = out_stride;
   p.err = ctx->dev_err;
-  const int64_t threads = tokens * 2 * cache->kv_heads * (cache->head_dim / 8);
-  const int64_t blocks = (threads + 255) / 256;
+  const int64_t blocks =
+      deal_rows(ctx, tokens, 2 * cache->kv_heads, 32 / (cache->head_dim / 16), &p.rows_per_warp, &p.chunks);
   if (blocks > INT32_MAX) return set_error(ctx, WX_ERR_UNSUPPORTED, "too many tokens in one call");
   ProfScope prof(ctx, kProfRow);
   const unsigned g = (unsigned)blocks;

@@ -2,6 +2,7 @@
 // wx_text_flash.cu): launch parameters, a sequence's bounds, 8-bit -> bf16.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp8.h>
 
 #include "wx_ptx.cuh"
 #include "wx_text.h"
@@ -109,6 +110,23 @@ __device__ __forceinline__ uint32_t bytes_to_bf16x2(uint32_t a, uint32_t b, int 
     const uint32_t w = __byte_perm(a, b, (uint32_t)(lo << 4 | hi << 12));
     return mul_bf16x2((w & 0x80008000u) | ((w >> 4) & 0x07f007f0u), 0x7b807b80u);  // 2^120
   }
+}
+
+// stored bytes 2 h, 2 h + 1 of a word, times a scale, rounded to a bf16 pair
+template <int FMT>
+__device__ __forceinline__ uint32_t bytes_times(uint32_t w, int h, float scale) {
+  float2 x;
+  if constexpr (FMT == kKvInt8) {  // 2^23 + (byte + 128) is an fp32 number whose low byte is byte + 128
+    w ^= 0x80808080u;
+    x = make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, h ? 0x7442 : 0x7440)),
+                    __uint_as_float(__byte_perm(w, 0x4b000000u, h ? 0x7443 : 0x7441)));
+    x = __fadd2_rn(x, make_float2(-8388736.f, -8388736.f));
+  } else {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * h)), __NV_E4M3);
+    x = __half22float2(__half2(r));
+  }
+  x = __fmul2_rn(x, make_float2(scale, scale));
+  return pack_bf16x2(x.x, x.y);
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
