@@ -527,6 +527,11 @@ def test_refusals():
     refused(bad, lambda: text.paged_attention(q, cache, cu, lens, table[0], 4))
     refused(bad, lambda: text.paged_attention(q, cache, cu, lens.long(), table, 4))
     refused(bad, lambda: text.paged_attention(_randn(g, 4, 4, 64), cache, cu, lens, table, 4))
+    # one page named so often that the walk over it could not be counted in 32 bits
+    deep = torch.zeros((64, 1 << 19), dtype=torch.int32, device="cuda")
+    mqa = text.PagedKVCache(1, 256, 64, 64)
+    refused(unsup, lambda: text.paged_attention(_randn(g, 64, 64, 64), mqa, _cu([1] * 64),
+                                                torch.ones(64, dtype=torch.int32, device="cuda"), deep, 1))
     refused(bad, lambda: cache.append(k, k, torch.zeros(3, dtype=torch.int64, device="cuda")))
     refused(bad, lambda: cache.append(q, q, torch.zeros(4, dtype=torch.int64, device="cuda")))
     refused(bad, lambda: text.PagedKVCache(2, 16, 2, 128, "int4"))

@@ -126,25 +126,6 @@ int make_tmap_bf16_3d(wx_ctx* ctx, CUtensorMap* map, const void* base, const uin
   return WX_OK;
 }
 
-int make_tmap_u8_rows(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t rows, uint32_t cols,
-                      uint32_t box_rows) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return set_error(ctx, WX_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  if (!aligned16(base) || (cols != 64 && cols != 128))
-    return set_error(ctx, WX_ERR_INVALID, "TMA byte rows need a 16-byte aligned base and 64 or 128 columns");
-  cuuint64_t gdim[2] = {cols, rows};
-  cuuint64_t gstride[1] = {cols};
-  cuuint32_t box[2] = {cols, box_rows};
-  cuuint32_t estride[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstride, box, estride,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return set_error(ctx, WX_ERR_CUDA, "cuTensorMapEncodeTiled (u8) failed (%d): rows=%llu cols=%u", (int)r,
-                     (unsigned long long)rows, cols);
-  return WX_OK;
-}
-
 int* arrival_counters(wx_ctx* ctx, int64_t n, int* status) {
   *status = WX_OK;
   if (n <= ctx->n_arrivals) return ctx->arrivals;

@@ -107,11 +107,6 @@ int make_tmap_u32_2d(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t r
 int make_tmap_bf16_3d(wx_ctx* ctx, CUtensorMap* map, const void* base, const uint64_t (&dims)[3],
                       const uint64_t (&ld)[2], const uint32_t (&box)[3]);
 
-// 2-D byte tensor map of contiguous rows of `cols` (64 or 128) bytes, box `box_rows` whole rows,
-// swizzled over the row's width, zero fill out of bounds.
-int make_tmap_u8_rows(wx_ctx* ctx, CUtensorMap* map, const void* base, uint64_t rows, uint32_t cols,
-                      uint32_t box_rows);
-
 // `n` counters on the device, zero between launches: a kernel that counts arrivals on them sets
 // each back to zero with the last arrival (every CTA arrives, whatever happened to its work).
 int* arrival_counters(wx_ctx* ctx, int64_t n, int* status);

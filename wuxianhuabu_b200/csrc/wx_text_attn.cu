@@ -13,575 +13,532 @@
 
 namespace wx {
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+// C[16 x 8] += A[16 x 16] B[16 x 8], bf16, fp32 accumulators. Lane (g, t) = (lane / 4, lane % 4)
+// holds C rows g (c0, c1) and g + 8 (c2, c3), columns 2t and 2t + 1; A rows g (a0, a2) and g + 8
+// (a1, a3), columns 2t.. (a0, a1) and 2t + 8.. (a2, a3); B column g, rows 2t.. (b0) and 2t + 8.. (b1).
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 x 8 matrix of bf16, lane (g, t) holding row g, columns 2t and 2t + 1, transposed
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// 16 bytes (4: plain) from global to shared memory, in the thread's open group of copies
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// waits until at most N of the thread's groups are open
+template <int N>
+__device__ __forceinline__ void copy_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // ------------------------------------------------- few query rows: text_rows_attn_kernel
-// For decoding and for a few new tokens: 16 flattened query rows share one walk over the keys.
-// 16 rows against 128-wide heads are 32 FLOP per K/V byte at bf16, far below the ridge, so the
-// walk is bound by the K/V bytes; the tensor work (mma.sync, M = 16) and the 8-bit expansion
-// stay in registers below that bound.
+// For decoding and for a few new tokens: 8 NT flattened query rows share a walk over the keys. So
+// few rows against 128-wide heads are a few FLOP per K/V byte, far below the ridge: the walk is
+// bound by the K/V bytes, and what has to be kept small beside them is the work per key. The
+// products are therefore turned round, the 16 keys of a step being the tensor tile's rows and the
+// query rows its columns (S^T = K Q^T, O^T += V^T P^T): no tile row is padding, a lane's K and V
+// scales are two numbers, and sums take 32 NT / (128 / HD) registers instead of twice that.
 //
-// A CTA's eight warps take 16-key steps of its key range in turn, each with its own ring of
-// TMA-filled stages (kStages deep, swizzled so that both fragment reads are conflict-free) and
-// its own running maximum and denominator; they are joined once, at the end of the range. A
-// step's keys and head columns are dealt to the fragments in the order that makes every
-// shared-memory read a 16-byte one and the products need no transposition: a dot product does
-// not care for the order of its terms, so q, K (head columns) and P, V (keys) are permuted alike.
+// Each warp keeps several steps in flight in a ring of its own, filled by 16-byte copies whose lanes
+// lie side by side in memory (copies of half lines, each lane its own operands, cost a third more
+// at bf16); 8-bit values become bf16 in registers, exactly. The keys and head columns of a step are
+// dealt to the fragments in the order in which they lie in memory: a dot product does not care for
+// the order of its terms, so q and K (head columns) and P and V (keys) are permuted alike, and the
+// head columns of O^T are put in order when they are written. (A ring of TMA boxes per warp spent a
+// third of each step on issuing its copies; one ring for the CTA, and tcgen05 with the keys as 128
+// rows, were slower still on 8-bit caches.)
 //
-// Work is split evenly: the (sequence, K/V head, row tile) items, each cut into units of 128
-// keys, form one line of units that is divided into equal runs, one per CTA. A CTA whose run
-// covers part of an item leaves its partial sums; the last to arrive joins them in key order
-// (so the result does not depend on who is last).
-template <int FMT, int HD>
+// A CTA's warps take 16-key steps of its key range in turn, each with its own running maximum and
+// denominator; they are joined once, at the end of the range. Work is split evenly: the (sequence,
+// K/V head, row tile) items, each cut into units of 128 keys, form one line of units that is divided
+// into equal runs, one per CTA. A CTA whose run covers part of an item leaves its partial sums; the
+// last to arrive joins them in key order (so the result does not depend on who is last).
+//
+// Measured, caches flushed from L2: 64 sequences, 32 / 8 heads of 128, 238,000 bf16 keys 191 us =
+// 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 53 us = 2.6 TB/s
+// (4.3 TB/s a further key: there the expansion and the exponentials are as long as the loads); a
+// call with a few keys 11 us, of which 7 on the device.
+constexpr int kUnit = 128;
+
+template <int FMT, int HD, int NT>
 struct RowsGeom {
-  static constexpr bool kWide = FMT != kKvBf16;               // 8-bit rows
-  static constexpr int kTiles = kWide ? 1 : HD / 64;          // boxes per 16-key K (or V) step
-  static constexpr int kRowBytes = kWide ? HD : 128;          // bytes of a box row (swizzle span)
-  static constexpr int kTileBytes = 16 * kRowBytes;
-  static constexpr int kKvBytes = kTiles * kTileBytes;        // K (or V) of a step
-  static constexpr int kStepBytes = 2 * kKvBytes;
-  static constexpr int kStages = kWide ? 4 : (HD == 128 ? 2 : 4);
-  static constexpr int kWarps = 8;
-  static constexpr int kRing = kWarps * kStages * kStepBytes;
-  static constexpr int kScales = kWide ? kWarps * kStages * 128 : 0;
+  static constexpr bool kWide = FMT != kKvBf16;  // 8-bit rows
+  // as many warps as registers (8-bit: 12 against 16, 53 : 54 us) and ring stages (bf16: 10 against
+  // 8, 191 : 196 us) allow; 16 rows take twice the registers
+  static constexpr int kWarps = NT == 1 ? (kWide ? 12 : 10) : 8;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kUnits16 = kWide ? HD / 64 : HD / 32;  // 16-byte units of a key that a lane reads
   static constexpr int kPitch = HD + 4;
-  static constexpr int kJoin = kWarps * 16 * (kPitch + 2) * 4;
-  static constexpr int kBars = kWarps * kStages * 8 + 64;
-  static constexpr int kSmem = kRing + kScales + kJoin + kBars + 1024;
+  static constexpr int kJoin = kWarps * kRows * (kPitch + 2) * 4 + 64;
+  // a step's keys, values (and scales), and as many steps in flight as shared memory holds, up to 6
+  static constexpr int kKvBytes = 16 * HD * (kWide ? 1 : 2);
+  static constexpr int kStep = 2 * kKvBytes + (kWide ? 128 : 0);
+  static constexpr int kFit = (227 * 1024 - kJoin) / (kWarps * kStep);
+  static constexpr int kStages = kFit < 6 ? kFit : 6;
+  static constexpr int kSmem = kWarps * kStages * kStep + kJoin;
 };
 
-constexpr int kUnit = 128;  // keys of a unit: one step of each warp
-
-template <int FMT, int HD>
-__global__ void __launch_bounds__(256, 1)
-    text_rows_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                          TextAttnParams p, int min_units) {
-  using G = RowsGeom<FMT, HD>;
+template <int FMT, int HD, int NT>
+__global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
+    text_rows_attn_kernel(const uint8_t* __restrict__ k_base, const uint8_t* __restrict__ v_base, int64_t k_stride,
+                          int64_t v_stride, TextAttnParams p, int min_units) {
+  using G = RowsGeom<FMT, HD, NT>;
   constexpr bool kW = G::kWide;
+  constexpr int kWarps = G::kWarps, kRows = G::kRows, kU = G::kUnits16;
+  constexpr int kMT = HD / 16;                 // 16-column tiles of O^T
+  constexpr int kRowBytes = kW ? HD : HD * 2;
   constexpr int kD = G::kStages;
-  constexpr int kNB = HD / 8;  // 8-column blocks of the output
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t sbase = smem_u32(smem);
+  extern __shared__ uint4 smem_raw[];          // [warp][stage][step]
+  // [warp][row][pitch], then [warp][row](maximum, denominator)
+  float* join = reinterpret_cast<float*>(smem_raw) + kWarps * kD * G::kStep / 4;
+  float* join_ml = join + kWarps * kRows * G::kPitch;
+  int* last_flag = reinterpret_cast<int*>(join_ml + kWarps * kRows * 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
-  float* join = reinterpret_cast<float*>(smem + G::kRing + G::kScales);
-  float* join_ml = join + G::kWarps * 16 * G::kPitch;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kRing + G::kScales + G::kJoin);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + G::kWarps * kD);
-  int* last_flag = const_cast<int*>(abort_flag) + 1;
-  auto stage = [&](int s) { return sbase + (uint32_t)((warp * kD + s) * G::kStepBytes); };
-  auto sscale = [&](int s) { return sbase + G::kRing + (uint32_t)((warp * kD + s) * 128); };
-  auto bar = [&](int s) { return smem_u32(bars + warp * kD + s); };
+  const uint32_t ring = smem_u32(smem_raw) + (uint32_t)(warp * kD * G::kStep);
 
-  if (lane == 0)
-    for (int s = 0; s < kD; ++s) mbar_init(bar(s), 1);
-  if (threadIdx.x == 0) *abort_flag = 0;
-  fence_mbar_init();
-  fence_proxy_async_smem();
-  __syncthreads();
-
-  // ---- the line of units, walked 32 sequences at a time by each warp for itself
-  auto seq_units = [&](int b, int& items) -> int64_t {
-    items = 0;
-    if (b >= p.batch) return 0;
+  // ---- the line of units, walked 32 sequences at a time by each warp for itself (32-bit
+  // arithmetic: 64-bit divisions were most of a short call's start)
+  auto line_of = [&](int b, unsigned& items, unsigned& nu, int& k16) {
+    items = nu = 0;
+    k16 = 0;
+    if (b >= p.batch) return;
     const Seq s = load_seq(p, b);
-    const int rt = (int)(((int64_t)s.lq * p.group + 15) / 16);
-    items = rt * p.hkv;
-    const int k16 = key_lo(p, s, 0) & ~15;
-    return (int64_t)items * max(1, (s.lk - k16 + kUnit - 1) / kUnit);
+    k16 = key_lo(p, s, 0) & ~15;
+    items = ((unsigned)(s.lq * p.group) + kRows - 1) / kRows * (unsigned)p.hkv;
+    nu = (unsigned)max(1, (s.lk - k16 + kUnit - 1) / kUnit);
   };
-  int64_t total = 0;
+  unsigned my_items = 0, my_nu = 0, total = 0;  // of sequence loaded + lane
+  int my_k16 = 0, loaded = -1;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    int it;
-    int64_t n = seq_units(b0 + lane, it);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    total += n;
+    line_of(b0 + lane, my_items, my_nu, my_k16);
+    loaded = b0;
+    total += __reduce_add_sync(0xffffffffu, my_items * my_nu);
   }
-  const int64_t per = max64(min_units, (total + gridDim.x - 1) / gridDim.x);
-  int64_t u = (int64_t)blockIdx.x * per;
-  const int64_t u_end = min64(total, u + per);
+  const unsigned per = max((unsigned)min_units, (total + gridDim.x - 1) / gridDim.x);
+  unsigned u = min(total, blockIdx.x * per);
+  const unsigned u_end = min(total, u + per);
 
-  // sequence group being walked: units and items before it
-  int wb = 0;
-  int64_t wu = 0;
-  int wi = 0;
+  int wb = 0;               // sequences before wb hold
+  unsigned wu = 0, wi = 0;  // this many units and items
   struct Piece {
     Seq s;
-    int b, h, rt, item;
-    int k_lo, k_hi;          // keys of this piece (k_lo a multiple of 16)
-    int64_t item_u0;         // the item's first unit, and its units
-    int nu;
-    int steps;               // 16-key steps of this piece for this warp
+    int b, h, rt;
+    unsigned item, item_u0, nu;  // the item, its first unit and its units
+    int k_lo, k_hi;              // keys of this piece (k_lo a multiple of 16)
+    int steps;                   // 16-key steps of this piece for this warp
   };
-  auto piece_at = [&](int64_t at, Piece& c) {
+  auto piece_at = [&](unsigned at, Piece& c) -> unsigned {
     while (true) {
-      int it;
-      const int64_t n = seq_units(wb + lane, it);
-      int64_t nc = n;
-      int ic = it;
+      if (loaded != wb) {
+        line_of(wb + lane, my_items, my_nu, my_k16);
+        loaded = wb;
+      }
+      const unsigned n = my_items * my_nu;
+      unsigned nc = n, ic = my_items;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t a = __shfl_up_sync(0xffffffffu, nc, o);
-        const int e = __shfl_up_sync(0xffffffffu, ic, o);
+        const unsigned a = __shfl_up_sync(0xffffffffu, nc, o), e = __shfl_up_sync(0xffffffffu, ic, o);
         if (lane >= o) {
           nc += a;
           ic += e;
         }
       }
-      const int64_t group_units = __shfl_sync(0xffffffffu, nc, 31);
-      if (at < wu + group_units) {
+      const unsigned all = __shfl_sync(0xffffffffu, nc, 31);
+      if (at < wu + all) {
         const int src = __ffs(__ballot_sync(0xffffffffu, at < wu + nc)) - 1;
         c.b = wb + src;
-        const int64_t b_u0 = wu + __shfl_sync(0xffffffffu, nc - n, src);
-        const int b_i0 = wi + __shfl_sync(0xffffffffu, ic - it, src);
+        const unsigned b_u0 = wu + __shfl_sync(0xffffffffu, nc - n, src);
+        const unsigned b_i0 = wi + __shfl_sync(0xffffffffu, ic - my_items, src);
         c.s = load_seq(p, c.b);
-        const int rts = (int)(((int64_t)c.s.lq * p.group + 15) / 16);
-        const int k16 = key_lo(p, c.s, 0) & ~15;
-        c.nu = max(1, (c.s.lk - k16 + kUnit - 1) / kUnit);
-        const int64_t in_b = at - b_u0;
-        const int i = (int)(in_b / c.nu);
-        const int u_in = (int)(in_b % c.nu);
-        c.h = i / rts;
-        c.rt = i % rts;
+        const unsigned rts = __shfl_sync(0xffffffffu, my_items, src) / (unsigned)p.hkv;
+        c.nu = __shfl_sync(0xffffffffu, my_nu, src);
+        const int k16 = __shfl_sync(0xffffffffu, my_k16, src);
+        const unsigned i = (at - b_u0) / c.nu, u_in = (at - b_u0) - i * c.nu;
+        c.h = (int)(i / rts);
+        c.rt = (int)(i % rts);
         c.item = b_i0 + i;
-        c.item_u0 = b_u0 + (int64_t)i * c.nu;
-        const int u_stop = (int)min64(c.nu, u_in + (u_end - at));
-        c.k_lo = k16 + u_in * kUnit;
-        c.k_hi = min(c.s.lk, k16 + u_stop * kUnit);
+        c.item_u0 = b_u0 + i * c.nu;
+        const unsigned units = min(c.nu - u_in, u_end - at);
+        c.k_lo = k16 + (int)u_in * kUnit;
+        c.k_hi = min(c.s.lk, c.k_lo + (int)units * kUnit);
         const int n16 = max(0, (c.k_hi - c.k_lo + 15) / 16);
-        c.steps = n16 > warp ? (n16 - warp + 7) / 8 : 0;
-        return u_stop - u_in;
+        c.steps = n16 > warp ? (n16 - warp + kWarps - 1) / kWarps : 0;
+        return units;
       }
-      wu += group_units;
+      wu += all;
       wi += __shfl_sync(0xffffffffu, ic, 31);
       wb += 32;
     }
   };
 
-  // ---- loads: step i of this warp starts at key k_lo + (i * 8 + warp) * 16; the pages of 32
+  // ---- loads: step i of this warp starts at key k_lo + (i * kWarps + warp) * 16; the pages of 32
   // consecutive steps are fetched at once, one per lane
-  uint32_t issued = 0, used = 0;  // steps loaded / consumed so far
-  bool ok = true;
   int page_of = 0;
-  auto load_step = [&](const Piece& c, int i) {
-    const int j0 = c.k_lo + (i * 8 + warp) * 16;
-    int row, x = 0;
-    if (p.block_table) {
-      if ((i & 31) == 0) {
-        const int jl = c.k_lo + ((i + lane) * 8 + warp) * 16;
-        page_of = 0;
-        if (jl < c.k_hi) {
-          page_of = p.block_table[c.b * p.blocks_per_seq + (jl >> p.page_shift)];
-          if (page_of < 0 || page_of >= p.pages) {
-            set_dev_error(p.err, kDevBadArgs);
-            page_of = 0;
-          }
+  auto first_key = [&](const Piece& c, int i) { return c.k_lo + (i * kWarps + warp) * 16; };
+  // row of the step's first key: of the cache, or of the packed keys
+  auto step_row = [&](const Piece& c, int i) -> int64_t {
+    const int j0 = first_key(c, i);
+    if (!p.block_table) return c.s.k0 + j0;
+    if ((i & 31) == 0) {
+      const int jl = first_key(c, i + lane);
+      page_of = 0;
+      if (jl < c.k_hi) {
+        page_of = p.block_table[c.b * p.blocks_per_seq + (jl >> p.page_shift)];
+        if (page_of < 0 || page_of >= p.pages) {
+          set_dev_error(p.err, kDevBadArgs);
+          page_of = 0;
         }
       }
-      const int page = __shfl_sync(0xffffffffu, page_of, i & 31);
-      row = (int)((((int64_t)page * p.hkv + c.h) << p.page_shift) | (j0 & ((1 << p.page_shift) - 1)));
-    } else {
-      row = (int)(c.s.k0 + j0);
-      x = c.h * HD;
     }
-    if (lane == 0) {
-      const int s = issued % kD;
-      mbar_arrive_expect_tx(bar(s), G::kStepBytes + (kW ? 128 : 0));
+    const int page = __shfl_sync(0xffffffffu, page_of, i & 31);
+    return (((int64_t)page * p.hkv + c.h) << p.page_shift) | (j0 & ((1 << p.page_shift) - 1));
+  };
+  // A step's rows are copied whole, 16 bytes a lane, the lanes of a copy side by side in memory. Their
+  // 16-byte units are swizzled such that the eight lanes of a read's phase, two rows of K by four
+  // units or four even rows of V by two, meet eight groups of banks. One group of copies per step; steps that a
+  // piece does not have are empty groups. (packed keys: rows past the sequence's last are not read,
+  // the last one stands in; a page is whole)
+  constexpr int kRU = kRowBytes / 16;   // units of a row
+  constexpr int kVN = kW ? 1 : HD / 64; // V units of a row that a lane reads
+  auto k_swz = [](int row) { return kRU == 4 ? 0 : (row & 1) << 2; };
+  auto v_swz = [](int row) { return kRU == 4 ? (row >> 1) & 3 : row & 6; };
+  auto load_step = [&](const Piece& c, int i, uint32_t stage) {
+    if (i < c.steps) {
+      const int64_t row = step_row(c, i);
+      const int left = p.block_table ? 15 : c.s.lk - 1 - first_key(c, i);
+      const int64_t col = (p.block_table ? 0 : (int64_t)c.h * kRowBytes) + lane % kRU * 16;
+      const uint8_t* kb = k_base + row * k_stride + col;
+      const uint8_t* vb = v_base + row * v_stride + col;
 #pragma unroll
-      for (int ch = 0; ch < G::kTiles; ++ch) {
-        tma_load_2d(stage(s) + ch * G::kTileBytes, &tmK, bar(s), x + ch * 64, row);
-        tma_load_2d(stage(s) + G::kKvBytes + ch * G::kTileBytes, &tmV, bar(s), x + ch * 64, row);
+      for (int x = 0; x < kRU / 2; ++x) {
+        const int r = x * (32 / kRU) + lane / kRU;
+        copy_async16(stage + (r * kRU + (lane % kRU ^ k_swz(r))) * 16, kb + (int64_t)min(r, left) * k_stride);
       }
-      if constexpr (kW) {
-        bulk_load(sscale(s), p.ks + row, 64, bar(s));
-        bulk_load(sscale(s) + 64, p.vs + row, 64, bar(s));
+#pragma unroll
+      for (int x = 0; x < kRU / 2; ++x) {
+        const int r = x * (32 / kRU) + lane / kRU;
+        copy_async16(stage + G::kKvBytes + (r * kRU + (lane % kRU ^ v_swz(r))) * 16,
+                     vb + (int64_t)min(r, left) * v_stride);
       }
+      if constexpr (kW)  // keys' scales, then values'
+        copy_async4(stage + 2 * G::kKvBytes + lane * 4, (lane < 16 ? p.ks : p.vs) + row + (lane & 15));
     }
-    ++issued;
+    copy_async_commit();
   };
-
-  // dealing of keys to fragment columns and of 16-byte chunks to lane groups
-  auto kp = [](int n) { return (kW && HD == 64) ? n : (n >> 1) | ((n & 1) << 2); };
-  auto swz = [](int row, int chunk) {  // byte offset of a 16-byte chunk in a swizzled box
-    return (kW && HD == 64) ? (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4))
-                            : (uint32_t)(row * 128 + ((chunk ^ (row & 7)) << 4));
+  struct Values {
+    uint4 v[4][kVN];
   };
-  // head column of output block j, fragment column n
-  auto out_dim = [&](int j, int n) {
-    if constexpr (!kW) return (j >> 3) * 64 + kp(n) * 8 + (j & 7);
-    else if constexpr (HD == 128) return kp(n) * 16 + j;
-    else return n * 8 + j;
+  auto word = [](const uint4& x, int i) -> uint32_t { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; };
+  // bf16 pair (keys of rows ra and rb) of this lane's d-th head column
+  auto value_pair = [&](const Values& f, int ra, int rb, int d) -> uint32_t {
+    if constexpr (kW)
+      return bytes_to_bf16x2<FMT>(word(f.v[ra][0], d >> 2), word(f.v[rb][0], d >> 2), d & 3, 4 + (d & 3));
+    else
+      return __byte_perm(word(f.v[ra][d >> 3], (d & 7) >> 1), word(f.v[rb][d >> 3], (d & 7) >> 1), d & 1 ? 0x7632 : 0x5410);
   };
+  // head column of this lane's d-th: the units of lane group g
+  auto column = [&](int d) { return kW ? g * (HD / 8) + d : (d >> 3) * 64 + g * 8 + (d & 7); };
 
   Piece cur;
+  uint32_t at_stage = 0;  // stage of the next step to be worked on
+  auto next_stage = [&](uint32_t x) { return x + 1 == (uint32_t)kD ? 0u : x + 1; };
+  auto first_loads = [&](const Piece& c) {
+    uint32_t to = at_stage;
+#pragma unroll
+    for (int i = 0; i < kD; ++i, to = next_stage(to)) load_step(c, i, ring + to * G::kStep);
+  };
   bool have = u < u_end;
-  int units = 0;
+  unsigned units = 0;
   if (have) {
     units = piece_at(u, cur);
-    for (int i = 0; i < kD && i < cur.steps; ++i) load_step(cur, i);
+    first_loads(cur);
   }
   while (have) {
-    const int64_t n_rows = (int64_t)cur.s.lq * p.group;
-    const int row0 = cur.rt * 16;
-    // ---- q fragments: rows g and g + 8, columns in the order of the K reads
-    uint32_t qf[HD / 16][4];
-    int lim_hi[2], lim_lo[2];
+    const int n_rows = cur.s.lq * p.group;
+    const int row0 = cur.rt * kRows;
+    // ---- q fragments: row 8 n + g, columns in the order of the K reads; the limits of rows 2t, 2t+1
+    uint32_t qf[NT][HD / 16][2];
+    int lim_hi[NT][2], lim_lo[NT][2];
 #pragma unroll
-    for (int hrow = 0; hrow < 2; ++hrow) {
-      const int r = row0 + g + 8 * hrow;
+    for (int n = 0; n < NT; ++n) {
+      const int r = row0 + 8 * n + g;
       const bool live = r < n_rows;
-      const int tok = live ? r / p.group : 0;
-      const int head = cur.h * p.group + (live ? r % p.group : 0);
-      lim_hi[hrow] = live ? key_hi(p, cur.s, tok) : 0;
-      lim_lo[hrow] = live ? key_lo(p, cur.s, tok) : 0;
-      const __nv_bfloat16* src = p.q + (cur.s.q0 + tok) * p.q_stride + (int64_t)head * HD;
-      if constexpr (!kW) {
+      const int tok = live ? (int)((unsigned)r / (unsigned)p.group) : 0;
+      const __nv_bfloat16* src = p.q + (cur.s.q0 + tok) * p.q_stride +
+                                 (int64_t)(cur.h * p.group + (live ? r - tok * p.group : 0)) * HD;
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (live) w = *reinterpret_cast<const uint4*>(src + (i >> 1) * 64 + ((i & 1) * 4 + t) * 8);
-          qf[2 * i][hrow] = w.x;
-          qf[2 * i][2 + hrow] = w.y;
-          qf[2 * i + 1][hrow] = w.z;
-          qf[2 * i + 1][2 + hrow] = w.w;
-        }
-      } else {
+      for (int i = 0; i < HD / 32; ++i) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (live)
+          w = __ldg(reinterpret_cast<const uint4*>(src + (kW ? (i >> 1) * 64 + t * 16 + (i & 1) * 8 : i * 32 + t * 8)));
+        qf[n][2 * i][0] = w.x;
+        qf[n][2 * i][1] = w.y;
+        qf[n][2 * i + 1][0] = w.z;
+        qf[n][2 * i + 1][1] = w.w;
+      }
 #pragma unroll
-        for (int i = 0; i < HD / 64; ++i) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (live) w = *reinterpret_cast<const uint4*>(src + i * 64 + t * 16 + e * 8);
-            qf[4 * i + 2 * e][hrow] = w.x;
-            qf[4 * i + 2 * e][2 + hrow] = w.y;
-            qf[4 * i + 2 * e + 1][hrow] = w.z;
-            qf[4 * i + 2 * e + 1][2 + hrow] = w.w;
-          }
-        }
+      for (int e = 0; e < 2; ++e) {
+        const int rr = row0 + 8 * n + 2 * t + e;
+        const bool here = rr < n_rows;
+        const int tk = here ? (int)((unsigned)rr / (unsigned)p.group) : 0;
+        lim_hi[n][e] = here ? key_hi(p, cur.s, tk) : 0;
+        lim_lo[n][e] = here ? key_lo(p, cur.s, tk) : 0;
       }
     }
     // a step between these sees no mask in any row of the tile
-    const int last_tok = (int)(min64(n_rows - 1, row0 + 15) / p.group);
-    const int free_hi = key_hi(p, cur.s, row0 / p.group);
+    const int last_tok = (int)((unsigned)(min(n_rows, row0 + kRows) - 1) / (unsigned)p.group);
+    const int free_hi = key_hi(p, cur.s, (int)((unsigned)row0 / (unsigned)p.group));
     const int free_lo = key_lo(p, cur.s, last_tok);
 
-    float acc[kNB][4];
+    float acc[NT][kMT][4];
 #pragma unroll
-    for (int j = 0; j < kNB; ++j)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int j = 0; j < kMT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][j][i] = 0.f;
+    float m[NT][2], l[NT][2];  // of rows 8 n + 2t + e; l: this lane's keys only
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+      }
 
-    for (int i = 0; i < cur.steps; ++i) {
-      const int s = used % kD;
-      const int j0 = cur.k_lo + (i * 8 + warp) * 16;
-      if (ok && !mbar_wait(bar(s), (used / kD) & 1, p.err, kDevTimeoutFull, abort_flag)) ok = false;
-      if (!ok) break;
-      const uint32_t sk = stage(s), sv = stage(s) + G::kKvBytes;
-      float sc[2][4];
+    for (int i = 0; i < cur.steps; ++i, at_stage = next_stage(at_stage)) {
+      const uint32_t stage = ring + at_stage * G::kStep;
+      copy_async_wait<kD - 1>();
+      __syncwarp();
+      const int j0 = first_key(cur, i);
+      const bool masked = j0 + 16 > free_hi || j0 < free_lo;
+      float sc[NT][4];
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nb][e] = 0.f;
-        const int row = nb * 8 + kp(g);
-        if constexpr (!kW) {
+        for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
 #pragma unroll
-          for (int c = 0; c < HD / 32; ++c) {
-            const uint4 w = lds128(sk + (c >> 1) * G::kTileBytes + swz(row, (c & 1) * 4 + t));
-            mma_bf16(sc[nb], qf[2 * c], w.x, w.y);
-            mma_bf16(sc[nb], qf[2 * c + 1], w.z, w.w);
+      for (int c = 0; c < kU; ++c) {
+        const uint32_t at = stage + (g * kRU + (c * 4 + t ^ k_swz(g))) * 16;
+        const uint4 kx = lds128(at), ky = lds128(at + 8 * kRowBytes);
+        if constexpr (kW) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = word(kx, e), y = word(ky, e);
+            const uint32_t a0 = bytes_to_bf16x2<FMT>(x, 0, 0, 1), a1 = bytes_to_bf16x2<FMT>(y, 0, 0, 1);
+            const uint32_t a2 = bytes_to_bf16x2<FMT>(x, 0, 2, 3), a3 = bytes_to_bf16x2<FMT>(y, 0, 2, 3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(sc[n], a0, a1, a2, a3, qf[n][4 * c + e][0], qf[n][4 * c + e][1]);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < HD / 64; ++c) {
-            const uint4 w = lds128(sk + swz(row, c * 4 + t));
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          for (int n = 0; n < NT; ++n) mma_bf16(sc[n], kx.x, ky.x, kx.y, ky.y, qf[n][2 * c][0], qf[n][2 * c][1]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              mma_bf16(sc[nb], qf[4 * c + e], bytes_to_bf16x2<FMT>(ww[e], 0, 0, 1),
-                       bytes_to_bf16x2<FMT>(ww[e], 0, 2, 3));
-          }
+          for (int n = 0; n < NT; ++n) mma_bf16(sc[n], kx.z, ky.z, kx.w, ky.w, qf[n][2 * c + 1][0], qf[n][2 * c + 1][1]);
         }
       }
-      // scores in base 2, scaled, masked; key of column e of block nb
-      const bool masked = j0 + 16 > free_hi || j0 < free_lo;
-      float vscale[2][2];
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb)
+      float f[2] = {p.sl2, p.sl2}, vs[2] = {1.f, 1.f};  // of keys g and g + 8
+      if constexpr (kW) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int kk = nb * 8 + kp(2 * t + e);
-          float f = p.sl2;
-          vscale[nb][e] = 1.f;
-          if constexpr (kW) {
-            f *= lds_f32(sscale(s) + kk * 4);
-            vscale[nb][e] = lds_f32(sscale(s) + 64 + kk * 4);
-          }
-          sc[nb][e] *= f;
-          sc[nb][2 + e] *= f;
-          if (masked) {
-            const int j = j0 + kk;
+          f[e] *= lds_f32(stage + 2 * G::kKvBytes + (e * 8 + g) * 4);
+          vs[e] = lds_f32(stage + 2 * G::kKvBytes + 64 + (e * 8 + g) * 4);
+        }
+      }
+      uint32_t pb[NT][2];
 #pragma unroll
-            for (int hrow = 0; hrow < 2; ++hrow)
-              if (j >= lim_hi[hrow] || j < lim_lo[hrow]) sc[nb][2 * hrow + e] = -INFINITY;
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sc[n][q] *= f[q >> 1];
+        if (masked) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int j = j0 + g + 8 * (q >> 1);
+            if (j >= lim_hi[n][q & 1] || j < lim_lo[n][q & 1]) sc[n][q] = -INFINITY;
           }
         }
-      float alpha[2];
-#pragma unroll
-      for (int hrow = 0; hrow < 2; ++hrow) {
-        float mx = fmaxf(fmaxf(sc[0][2 * hrow], sc[0][2 * hrow + 1]), fmaxf(sc[1][2 * hrow], sc[1][2 * hrow + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[hrow], mx);
-        const float mu = mn == -INFINITY ? 0.f : mn;
-        alpha[hrow] = exp2_approx(m[hrow] - mu);
-        m[hrow] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
+        // The maximum is moved only when it has grown by 2^8: most steps leave O^T alone and take no
+        // more than a vote, and the weights stay below 2^8, far from fp32's and bf16's range
+        const float mx[2] = {fmaxf(sc[n][0], sc[n][2]), fmaxf(sc[n][1], sc[n][3])};
+        auto grown = [&](int e) { return mx[e] > m[n][e] + 8.f || (m[n][e] == -INFINITY && mx[e] > -INFINITY); };
+        if (__any_sync(0xffffffffu, grown(0) || grown(1))) {
+          float alpha[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float& x = sc[nb][2 * hrow + e];
-            const bool off = x == -INFINITY;
-            x = exp2_approx(x - mu);
-            sum += x;
-            // a masked key's scale may be anything: its weight is 0, not 0 * scale
-            if constexpr (kW) x = off ? 0.f : x * vscale[nb][e];
+            float x = mx[e];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            x = fmaxf(x, m[n][e]);
+            alpha[e] = x == -INFINITY ? 1.f : exp2_approx(m[n][e] - x);
+            m[n][e] = x;
+            l[n][e] *= alpha[e];
           }
-        l[hrow] = l[hrow] * alpha[hrow] + sum;
-      }
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-        for (int j = 0; j < kNB; ++j) {
-          acc[j][0] *= alpha[0];
-          acc[j][1] *= alpha[0];
-          acc[j][2] *= alpha[1];
-          acc[j][3] *= alpha[1];
+          for (int j = 0; j < kMT; ++j) {
+            acc[n][j][0] *= alpha[0];
+            acc[n][j][1] *= alpha[1];
+            acc[n][j][2] *= alpha[0];
+            acc[n][j][3] *= alpha[1];
+          }
         }
-      }
-      // P rounded to bf16 for the tensor product (the denominator sums the unrounded values)
-      const uint32_t pf[4] = {pack_bf16x2(sc[0][0], sc[0][1]), pack_bf16x2(sc[0][2], sc[0][3]),
-                              pack_bf16x2(sc[1][0], sc[1][1]), pack_bf16x2(sc[1][2], sc[1][3])};
-      const int vr[4] = {kp(2 * t), kp(2 * t + 1), 8 + kp(2 * t), 8 + kp(2 * t + 1)};
-      if constexpr (!kW) {
-        bool slow = false;
 #pragma unroll
-        for (int c = 0; c < G::kTiles; ++c) {
-          uint32_t w[4][4];
+        for (int e = 0; e < 2; ++e) {
+          const float mu = m[n][e] == -INFINITY ? 0.f : m[n][e];
+          const bool off0 = sc[n][e] == -INFINITY, off1 = sc[n][2 + e] == -INFINITY;
+          const float x0 = exp2_approx(sc[n][e] - mu), x1 = exp2_approx(sc[n][2 + e] - mu);
+          l[n][e] += x0 + x1;
+          // an unseen key's scale may be anything: its weight is 0, not 0 * scale
+          sc[n][e] = kW && off0 ? 0.f : x0 * vs[0];
+          sc[n][2 + e] = kW && off1 ? 0.f : x1 * vs[1];
+        }
+        // P rounded to bf16 for the tensor product (the denominator sums the unrounded values)
+        pb[n][0] = transpose_8x8(pack_bf16x2(sc[n][0], sc[n][1]));
+        pb[n][1] = transpose_8x8(pack_bf16x2(sc[n][2], sc[n][3]));
+      }
+      Values vf;
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+        for (int e = 0; e < kVN; ++e) {
+          const int r = 2 * t + (rr & 1) + (rr >> 1) * 8;
+          const uint32_t at = stage + G::kKvBytes + r * kRowBytes;
+          if constexpr (kRU > 4) {
+            vf.v[rr][e] = lds128(at + ((e * 8 + g) ^ v_swz(r)) * 16);
+          } else {
+            const uint2 x = lds64(at + ((g >> 1) ^ v_swz(r)) * 16 + (g & 1) * 8);
+            vf.v[rr][e] = make_uint4(x.x, x.y, 0, 0);
+          }
+        }
+      bool slow = false;
+      if constexpr (!kW) {
+        if (masked) {
+          // 0 * NaN is NaN: keys past the end are zeroed; with a non-finite value at a key that only
+          // some rows see, this step's products go by scalar sums
+          bool odd = false;
 #pragma unroll
           for (int rr = 0; rr < 4; ++rr) {
-            const uint4 x = lds128(sv + c * G::kTileBytes + swz(vr[rr], kp(g)));
-            w[rr][0] = x.x;
-            w[rr][1] = x.y;
-            w[rr][2] = x.z;
-            w[rr][3] = x.w;
-          }
-          if (masked) {
-            // keys past the end are another sequence's or nobody's: zero them (0 * NaN is NaN).
-            // A non-finite value at a key that only some rows see: the whole step goes by
-            // scalar sums below.
-            bool odd = false;
+            const bool past = j0 + 2 * t + (rr & 1) + (rr >> 1) * 8 >= cur.s.lk;
 #pragma unroll
-            for (int rr = 0; rr < 4; ++rr)
+            for (int e = 0; e < HD / 64; ++e) {
+              if (past) vf.v[rr][e] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if (j0 + vr[rr] >= cur.s.lk) w[rr][e] = 0;
-                odd |= (w[rr][e] & 0x7f80u) == 0x7f80u || (w[rr][e] & 0x7f800000u) == 0x7f800000u;
+              for (int q = 0; q < 4; ++q) {
+                const uint32_t x = word(vf.v[rr][e], q);
+                odd |= (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u;
               }
-            if (c == 0) {
-              // (both halves are checked before the first product)
-              if constexpr (G::kTiles == 2) {
+            }
+          }
+          slow = __any_sync(0xffffffffu, odd);
+          if (slow) {
+#pragma unroll 1
+            for (int kk = 0; kk < 16; ++kk) {
+              const int from = g * 4 + ((kk & 7) >> 1), rr = (kk & 1) + 2 * (kk >> 3);
+              const int j = j0 + kk;
 #pragma unroll
-                for (int rr = 0; rr < 4; ++rr) {
-                  const uint4 x = lds128(sv + G::kTileBytes + swz(vr[rr], kp(g)));
-                  const uint32_t y[4] = {x.x, x.y, x.z, x.w};
+              for (int n = 0; n < NT; ++n) {
+                float w[2];
 #pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    odd |= j0 + vr[rr] < cur.s.lk &&
-                           ((y[e] & 0x7f80u) == 0x7f80u || (y[e] & 0x7f800000u) == 0x7f800000u);
+                for (int e = 0; e < 2; ++e)
+                  w[e] = round_bf16(__shfl_sync(0xffffffffu, kk < 8 ? sc[n][e] : sc[n][2 + e], (kk & 7) * 4 + t));
+#pragma unroll
+                for (int d = 0; d < HD / 8; ++d) {
+                  uint32_t mine = 0;
+#pragma unroll
+                  for (int q = 0; q < 4; ++q)
+                    if (q == rr) mine = word(vf.v[q][d >> 3], (d & 7) >> 1);
+                  // (every lane offers its row rr; the wanted key is that of lane `from`)
+                  const uint32_t x = __shfl_sync(0xffffffffu, mine, from);
+                  const float v = d & 1 ? bf16_hi(x) : bf16_lo(x);
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (j < lim_hi[n][e] && j >= lim_lo[n][e]) acc[n][d >> 1][2 * (d & 1) + e] += w[e] * v;
                 }
               }
-              slow = __any_sync(0xffffffffu, odd);
             }
-            if (slow) break;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            mma_bf16(acc[c * 8 + 2 * e], pf, __byte_perm(w[0][e], w[1][e], 0x5410),
-                     __byte_perm(w[2][e], w[3][e], 0x5410));
-            mma_bf16(acc[c * 8 + 2 * e + 1], pf, __byte_perm(w[0][e], w[1][e], 0x7632),
-                     __byte_perm(w[2][e], w[3][e], 0x7632));
           }
         }
-        if (slow) {
-#pragma unroll 1
-          for (int kk = 0; kk < 16; ++kk) {
-            const int n = ((kk & 3) << 1) | ((kk & 7) >> 2);  // fragment column that holds this key
-            const int src = (lane & ~3) | (n >> 1);
-            const float a0 = kk < 8 ? ((n & 1) ? sc[0][1] : sc[0][0]) : ((n & 1) ? sc[1][1] : sc[1][0]);
-            const float a1 = kk < 8 ? ((n & 1) ? sc[0][3] : sc[0][2]) : ((n & 1) ? sc[1][3] : sc[1][2]);
-            const float p0 = round_bf16(__shfl_sync(0xffffffffu, a0, src));
-            const float p1 = round_bf16(__shfl_sync(0xffffffffu, a1, src));
-            const int j = j0 + kk;
-            const bool see0 = j < lim_hi[0] && j >= lim_lo[0], see1 = j < lim_hi[1] && j >= lim_lo[1];
-#pragma unroll
-            for (int jb = 0; jb < kNB; ++jb)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int chunk = kp(2 * t + e);
-                const float v = __uint_as_float(
-                    lds_u16(sv + (jb >> 3) * G::kTileBytes + swz(kk, chunk) + (uint32_t)(jb & 7) * 2) << 16);
-                if (see0) acc[jb][e] += p0 * v;
-                if (see1) acc[jb][2 + e] += p1 * v;
-              }
-          }
-        }
-      } else if constexpr (HD == 128) {
-        uint32_t w[4][4];
-#pragma unroll
-        for (int rr = 0; rr < 4; ++rr) {
-          const uint4 x = lds128(sv + swz(vr[rr], kp(g)));
-          w[rr][0] = x.x;
-          w[rr][1] = x.y;
-          w[rr][2] = x.z;
-          w[rr][3] = x.w;
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          mma_bf16(acc[j], pf, bytes_to_bf16x2<FMT>(w[0][j >> 2], w[1][j >> 2], j & 3, 4 + (j & 3)),
-                   bytes_to_bf16x2<FMT>(w[2][j >> 2], w[3][j >> 2], j & 3, 4 + (j & 3)));
-      } else {
-        uint32_t w[4][2];
-#pragma unroll
-        for (int rr = 0; rr < 4; ++rr) {
-          const uint2 x = lds64(sv + swz(vr[rr], g >> 1) + (uint32_t)(g & 1) * 8);
-          w[rr][0] = x.x;
-          w[rr][1] = x.y;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          mma_bf16(acc[j], pf, bytes_to_bf16x2<FMT>(w[0][j >> 2], w[1][j >> 2], j & 3, 4 + (j & 3)),
-                   bytes_to_bf16x2<FMT>(w[2][j >> 2], w[3][j >> 2], j & 3, 4 + (j & 3)));
       }
-      ++used;
-      __syncwarp();  // every lane has read the stage
-      if (i + kD < cur.steps) load_step(cur, i + kD);
+      if (!slow) {
+#pragma unroll
+        for (int j = 0; j < kMT; ++j) {
+          const uint32_t a0 = value_pair(vf, 0, 1, 2 * j), a1 = value_pair(vf, 0, 1, 2 * j + 1);
+          const uint32_t a2 = value_pair(vf, 2, 3, 2 * j), a3 = value_pair(vf, 2, 3, 2 * j + 1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_bf16(acc[n][j], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+        }
+      }
+      __syncwarp();  // the stage has been read
+      load_step(cur, i + kD, stage);
     }
 
     // ---- the next piece's first loads go out before this one is joined
     const Piece done = cur;
-    const int64_t u_done = u;
+    const unsigned u_done = u;
     u += units;
     have = u < u_end;
     if (have) {
       units = piece_at(u, cur);
-      if (ok)
-        for (int i = 0; i < kD && i < cur.steps; ++i) load_step(cur, i);
+      first_loads(cur);
     }
 
-    // ---- join the eight warps
+    // ---- join the warps
 #pragma unroll
-    for (int hrow = 0; hrow < 2; ++hrow) {
-      l[hrow] += __shfl_xor_sync(0xffffffffu, l[hrow], 1);
-      l[hrow] += __shfl_xor_sync(0xffffffffu, l[hrow], 2);
-      if (t == 0) {
-        join_ml[(warp * 16 + g + 8 * hrow) * 2] = m[hrow];
-        join_ml[(warp * 16 + g + 8 * hrow) * 2 + 1] = l[hrow];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[n][e];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        const int row = warp * kRows + 8 * n + 2 * t + e;
+        if (g == 0) *reinterpret_cast<float2*>(join_ml + row * 2) = make_float2(m[n][e], x);
+        if (done.steps > 0) {
+          float* dst = join + row * G::kPitch;
+#pragma unroll
+          for (int d = 0; d < HD / 8; d += 4)
+            *reinterpret_cast<float4*>(dst + column(d)) =
+                make_float4(acc[n][d >> 1][e], acc[n][d >> 1][2 + e], acc[n][(d >> 1) + 1][e], acc[n][(d >> 1) + 1][2 + e]);
+        }
       }
-    }
-    if (done.steps > 0) {
-#pragma unroll
-      for (int j = 0; j < kNB; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          join[(warp * 16 + g + 8 * (e >> 1)) * G::kPitch + out_dim(j, 2 * t + (e & 1))] = acc[j][e];
-    }
     __syncthreads();
-    constexpr int kPer = HD / 16;  // columns of a thread
-    const int jr = threadIdx.x >> 4, jc = (threadIdx.x & 15) * kPer;
-    float M = -INFINITY, L = 0.f, o[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) M = fmaxf(M, join_ml[(w * 16 + jr) * 2]);
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const float lw = join_ml[(w * 16 + jr) * 2 + 1];
-      if (lw == 0.f) continue;
-      const float f = exp2_approx(join_ml[(w * 16 + jr) * 2] - M);
-      L += lw * f;
-#pragma unroll
-      for (int i = 0; i < kPer; i += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(&join[(w * 16 + jr) * G::kPitch + jc + i]);
-        o[i] += x.x * f;
-        o[i + 1] += x.y * f;
-        o[i + 2] += x.z * f;
-        o[i + 3] += x.w * f;
-      }
-    }
     const bool whole = u_done <= done.item_u0 && u >= done.item_u0 + done.nu;
-    bool write = whole;
-    if (!whole) {
-      // this CTA's piece of an item: slot 0 if the item began in an earlier CTA, 1 if it goes on
-      const int slot = 2 * blockIdx.x + (done.item_u0 >= (int64_t)blockIdx.x * per ? 1 : 0);
-      float* dst = p.part + ((int64_t)slot * 16 + jr) * HD + jc;
+    const unsigned c0 = done.item_u0 / per, c1 = (done.item_u0 + done.nu - 1) / per;  // CTAs of this item
+    constexpr int kPer = HD / 16;  // columns of a thread, 16 threads to a row
+    constexpr int kGroups = 2 * kWarps / kRows;  // groups of threads that cover the rows
+    const int jr = (threadIdx.x >> 4) % kRows, jg = (threadIdx.x >> 4) / kRows, jc = (threadIdx.x & 15) * kPer;
+    float o[kPer] = {};
+    float M = -INFINITY, L = 0.f;
+    auto add = [&](const float4& x, int i, float f) {
+      o[i] += x.x * f;
+      o[i + 1] += x.y * f;
+      o[i + 2] += x.z * f;
+      o[i + 3] += x.w * f;
+    };
+    auto clear = [&]() {
+      M = -INFINITY;
+      L = 0.f;
 #pragma unroll
-      for (int i = 0; i < kPer; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-      if ((threadIdx.x & 15) == 0) {
-        p.part_ml[((int64_t)slot * 16 + jr) * 2] = M;
-        p.part_ml[((int64_t)slot * 16 + jr) * 2 + 1] = L;
-      }
-      __threadfence();
-      __syncthreads();
-      const int c0 = (int)(done.item_u0 / per), c1 = (int)((done.item_u0 + done.nu - 1) / per);
-      if (threadIdx.x == 0) {
-        // (sequences that overlap in cu_q could count more items than there are counters)
-        const bool known = done.item < p.n_items;
-        const int before = known ? atomicAdd(p.counters + done.item, 1) : -1;
-        *last_flag = before == c1 - c0;
-        if (before == c1 - c0) p.counters[done.item] = 0;
-        if (!known) set_dev_error(p.err, kDevBadArgs);
-      }
-      __syncthreads();
-      write = *last_flag != 0;
-      if (write) {
-        __threadfence();
-        M = -INFINITY;
-        L = 0.f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) o[i] = 0.f;
-        for (int c = c0; c <= c1; ++c) {
-          const int sl = 2 * c + (done.item_u0 >= (int64_t)c * per ? 1 : 0);
-          M = fmaxf(M, __ldcg(p.part_ml + ((int64_t)sl * 16 + jr) * 2));
-        }
-        for (int c = c0; c <= c1; ++c) {
-          const int sl = 2 * c + (done.item_u0 >= (int64_t)c * per ? 1 : 0);
-          const float lw = __ldcg(p.part_ml + ((int64_t)sl * 16 + jr) * 2 + 1);
-          if (lw == 0.f) continue;
-          const float f = exp2_approx(__ldcg(p.part_ml + ((int64_t)sl * 16 + jr) * 2) - M);
-          L += lw * f;
-#pragma unroll
-          for (int i = 0; i < kPer; i += 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part + ((int64_t)sl * 16 + jr) * HD + jc + i));
-            o[i] += x.x * f;
-            o[i + 1] += x.y * f;
-            o[i + 2] += x.z * f;
-            o[i + 3] += x.w * f;
-          }
-        }
-      }
-    }
-    const int r = done.rt * 16 + jr;
-    if (write && r < (int64_t)done.s.lq * p.group) {
-      const int64_t tok = done.s.q0 + r / p.group;
-      const int head = done.h * p.group + r % p.group;
+      for (int i = 0; i < kPer; ++i) o[i] = 0.f;
+    };
+    auto write = [&]() {
+      const int r = done.rt * kRows + jr;
+      if (r >= done.s.lq * p.group) return;
+      const int tk = (int)((unsigned)r / (unsigned)p.group);
+      const int64_t tok = done.s.q0 + tk;
+      const int head = done.h * p.group + r - tk * p.group;
       const float inv = L == 0.f ? 0.f : 1.f / L;
       uint32_t w[kPer / 2];
 #pragma unroll
@@ -591,11 +548,101 @@ __global__ void __launch_bounds__(256, 1)
       else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
       if (p.lse && (threadIdx.x & 15) == 0)
         p.lse[tok * p.hq + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    };
+    // partial sums of CTA c for this item: slot 0 if the item began in an earlier CTA, 1 if there
+    auto slot_row = [&](unsigned c, int row) -> int64_t {
+      return (int64_t)(2 * c + (done.item_u0 >= c * per ? 1 : 0)) * kRows + row;
+    };
+    if (jg == 0) {
+      clear();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, join_ml[(w * kRows + jr) * 2]);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 ml = *reinterpret_cast<const float2*>(join_ml + (w * kRows + jr) * 2);
+        if (ml.y == 0.f) continue;
+        const float f = exp2_approx(ml.x - M);
+        L += ml.y * f;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4)
+          add(*reinterpret_cast<const float4*>(join + (w * kRows + jr) * G::kPitch + jc + i), i, f);
+      }
+      if (whole) {
+        write();
+      } else {
+        const int64_t at = slot_row(blockIdx.x, jr);
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4)
+          *reinterpret_cast<float4*>(p.part + at * HD + jc + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        if ((threadIdx.x & 15) == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(M, L);
+      }
+    }
+    if (!whole) {
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        // (sequences that overlap in cu_q could count more items than there are counters)
+        const bool known = (int64_t)done.item < p.n_items;
+        const int before = known ? atomicAdd(p.counters + done.item, 1) : -1;
+        *last_flag = before == (int)(c1 - c0);
+        if (*last_flag) p.counters[done.item] = 0;
+        if (!known) set_dev_error(p.err, kDevBadArgs);
+      }
+      __syncthreads();
+      if (*last_flag) {
+        // All pieces' maxima and denominators at once, then the thread groups share the pieces, four
+        // in flight each: one after the other, the latency of 20 pieces was 11 us of a call.
+        __threadfence();
+        const int n = (int)(c1 - c0) + 1;
+        for (int i = threadIdx.x; i < n * kRows; i += G::kThreads)
+          *reinterpret_cast<float2*>(join + 2 * i) =
+              __ldcg(reinterpret_cast<const float2*>(p.part_ml + slot_row(c0 + i / kRows, i % kRows) * 2));
+        __syncthreads();
+        clear();
+        for (int c = 0; c < n; ++c) M = fmaxf(M, join[2 * (c * kRows + jr)]);
+        for (int c = jg < kGroups ? jg : n; c < n; c += 4 * kGroups) {
+          float4 x[4][kPer / 4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float* src = p.part + slot_row(c0 + min(c + q * kGroups, n - 1), jr) * HD + jc;
+#pragma unroll
+            for (int i = 0; i < kPer / 4; ++i) x[q][i] = __ldcg(reinterpret_cast<const float4*>(src) + i);
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (c + q * kGroups >= n) continue;
+            const float2 ml = *reinterpret_cast<const float2*>(join + 2 * ((c + q * kGroups) * kRows + jr));
+            if (ml.y == 0.f) continue;
+            const float f = exp2_approx(ml.x - M);
+            L += ml.y * f;
+#pragma unroll
+            for (int i = 0; i < kPer; i += 4) add(x[q][i / 4], i, f);
+          }
+        }
+        if constexpr (kGroups > 1) {
+          __syncthreads();
+          float* mine = join + ((jg * kRows + jr) * 16 + (threadIdx.x & 15)) * (kPer + 1);
+          if (jg > 0 && jg < kGroups) {
+            mine[kPer] = L;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) mine[i] = o[i];
+          }
+          __syncthreads();
+          if (jg == 0) {
+#pragma unroll
+            for (int w = 1; w < kGroups; ++w) {
+              const float* src = mine + w * kRows * 16 * (kPer + 1);
+              L += src[kPer];
+#pragma unroll
+              for (int i = 0; i < kPer; ++i) o[i] += src[i];
+            }
+          }
+        }
+        if (jg == 0) write();
+      }
     }
     __syncthreads();  // the join buffer is free again
   }
-  // after a wait that ran out: copies still in flight land before the CTA's memory goes away
-  for (; used < issued; ++used) mbar_drain(bar(used % kD), (used / kD) & 1);
 }
 
 // --------------------------------------------------------------------- host side
@@ -638,45 +685,48 @@ static void fill_params(wx_ctx* ctx, const wx_attn_dims* d, const void* q, int64
   p.err = ctx->dev_err;
 }
 
-template <int FMT, int HD>
+template <int FMT, int HD, int NT>
 static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
-  using G = RowsGeom<FMT, HD>;
-  const int grid = ctx->num_sms;
-  const int64_t items = (int64_t)p.hkv * (p.total_q * p.group / 16 + p.batch);
-  CUtensorMap tk, tv;
+  using G = RowsGeom<FMT, HD, NT>;
+  const int grid = std::min(ctx->num_sms, G::kWarps * (G::kPitch + 2) / 2);  // (an item's pieces: the join buffer)
+  const int64_t items = (int64_t)p.hkv * (p.total_q * p.group / G::kRows + p.batch);
+  // the line of units is counted in 32 bits (only block tables that repeat pages get near)
+  if (p.block_table && items > UINT32_MAX / ((p.blocks_per_seq << p.page_shift) / kUnit + 1))
+    return set_error(ctx, WX_ERR_UNSUPPORTED, "batch * kv_heads * blocks_per_seq too large (2^32 units of 128 keys)");
+  const size_t rows = (size_t)grid * 2 * G::kRows;
   int st;
-  if (FMT == kKvBf16) {
-    if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, 16))) return st;
-    if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, 16))) return st;
-  } else {
-    if ((st = make_tmap_u8_rows(ctx, &tk, kv.k, kv.rows, (uint32_t)kv.cols, 16))) return st;
-    if ((st = make_tmap_u8_rows(ctx, &tv, kv.v, kv.rows, (uint32_t)kv.cols, 16))) return st;
-  }
   Carve c;
-  const size_t o_part = c.take((size_t)grid * 2 * 16 * HD * 4), o_ml = c.take((size_t)grid * 2 * 16 * 8);
+  const size_t o_part = c.take(rows * HD * 4), o_ml = c.take(rows * 8);
   uint8_t* ws = static_cast<uint8_t*>(workspace(ctx, c.off, &st));
   if (!ws) return st;
   p.part = reinterpret_cast<float*>(ws + o_part);
   p.part_ml = reinterpret_cast<float*>(ws + o_ml);
   p.n_items = items;
   if (!(p.counters = arrival_counters(ctx, items, &st))) return st;
-  auto fn = text_rows_attn_kernel<FMT, HD>;
+  auto fn = text_rows_attn_kernel<FMT, HD, NT>;
   if ((st = ensure_smem_attr(ctx, (const void*)fn, G::kSmem, "text_rows_attn"))) return st;
+  const int64_t bytes = G::kWide ? 1 : 2;
   ProfScope prof(ctx, kProfAttn);
-  fn<<<grid, 256, G::kSmem, ctx->stream>>>(tk, tv, p, 2);
+  fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(static_cast<const uint8_t*>(kv.k), static_cast<const uint8_t*>(kv.v),
+                                                   (int64_t)kv.k_stride * bytes, (int64_t)kv.v_stride * bytes, p, 2);
   return launch_status(ctx, "text_rows_attn");
 }
 
-// Up to 16 flattened rows a sequence (a decoding step, a few drafted tokens) fill one tile of the
-// rows kernel, which is bound by the K/V bytes; more rows go to the tcgen05 kernel.
+template <int FMT>
+static int launch_rows_attn(wx_ctx* ctx, int head_dim, int64_t rows, const TextAttnParams& p, const KvSource& kv) {
+  if (head_dim == 128)
+    return rows <= 8 ? launch_rows_attn<FMT, 128, 1>(ctx, p, kv) : launch_rows_attn<FMT, 128, 2>(ctx, p, kv);
+  return rows <= 8 ? launch_rows_attn<FMT, 64, 1>(ctx, p, kv) : launch_rows_attn<FMT, 64, 2>(ctx, p, kv);
+}
+
+// Few flattened rows a sequence (a decoding step, a few drafted tokens): the rows kernel, which is
+// bound by the K/V bytes; more rows go to the tcgen05 kernel.
 static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParams& p, const KvSource& kv) {
-  const bool big = d->head_dim == 128;
-  if ((int64_t)d->max_q * p.group > 16) return text_flash(ctx, p, d->head_dim, kv);
-  if (kv.format == kKvInt8)
-    return big ? launch_rows_attn<kKvInt8, 128>(ctx, p, kv) : launch_rows_attn<kKvInt8, 64>(ctx, p, kv);
-  if (kv.format == kKvE4m3)
-    return big ? launch_rows_attn<kKvE4m3, 128>(ctx, p, kv) : launch_rows_attn<kKvE4m3, 64>(ctx, p, kv);
-  return big ? launch_rows_attn<kKvBf16, 128>(ctx, p, kv) : launch_rows_attn<kKvBf16, 64>(ctx, p, kv);
+  const int64_t rows = (int64_t)d->max_q * p.group;
+  if (rows > (kv.format == kKvBf16 ? 16 : 64)) return text_flash(ctx, p, d->head_dim, kv);
+  if (kv.format == kKvInt8) return launch_rows_attn<kKvInt8>(ctx, d->head_dim, rows, p, kv);
+  if (kv.format == kKvE4m3) return launch_rows_attn<kKvE4m3>(ctx, d->head_dim, rows, p, kv);
+  return launch_rows_attn<kKvBf16>(ctx, d->head_dim, rows, p, kv);
 }
 
 }  // namespace wx
