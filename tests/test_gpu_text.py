@@ -602,3 +602,24 @@ def test_calls_on_two_streams_share_the_workspace_safely():
     torch.cuda.synchronize()
     _check_device()
     assert all(torch.equal(o, want) for o in outs)
+
+
+# The states are normalised and each of the 2 x 2 sublayers rounds its input, products and sum to
+# bf16 (2^-9 rms of the value, some 6 roundings): sqrt(24) 2^-9 = 0.01 between two orders of the
+# same arithmetic. An 8-bit cache adds at most half a step of the row's largest value to every K
+# and V entry (1 / 254 of 2.5 to 3 standard deviations, e4m3 2^-4 of the entry: 0.036 rms); the
+# largest of these reaches the states through the attention's share of them. Five times that.
+@pytest.mark.parametrize("fmt,bound", [("bf16", 0.05), ("int8", 0.1), ("e4m3", 0.2)])
+def test_example_runs_the_operators_together(fmt, bound):
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "encode_prompt.py"
+    spec = importlib.util.spec_from_file_location("encode_prompt", path)
+    module = importlib.util.module_from_spec(spec)
+    import sys
+    sys.modules["encode_prompt"] = module  # (dataclasses look their module up)
+    spec.loader.exec_module(module)
+    r = module.main(["--cache", fmt, "--new", "5"])
+    assert r["finite"] and r["tokens"] == [82, 26]
+    assert r["conditions"] == [(82, 256), (26, 256)]
+    assert r["stepwise"] < bound and r["chunked"] < bound, r
