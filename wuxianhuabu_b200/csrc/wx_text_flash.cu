@@ -21,6 +21,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "wx_text_dev.cuh"
 
@@ -41,7 +42,7 @@ struct TfGeom {
   static constexpr int kThreads = kWide ? 512 : 384;
   static constexpr int kKStages = kWide ? 2 : 3;
   // registers of the control (and conversion) warps and of the softmax warps after setmaxnreg
-  static constexpr int kRegsLow = kWide ? 56 : 72, kRegsHigh = kWide ? 200 : 216;
+  static constexpr int kRegsLow = kWide ? 96 : 72, kRegsHigh = kWide ? 160 : 216;
   static constexpr int kRegsUsed = kRegsLow * (kThreads - 256) + kRegsHigh * 256;
   static_assert(kRegsUsed <= 65536 / kThreads / 8 * 8 * kThreads, "register split exceeds the launch");
   static constexpr int kTile = 128 * HD * 2;
@@ -119,6 +120,28 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// The shape of a matrix fragment, 16 lanes by 8 columns of 32 bits a repeat: thread (g, t) =
+// (lane / 4, lane % 4) holds columns 2t and 2t + 1 of lane g (first two registers) and of lane g + 8.
+__device__ __forceinline__ void tmem_ld_frag4(uint32_t taddr, float* v) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_frag4(uint32_t taddr, const float* v) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+               : "memory");
+}
+// waits for the thread's loads, of which v is one: nothing that uses v moves before it
+__device__ __forceinline__ void tmem_wait_ld32(float (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])::"memory");
+}
+// 16 lanes by 4 columns a repeat: column t of lane g, then of lane g + 8
+__device__ __forceinline__ void tmem_st_half4(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // Zeroes the non-finite values of row r of a V tile and notes their columns in `entry`.
 template <int HD>
 __device__ __noinline__ void remember_row(uint32_t row, int r, int key, uint32_t* entry) {
@@ -137,11 +160,6 @@ __device__ __noinline__ void remember_row(uint32_t row, int r, int key, uint32_t
   for (int e = 0; e < 4; ++e) entry[1 + e] = mask[e];
 }
 
-__device__ __forceinline__ float4 lds_f4(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
-  return v;
-}
 __device__ __forceinline__ float2 lds_f2(uint32_t a) {
   float2 v;
   asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
@@ -658,6 +676,154 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kBTfTurn + X));
     };
+    // One tile of an 8-bit cache, in matrix fragments: a thread has 32 columns of the four rows
+    // lane / 4 + 8 j instead of all columns of one, so that it reads 32 scales of each kind, not 128
+    // (as broadcasts these took as long as the products). S is read twice, a quarter at a time, rather
+    // than kept: unrolled over 128 registers the tile's code did not stay in the instruction cache
+    // beside the conversion's. 1324 tokens over 26,383 cached e4m3 keys, 32 / 8 heads: 942 us with a
+    // row per thread, 856 in fragments unrolled, 664 like this (bf16, a row per thread and unrolled:
+    // 420, and rolled it loses a tenth).
+    auto frag_tile = [&](uint32_t g, int t, int a0, bool masked, int hi, int lo, float (&m)[4], float (&l)[4]) -> bool {
+      const int tq = lane & 3;
+      const uint32_t scales = sbase + G::kScaleOff + (g % kTfScales) * 1024 + tq * 8;
+      if (!mbar_wait(bar(kBTfScale + g % kTfScales), (g / kTfScales) & 1, p.err, kDevTimeoutFull, abort_flag)) return false;
+      const float2 sl2x2 = make_float2(p.sl2, p.sl2);
+      // bits of this thread's columns that row j sees
+      uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+      if (masked) {
+        auto below = [&](int limit) -> uint32_t {  // of its columns before `limit`
+          const int x = max(0, limit - t * 128 - 2 * tq), n = 2 * (x >> 3) + min(2, x & 7);
+          return n >= 32 ? ~0u : (1u << n) - 1u;
+        };
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int from = (lane >> 2) + 8 * j;
+          keep[j] = below(__shfl_sync(0xffffffffu, hi, from)) & ~below(__shfl_sync(0xffffffffu, lo, from));
+        }
+      }
+      // the row maxima, in base 2 and scaled
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      auto maxima = [&](auto mk) {
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          float v[2][16];  // [16 lanes][column / 8][row g, row g + 8][2]
+          tmem_ld_frag4(tS + x * 32, v[0]);
+          tmem_ld_frag4(tS + (1u << 20) + x * 32, v[1]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __fmul2_rn(lds_f2(scales + x * 128 + k * 32), sl2x2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float* s = v[j >> 1] + k * 4 + (j & 1) * 2;
+              float2 y = __fmul2_rn(make_float2(s[0], s[1]), f);
+              if constexpr (decltype(mk)::value) {
+                const uint32_t bits = keep[j] >> (8 * x + 2 * k);
+                if (!(bits & 1u)) y.x = -INFINITY;
+                if (!(bits & 2u)) y.y = -INFINITY;
+              }
+              mx[j] = max3_f(mx[j], y.x, y.y);
+            }
+          }
+        }
+      };
+      if (masked) maxima(std::true_type{});
+      else maxima(std::false_type{});
+      bool grown = t == a0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) grown |= mx[j] - m[j] > 8.0f;
+      // as for rows below; without growth by 2^8 the maxima need not even be gathered
+      if (__any_sync(0xffffffffu, grown)) {
+        float alpha[4];
+        bool need = false;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
+          alpha[j] = 1.f;
+          if (t == a0) {
+            m[j] = mx[j];
+          } else if (mx[j] - m[j] > 8.0f) {
+            alpha[j] = exp2_approx(m[j] - mx[j]);
+            m[j] = mx[j];
+            l[j] *= alpha[j];
+            need = true;
+          }
+        }
+        if (__any_sync(0xffffffffu, need)) {
+          // PV(t-1) completed before S(t) (the tensor pipe runs in order): O is stable
+#pragma unroll 1
+          for (int c = 0; c < HD / 16; ++c) {
+            const uint32_t at = tO + ((uint32_t)(c & 1) << 20) + (c >> 1) * 32;
+            const float a = c & 1 ? alpha[2] : alpha[0], b = c & 1 ? alpha[3] : alpha[1];
+            float o[16];
+            tmem_ld_frag4(at, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= i & 2 ? b : a;
+            tmem_st_frag4(at, o);
+          }
+        }
+      }
+      float2 rs[4];
+      float nmu[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        rs[j] = make_float2(0.f, 0.f);
+        nmu[j] = m[j] == -INFINITY ? 0.f : -m[j];
+      }
+      auto weights = [&](auto mk, int c, const float (&v)[32]) {  // columns 32 c .. 32 c + 31
+        uint32_t pk[2][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 ks = __fmul2_rn(lds_f2(scales + (c * 4 + i) * 32), sl2x2);
+          const float2 vs = lds_f2(scales + 512 + (c * 4 + i) * 32);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float* s = v + (j >> 1) * 16 + i * 4 + (j & 1) * 2;
+            const float2 a = __ffma2_rn(make_float2(s[0], s[1]), ks, make_float2(nmu[j], nmu[j]));
+            float2 e = make_float2(exp2_approx(a.x), exp2_approx(a.y));
+            float2 w = __fmul2_rn(e, vs);
+            if constexpr (decltype(mk)::value) {  // an unseen key's scales may be anything: its weight is 0, not 0 * scale
+              const uint32_t bits = keep[j] >> (8 * c + 2 * i);
+              if (!(bits & 1u)) e.x = w.x = 0.f;
+              if (!(bits & 2u)) e.y = w.y = 0.f;
+            }
+            rs[j] = __fadd2_rn(rs[j], e);
+            pk[j >> 1][2 * i + (j & 1)] = pack_bf16x2(w.x, w.y);
+          }
+        }
+        tmem_st_half4(tS + c * 16, pk[0]);
+        tmem_st_half4(tS + (1u << 20) + c * 16, pk[1]);
+      };
+      auto load = [&](int c, float (&v)[32]) {
+        tmem_ld_frag4(tS + c * 32, v);
+        tmem_ld_frag4(tS + (1u << 20) + c * 32, v + 16);
+      };
+      auto publish = [&](int c) {
+        tmem_wait_st();  // this quarter of P is in TMEM (over S that has been read): its products may start
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kBTfPFull + X * 4 + c));
+      };
+      if (!my_turn(g)) return false;
+      auto walk = [&](auto mk) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float v0[32];
+          load(c, v0);
+          tmem_wait_ld32(v0);
+          weights(mk, c, v0);
+          if (c == 3) pass_turn();
+          publish(c);
+        }
+      };
+      if (masked) walk(std::true_type{});
+      else walk(std::false_type{});
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l[j] += rs[j].x + rs[j].y;
+      return true;
+    };
     bool ok = true;
     const TfItem* at = take_item(0);
     if (at) load_q(*at);
@@ -675,7 +841,14 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         lo = key_lo(p, s, tok);
       }
       bool q_sent = false;
+      // (8-bit: of the four rows of the thread's fragments, l over the thread's columns)
       float m = -INFINITY, l = 0.f;
+      float m4[4], l4[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        m4[j] = -INFINITY;
+        l4[j] = 0.f;
+      }
       for (int t = t0; t < t1; ++t) {
         if (t < a0 || t >= a1) {  // the other slot's alone
           if (!(ok = my_turn(both + (uint32_t)(t - t0)))) break;
@@ -694,13 +867,21 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           q_sent = true;
         }
         const bool masked = it.masked(t);
+        if constexpr (kW) {
+          const uint32_t g = both + (uint32_t)(t - t0);
+          if (!frag_tile(g, t, a0, masked, hi, lo, m4, l4)) {
+            ok = false;
+            break;
+          }
+          continue;
+        }
         const int lim = hi - t * 128, from = lo - t * 128;
         // bits of the keys 32 c .. 32 c + 31 that this row sees
         auto keep_bits = [&](int c) -> uint32_t {
           const int a = min(32, max(0, lim - c * 32)), b = min(32, max(0, from - c * 32));
           return (a == 32 ? ~0u : (1u << a) - 1u) & ~(b == 32 ? ~0u : (1u << b) - 1u);
         };
-        if (!kW && masked) {
+        if (masked) {
           // a short loop over S in TMEM: few tiles are masked, and unrolled over 128 registers this
           // code left the instruction cache between two of them (2 to 4 us a tile instead of 0.5)
 #pragma unroll 1
@@ -720,32 +901,6 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<float(*)[32]>(v + c * 32));
         tmem_wait_ld();
-        uint32_t scales = 0;
-        if constexpr (kW) {
-          const uint32_t g = both + (uint32_t)(t - t0);
-          scales = sbase + G::kScaleOff + (g % kTfScales) * 1024;
-          if (!mbar_wait(bar(kBTfScale + g % kTfScales), (g / kTfScales) & 1, p.err, kDevTimeoutFull, abort_flag)) {
-            ok = false;
-            break;
-          }
-#pragma unroll
-          for (int i = 0; i < 128; i += 4) {
-            const float4 f = lds_f4(scales + i * 4);
-            v[i] *= f.x;
-            v[i + 1] *= f.y;
-            v[i + 2] *= f.z;
-            v[i + 3] *= f.w;
-          }
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const uint32_t keep = keep_bits(c);
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(keep >> i & 1u)) v[c * 32 + i] = -INFINITY;
-            }
-          }
-        }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 128; i += 8) {
@@ -793,18 +948,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
             const float2 a = __ffma2_rn(make_float2(v[32 * c + 2 * i], v[32 * c + 2 * i + 1]), sl2x2, nmu2);
             const float2 e = make_float2(exp2_approx(a.x), exp2_approx(a.y));
             rs[i & 3] = __fadd2_rn(rs[i & 3], e);
-            if constexpr (kW) {
-              const float2 f = lds_f2(scales + 512 + (32 * c + 2 * i) * 4);
-              pk[i] = pack_bf16x2(e.x * f.x, e.y * f.y);
-            } else {
-              pk[i] = pack_bf16x2(e.x, e.y);
-            }
-          }
-          if (kW && masked) {  // an unseen key's scale may be anything: its weight is 0, not 0 * scale
-            const uint32_t keep = keep_bits(c);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              pk[i] &= (keep >> (2 * i) & 1u ? 0xffffu : 0u) | (keep >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+            pk[i] = pack_bf16x2(e.x, e.y);
           }
           tmem_st16(tS + c * 16, pk);
           if (c == 3) pass_turn();
@@ -818,6 +962,20 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       }
       mine += (uint32_t)(a1 - a0);
       both += (uint32_t)(t1 - t0);
+      if constexpr (kW) {  // back to the thread's own row
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x = l4[j];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          const float lj = __shfl_sync(0xffffffffu, x, (lane & 7) * 4);
+          const float mj = __shfl_sync(0xffffffffu, m4[j], (lane & 7) * 4);
+          if ((lane >> 3) == j) {
+            l = lj;
+            m = mj;
+          }
+        }
+      }
       // the next item's Q goes in first: its products then run while this item's rows are written
       const TfItem* next = ok ? take_item(n + 1) : nullptr;
       if (next && !q_sent) load_q(*next);
@@ -878,7 +1036,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       if (lane == 0 && any) mbar_arrive(bar(kBTfOEmpty + X));
       if (ok && live && p.lse)
         p.lse[((int64_t)it.q0 + tok) * p.hq + it.h * p.group + my_g] =
-            l == 0.f ? -INFINITY : (m * p.sl2 + __log2f(l)) * 0.69314718055994531f;
+            l == 0.f ? -INFINITY : ((kW ? m : m * p.sl2) + __log2f(l)) * 0.69314718055994531f;
       drop_item(n);
       at = next;
     }
