@@ -473,6 +473,56 @@ def test_paged_attention_is_deterministic_and_alone_or_in_a_batch(q_lens):
     _check_device()
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3"])
+@pytest.mark.parametrize("q_lens,kv_lens,hq,hkv,hd,page,window", [
+    ([90], [4100], 8, 2, 128, 64, 0),                      # one item, cut into pieces of its keys
+    ([70, 0, 200, 66], [2049, 300, 1025, 0], 4, 1, 64, 16, 0),  # some cut, some not, one without keys
+    ([130, 66], [6000, 2048], 4, 4, 128, 32, 2500),        # a window that pieces begin inside
+    ([150], [2900], 1, 1, 64, 256, 0),
+])
+def test_paged_attention_few_rows_long_keys(fmt, q_lens, kv_lens, hq, hkv, hd, page, window):
+    test_paged_attention(fmt, q_lens, kv_lens, hq, hkv, hd, page, window)
+
+
+@pytest.mark.parametrize("hd,causal,window", [(128, True, 0), (64, False, 0), (128, True, 1700)])
+def test_prompt_attention_few_rows_long_keys(hd, causal, window):
+    test_prompt_attention_with_other_key_lengths([50, 3], [5003, 1024], 8, 2, hd, causal, window)
+
+
+def test_pieces_of_long_keys_ignore_what_a_row_does_not_see():
+    """NaN in the value of a key that only the last rows see, and past the end of the last page."""
+    text = _text()
+    g = _gen(12)
+    n, nq = 3000, 80
+    cache, table, q, ks, vs = _paged(g, "bf16", [nq], [n], 4, 1, 128, 64)
+    page, off = int(table[0, (n - 20) // 64]), (n - 20) % 64
+    cache.v[page, :, off, 5] = math.nan
+    cache.v[int(table[0, n // 64]), :, n % 64:] = math.inf
+    out = text.paged_attention(q, cache, _cu([nq]), torch.tensor([n], dtype=torch.int32, device="cuda"), table, nq)
+    _check_device()
+    sees = torch.arange(nq, device="cuda") + n - nq >= n - 20
+    assert torch.isnan(out[sees][:, :, 5]).all()
+    rest = torch.ones(128, dtype=torch.bool, device="cuda")
+    rest[5] = False
+    ref, rl, mag = ref_attention(q, ks[0], vs[0], 1 / math.sqrt(128), True, 0)
+    assert_attention(out[~sees], None, ref[~sees], rl[~sees], mag[~sees], "rows before the key")
+    assert_attention(out[sees][..., rest], None, ref[sees][..., rest], rl[sees], mag[sees][..., rest], "other columns")
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_pieces_are_joined_in_order(fmt):
+    text = _text()
+    g = _gen(78)
+    kv, nq = [9000, 2500], [100, 77]
+    cache, table, q, _, _ = _paged(g, fmt, nq, kv, 8, 2, 128, 64)
+    lens = torch.tensor(kv, dtype=torch.int32, device="cuda")
+    first = text.paged_attention(q, cache, _cu(nq), lens, table, max(nq), return_lse=True)
+    for _ in range(10):
+        again = text.paged_attention(q, cache, _cu(nq), lens, table, max(nq), return_lse=True)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    _check_device()
+
+
 def test_paged_equals_prompt_attention():
     """A prompt written to a bf16 cache and attended as one chunk gives what the packed call gives."""
     text = _text()

@@ -32,6 +32,8 @@ constexpr int kTfRaw = 3;       // 8-bit: raw half tiles (64 keys) in flight
 constexpr int kTfScales = 4;    // 8-bit: tiles of scales kept
 constexpr int kTfItems = 2;     // item slots: the one at work and the next
 constexpr int kTfChunk = 128 * 128;  // one 64-column SW128 chunk of a 128-row tile
+constexpr int kTfWaves = 3;          // pieces for each SM below which items are cut up
+constexpr int kTfMinTiles = 8;       // tiles of a piece of an item: its start and end cost one or two
 constexpr int64_t kTfL2 = int64_t(48) << 20;
 constexpr int kTfBadRows = 1024;     // V rows with non-finite values remembered per item
 constexpr int kTfBadWords = 5;       // key, 128-bit column mask
@@ -63,6 +65,7 @@ struct TfItem {
   int a0, a1, b0, b1;    // key tiles [a0, a1) of slot A, [b0, b1) of slot B
   int free_hi, free_lo;  // tiles inside [free_lo, free_hi) are unmasked for every row
   int bad;               // V rows with non-finite values found in masked tiles
+  int piece, pieces;     // this part of the item's key tiles, and how many it was cut into
   __device__ int lo(int X) const { return X ? b0 : a0; }
   __device__ int hi(int X) const { return X ? b1 : a1; }
   __device__ int first() const { return a1 <= a0 ? b0 : b1 <= b0 ? a0 : min(a0, b0); }
@@ -173,7 +176,24 @@ struct TfParams {
   int* next;           // [2] items handed out, CTAs that have finished (0, 0 between launches)
   uint32_t* bad_rows;  // [CTA][kTfItems][kTfBadRows][kTfBadWords]
   const uint8_t *k8, *v8;  // rows of an 8-bit cache
+  int splits;              // at most this many pieces of an item
+  float* part;             // [splits][total_q * hq][HD] sums of the pieces' rows (items cut up only)
+  float2* part_ml;         // [splits][total_q * hq] maximum (base 2) and denominator
 };
+
+// Key tiles that tokens [k0, k0 + tt) of a sequence see: [x.x, x.y)
+__device__ __forceinline__ int2 slot_tiles(const TextAttnParams& p, const Seq& s, int k0, int tt) {
+  const int k1 = min(s.lq, k0 + tt);
+  if (k0 >= k1) return make_int2(0, 0);
+  const int hi = key_hi(p, s, k1 - 1), lo = key_lo(p, s, k0);
+  return hi > lo ? make_int2(lo >> 7, (hi + 127) >> 7) : make_int2(0, 0);
+}
+// The item's tiles [first, last) and the pieces that they are cut into, of at least kTfMinTiles
+__device__ __forceinline__ void cut_item(int2 a, int2 b, int splits, int& first, int& last, int& pieces) {
+  first = a.y <= a.x ? b.x : b.y <= b.x ? a.x : min(a.x, b.x);
+  last = max(first, max(a.y > a.x ? a.y : 0, b.y > b.x ? b.y : 0));
+  pieces = min(splits, max(1, (last - first) / kTfMinTiles));
+}
 
 template <int FMT, int HD>
 __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
@@ -442,12 +462,13 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     auto seq_items = [&](int b) -> int {
       if (b >= p.batch) return 0;
       const Seq s = load_seq(p, b);
-      return (int)((unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt)) * p.hkv;
+      return (int)((unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt)) * p.hkv * tp.splits;
     };
     int wb = 0;
     int wi = 0;  // items of the sequences before wb
-    // item number `at` into its slot (every lane works it out, lane 0 writes); false: no such item
-    auto find = [&](int at, TfItem* dst) -> bool {
+    // piece number `at` into its slot (every lane works it out, lane 0 writes); 0: no such piece, 2: an
+    // item that has fewer
+    auto find = [&](int at, TfItem* dst) -> int {
       while (wb < p.batch) {
         const int n = seq_items(wb + lane);
         int nc = n;
@@ -459,7 +480,9 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         const int all = __shfl_sync(0xffffffffu, nc, 31);
         if (at < wi + all) {
           const int src = __ffs(__ballot_sync(0xffffffffu, at < wi + nc)) - 1;
-          const unsigned in_b = (unsigned)(at - wi - __shfl_sync(0xffffffffu, nc - n, src));
+          const unsigned of_b = (unsigned)(at - wi - __shfl_sync(0xffffffffu, nc - n, src));
+          const unsigned in_b = of_b / (unsigned)tp.splits;
+          int found = 1;
           if (lane == 0) {
             const Seq s = load_seq(p, wb + src);
             const unsigned tiles = (unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt);
@@ -477,29 +500,30 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
             dst->lk = s.lk;
             dst->q0 = (int)s.q0;
             dst->k0 = (int)s.k0;
-#pragma unroll 1
-            for (int X = 0; X < 2; ++X) {
-              const int k0 = tok0 + X * tp.tt, k1 = min(s.lq, k0 + tp.tt);  // tokens [k0, k1)
-              int x0 = 0, x1 = 0;
-              if (k0 < k1) {
-                const int hi = key_hi(p, s, k1 - 1), lo = key_lo(p, s, k0);
-                if (hi > lo) {
-                  x0 = lo >> 7;
-                  x1 = (hi + 127) >> 7;
-                }
-              }
-              (X ? dst->b0 : dst->a0) = x0;
-              (X ? dst->b1 : dst->a1) = x1;
-            }
+            int2 a = slot_tiles(p, s, tok0, tp.tt), b = slot_tiles(p, s, tok0 + tp.tt, tp.tt);
+            int first, last, pieces;
+            cut_item(a, b, tp.splits, first, last, pieces);
+            const int piece = (int)(of_b - in_b * (unsigned)tp.splits), per = (last - first + pieces - 1) / pieces;
+            first += piece * per;
+            last = min(last, first + per);
+            a = make_int2(max(a.x, first), min(a.y, last));
+            b = make_int2(max(b.x, first), min(b.y, last));
+            dst->a0 = a.y > a.x ? a.x : 0;
+            dst->a1 = a.y > a.x ? a.y : 0;
+            dst->b0 = b.y > b.x ? b.x : 0;
+            dst->b1 = b.y > b.x ? b.y : 0;
+            dst->piece = piece;
+            dst->pieces = pieces;
+            if (piece >= pieces) found = 2;
             dst->free_hi = key_hi(p, s, tok0);
             dst->free_lo = key_lo(p, s, min(s.lq, tok0 + 2 * tp.tt) - 1);
           }
-          return true;
+          return __shfl_sync(0xffffffffu, found, 0);
         }
         wi += all;
         wb += 32;
       }
-      return false;
+      return 0;
     };
     uint32_t nv = 0;                 // V tiles of the items before
     uint32_t raw[kTfVStages] = {};   // masked tiles mended per stage
@@ -513,11 +537,13 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     bool ok = true;
     // finds the item that comes n-th on this CTA and announces it, once its slot is free
     auto announce = [&](int n) -> bool {
-      const int at = hand_out();
+      int at = hand_out();
       if (n >= kTfItems && ok &&
           !mbar_wait(bar(kBTfItemEmpty + n % kTfItems), ((n / kTfItems) & 1) ^ 1u, p.err, kDevTimeoutOther, abort_flag))
         ok = false;
-      const bool more = ok && find(at, items + n % kTfItems);
+      int found = 0;
+      while (ok && (found = find(at, items + n % kTfItems)) == 2) at = hand_out();
+      const bool more = found != 0;
       if (!more && lane == 0) items[n % kTfItems].valid = 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kBTfItemFull + n % kTfItems));
@@ -984,8 +1010,12 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : __fdividef(1.0f, l);
       const int bad = any ? *reinterpret_cast<const volatile int*>(&it.bad) : 0;
+      const bool cut = it.pieces > 1;
+      const bool write = ok && live && WX_IN_BOUNDS(p.err, it.q0 + tok < p.total_q);
+      const int64_t at_row = ((int64_t)it.q0 + tok) * p.hq + it.h * p.group + my_g;
+      const int64_t at_part = it.piece * (p.total_q * p.hq) + at_row;
       __nv_bfloat16* row = p.out + ((int64_t)it.q0 + tok) * p.out_stride + (int64_t)(it.h * p.group + my_g) * HD;
-      if (!ok || !live || !WX_IN_BOUNDS(p.err, it.q0 + tok < p.total_q)) row = nullptr;
+      if (!write || cut) row = nullptr;
       // 16-byte units are exchanged between two neighbouring lanes, so that a store covers 32
       // bytes (a whole sector) of each row: `even` is the row of the lower lane, `odd` the other's
       const auto other = reinterpret_cast<__nv_bfloat16*>(
@@ -1015,6 +1045,15 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           for (int i = 0; i < 16; ++i)
             if (hit >> i & 1u) o[i] = __int_as_float(0x7fc00000);
         }
+        if (cut) {
+          if (write) {
+            float* dst = tp.part + at_part * HD + c * 16;
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+          continue;
+        }
         uint4 w0 = make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
                               pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
         uint4 w1 = make_uint4(pack_bf16x2(o[8] * inv, o[9] * inv), pack_bf16x2(o[10] * inv, o[11] * inv),
@@ -1034,9 +1073,9 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0 && any) mbar_arrive(bar(kBTfOEmpty + X));
-      if (ok && live && p.lse)
-        p.lse[((int64_t)it.q0 + tok) * p.hq + it.h * p.group + my_g] =
-            l == 0.f ? -INFINITY : ((kW ? m : m * p.sl2) + __log2f(l)) * 0.69314718055994531f;
+      const float m2 = kW ? m : m * p.sl2;
+      if (cut && write) tp.part_ml[at_part] = make_float2(m2, l);
+      if (!cut && write && p.lse) p.lse[at_row] = l == 0.f ? -INFINITY : (m2 + __log2f(l)) * 0.69314718055994531f;
       drop_item(n);
       at = next;
     }
@@ -1048,6 +1087,55 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// Rows of items that were cut up: sums of the pieces, in order, brought to one maximum. A warp a row.
+template <int HD>
+__global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
+  const TextAttnParams& p = tp.a;
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = p.total_q * p.hq;
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t token = row / p.hq;
+  int b = 0;  // last sequence that begins at or before the token
+  for (int n = p.batch; n > 1;) {
+    const int half = n / 2;
+    if (p.cu_q[b + half] <= token) b += half;
+    n -= half;
+  }
+  const Seq s = load_seq(p, b);
+  const int64_t tok = token - s.q0;
+  if (tok < 0 || tok >= s.lq) return;
+  const int tok0 = (int)tok / (2 * tp.tt) * (2 * tp.tt);
+  int first, last, pieces;
+  cut_item(slot_tiles(p, s, tok0, tp.tt), slot_tiles(p, s, tok0 + tp.tt, tp.tt), tp.splits, first, last, pieces);
+  if (pieces < 2) return;
+  constexpr int kPer = HD / 32;
+  float o[kPer] = {};
+  float M = -INFINITY, L = 0.f;
+  for (int i = 0; i < pieces; ++i) {
+    const float2 ml = tp.part_ml[i * rows + row];
+    if (ml.y != 0.f) M = fmaxf(M, ml.x);
+  }
+#pragma unroll 4
+  for (int i = 0; i < pieces; ++i) {
+    const float2 ml = tp.part_ml[i * rows + row];
+    if (ml.y == 0.f) continue;  // (nothing seen: its sums may be anything)
+    const float f = exp2_approx(ml.x - M);
+    L += ml.y * f;
+    const float* src = tp.part + (i * rows + row) * HD + lane * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; e += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(src + e);
+      o[e] += x.x * f;
+      o[e + 1] += x.y * f;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : __fdividef(1.0f, L);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + token * p.out_stride + (row - token * p.hq) * HD + lane * kPer);
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) dst[e / 2] = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
 template <int FMT, int HD>
@@ -1065,14 +1153,27 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   if (!regs_ok) return set_error(ctx, WX_ERR_CUDA, "text_flash: register split does not fit");
   const TextAttnParams& p = tp.a;
   const int64_t items = (int64_t)p.hkv * (p.total_q / (2 * tp.tt) + p.batch);
-  const int grid = (int)std::min<int64_t>(ctx->num_sms, items);
-  void* ws = workspace(ctx, (size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4, &st);
+  // Too few items to level the SMs out are cut into pieces of their keys, as many as give kTfWaves
+  // to an SM and as the longest range that a row can see allows.
+  int64_t keys = p.block_table ? p.blocks_per_seq << p.page_shift : p.total_k;
+  if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 2 * tp.tt);
+  tp.splits = (int)std::max<int64_t>(1, std::min((kTfWaves * ctx->num_sms + items - 1) / items, keys / (128 * kTfMinTiles)));
+  const int grid = (int)std::min<int64_t>(ctx->num_sms, items * tp.splits);
+  const int64_t rows = tp.splits > 1 ? p.total_q * p.hq * tp.splits : 0;
+  Carve c;
+  const size_t o_bad = c.take((size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4);
+  const size_t o_part = c.take((size_t)rows * HD * 4), o_ml = c.take((size_t)rows * 8);
+  uint8_t* ws = static_cast<uint8_t*>(workspace(ctx, c.off, &st));
   if (!ws) return st;
-  tp.bad_rows = static_cast<uint32_t*>(ws);
+  tp.bad_rows = reinterpret_cast<uint32_t*>(ws + o_bad);
+  tp.part = reinterpret_cast<float*>(ws + o_part);
+  tp.part_ml = reinterpret_cast<float2*>(ws + o_ml);
   if (!(tp.next = arrival_counters(ctx, 2, &st))) return st;
   ProfScope prof(ctx, kProfAttn);
   fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(tq, tk, tv, tp);
-  return launch_status(ctx, "text_flash");
+  if (tp.splits == 1) return launch_status(ctx, "text_flash");
+  text_flash_join_kernel<HD><<<(unsigned)((p.total_q * p.hq + 7) / 8), 256, 0, ctx->stream>>>(tp);
+  return launch_status(ctx, "text_flash", 2);
 }
 
 int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv) {
