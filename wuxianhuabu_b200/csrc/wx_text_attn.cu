@@ -719,11 +719,14 @@ static int launch_rows_attn(wx_ctx* ctx, int head_dim, int64_t rows, const TextA
   return rows <= 8 ? launch_rows_attn<FMT, 64, 1>(ctx, p, kv) : launch_rows_attn<FMT, 64, 2>(ctx, p, kv);
 }
 
-// Few flattened rows a sequence (a decoding step, a few drafted tokens): the rows kernel, which is
-// bound by the K/V bytes; more rows go to the tcgen05 kernel.
+// Few flattened rows a sequence (a decoding step, a few drafted tokens) go to the rows kernel, which
+// reads the keys once per 16 rows, more to the tcgen05 kernel, which does so once per 256. Rows : tcgen05
+// at 32 sequences of 8,000 keys, 32 / 8 heads of 128: 24 rows 326 : 253 us at bf16 and 338 : 382 at
+// int8, 64 rows 618 : 259 and 657 : 390; one sequence of 65,536 keys, 24 rows 92 : 114 and 102 : 136,
+// 48 rows 121 : 118 and 142 : 142.
 static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParams& p, const KvSource& kv) {
   const int64_t rows = (int64_t)d->max_q * p.group;
-  if (rows > (kv.format == kKvBf16 ? 16 : 64)) return text_flash(ctx, p, d->head_dim, kv);
+  if (rows > (kv.format == kKvBf16 ? 16 : 48)) return text_flash(ctx, p, d->head_dim, kv);
   if (kv.format == kKvInt8) return launch_rows_attn<kKvInt8>(ctx, d->head_dim, rows, p, kv);
   if (kv.format == kKvE4m3) return launch_rows_attn<kKvE4m3>(ctx, d->head_dim, rows, p, kv);
   return launch_rows_attn<kKvBf16>(ctx, d->head_dim, rows, p, kv);
