@@ -67,15 +67,15 @@ __device__ __forceinline__ void copy_async_wait() {
 // last to arrive joins them in key order (so the result does not depend on who is last).
 //
 // Measured, caches flushed from L2: 64 sequences, 32 / 8 heads of 128, 238,000 bf16 keys 191 us =
-// 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 53 us = 2.6 TB/s
-// (4.3 TB/s a further key: there the expansion and the exponentials are as long as the loads); a
+// 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 51 us = 2.7 TB/s
+// (4.3 TB/s a further key: the integer pipe, which expands the bytes, is the bound: issue slots 53 % busy, DRAM 34 %); a
 // call with a few keys 11 us, of which 7 on the device.
 constexpr int kUnit = 128;
 
 template <int FMT, int HD, int NT>
 struct RowsGeom {
   static constexpr bool kWide = FMT != kKvBf16;  // 8-bit rows
-  // as many warps as registers (8-bit: 12 against 16, 53 : 54 us) and ring stages (bf16: 10 against
+  // as many warps as registers (8-bit: 12 against 16, 51 : 51 us) and ring stages (bf16: 10 against
   // 8, 191 : 196 us) allow; 16 rows take twice the registers
   static constexpr int kWarps = NT == 1 ? (kWide ? 12 : 10) : 8;
   static constexpr int kThreads = 32 * kWarps;
@@ -187,12 +187,13 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
 
   // ---- loads: step i of this warp starts at key k_lo + (i * kWarps + warp) * 16; the pages of 32
   // consecutive steps are fetched at once, one per lane
+  const bool paged = kW || p.block_table;
   int page_of = 0;
   auto first_key = [&](const Piece& c, int i) { return c.k_lo + (i * kWarps + warp) * 16; };
   // row of the step's first key: of the cache, or of the packed keys
   auto step_row = [&](const Piece& c, int i) -> int64_t {
     const int j0 = first_key(c, i);
-    if (!p.block_table) return c.s.k0 + j0;
+    if (!paged) return c.s.k0 + j0;
     if ((i & 31) == 0) {
       const int jl = first_key(c, i + lane);
       page_of = 0;
@@ -216,26 +217,28 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   constexpr int kVN = kW ? 1 : HD / 64; // V units of a row that a lane reads
   auto k_swz = [](int row) { return kRU == 4 ? 0 : (row & 1) << 2; };
   auto v_swz = [](int row) { return kRU == 4 ? (row >> 1) & 3 : row & 6; };
+  const float* scale_at = kW ? (lane < 16 ? p.ks : p.vs) + (lane & 15) : nullptr;
   auto load_step = [&](const Piece& c, int i, uint32_t stage) {
     if (i < c.steps) {
       const int64_t row = step_row(c, i);
-      const int left = p.block_table ? 15 : c.s.lk - 1 - first_key(c, i);
-      const int64_t col = (p.block_table ? 0 : (int64_t)c.h * kRowBytes) + lane % kRU * 16;
-      const uint8_t* kb = k_base + row * k_stride + col;
-      const uint8_t* vb = v_base + row * v_stride + col;
+      // (an 8-bit cache is paged: its 16 rows lie together)
+      const int64_t kst = kW ? kRowBytes : k_stride, vst = kW ? kRowBytes : v_stride;
+      const int left = paged ? 15 : c.s.lk - 1 - first_key(c, i);
+      const int64_t col = (paged ? 0 : (int64_t)c.h * kRowBytes) + lane % kRU * 16;
+      const uint8_t* kb = k_base + row * kst + col;
+      const uint8_t* vb = v_base + row * vst + col;
 #pragma unroll
       for (int x = 0; x < kRU / 2; ++x) {
         const int r = x * (32 / kRU) + lane / kRU;
-        copy_async16(stage + (r * kRU + (lane % kRU ^ k_swz(r))) * 16, kb + (int64_t)min(r, left) * k_stride);
+        copy_async16(stage + (r * kRU + (lane % kRU ^ k_swz(r))) * 16, kb + (int64_t)(kW ? r : min(r, left)) * kst);
       }
 #pragma unroll
       for (int x = 0; x < kRU / 2; ++x) {
         const int r = x * (32 / kRU) + lane / kRU;
         copy_async16(stage + G::kKvBytes + (r * kRU + (lane % kRU ^ v_swz(r))) * 16,
-                     vb + (int64_t)min(r, left) * v_stride);
+                     vb + (int64_t)(kW ? r : min(r, left)) * vst);
       }
-      if constexpr (kW)  // keys' scales, then values'
-        copy_async4(stage + 2 * G::kKvBytes + lane * 4, (lane < 16 ? p.ks : p.vs) + row + (lane & 15));
+      if constexpr (kW) copy_async4(stage + 2 * G::kKvBytes + lane * 4, scale_at + row);  // keys' scales, then values'
     }
     copy_async_commit();
   };
@@ -398,12 +401,19 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float mu = m[n][e] == -INFINITY ? 0.f : m[n][e];
-          const bool off0 = sc[n][e] == -INFINITY, off1 = sc[n][2 + e] == -INFINITY;
           const float x0 = exp2_approx(sc[n][e] - mu), x1 = exp2_approx(sc[n][2 + e] - mu);
           l[n][e] += x0 + x1;
-          // an unseen key's scale may be anything: its weight is 0, not 0 * scale
-          sc[n][e] = kW && off0 ? 0.f : x0 * vs[0];
-          sc[n][2 + e] = kW && off1 ? 0.f : x1 * vs[1];
+          float w0 = x0, w1 = x1;
+          if constexpr (kW) {
+            w0 *= vs[0];
+            w1 *= vs[1];
+            if (masked) {  // an unseen key's scale may be anything: its weight is 0, not 0 * scale
+              if (sc[n][e] == -INFINITY) w0 = 0.f;
+              if (sc[n][2 + e] == -INFINITY) w1 = 0.f;
+            }
+          }
+          sc[n][e] = w0;
+          sc[n][2 + e] = w1;
         }
         // P rounded to bf16 for the tensor product (the denominator sums the unrounded values)
         pb[n][0] = transpose_8x8(pack_bf16x2(sc[n][0], sc[n][1]));
