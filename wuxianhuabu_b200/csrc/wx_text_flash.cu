@@ -43,6 +43,9 @@ struct TfGeom {
   static constexpr bool kWide = FMT != kKvBf16;
   static constexpr int kThreads = kWide ? 512 : 384;
   static constexpr int kKStages = kWide ? 2 : 3;
+  // quarters of P that are handed over first, together; each hand-over waits for its stores, and a
+  // tile's last products should be few (9001 + 5003 + 2380 tokens: 1: 808, 2: 795, 3: 800, 4: 840 us)
+  static constexpr int kFirstP = kWide ? 1 : 2;
   // registers of the control (and conversion) warps and of the softmax warps after setmaxnreg
   static constexpr int kRegsLow = kWide ? 96 : 72, kRegsHigh = kWide ? 160 : 216;
   static constexpr int kRegsUsed = kRegsLow * (kThreads - 256) + kRegsHigh * 256;
@@ -408,8 +411,10 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           if (t >= a0 && t < a1) {
             const uint64_t dv = fresh64(smem_desc_sw128(sV(sv), kTfChunk, 1024));
 #pragma unroll
-            for (int part = 0; part < 4; ++part) {
-              if (!mbar_wait(bar(kBTfPFull + X * 4 + part), (mine + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax,
+            for (int part = 0; part < 4; ++part) {  // (the first kFirstP quarters come together)
+              const int full = part < G::kFirstP ? G::kFirstP - 1 : part;
+              if ((part == 0 || part >= G::kFirstP) &&
+                  !mbar_wait(bar(kBTfPFull + X * 4 + full), (mine + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax,
                              abort_flag)) {
                 ok = false;
                 break;
@@ -978,6 +983,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           }
           tmem_st16(tS + c * 16, pk);
           if (c == 3) pass_turn();
+          if (c + 1 < G::kFirstP) continue;
           tmem_wait_st();  // this quarter of P is in TMEM: its products may start
           tc_fence_before();
           __syncwarp();
