@@ -1119,22 +1119,48 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   constexpr int kPer = HD / 32;
   float o[kPer] = {};
   float M = -INFINITY, L = 0.f;
-  for (int i = 0; i < pieces; ++i) {
-    const float2 ml = tp.part_ml[i * rows + row];
-    if (ml.y != 0.f) M = fmaxf(M, ml.x);
-  }
-#pragma unroll 4
-  for (int i = 0; i < pieces; ++i) {
-    const float2 ml = tp.part_ml[i * rows + row];
-    if (ml.y == 0.f) continue;  // (nothing seen: its sums may be anything)
-    const float f = exp2_approx(ml.x - M);
-    L += ml.y * f;
-    const float* src = tp.part + (i * rows + row) * HD + lane * kPer;
+  auto piece = [&](int i) { return i < pieces ? tp.part_ml[i * rows + row] : make_float2(-INFINITY, 0.f); };
+  for (int c = 0; c < pieces; c += 32) {
+    const float2 ml = piece(c + lane);
+    float m = ml.y != 0.f ? ml.x : -INFINITY;
 #pragma unroll
-    for (int e = 0; e < kPer; e += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(src + e);
-      o[e] += x.x * f;
-      o[e + 1] += x.y * f;
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    M = fmaxf(M, m);
+  }
+  for (int c = 0; c < pieces; c += 32) {
+    const float2 ml = piece(c + lane);
+    const float f = ml.y != 0.f ? exp2_approx(ml.x - M) : 0.f;
+    const uint32_t seen = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    float l = ml.y != 0.f ? ml.y * f : 0.f;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    L += l;
+    const int n = min(32, pieces - c);
+#pragma unroll 1
+    for (int i = 0; i < n; i += 8) {  // eight pieces' rows in flight
+      float x[8][kPer];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float* src = tp.part + (min(c + i + q, pieces - 1) * rows + row) * HD + lane * kPer;
+        if constexpr (kPer == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(src);
+          x[q][0] = y.x;
+          x[q][1] = y.y;
+          x[q][2] = y.z;
+          x[q][3] = y.w;
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(src);
+          x[q][0] = y.x;
+          x[q][1] = y.y;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float w = __shfl_sync(0xffffffffu, f, (i + q) & 31);
+        if (i + q < n && (seen >> (i + q) & 1u))  // (nothing seen: its sums may be anything)
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) o[e] += x[q][e] * w;
+      }
     }
   }
   const float inv = L == 0.f ? 0.f : __fdividef(1.0f, L);
