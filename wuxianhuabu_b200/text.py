@@ -71,7 +71,7 @@ def _same_device(*ts: torch.Tensor) -> int:
 def _out_rows(like: torch.Tensor, n: int, h: int, d: int, out: Optional[torch.Tensor], msg: str):
     """The output tensor (a new one without ``out``) and its token stride."""
     if out is None:
-        return like.new_empty((n, h, d)), h * d
+        return torch.empty_like(like), h * d  # (rows of contiguous heads: never anything but contiguous)
     if out.shape != like.shape:
         raise _invalid(msg)
     return out, _rows(out, "out")[3]
@@ -220,7 +220,7 @@ class PagedKVCache:
         """k and v of the slots as bf16 [tokens, kv_heads, head_dim] (< 0: zeros)."""
         at = _need_ints(torch.int64, None, "slots", slots)
         n, h, d = slots.numel(), self.kv_heads, self.head_dim
-        k = torch.empty((n, h, d), dtype=torch.bfloat16, device=self.k.device)
+        k = slots.new_empty((n, h, d), dtype=torch.bfloat16)
         v = torch.empty_like(k)
         context(_same_device(self.k, slots)).call("wx_kv_read", self._desc, at, n, k.data_ptr(), v.data_ptr(), h * d)
         return k, v
@@ -229,7 +229,7 @@ class PagedKVCache:
 def _attn_out(q: torch.Tensor, out: Optional[torch.Tensor], return_lse: bool):
     n, h, d, stride = _rows(q, "q")
     o, ostride = _out_rows(q, n, h, d, out, "out must have q's shape")
-    lse = torch.empty((n, h), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((n, h), dtype=torch.float32) if return_lse else None
     return n, h, d, stride, o, ostride, lse
 
 
