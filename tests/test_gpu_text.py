@@ -540,6 +540,36 @@ def test_paged_equals_prompt_attention():
     assert_attention(b, None, ref, rl, mag, "paged")
 
 
+@pytest.mark.parametrize("fmt,pages", [("bf16", 9000), ("int8", 18000)])
+@pytest.mark.parametrize("q_len", [1, 70])
+def test_cache_beyond_32_bit_offsets(fmt, pages, q_len):
+    """More than 2^32 bytes of keys: pages from the end, the middle and the start of the cache."""
+    text = _text()
+    g = _gen(q_len)
+    hq, hkv, hd, page, n = 16, 8, 128, 256, 600
+    cache = text.PagedKVCache(pages, page, hkv, hd, fmt)
+    assert cache.k.numel() * cache.k.element_size() > 1 << 32
+    table = torch.tensor([[pages - 1, pages // 2, 0]], dtype=torch.int32, device="cuda")
+    j = torch.arange(n, device="cuda")
+    slots = table[0].long()[j // page] * page + j % page
+    k, v = _randn(g, n, hkv, hd), _randn(g, n, hkv, hd)
+    cache.append(k, v, slots)
+    ks, vs = cache.read(slots)
+    if fmt == "bf16":
+        assert torch.equal(ks, k) and torch.equal(vs, v)
+    else:
+        pg, off = table[0].long()[j // page], j % page
+        ks = cache.k[pg, :, off].to(F64) * cache.k_scale[pg, :, off].to(F64)[..., None]
+        vs = cache.v[pg, :, off].to(F64) * cache.v_scale[pg, :, off].to(F64)[..., None]
+        assert ((ks - k.to(F64)).abs() <= 0.5001 * cache.k_scale[pg, :, off].to(F64)[..., None]).all()
+    q = _randn(g, q_len, hq, hd)
+    out, lse = text.paged_attention(q, cache, _cu([q_len]), torch.tensor([n], dtype=torch.int32, device="cuda"),
+                                    table, q_len, return_lse=True)
+    _check_device()
+    ref, rl, mag = ref_attention(q, ks, vs, 1 / math.sqrt(hd), True, 0)
+    assert_attention(out, lse, ref, rl, mag, fmt)
+
+
 # ---------------------------------------------------------------------------------- refusals
 def test_refusals():
     text = _text()

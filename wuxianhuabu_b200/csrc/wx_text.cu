@@ -326,7 +326,7 @@ int check_kv_cache(wx_ctx* ctx, const wx_kv_cache* c) {
   WX_CHECK_ARG(ctx, c->format == WX_KV_BF16 || (c->k_scale && c->v_scale));
   WX_CHECK_ARG(ctx, aligned16(c->k) && aligned16(c->v) && aligned16(c->k_scale) && aligned16(c->v_scale));
   // rows of the cache are indexed by 32-bit tile coordinates
-  if (c->pages > INT32_MAX || c->pages * c->kv_heads * c->page_size > INT32_MAX)
+  if (c->pages > INT32_MAX / c->page_size / c->kv_heads)
     return set_error(ctx, WX_ERR_UNSUPPORTED, "pages * kv_heads * page_size must be below 2^31");
   return WX_OK;
 }
