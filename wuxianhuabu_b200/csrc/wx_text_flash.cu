@@ -55,7 +55,7 @@ struct TfGeom {
   // tile's last products should be few (9001 + 5003 + 2380 tokens: 1: 808, 2: 795, 3: 800, 4: 840 us)
   static constexpr int kFirstP = kWide ? 1 : 2;
   // registers of the control (and conversion) warps and of the softmax warps after setmaxnreg
-  static constexpr int kRegsLow = kWide ? 96 : 72, kRegsHigh = kWide ? 160 : 216;
+  static constexpr int kRegsLow = kWide ? 104 : 72, kRegsHigh = kWide ? 152 : 216;
   static constexpr int kRegsUsed = kRegsLow * (kThreads - 256) + kRegsHigh * 256;
   static_assert(kRegsUsed <= 65536 / kThreads / 8 * 8 * kThreads, "register split exceeds the launch");
   static constexpr int kTile = 128 * HD * 2;
@@ -111,11 +111,11 @@ __device__ __forceinline__ float max3_f(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// a value the compiler recomputes where it is used (keeps descriptors out of registers)
-__device__ __forceinline__ uint64_t fresh64(uint64_t v) {
-  uint64_t r;
-  asm volatile("mov.b64 %0, %1;" : "=l"(r) : "l"(v));
-  return r;
+// true in one lane of the (converged) warp, the same each time
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+  return yes != 0;
 }
 __device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -382,90 +382,98 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
   } else if (warp == 1 || warp == 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLow));
     // ------------------------------------------------------------ MMA issuer of slot X
-    const int X = warp - 1;
+    const int X = __shfl_sync(0xffffffffu, warp, 0) - 1;
     constexpr uint32_t idesc_s = idesc_bf16_f32(128, 128, false, false);
     constexpr uint32_t idesc_o = idesc_bf16_f32(128, HD, false, true);  // P from TMEM, V MN-major
     const uint32_t tS = tmem + (uint32_t)(X * 128);
     const uint32_t tO = tmem + 256 + (uint32_t)(X * 128);
-    const uint64_t dq = fresh64(smem_desc_sw128(sQ(X), 16, 1024));
+    const uint64_t dq = smem_desc_sw128(sQ(X), 16, 1024);
     uint32_t kv = 0;    // tiles of all items before this one (K and V alike)
     uint32_t mine = 0;  // tiles of this slot so far
     uint32_t n_o = 0;   // items in which this slot had tiles
     bool ok = true, issued = false;
+    // The whole warp walks the tiles, one elected lane issues, from descriptors in uniform registers
+    // (long prompts 793 -> 784 us against lane 0 walking alone).
+    auto wait = [&](int which, uint32_t parity, int code) -> bool {
+      return __all_sync(0xffffffffu, mbar_wait(bar(which), parity, p.err, code, abort_flag));
+    };
     for (int n = 0; ok; ++n) {
       const TfItem* at = take_item(n);
-      if (!at) break;
+      if (!__all_sync(0xffffffffu, at != nullptr)) break;
       const TfItem& it = *at;
       const int t0 = it.first(), t1 = it.last();
       const bool any = it.hi(X) > it.lo(X);
       const int a0 = any ? it.lo(X) : t1, a1 = any ? it.hi(X) : t1;
-      if (lane == 0) {
-        if (any) ok = mbar_wait(bar(kBTfQFull + X), n_o & 1, p.err, kDevTimeoutSoftmax, abort_flag);
-        // step t: O += P(t) V(t), then S(t + 1); a tile that only the other slot works on is
-        // just given back
+      if (any) ok = wait(kBTfQFull + X, n_o & 1, kDevTimeoutSoftmax);
+      // step t: O += P(t) V(t), then S(t + 1); a tile that only the other slot works on is
+      // just given back
 #pragma unroll 1
-        for (int t = t0 - 1; t < t1 && ok; ++t) {
-          // V(t) and K(t+1) are waited for before P(t): PV(t) and S(t+1) then go out back to back
-          const uint32_t cv = kv + (uint32_t)(t - t0), ck = cv + 1;
-          const uint32_t sv = cv % kTfVStages, sk = ck % kKStages;
-          if (t >= t0)
-            ok = mbar_wait(bar(kBTfVFull + sv), (cv / kTfVStages) & 1, p.err, kDevTimeoutFull, abort_flag);
-          if (ok && t + 1 < t1)
-            ok = mbar_wait(bar(kBTfKFull + sk), (ck / kKStages) & 1, p.err, kDevTimeoutFull, abort_flag);
-          // the first product of an item overwrites O: the last epilogue must have read it
-          if (ok && t == a0 && n_o > 0)
-            ok = mbar_wait(bar(kBTfOEmpty + X), (n_o - 1) & 1, p.err, kDevTimeoutSoftmax, abort_flag);
-          if (!ok) break;
-          if (t >= a0 && t < a1) {
-            const uint64_t dv = fresh64(smem_desc_sw128(sV(sv), kTfChunk, 1024));
+      for (int t = t0 - 1; t < t1 && ok; ++t) {
+        // V(t) and K(t+1) are waited for before P(t): PV(t) and S(t+1) then go out back to back
+        const uint32_t cv = kv + (uint32_t)(t - t0), ck = cv + 1;
+        const uint32_t sv = cv % kTfVStages, sk = ck % kKStages;
+        if (t >= t0) ok = wait(kBTfVFull + sv, (cv / kTfVStages) & 1, kDevTimeoutFull);
+        if (ok && t + 1 < t1) ok = wait(kBTfKFull + sk, (ck / kKStages) & 1, kDevTimeoutFull);
+        // the first product of an item overwrites O: the last epilogue must have read it
+        if (ok && t == a0 && n_o > 0) ok = wait(kBTfOEmpty + X, (n_o - 1) & 1, kDevTimeoutSoftmax);
+        if (!ok) break;
+        if (t >= a0 && t < a1) {
+          const uint64_t dv = smem_desc_sw128(sV(sv), kTfChunk, 1024);
 #pragma unroll
-            for (int part = 0; part < 4; ++part) {  // (the first kFirstP quarters come together)
-              const int full = part < G::kFirstP ? G::kFirstP - 1 : part;
-              if ((part == 0 || part >= G::kFirstP) &&
-                  !mbar_wait(bar(kBTfPFull + X * 4 + full), (mine + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax,
-                             abort_flag)) {
-                ok = false;
-                break;
-              }
-              tc_fence_after();
+          for (int part = 0; part < 4; ++part) {  // (the first kFirstP quarters come together)
+            const int full = part < G::kFirstP ? G::kFirstP - 1 : part;
+            if ((part == 0 || part >= G::kFirstP) &&
+                !wait(kBTfPFull + X * 4 + full, (mine + (uint32_t)(t - a0)) & 1, kDevTimeoutSoftmax)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
               for (int k2 = 0; k2 < 2; ++k2) {
                 const int kk = part * 2 + k2;
                 umma_bf16_ts(tO, tS + kk * 8, dv + (uint64_t)(kk * (2048 >> 4)), idesc_o, (t > a0 || kk > 0) ? 1u : 0u);
               }
             }
-            if (!ok) break;
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (elect_one()) {
             umma_commit(bar(kBTfVEmpty + sv));
             if (t == a1 - 1) umma_commit(bar(kBTfOFull + X));
-          } else if (t >= t0) {
-            mbar_arrive(bar(kBTfVEmpty + sv));
           }
-          if (t + 1 >= a0 && t + 1 < a1) {
-            tc_fence_after();
-            const uint64_t dk = fresh64(smem_desc_sw128(sK(sk), 16, 1024));
+          __syncwarp();
+        } else if (t >= t0) {
+          if (lane == 0) mbar_arrive(bar(kBTfVEmpty + sv));
+        }
+        if (t + 1 >= a0 && t + 1 < a1) {
+          tc_fence_after();
+          const uint64_t dk = smem_desc_sw128(sK(sk), 16, 1024);
+          if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk) {
               const uint32_t off = ((kk >> 2) * kTfChunk + (kk & 3) * 32) >> 4;
               umma_bf16(tS, dq + off, dk + off, idesc_s, kk > 0 ? 1u : 0u);
             }
-            issued = true;
             umma_commit(bar(kBTfSFull + X));
             umma_commit(bar(kBTfKEmpty + sk));
-          } else if (t + 1 < t1) {
-            mbar_arrive(bar(kBTfKEmpty + sk));
           }
+          __syncwarp();
+          issued = true;
+        } else if (t + 1 < t1) {
+          if (lane == 0) mbar_arrive(bar(kBTfKEmpty + sk));
         }
-        mine += (uint32_t)(a1 - a0);
-        kv += (uint32_t)(t1 - t0);
-        n_o += any ? 1 : 0;
       }
+      mine += (uint32_t)(a1 - a0);
+      kv += (uint32_t)(t1 - t0);
+      n_o += any ? 1 : 0;
       drop_item(n);
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
     }
-    if (lane == 0 && issued) {  // every MMA of this thread completes before TMEM is released
+    if (issued && elect_one()) {  // every MMA of this thread completes before TMEM is released
       umma_commit(bar(kBTfDrain + X));
       mbar_drain(bar(kBTfDrain + X), 0);
     }
+    __syncwarp();
   } else if (warp == 3) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kRegsLow));
     // ------------------------------------------------------------ items, and masked V tiles
