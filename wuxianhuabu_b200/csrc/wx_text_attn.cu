@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
           for (int n = 0; n < NT; ++n) mma_bf16(sc[n], kx.z, ky.z, kx.w, ky.w, qf[n][2 * c + 1][0], qf[n][2 * c + 1][1]);
         }
       }
-      float f[2] = {p.sl2, p.sl2}, vs[2] = {1.f, 1.f};  // of keys g and g + 8
+      const float k_unit = p.sl2 * kByteUnit<FMT>;
+      float f[2] = {k_unit, k_unit}, vs[2] = {1.f, 1.f};  // of keys g and g + 8
       if constexpr (kW) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -549,7 +550,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
       const int tk = (int)((unsigned)r / (unsigned)p.group);
       const int64_t tok = done.s.q0 + tk;
       const int head = done.h * p.group + r - tk * p.group;
-      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const float inv = L == 0.f ? 0.f : kByteUnit<FMT> / L;
       uint32_t w[kPer / 2];
 #pragma unroll
       for (int i = 0; i < kPer; i += 2) w[i / 2] = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
@@ -775,6 +776,7 @@ int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int
   if (st) return st;
   if ((st = check_kv_cache(ctx, cache))) return st;
   WX_CHECK_ARG(ctx, cache->kv_heads == dims->kv_heads && cache->head_dim == dims->head_dim);
+  WX_CHECK_ARG(ctx, cache->format != WX_KV_INT8 || dims->scale < 0x1p100f);  // (int8 scores are formed in units of 2^13)
   if (dims->total_q == 0 || dims->batch == 0) return WX_OK;
   WX_CHECK_ARG(ctx, kv_lens && block_table && blocks_per_seq > 0);
   WX_CHECK_ARG(ctx, blocks_per_seq <= INT32_MAX / cache->page_size);

@@ -89,12 +89,16 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 // ------------------------------------------------------------------ 8-bit -> bf16
-// Two stored bytes -> a bf16 pair, exactly. int8: 128 + low 7 bits and 128 or 256 (sign bit)
-// are both bf16 numbers whose difference is the value. e4m3: its 7 low bits are the top of a
-// bf16 with the exponent off by 120 (a bf16 product by 2^120 also sets subnormals right).
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
+// Two stored bytes -> a bf16 pair, exactly, in units of kByteUnit. int8: byte + 128 as the bits of a
+// bf16 is (byte + 128) * 2^-133 (subnormal or the first binade: one line), so one fused product with 2^120
+// and sum gives byte * 2^-13. e4m3: its 7 low bits are the top of a bf16 with the exponent off by 120 (a
+// bf16 product by 2^120 also sets subnormals right).
+template <int FMT>
+constexpr float kByteUnit = FMT == kKvInt8 ? 8192.f : 1.f;
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
@@ -104,8 +108,11 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 template <int FMT>
 __device__ __forceinline__ uint32_t bytes_to_bf16x2(uint32_t a, uint32_t b, int lo, int hi) {
   if constexpr (FMT == kKvInt8) {
-    const uint32_t w = __byte_perm(a, b, (uint32_t)(lo | hi << 8));
-    return sub_bf16x2((w & 0x007f007fu) | 0x43004300u, (w & 0x00800080u) | 0x43004300u);
+    a ^= 0x80808080u;
+    // (bytes of one word are put between zeros at once)
+    const uint32_t w = hi < 4 ? __byte_perm(a, 0u, (uint32_t)(0x4040 | lo | hi << 8))
+                              : __byte_perm(a, b ^ 0x80808080u, (uint32_t)(lo | hi << 8)) & 0x00ff00ffu;
+    return fma_bf16x2(w, 0x7b807b80u, 0xbc80bc80u);  // * 2^120 - 2^-6
   } else {
     const uint32_t w = __byte_perm(a, b, (uint32_t)(lo << 4 | hi << 12));
     return mul_bf16x2((w & 0x80008000u) | ((w >> 4) & 0x07f007f0u), 0x7b807b80u);  // 2^120

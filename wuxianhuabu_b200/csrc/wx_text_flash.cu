@@ -734,7 +734,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       const int tq = lane & 3;
       const uint32_t scales = sbase + G::kScaleOff + (g % kTfScales) * 1024 + tq * 8;
       if (!mbar_wait(bar(kBTfScale + g % kTfScales), (g / kTfScales) & 1, p.err, kDevTimeoutFull, abort_flag)) return false;
-      const float2 sl2x2 = make_float2(p.sl2, p.sl2);
+      const float k_unit = p.sl2 * kByteUnit<FMT>;
+      const float2 sl2x2 = make_float2(k_unit, k_unit);
       // bits of this thread's columns that row j sees
       uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
       if (masked) {
@@ -1030,7 +1031,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       if (ok && any) ok = mbar_wait(bar(kBTfOFull + X), n_o & 1, p.err, kDevTimeoutSoftmax, abort_flag);
       n_o += any ? 1 : 0;
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : __fdividef(1.0f, l);
+      const float inv = l == 0.f ? 0.f : __fdividef(kByteUnit<FMT>, l);
       const int bad = any ? *reinterpret_cast<const volatile int*>(&it.bad) : 0;
       const bool cut = it.pieces > 1;
       const bool write = ok && live && WX_IN_BOUNDS(p.err, it.q0 + tok < p.total_q);
@@ -1072,7 +1073,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
             float* dst = tp.part + at_part * HD + c * 16;
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              *reinterpret_cast<float4*>(dst + i) =
+                  make_float4(o[i] * kByteUnit<FMT>, o[i + 1] * kByteUnit<FMT>, o[i + 2] * kByteUnit<FMT>, o[i + 3] * kByteUnit<FMT>);
           }
           continue;
         }
