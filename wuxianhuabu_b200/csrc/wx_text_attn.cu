@@ -67,9 +67,9 @@ __device__ __forceinline__ void copy_async_wait() {
 // last to arrive joins them in key order (so the result does not depend on who is last).
 //
 // Measured, caches flushed from L2: 64 sequences, 32 / 8 heads of 128, 238,000 bf16 keys 191 us =
-// 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 51 us = 2.7 TB/s
-// (4.3 TB/s a further key: the integer pipe, which expands the bytes, is the bound: issue slots 53 % busy, DRAM 34 %); a
-// call with a few keys 11 us, of which 7 on the device.
+// 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 48 us = 2.9 TB/s
+// (the expansion's instructions are the bound: issue slots 53 % busy, DRAM 34 %); a call with a few
+// keys 11 us, of which 7 on the device.
 constexpr int kUnit = 128;
 
 template <int FMT, int HD, int NT>
@@ -731,13 +731,16 @@ static int launch_rows_attn(wx_ctx* ctx, int head_dim, int64_t rows, const TextA
 }
 
 // Few flattened rows a sequence (a decoding step, a few drafted tokens) go to the rows kernel, which
-// reads the keys once per 16 rows, more to the tcgen05 kernel, which does so once per 256. Rows : tcgen05
-// at 32 sequences of 8,000 keys, 32 / 8 heads of 128: 24 rows 326 : 253 us at bf16 and 338 : 382 at
-// int8, 64 rows 618 : 259 and 657 : 390; one sequence of 65,536 keys, 24 rows 92 : 114 and 102 : 136,
-// 48 rows 121 : 118 and 142 : 142.
+// walks the keys once per 16 rows, more to the tcgen05 kernel, which does so once per 256. Rows : tcgen05
+// in us, 32 / 8 heads of 128:                 bf16        e4m3        int8
+//   32 sequences of 8,000 keys, 24 to 32 rows   326 : 253   294 : 388   244 : 376
+//                               48 rows                     431 : 392   358 : 382
+//                               64 rows         618 : 259   565 : 396   465 : 386
+//   1 sequence of 65,536 keys, 24 to 32 rows     92 : 87     91 : 116    80 : 114
+//                              48 rows          121 : 89    125 : 118   105 : 114
 static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParams& p, const KvSource& kv) {
   const int64_t rows = (int64_t)d->max_q * p.group;
-  if (rows > (kv.format == kKvBf16 ? 16 : 48)) return text_flash(ctx, p, d->head_dim, kv);
+  if (rows > (kv.format == kKvBf16 ? 16 : kv.format == kKvE4m3 ? 32 : 48)) return text_flash(ctx, p, d->head_dim, kv);
   if (kv.format == kKvInt8) return launch_rows_attn<kKvInt8>(ctx, d->head_dim, rows, p, kv);
   if (kv.format == kKvE4m3) return launch_rows_attn<kKvE4m3>(ctx, d->head_dim, rows, p, kv);
   return launch_rows_attn<kKvBf16>(ctx, d->head_dim, rows, p, kv);
