@@ -703,7 +703,7 @@ typedef struct wx_attn_dims {
   int32_t head_dim;
   int32_t causal;
   int32_t window; /* 0: none; needs causal */
-  float scale;    /* > 0 */
+  float scale;    /* > 0; over an int8 cache below 2^100 */
 } wx_attn_dims;
 /* Whole prompts, packed: sequence b has query rows cu_q[b]..cu_q[b+1] of q [total_q, q_heads,
  * head_dim] and key rows cu_k[b]..cu_k[b+1] of k, v [total_k, kv_heads, head_dim] (cu arrays on
@@ -713,7 +713,8 @@ int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, in
                         const int32_t* cu_k, void* out, int64_t out_stride, float* lse);
 /* New tokens (1 per sequence when decoding, a chunk of a prompt otherwise) over the paged cache
  * that holds them already: sequence b has kv_lens[b] cached tokens in pages block_table[b,
- * 0..], its queries being the last ones. Block entries beyond the length are not read. */
+ * 0..], its queries being the last ones. Block entries beyond the length are not read. Few query
+ * rows: batch * kv_heads * blocks_per_seq * page_size / 128 must stay below 2^32. */
 int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
                        const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
                        const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride, float* lse);

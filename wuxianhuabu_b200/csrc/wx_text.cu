@@ -132,16 +132,17 @@ __device__ __forceinline__ float quantise(const float (&x)[N], uint32_t (&w)[N /
 }
 
 template <int FMT, int HD, int W, bool INTERLEAVED>
-__global__ void __launch_bounds__(256, 4) text_rows_kernel(RowsParams p) {
+__global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
   constexpr int kLanes = HD / (2 * W);  // lanes of a row
   constexpr int kRows = 32 / kLanes;    // rows of a warp at a time
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes;
   const int per_token = p.nq + 2 * p.nkv;
-  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int64_t t = w / p.chunks;
+  // a block: eight tokens, the same chunk of each
+  const unsigned blk = blockIdx.x / (unsigned)p.chunks;
+  const int64_t t = (int64_t)blk * 8 + (threadIdx.x >> 5);
   if (t >= p.tokens) return;
-  const int r0 = (int)(w % p.chunks) * p.rows_per_warp;
+  const int r0 = (int)(blockIdx.x - blk * (unsigned)p.chunks) * p.rows_per_warp;
   const int r1 = min(per_token, r0 + p.rows_per_warp);
 
   const bool turn = j < p.rot / (2 * W);
@@ -267,10 +268,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p) {
   constexpr int kVec = FMT == kKvBf16 ? 2 : 1;  // 16-byte units of 16 values
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes;
-  const int64_t w = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int64_t t = w / p.chunks;
+  const unsigned blk = blockIdx.x / (unsigned)p.chunks;  // (as above)
+  const int64_t t = (int64_t)blk * 8 + (threadIdx.x >> 5);
   if (t >= p.tokens) return;
-  const int r0 = (int)(w % p.chunks) * p.rows_per_warp;
+  const int r0 = (int)(blockIdx.x - blk * (unsigned)p.chunks) * p.rows_per_warp;
   const int r1 = min(2 * p.nkv, r0 + p.rows_per_warp);
   int64_t slot = p.slots[t];
   if (slot >= p.n_slots) {
@@ -346,7 +347,7 @@ static int64_t deal_rows(wx_ctx* ctx, int64_t tokens, int per_token, int rows_at
          tokens * ((per_token + *rows_per_warp - 1) / *rows_per_warp) < (int64_t)ctx->num_sms * 64)
     *rows_per_warp /= 2;
   *chunks = (per_token + *rows_per_warp - 1) / *rows_per_warp;
-  return (tokens * *chunks + 7) / 8;  // blocks of 8 warps
+  return (tokens + 7) / 8 * *chunks;  // blocks of 8 warps
 }
 
 template <int FMT, int HD, int W>
