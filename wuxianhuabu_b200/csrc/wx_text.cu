@@ -43,10 +43,10 @@ __global__ void rope_table_kernel(RopeFreqs f, int nf, int64_t positions, double
 // Bound by HBM: each value is read once and written once, the table row of a token (rot * 4 bytes)
 // is shared by its heads. A warp issues the loads of all its rows (up to kRowGroups groups) before
 // the first store: the outputs may alias the inputs, so the compiler could not.
-// Measured, inputs flushed from L2: rope of 8,192 tokens, 32 + 8 heads of 128, 34.8 us = 4.9 TB/s (one
-// group at a time 49); 4,096 tokens with rope into an int8 cache and read back, 38.9 us for both. A
-// warp's rows after its first few wait for their own loads only; larger launches would go nearer to
-// the copy's 6.5 TB/s. 300 tokens take 3 us on the device, a third of the call.
+// Measured: rope of 8,192 tokens, 32 + 8 heads of 128, 36 us after a flush that leaves L2 dirty, 31.7 us
+// = 5.45 TB/s with clean lines (three or two groups in flight 43 and 67, five 38); 4,096 tokens
+// with rope into an int8 cache and read back, 40 us for both (35.6). 300 tokens take 3 us on the
+// device, a third of the call.
 constexpr int kRowGroups = 4;
 
 struct RowsParams {
