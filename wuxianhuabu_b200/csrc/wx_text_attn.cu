@@ -141,8 +141,11 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     int k_lo, k_hi;              // keys of this piece (k_lo a multiple of 16)
     int steps;                   // 16-key steps of this piece for this warp
   };
+  // the sequence found last: its first unit and item, the end of its units, its row tiles and first key
+  unsigned b_u0 = 0, b_end = 0, b_i0 = 0, rts = 1;
+  int k16 = 0;
   auto piece_at = [&](unsigned at, Piece& c) -> unsigned {
-    while (true) {
+    while (at >= b_end) {
       if (loaded != wb) {
         line_of(wb + lane, my_items, my_nu, my_k16);
         loaded = wb;
@@ -161,28 +164,30 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
       if (at < wu + all) {
         const int src = __ffs(__ballot_sync(0xffffffffu, at < wu + nc)) - 1;
         c.b = wb + src;
-        const unsigned b_u0 = wu + __shfl_sync(0xffffffffu, nc - n, src);
-        const unsigned b_i0 = wi + __shfl_sync(0xffffffffu, ic - my_items, src);
+        b_u0 = wu + __shfl_sync(0xffffffffu, nc - n, src);
+        b_end = wu + __shfl_sync(0xffffffffu, nc, src);
+        b_i0 = wi + __shfl_sync(0xffffffffu, ic - my_items, src);
         c.s = load_seq(p, c.b);
-        const unsigned rts = __shfl_sync(0xffffffffu, my_items, src) / (unsigned)p.hkv;
+        rts = __shfl_sync(0xffffffffu, my_items, src) / (unsigned)p.hkv;
         c.nu = __shfl_sync(0xffffffffu, my_nu, src);
-        const int k16 = __shfl_sync(0xffffffffu, my_k16, src);
-        const unsigned i = (at - b_u0) / c.nu, u_in = (at - b_u0) - i * c.nu;
-        c.h = (int)(i / rts);
-        c.rt = (int)(i % rts);
-        c.item = b_i0 + i;
-        c.item_u0 = b_u0 + i * c.nu;
-        const unsigned units = min(c.nu - u_in, u_end - at);
-        c.k_lo = k16 + (int)u_in * kUnit;
-        c.k_hi = min(c.s.lk, c.k_lo + (int)units * kUnit);
-        const int n16 = max(0, (c.k_hi - c.k_lo + 15) / 16);
-        c.steps = n16 > warp ? (n16 - warp + kWarps - 1) / kWarps : 0;
-        return units;
+        k16 = __shfl_sync(0xffffffffu, my_k16, src);
+        break;
       }
       wu += all;
       wi += __shfl_sync(0xffffffffu, ic, 31);
       wb += 32;
     }
+    const unsigned i = (at - b_u0) / c.nu, u_in = (at - b_u0) - i * c.nu;
+    c.h = (int)(i / rts);
+    c.rt = (int)(i % rts);
+    c.item = b_i0 + i;
+    c.item_u0 = b_u0 + i * c.nu;
+    const unsigned units = min(c.nu - u_in, u_end - at);
+    c.k_lo = k16 + (int)u_in * kUnit;
+    c.k_hi = min(c.s.lk, c.k_lo + (int)units * kUnit);
+    const int n16 = max(0, (c.k_hi - c.k_lo + 15) / 16);
+    c.steps = n16 > warp ? (n16 - warp + kWarps - 1) / kWarps : 0;
+    return units;
   };
 
   // ---- loads: step i of this warp starts at key k_lo + (i * kWarps + warp) * 16; the pages of 32
