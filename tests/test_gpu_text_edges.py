@@ -1,0 +1,85 @@
+"""The text-side operators where a mask, a value or a length is extreme: windows near the integer
+limit, infinities and NaN in keys and values that some rows see, NaN codes in an e4m3 cache.
+
+Attention is compared with its definition in 64 bits; the tolerance of finite outputs is that of the
+weights' and the output's rounding to bf16 (2^-8 of the sum of |w v|, 2^-8 of the output) and 2^-14 of the
+weights for scores and exponentials in fp32. NaN, +inf and -inf have to stand exactly where the
+definition puts them.
+"""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_text import BF16, F64, _check_device, _cu, _gen, _paged, _randn, _text, ref_attention
+
+pytestmark = pytest.mark.gpu
+INT_MAX = 2 ** 31 - 1
+
+
+def assert_same(out, lse, ref, rlse, mag, what=""):
+    for name, is_it in (("NaN", torch.isnan), ("+inf", torch.isposinf), ("-inf", torch.isneginf)):
+        assert torch.equal(is_it(out), is_it(ref)), f"{what}: {name} at other places"
+        if lse is not None:
+            assert torch.equal(is_it(lse), is_it(rlse)), f"{what}: {name} of lse at other places"
+    ok = torch.isfinite(ref)
+    tol = 2.0 ** -8 * (ref.abs() + mag) * (1 + 2.0 ** -7) + 2.0 ** -14 * mag
+    over = ((out.to(F64) - ref).abs() > tol) & ok
+    assert not over.any(), f"{what}: {int(over.sum())} outputs off"
+    if lse is not None:
+        fin = torch.isfinite(rlse)
+        e = (lse.to(F64) - rlse)[fin].abs()
+        assert e.numel() == 0 or float((e - 2.0 ** -20 * rlse[fin].abs()).max()) < 2e-5, f"{what}: lse"
+
+
+# ---------------------------------------------------------------------------------- windows
+@pytest.mark.parametrize("window", [INT_MAX, INT_MAX - 7, 2 ** 30, 2 ** 31, 2 ** 32 + 3])
+@pytest.mark.parametrize("lens_q,lens_k,hq,hkv,hd", [
+    ([5, 3], [3, 3], 4, 2, 128),            # few rows
+    ([16, 7, 2], [2, 0, 40], 2, 2, 64),
+    ([130, 300], [20, 290], 8, 2, 128),     # many rows
+    ([400], [130], 4, 4, 64),
+])
+def test_a_window_that_holds_every_key_hides_none(lens_q, lens_k, hq, hkv, hd, window):
+    """More query than key rows (some see nothing) under windows up to and beyond the 32-bit limit."""
+    text = _text()
+    g = _gen(sum(lens_q) + hd)
+    q = _randn(g, sum(lens_q), hq, hd)
+    k, v = _randn(g, sum(lens_k), hkv, hd), _randn(g, sum(lens_k), hkv, hd)
+    out, lse = text.prompt_attention(q, k, v, _cu(lens_q), max(lens_q), window=window, cu_seqlens_k=_cu(lens_k),
+                                     return_lse=True)
+    _check_device()
+    a = b = 0
+    for n, m in zip(lens_q, lens_k):
+        ref, rl, mag = ref_attention(q[a:a + n], k[b:b + m], v[b:b + m], 1 / math.sqrt(hd), True, 0)
+        assert_same(out[a:a + n], lse[a:a + n], ref, rl, mag, f"{n} over {m}")
+        a, b = a + n, b + m
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("q_lens,kv_lens", [([9, 30], [4, 20]), ([3], [1]), ([200], [150])])
+def test_a_window_that_holds_the_whole_cache_hides_nothing(fmt, q_lens, kv_lens):
+    text = _text()
+    g = _gen(sum(q_lens))
+    cache, table, q, ks, vs = _paged(g, fmt, q_lens, kv_lens, 4, 2, 128, 16)
+    lens = torch.tensor(kv_lens, dtype=torch.int32, device="cuda")
+    out, lse = text.paged_attention(q, cache, _cu(q_lens), lens, table, max(q_lens), window=INT_MAX, return_lse=True)
+    _check_device()
+    a = 0
+    for n, k, v in zip(q_lens, ks, vs):
+        ref, rl, mag = ref_attention(q[a:a + n], k, v, 1 / math.sqrt(128), True, 0)
+        assert_same(out[a:a + n], lse[a:a + n], ref, rl, mag, f"{n} over {k.shape[0]}")
+        a += n
+
+
+def test_windows_below_zero_are_refused_whatever_their_low_bits():
+    text = _text()
+    from wuxianhuabu_b200 import _lib, h3
+    g = _gen(1)
+    q = _randn(g, 4, 2, 64)
+    for window in (-1, -2 ** 32, -2 ** 32 + 5):
+        with pytest.raises(h3.WxError) as e:
+            text.prompt_attention(q, q, q, _cu([4]), 4, window=window)
+        assert e.value.status == _lib.WX_ERR_INVALID
+
+

@@ -74,12 +74,14 @@ __device__ __forceinline__ Seq load_seq(const TextAttnParams& p, int b) {
   return s;
 }
 
-// keys [lo, hi) that query token `tok` of a sequence sees
+// Keys [lo, hi) that query token `tok` of a sequence sees. In 32 bits for every length and window:
+// tok - lq is above -2^31 and below 0, and a window is taken off a number that is not below 0 (off a
+// negative one, one near 2^31 would wrap to a bound beyond every key).
 __device__ __forceinline__ int key_hi(const TextAttnParams& p, const Seq& s, int tok) {
-  return p.causal ? max(0, min(s.lk, tok + s.lk - s.lq + 1)) : s.lk;
+  return p.causal ? max(0, min(s.lk, tok - s.lq + s.lk + 1)) : s.lk;
 }
 __device__ __forceinline__ int key_lo(const TextAttnParams& p, const Seq& s, int tok) {
-  return p.window > 0 ? max(0, tok + s.lk - s.lq - p.window + 1) : 0;
+  return p.window > 0 ? max(0, max(0, tok - s.lq + s.lk + 1) - p.window) : 0;
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {

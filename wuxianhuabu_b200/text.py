@@ -240,9 +240,15 @@ def _batch_of(cu_seqlens: torch.Tensor) -> int:
     return batch
 
 
+def _int32(n: int) -> int:
+    """n, or the int32 nearest to it (a struct's field would keep the low bits)."""
+    return max(-1 << 31, min(n, (1 << 31) - 1))
+
+
 def _dims(n: int, batch: int, max_len: int, h: int, hk: int, d: int, causal: bool, window: int,
           scale: Optional[float]):
-    return C.byref(AttnDims(n, batch, max_len, h, hk, d, causal, window, d ** -0.5 if scale is None else scale))
+    return C.byref(AttnDims(n, batch, _int32(max_len), h, hk, d, causal, _int32(window),
+                            d ** -0.5 if scale is None else scale))
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_len: int,
