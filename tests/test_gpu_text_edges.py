@@ -83,3 +83,57 @@ def test_windows_below_zero_are_refused_whatever_their_low_bits():
         assert e.value.status == _lib.WX_ERR_INVALID
 
 
+# ------------------------------------------------------------- infinities and NaN in values
+def _spoil(v, first, last):
+    """Infinities and NaN in values at keys of [first, last): of one sign, of both in a column, NaN beside
+    infinity, in the first and the last columns."""
+    at = torch.linspace(first, last - 1, 7, device=v.device).long().tolist()
+    v[at[0], 0, 0], v[at[1], 0, -1] = math.inf, -math.inf
+    v[at[2], -1, 3], v[at[4], -1, 3] = math.inf, -math.inf
+    v[at[2], -1, 33], v[at[3], -1, 33] = math.inf, math.inf
+    v[at[4], 0, 40], v[at[6], 0, 40] = -math.inf, math.nan
+    v[at[5], -1, -2], v[at[6], 0, 17] = -math.inf, math.inf
+
+
+@pytest.mark.parametrize("hd,hq,hkv", [(128, 8, 2), (64, 4, 2), (64, 3, 3)])
+@pytest.mark.parametrize("lens,causal,window,first,last", [
+    ([300], True, 0, 0, 300),        # tiles that every row sees, and tiles under the diagonal
+    ([300], True, 0, 250, 300),
+    ([220, 260], True, 90, 0, 480),  # and tiles that the window cuts
+    ([200], False, 0, 30, 200),
+])
+def test_prompt_attention_keeps_infinities(hd, hq, hkv, lens, causal, window, first, last):
+    text = _text()
+    g = _gen(sum(lens) + hd)
+    n = sum(lens)
+    q, k, v = _randn(g, n, hq, hd), _randn(g, n, hkv, hd), _randn(g, n, hkv, hd)
+    _spoil(v, first, last)
+    out, lse = text.prompt_attention(q, k, v, _cu(lens), max(lens), causal=causal, window=window, return_lse=True)
+    _check_device()
+    a = 0
+    for m in lens:
+        s = slice(a, a + m)
+        ref, rl, mag = ref_attention(q[s], k[s], v[s], 1 / math.sqrt(hd), causal, window)
+        assert_same(out[s], lse[s], ref, rl, mag, f"len {m}")
+        a += m
+
+
+@pytest.mark.parametrize("hd,hq,hkv,page", [(128, 4, 2, 16), (64, 4, 2, 64), (128, 16, 8, 32)])
+@pytest.mark.parametrize("nq,n,window", [(1, 200, 0), (3, 200, 0), (7, 150, 60), (5, 4, 0), (100, 260, 0), (90, 2300, 0)])
+def test_paged_attention_keeps_infinities(hd, hq, hkv, page, nq, n, window):
+    """Values of the last keys, which only some of the new tokens see, and of keys that all of them see."""
+    text = _text()
+    g = _gen(nq + n + hd)
+    cache, table, q, ks, vs = _paged(g, "bf16", [nq], [n], hq, hkv, hd, page)
+    first = max(0, n - 2 * nq)
+    _spoil(vs[0], first, n)
+    j = torch.arange(n, device="cuda")
+    cache.append(ks[0], vs[0], table[0].long()[j // page] * page + j % page)
+    out, lse = text.paged_attention(q, cache, _cu([nq]), torch.tensor([n], dtype=torch.int32, device="cuda"), table, nq,
+                                    window=window, return_lse=True)
+    _check_device()
+    # (the definition's product takes lq * lk * hd numbers a head: the keys before `first` are finite)
+    ref, rl, mag = ref_attention(q, ks[0], vs[0], 1 / math.sqrt(hd), True, window)
+    assert_same(out, lse, ref, rl, mag)
+
+

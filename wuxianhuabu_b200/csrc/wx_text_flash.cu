@@ -43,8 +43,10 @@ constexpr int kTfChunk = 128 * 128;  // one 64-column SW128 chunk of a 128-row t
 constexpr int kTfWaves = 3;          // pieces for each SM below which items are cut up
 constexpr int kTfMinTiles = 8;       // tiles of a piece of an item: its start and end cost one or two
 constexpr int64_t kTfL2 = int64_t(48) << 20;
-constexpr int kTfBadRows = 1024;     // V rows with non-finite values remembered per item
-constexpr int kTfBadWords = 5;       // key, 128-bit column mask
+// V rows with non-finite values remembered per item: every row of its masked tiles (an item's 256 tokens
+// end, and where a window cuts begin, in up to three tiles each)
+constexpr int kTfBadRows = 6 * 128;
+constexpr int kTfBadWords = 9;       // key, columns with +infinity or NaN, columns with -infinity or NaN
 
 template <int FMT, int HD>
 struct TfGeom {
@@ -156,22 +158,30 @@ __device__ __forceinline__ void tmem_st_half4(uint32_t taddr, const uint32_t* v)
                : "memory");
 }
 
-// Zeroes the non-finite values of row r of a V tile and notes their columns in `entry`.
+// Zeroes the non-finite values of row r of a V tile and notes their columns and signs in `entry`.
 template <int HD>
 __device__ __noinline__ void remember_row(uint32_t row, int r, int key, uint32_t* entry) {
-  uint32_t mask[4] = {0, 0, 0, 0};
+  uint32_t plus[4] = {0, 0, 0, 0}, minus[4] = {0, 0, 0, 0};
 #pragma unroll 1
   for (int d = 0; d < HD; ++d) {
     const uint32_t at = row + (d >> 6) * kTfChunk + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2;
-    if ((lds_u16(at) & 0x7f80u) != 0x7f80u) continue;
+    const uint32_t x = lds_u16(at);
+    if ((x & 0x7f80u) != 0x7f80u) continue;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) mask[e] |= (d >> 5) == e ? 1u << (d & 31) : 0u;
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t bit = (d >> 5) == e ? 1u << (d & 31) : 0u;
+      if (x != 0xff80u) plus[e] |= bit;
+      if (x != 0x7f80u) minus[e] |= bit;
+    }
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((uint16_t)0) : "memory");
   }
   if (!entry) return;
   entry[0] = (uint32_t)key;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) entry[1 + e] = mask[e];
+  for (int e = 0; e < 4; ++e) {
+    entry[1 + e] = plus[e];
+    entry[5 + e] = minus[e];
+  }
 }
 
 __device__ __forceinline__ float2 lds_f2(uint32_t a) {
@@ -1054,19 +1064,25 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[i] = 0.f;
         }
-        if (bad) {  // non-finite values of V that this row does see
+        if (bad) {  // non-finite values of V that this row does see: infinities add up, both signs to NaN
           const int col = c * 16;
-          uint32_t hit = bad > kTfBadRows ? ~0u : 0u;
+          uint32_t plus = 0u, minus = 0u;
           const uint32_t* list =
               tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
 #pragma unroll 1
           for (int e = 0; e < min(bad, kTfBadRows); ++e) {
-            const int key = (int)__ldcg(list + e * kTfBadWords);
-            if (key >= lo && key < hi) hit |= __ldcg(list + e * kTfBadWords + 1 + (col >> 5)) >> (col & 31);
+            const uint32_t* entry = list + e * kTfBadWords;
+            const int key = (int)__ldcg(entry);
+            if (key >= lo && key < hi) {
+              plus |= __ldcg(entry + 1 + (col >> 5)) >> (col & 31);
+              minus |= __ldcg(entry + 5 + (col >> 5)) >> (col & 31);
+            }
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (hit >> i & 1u) o[i] = __int_as_float(0x7fc00000);
+          for (int i = 0; i < 16; ++i) {
+            if (plus >> i & 1u) o[i] += INFINITY;
+            if (minus >> i & 1u) o[i] -= INFINITY;
+          }
         }
         if (cut) {
           if (write) {
