@@ -676,7 +676,8 @@ typedef struct wx_kv_cache {
  * offset (device; < 0 skips the token). 8-bit formats: scale = amax / 127 (int8) or
  * amax / 448 (e4m3) of the row, value = x * (127 | 448) / amax to nearest even; a row with
  * infinity or NaN gets scale NaN (it reads back as NaN), one below 2^-100 throughout zeros.
- * A slot beyond the cache is skipped and sets the device error word. */
+ * A slot beyond the cache is skipped and sets the device error word. The writes store no e4m3 NaN
+ * code (0x7f, 0xff); in a cache that was filled elsewhere one is NaN to every call that sees it. */
 int wx_kv_append(wx_ctx* ctx, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
                  int64_t v_stride, int64_t tokens, const int64_t* slots);
 /* wx_rope_apply of q into q_out and of k, and wx_kv_append, in one launch: the turned k is

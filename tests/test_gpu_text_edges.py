@@ -137,3 +137,75 @@ def test_paged_attention_keeps_infinities(hd, hq, hkv, page, nq, n, window):
     assert_same(out, lse, ref, rl, mag)
 
 
+# --------------------------------------------------------------- NaN codes of an e4m3 cache
+def _with_nan_codes(cache, table, page, ks, vs, spots):
+    """NaN codes at spots (kind, key, head, column) of sequence 0; the expected values with them."""
+    for i, (kind, j, h, c) in enumerate(spots):
+        at = int(table[0, j // page])
+        buf, ref = (cache.k, ks[0]) if kind == "k" else (cache.v, vs[0])
+        buf.view(torch.uint8)[at, h, j % page, c] = 0x7f if i % 2 else 0xff
+        ref[j, h, c] = math.nan
+
+
+@pytest.mark.parametrize("hd,hq,hkv,page", [(128, 8, 2, 64), (64, 4, 4, 16), (128, 16, 2, 128)])
+@pytest.mark.parametrize("nq,n,window", [(1, 150, 0), (2, 700, 0), (6, 150, 0), (6, 400, 130), (90, 150, 0), (300, 333, 0),
+                                         (64, 3000, 0)])
+@pytest.mark.parametrize("kind", ["v", "k"])
+def test_nan_codes_of_an_e4m3_cache_are_nan(hd, hq, hkv, page, nq, n, window, kind):
+    """Written by somebody else (this package's writes saturate): NaN for the rows that see them, in all
+    columns for a key, in its own column for a value, and to nobody else; kv_read says the same."""
+    text = _text()
+    g = _gen(nq + n + hd)
+    cache, table, q, ks, vs = _paged(g, "e4m3", [nq], [n], hq, hkv, hd, page)
+    if kind == "v":
+        spots = [("v", 0, 0, 0), ("v", n // 2, hkv - 1, 37), ("v", n // 2, hkv - 1, hd - 1), ("v", n - 1, 0, 5),
+                 ("v", n - 1, hkv - 1, 16), ("v", max(0, n - nq // 2 - 1), 0, 63), ("v", n - n // 3, 0, 5)]
+    else:
+        spots = [("k", n - 1, 0, 9), ("k", max(0, n - nq // 2 - 1), hkv - 1, hd - 1), ("k", n - 2, hkv - 1, 0)]
+    _with_nan_codes(cache, table, page, ks, vs, spots)
+    last = int(table[0, (n - 1) // page])
+    if n % page:  # behind the last key: NaN codes and scales that nobody sees
+        for t in (cache.k, cache.v):
+            t.view(torch.uint8)[last, :, n % page:] = 0x7f
+        cache.k_scale[last, :, n % page:] = math.nan
+        cache.v_scale[last, :, n % page:] = math.nan
+    out, lse = text.paged_attention(q, cache, _cu([nq]), torch.tensor([n], dtype=torch.int32, device="cuda"), table, nq,
+                                    window=window, return_lse=True)
+    j = torch.arange(n, device="cuda")
+    kr, vr = cache.read(table[0].long()[j // page] * page + j % page)
+    _check_device()
+    assert torch.equal(torch.isnan(kr), torch.isnan(ks[0])) and torch.equal(torch.isnan(vr), torch.isnan(vs[0]))
+    scale = 1 / math.sqrt(hd)
+    if kind == "v":
+        # the definition with zeros in those places, and NaN for the rows and columns that see one
+        ref, rl, mag = ref_attention(q, ks[0], torch.nan_to_num(vs[0], nan=0.0), scale, True, window)
+        i = torch.arange(nq, device="cuda")[:, None] + (n - nq)
+        sees = (j[None] <= i) & ((j[None] > i - window) if window else torch.ones_like(j[None] <= i))
+        hit = torch.einsum("ij,jhd->ihd", sees.float(), torch.isnan(vs[0]).float()) > 0
+        ref[hit.repeat_interleave(hq // hkv, 1)] = math.nan
+    else:
+        ref, rl, mag = ref_attention(q, ks[0], vs[0], scale, True, window)
+    assert_same(out, lse, ref, rl, mag)
+
+
+def test_every_e4m3_code_reads_as_itself():
+    """All 256 codes, in a cache made elsewhere: read back, and as the value of the only key of a sequence."""
+    text = _text()
+    codes = torch.arange(256, dtype=torch.uint8, device="cuda").view(2, 1, 1, 128).expand(2, 1, 16, 128).contiguous()
+    v = codes.view(torch.float8_e4m3fn)
+    ones = torch.ones((2, 1, 16), dtype=torch.float32, device="cuda")
+    zeros = torch.zeros_like(codes).view(torch.float8_e4m3fn)
+    cache = text.PagedKVCache.from_tensors(zeros, v, ones, ones.clone())
+    want = v.float()[:, 0, 0]
+    got = cache.read(torch.tensor([3, 20], device="cuda"))[1][:, 0].float()
+    q = torch.ones((2, 1, 128), dtype=BF16, device="cuda")
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    lens = torch.ones(2, dtype=torch.int32, device="cuda")
+    few = text.paged_attention(q, cache, _cu([1, 1]), lens, table, 1)[:, 0].float()
+    many = text.paged_attention(torch.ones((200, 1, 128), dtype=BF16, device="cuda"), cache, _cu([100, 100]), lens, table,
+                                100)[[99, 199], 0].float()
+    _check_device()
+    for x in (got, few, many):
+        assert torch.equal(torch.nan_to_num(x, nan=1e9), torch.nan_to_num(want, nan=1e9))
+
+

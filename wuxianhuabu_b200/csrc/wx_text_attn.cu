@@ -440,6 +440,41 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
           }
         }
       bool slow = false;
+      if constexpr (FMT == kKvE4m3) {
+        if (masked) {
+          // NaN codes of values that only some rows see: zero in the products, NaN in their columns of the
+          // rows that do see them (int8 has none; a NaN scale is the weight's, and that is 0 where unseen)
+          uint32_t codes[4], odd = 0;  // of this lane's keys, a bit a column
+#pragma unroll
+          for (int rr = 0; rr < 4; ++rr) {
+            uint4& x = vf.v[rr][0];
+            codes[rr] = nan_code_mask(x.x) | nan_code_mask(x.y) << 4;
+            if constexpr (HD == 128) codes[rr] |= nan_code_mask(x.z) << 8 | nan_code_mask(x.w) << 12;
+            odd |= codes[rr];
+          }
+          if (__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+            for (int rr = 0; rr < 4; ++rr) {
+              uint4& x = vf.v[rr][0];
+              x = make_uint4(without_nan_codes(x.x), without_nan_codes(x.y), without_nan_codes(x.z), without_nan_codes(x.w));
+            }
+#pragma unroll 1
+            for (int kk = 0; kk < 16; ++kk) {
+              const int from = g * 4 + ((kk & 7) >> 1), rr = (kk & 1) + 2 * (kk >> 3), j = j0 + kk;
+              const uint32_t mine = rr == 0 ? codes[0] : rr == 1 ? codes[1] : rr == 2 ? codes[2] : codes[3];
+              const uint32_t x = __shfl_sync(0xffffffffu, mine, from);
+#pragma unroll
+              for (int d = 0; d < HD / 8; ++d)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if ((x >> d & 1u) && j < lim_hi[n][e] && j >= lim_lo[n][e])
+                      acc[n][d >> 1][2 * (d & 1) + e] = __int_as_float(0x7fc00000);
+            }
+          }
+        }
+      }
       if constexpr (!kW) {
         if (masked) {
           // 0 * NaN is NaN: keys past the end are zeroed; with a non-finite value at a key that only

@@ -77,7 +77,7 @@ struct TfItem {
   int lq, lk, q0, k0;
   int a0, a1, b0, b1;    // key tiles [a0, a1) of slot A, [b0, b1) of slot B
   int free_hi, free_lo;  // tiles inside [free_lo, free_hi) are unmasked for every row
-  int bad;               // V rows with non-finite values found in masked tiles
+  int bad;               // V rows with non-finite values (8-bit: NaN codes) found in masked tiles
   int piece, pieces;     // this part of the item's key tiles, and how many it was cut into
   __device__ int lo(int X) const { return X ? b0 : a0; }
   __device__ int hi(int X) const { return X ? b1 : a1; }
@@ -181,6 +181,45 @@ __device__ __noinline__ void remember_row(uint32_t row, int r, int key, uint32_t
   for (int e = 0; e < 4; ++e) {
     entry[1 + e] = plus[e];
     entry[5 + e] = minus[e];
+  }
+}
+
+// The same for the NaN codes of 64 raw e4m3 rows from `key0`, before 128 threads expand them: each thread
+// looks at the 16 bytes that it will expand itself (HD / 16 lanes a row), zeroes the codes there, and
+// their columns go to a new entry of the item's list, one a row. Behind the last key nobody sees them.
+template <int HD>
+__device__ __noinline__ void remember_codes(uint32_t raw, int tid, int key0, int lk, int& bad, uint32_t* list) {
+  constexpr int kLanes = HD / 16;
+  const int c = tid % kLanes;
+#pragma unroll 1
+  for (int u = tid; u < 64 * kLanes; u += 128) {
+    const uint32_t at = raw + (uint32_t)u * 16;
+    const uint4 w = lds128(at);
+    const uint32_t bits =
+        nan_code_mask(w.x) | nan_code_mask(w.y) << 4 | nan_code_mask(w.z) << 8 | nan_code_mask(w.w) << 12;
+    if (!__any_sync(0xffffffffu, bits != 0)) continue;
+    sts128(at, make_uint4(without_nan_codes(w.x), without_nan_codes(w.y), without_nan_codes(w.z), without_nan_codes(w.w)));
+    uint32_t mask[4], any = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      mask[e] = (c >> 1) == e ? bits << (16 * (c & 1)) : 0u;
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) mask[e] |= __shfl_xor_sync(0xffffffffu, mask[e], o);
+      any |= mask[e];
+    }
+    const int key = key0 + u / kLanes;
+    if (c == 0 && any && key < lk) {
+      const int slot = atomicAdd(&bad, 1);
+      if (slot < kTfBadRows) {
+        uint32_t* entry = list + slot * kTfBadWords;
+        entry[0] = (uint32_t)key;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) entry[1 + e] = entry[5 + e] = mask[e];
+      }
+      __threadfence_block();
+    }
+    __syncwarp();
+    fence_proxy_async_smem();  // the rows that are copied here next come after these zeros
   }
 }
 
@@ -311,7 +350,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         return (((int64_t)page * p.hkv + it.h) << p.page_shift) | (j & ((1 << p.page_shift) - 1));
       };
       // 8-bit: a tile in two halves of 64 raw rows, its scales with the keys; rows past the
-      // sequence's last key are not loaded (what stands there is finite, and masked)
+      // sequence's last key are not loaded (any byte expands to a finite value or, in K, NaN: masked)
       auto load_raw = [&](bool is_k, int t) -> bool {
         const int per_half = 64 / tp.box;
         const int page = page_of(t * boxes, lane % boxes);
@@ -654,6 +693,9 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       const TfItem* at = take_item(n);
       if (!at) break;
       const int t0 = at->first(), tiles = at->last() - t0;
+      const uint32_t at_first = nk;  // (K and V tiles before this item: as many)
+      uint32_t* list =
+          tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
 #pragma unroll 1
       for (int i = 0; i < 2 * tiles && ok; ++i) {  // in the producer's order
         const bool tail = i >= 2 * tiles - 1;
@@ -666,12 +708,17 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           break;
         }
         const uint32_t dst = is_k ? sK(s) : sV(s);
+        const int t = t0 + (int)(cnt - at_first);
+        const bool masked = at->masked(t);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half, ++nr) {
           const uint32_t rs = nr % kTfRaw;
           if (ok && !mbar_wait(bar(kBTfRawFull + rs), (nr / kTfRaw) & 1, p.err, kDevTimeoutFull, abort_flag)) ok = false;
           if (!ok) break;
           const uint32_t raw = sbase + G::kRawOff + rs * G::kRawBytes;
+          // (NaN codes do what they should in a key and in a value that every row sees)
+          if (FMT == kKvE4m3 && !is_k && masked)
+            remember_codes<HD>(raw, tid, t * 128 + half * 64, at->lk, items[n % kTfItems].bad, list);
 #pragma unroll
           for (int j = 0; j < 64 * HD / 16 / 128; ++j) {
             const int u = j * 128 + tid, row = half * 64 + u / (HD / 16), c = u % (HD / 16);
