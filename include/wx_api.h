@@ -146,13 +146,16 @@ typedef struct wx_mod_run {
 /* ------------------------------------------------------------- context */
 int wx_ctx_create(int device, wx_ctx** out);
 int wx_ctx_destroy(wx_ctx* ctx);
-/* stream: a cudaStream_t (NULL = legacy default stream) */
+/* stream: a cudaStream_t (NULL = legacy default stream). A stream that is being captured is
+ * allowed: the captured work keeps scratch of its own, which lives as long as the context, so
+ * replays of its graphs may run beside direct calls. All that was captured through one context
+ * shares it: order the replays among each other, and branches of a capture too. */
 int wx_ctx_set_stream(wx_ctx* ctx, void* stream);
 const char* wx_last_error(wx_ctx* ctx);
 /* synchronises the stream and returns WX_ERR_DEVICE if a kernel set the
  * device error word since the last call (the word is cleared) */
 int wx_ctx_check_device(wx_ctx* ctx);
-/* bytes currently held by the context workspace arena */
+/* bytes currently held by the context's workspace (direct and captured work) */
 size_t wx_ctx_workspace_bytes(wx_ctx* ctx);
 /* number of kernels this context has launched so far */
 int64_t wx_ctx_launch_count(wx_ctx* ctx);

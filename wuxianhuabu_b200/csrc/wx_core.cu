@@ -30,25 +30,49 @@ int set_error(wx_ctx* ctx, int status, const char* fmt, ...) {
   return status;
 }
 
+static bool stream_capturing(wx_ctx* ctx) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess) {  // (the legacy stream beside another's capture)
+    cudaGetLastError();
+    return false;
+  }
+  return st != cudaStreamCaptureStatusNone;
+}
+
+// Allows this thread what a capture under way would refuse (allocation): it is not part of the graph.
+struct OutsideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 void* workspace(wx_ctx* ctx, size_t bytes, int* status) {
   *status = WX_OK;
-  if (bytes <= ctx->ws_bytes) return ctx->ws;
-  if (ctx->ws) {
+  const bool capturing = stream_capturing(ctx);
+  wx_ctx::Scratch& own = capturing ? ctx->captured : ctx->direct;
+  if (bytes <= own.ws_bytes) return own.ws;
+  OutsideCapture outside;
+  size_t want = (bytes + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
+  if (own.ws && capturing) {
+    want = std::max(want, 2 * own.ws_bytes);  // (the retired buffers stay below the one in use)
+    ctx->retired.push_back(own.ws);
+    ctx->retired_bytes += own.ws_bytes;
+  } else if (own.ws) {
     // the arena may still be read by work queued on the stream
     cudaStreamSynchronize(ctx->stream);
-    cudaFree(ctx->ws);
-    ctx->ws = nullptr;
-    ctx->ws_bytes = 0;
+    cudaFree(own.ws);
   }
-  size_t want = (bytes + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
-  cudaError_t e = cudaMalloc(&ctx->ws, want);
+  own.ws = nullptr;
+  own.ws_bytes = 0;
+  cudaError_t e = cudaMalloc(&own.ws, want);
   if (e != cudaSuccess) {
-    ctx->ws = nullptr;
+    cudaGetLastError();
+    own.ws = nullptr;
     *status = set_error(ctx, WX_ERR_NOMEM, "workspace of %zu bytes: %s", want, cudaGetErrorString(e));
     return nullptr;
   }
-  ctx->ws_bytes = want;
-  return ctx->ws;
+  own.ws_bytes = want;
+  return own.ws;
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -126,26 +150,45 @@ int make_tmap_bf16_3d(wx_ctx* ctx, CUtensorMap* map, const void* base, const uin
   return WX_OK;
 }
 
+// zeroes n counters before it returns, on a stream of its own (the context's may be capturing)
+static cudaError_t zero_now(int* p, int64_t n) {
+  cudaStream_t s = nullptr;
+  cudaError_t e = cudaStreamCreateWithFlags(&s, cudaStreamNonBlocking);
+  if (e != cudaSuccess) return e;
+  e = cudaMemsetAsync(p, 0, (size_t)n * sizeof(int), s);
+  const cudaError_t done = cudaStreamSynchronize(s);
+  cudaStreamDestroy(s);
+  return e != cudaSuccess ? e : done;
+}
+
 int* arrival_counters(wx_ctx* ctx, int64_t n, int* status) {
   *status = WX_OK;
-  if (n <= ctx->n_arrivals) return ctx->arrivals;
-  if (ctx->arrivals) {
+  const bool capturing = stream_capturing(ctx);
+  wx_ctx::Scratch& own = capturing ? ctx->captured : ctx->direct;
+  if (n <= own.n_arrivals) return own.arrivals;
+  OutsideCapture outside;
+  int64_t want = std::max<int64_t>((n + 4095) & ~int64_t(4095), 16384);
+  if (own.arrivals && capturing) {
+    want = std::max(want, 2 * own.n_arrivals);
+    ctx->retired.push_back(own.arrivals);
+    ctx->retired_bytes += (size_t)own.n_arrivals * sizeof(int);
+  } else if (own.arrivals) {
     cudaStreamSynchronize(ctx->stream);  // queued work may still count on them
-    cudaFree(ctx->arrivals);
-    ctx->arrivals = nullptr;
-    ctx->n_arrivals = 0;
+    cudaFree(own.arrivals);
   }
-  const int64_t want = std::max<int64_t>((n + 4095) & ~int64_t(4095), 16384);
-  cudaError_t e = cudaMalloc(&ctx->arrivals, (size_t)want * sizeof(int));
-  if (e == cudaSuccess) e = cudaMemsetAsync(ctx->arrivals, 0, (size_t)want * sizeof(int), ctx->stream);
+  own.arrivals = nullptr;
+  own.n_arrivals = 0;
+  cudaError_t e = cudaMalloc(&own.arrivals, (size_t)want * sizeof(int));
+  if (e == cudaSuccess) e = zero_now(own.arrivals, want);
   if (e != cudaSuccess) {
-    if (ctx->arrivals) cudaFree(ctx->arrivals);
-    ctx->arrivals = nullptr;
+    cudaGetLastError();
+    if (own.arrivals) cudaFree(own.arrivals);
+    own.arrivals = nullptr;
     *status = set_error(ctx, WX_ERR_NOMEM, "%lld arrival counters: %s", (long long)want, cudaGetErrorString(e));
     return nullptr;
   }
-  ctx->n_arrivals = want;
-  return ctx->arrivals;
+  own.n_arrivals = want;
+  return own.arrivals;
 }
 
 int launch_status(wx_ctx* ctx, const char* what, int n) {
@@ -361,8 +404,11 @@ int wx_ctx_destroy(wx_ctx* ctx) {
   if (ctx->aux) cudaStreamDestroy(ctx->aux);
   if (ctx->fork) cudaEventDestroy(ctx->fork);
   if (ctx->join) cudaEventDestroy(ctx->join);
-  if (ctx->ws) cudaFree(ctx->ws);
-  if (ctx->arrivals) cudaFree(ctx->arrivals);
+  for (wx_ctx::Scratch* own : {&ctx->direct, &ctx->captured}) {
+    if (own->ws) cudaFree(own->ws);
+    if (own->arrivals) cudaFree(own->arrivals);
+  }
+  for (void* p : ctx->retired) cudaFree(p);
   if (ctx->dev_err) cudaFree(ctx->dev_err);
   delete ctx;
   return WX_OK;
@@ -421,7 +467,9 @@ int wx_ctx_synchronize(wx_ctx* ctx) {
   return WX_OK;
 }
 
-size_t wx_ctx_workspace_bytes(wx_ctx* ctx) { return ctx ? ctx->ws_bytes : 0; }
+size_t wx_ctx_workspace_bytes(wx_ctx* ctx) {
+  return ctx ? ctx->direct.ws_bytes + ctx->captured.ws_bytes + ctx->retired_bytes : 0;
+}
 
 int64_t wx_ctx_launch_count(wx_ctx* ctx) { return ctx ? ctx->launches : -1; }
 

@@ -15,8 +15,18 @@ struct wx_ctx {
   int num_sms = 148;
   cudaStream_t stream = nullptr;
   int* dev_err = nullptr;         // device error word (wx::DevErr)
-  void* ws = nullptr;             // workspace arena
-  size_t ws_bytes = 0;
+  // Workspace arena, and arrival counters of kernels whose CTAs join partial results
+  // (arrival_counters). Direct calls use one set. Work captured into a CUDA graph uses the other: a
+  // graph keeps the addresses, so its buffers are never freed while the context lives (one that has
+  // become too small goes to `retired`), and a replay shares nothing with direct calls beside it.
+  struct Scratch {
+    void* ws = nullptr;
+    size_t ws_bytes = 0;
+    int* arrivals = nullptr;
+    int64_t n_arrivals = 0;
+  } direct, captured;
+  std::vector<void*> retired;
+  size_t retired_bytes = 0;
   std::string last_error;
   int64_t launches = 0;  // kernels launched through this context
   // sequence-parallel group (Ulysses): NCCL communicator, size, rank
@@ -54,9 +64,6 @@ struct wx_ctx {
   void* p2p_peer[8] = {};
   int* p2p_counters = nullptr;
   uint32_t p2p_epoch = 0;
-  // arrival counters of kernels whose CTAs join partial results (arrival_counters)
-  int* arrivals = nullptr;
-  int64_t n_arrivals = 0;
   // limit of the cross-GPU flag waits (sequence-parallel exchange, wx_ctx_wait_flags)
   uint64_t peer_wait_ns = 10000000000ull;
 };
@@ -79,7 +86,8 @@ int set_error(wx_ctx* ctx, int status, const char* fmt, ...);
   } while (0)
 
 // Returns a device buffer of at least `bytes` from the context arena (grown on
-// demand; contents undefined; valid until the next call that grows it).
+// demand, during a stream capture too; contents undefined; valid until the next call that
+// grows it, and for the graph that a capture makes as long as the context).
 void* workspace(wx_ctx* ctx, size_t bytes, int* status);
 
 // Carves 256-byte-aligned sub-buffers out of one arena request.
