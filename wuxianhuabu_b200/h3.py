@@ -53,6 +53,11 @@ _current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
+def _capturing(s: torch.cuda.Stream) -> bool:
+    with torch.cuda.stream(s):
+        return torch.cuda.is_current_stream_capturing()
+
+
 class Context:
     """One libwx context per CUDA device; calls are ordered on torch's current stream."""
 
@@ -67,22 +72,40 @@ class Context:
         if st != 0:
             raise WxError(st, f"wx_ctx_create(device={device}) failed")
         self.h = h
-        self._stream: Optional[torch.cuda.Stream] = None
-        self._raw_stream: Optional[int] = None  # the context's stream, as set last
+        self._raw_stream: Optional[int] = None  # the context's stream, where it need not be looked at again
+        self._direct: Optional[torch.cuda.Stream] = None    # last stream of direct calls,
+        self._done: Optional[torch.cuda.Event] = None       # or, if it was a caller's own, the calls on it
+        self._captured: Optional[torch.cuda.Stream] = None  # last stream of captured calls
+        self._record = False  # the next call is on a caller's own stream
 
     def sync_stream(self) -> None:
+        """Puts the context on torch's current stream. Its scratch is shared (direct calls have one set,
+        captured ones another): a direct call waits for the direct calls on the last stream, a captured
+        one for those on another branch of its capture."""
         raw = _current_raw_stream(self.device)
         if raw == self._raw_stream:
             return
         s = torch.cuda.current_stream(self.device)
-        # the context's workspace is shared: a call on another stream waits for the calls queued on
-        # the last one (a capture orders its own work and must not reach outside)
-        if self._stream is not None and not torch.cuda.is_current_stream_capturing():
-            s.wait_stream(self._stream)
-        check(self.lib.wx_ctx_set_stream(self.h, C.c_void_p(s.cuda_stream)), self.h)
-        self._stream, self._raw_stream = s, raw
+        # a stream that torch wraps for a caller has its handle as its id. The caller may destroy it
+        # after a call, and may get the same handle again: what is kept of it is an event
+        theirs = raw != 0 and s.stream_id == raw
+        if _capturing(s):
+            for last in (self._captured, self._direct):  # (a stream of direct calls may be captured since)
+                if last is not None and last.cuda_stream != raw and _capturing(last):
+                    s.wait_stream(last)
+            self._captured, self._record, again = None if theirs else s, False, True
+        else:
+            if self._done is not None:
+                s.wait_event(self._done)
+            elif self._direct is not None and self._direct.cuda_stream != raw and not _capturing(self._direct):
+                s.wait_stream(self._direct)
+            self._direct, self._done, self._record, again = (None, self._done, True, True) if theirs else \
+                (s, None, False, False)
+        check(self.lib.wx_ctx_set_stream(self.h, C.c_void_p(raw)), self.h)
+        self._raw_stream = None if again else raw
 
     def check_device(self) -> None:
+        self.sync_stream()
         check(self.lib.wx_ctx_check_device(self.h), self.h)
 
     def sp_exchange(self) -> int:
@@ -93,6 +116,9 @@ class Context:
     def call(self, name: str, *args) -> None:
         self.sync_stream()
         st = getattr(self.lib, name)(self.h, *args)
+        if self._record:
+            self._done = torch.cuda.Event()
+            self._done.record(torch.cuda.current_stream(self.device))
         if st:
             check(st, self.h)
 
