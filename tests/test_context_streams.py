@@ -1,5 +1,6 @@
-"""How a Context follows torch's streams, on fakes of both (no GPU): which streams wait for which, and that a
-caller's own stream is not touched after it is gone."""
+"""How a Context follows torch's streams, on fakes of both (no GPU): which streams wait for which, that a
+caller's own stream is not touched after it is gone, and that threads do not change each other's stream
+between setting it and launching on it."""
 import contextlib
 import threading
 import time
@@ -168,3 +169,44 @@ def test_branches_of_a_capture_on_the_stream_used_before(world):
     with world.on(b):
         ctx.call("work", "3")
     assert "2" in b.after
+
+def test_threads_keep_their_streams(world):
+    """More threads than streams' worth of luck: every launch is on its own thread's stream."""
+    ctx = h3.Context(0)
+    failed = []
+
+    def run(i):
+        try:
+            with world.on(FakeStream(world, 16 * (i + 1), f"s{i}")):
+                for k in range(30):
+                    ctx.call("work", f"{i}.{k}")
+        except BaseException as e:  # noqa: BLE001 (reported below)
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed[0]
+    assert len(world.log) == 120
+
+
+def test_threads_share_one_context(world, monkeypatch):
+    made = []
+
+    class Slow(h3.Context):
+        def __init__(self, device):
+            time.sleep(0.01)
+            super().__init__(device)
+            made.append(self)
+
+    monkeypatch.setattr(h3, "Context", Slow)
+    monkeypatch.setattr(h3, "_contexts", {})
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(h3.context(0))) for _ in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and all(c is made[0] for c in got)

@@ -1,5 +1,7 @@
-"""Text-side calls on several streams: a caller's own stream, branches of a capture. Each call has inputs of
+"""Text-side calls on several streams: a caller's own stream, branches of a capture, threads. Each call has inputs of
 its own, and is compared with the same call alone."""
+import threading
+
 import pytest
 import torch
 
@@ -76,3 +78,35 @@ def test_streams_with_inputs_of_their_own():
     torch.cuda.synchronize()
     _check_device()
     assert all(_same(o, wants[i % 3]) for i, o in enumerate(got))
+
+
+def test_threads_with_streams_of_their_own():
+    """Threads share the device's context: each one's calls go to its own stream, behind its own inputs."""
+    steps = [Step("bf16", 9000, 1, 9), Step("int8", 8000, 3, 10), Step("bf16", 7000, 100, 11), Step("e4m3", 5000, 2, 12)]
+    wants = [[] for _ in steps]
+    for i, s in enumerate(steps):
+        for seed in range(10):
+            s.refresh(100 * i + seed)
+            wants[i].append(_clone(s.run()))
+    torch.cuda.synchronize()
+    got, failed = [[] for _ in steps], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for seed in range(10):
+                    steps[i].refresh(100 * i + seed)  # (queued on this thread's stream: the call has to follow it)
+                    got[i].append(_clone(steps[i].run()))
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:  # noqa: BLE001 (reported below)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(steps))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed[0]
+    _check_device()
+    for g, w in zip(got, wants):
+        assert all(_same(x, y) for x, y in zip(g, w))

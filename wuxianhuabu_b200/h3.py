@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import threading
 from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
@@ -59,7 +60,8 @@ def _capturing(s: torch.cuda.Stream) -> bool:
 
 
 class Context:
-    """One libwx context per CUDA device; calls are ordered on torch's current stream."""
+    """One libwx context per CUDA device; calls are ordered on torch's current stream. Threads may
+    share it, each with a current stream of its own: one call is made at a time."""
 
     def __init__(self, device: int = 0):
         self.lib = _lib.load()
@@ -72,6 +74,7 @@ class Context:
         if st != 0:
             raise WxError(st, f"wx_ctx_create(device={device}) failed")
         self.h = h
+        self._lock = threading.RLock()  # over the stream that is set and the call that goes out on it
         self._raw_stream: Optional[int] = None  # the context's stream, where it need not be looked at again
         self._direct: Optional[torch.cuda.Stream] = None    # last stream of direct calls,
         self._done: Optional[torch.cuda.Event] = None       # or, if it was a caller's own, the calls on it
@@ -82,6 +85,10 @@ class Context:
         """Puts the context on torch's current stream. Its scratch is shared (direct calls have one set,
         captured ones another): a direct call waits for the direct calls on the last stream, a captured
         one for those on another branch of its capture."""
+        with self._lock:
+            self._follow_stream()
+
+    def _follow_stream(self) -> None:
         raw = _current_raw_stream(self.device)
         if raw == self._raw_stream:
             return
@@ -105,8 +112,9 @@ class Context:
         self._raw_stream = None if again else raw
 
     def check_device(self) -> None:
-        self.sync_stream()
-        check(self.lib.wx_ctx_check_device(self.h), self.h)
+        with self._lock:
+            self._follow_stream()
+            check(self.lib.wx_ctx_check_device(self.h), self.h)
 
     def sp_exchange(self) -> int:
         """Sequence-parallel exchange path: 1 NVLink peer memory, 0 NCCL all-to-alls,
@@ -114,13 +122,14 @@ class Context:
         return int(self.lib.wx_ctx_sp_exchange(self.h))
 
     def call(self, name: str, *args) -> None:
-        self.sync_stream()
-        st = getattr(self.lib, name)(self.h, *args)
-        if self._record:
-            self._done = torch.cuda.Event()
-            self._done.record(torch.cuda.current_stream(self.device))
-        if st:
-            check(st, self.h)
+        with self._lock:
+            self._follow_stream()
+            st = getattr(self.lib, name)(self.h, *args)
+            if self._record:
+                self._done = torch.cuda.Event()
+                self._done.record(torch.cuda.current_stream(self.device))
+            if st:
+                check(st, self.h)
 
     TRACE_PHASES = ("norm1", "qkv", "rope", "attn", "out", "mlp")
     TRACE_MODES = ("dense", "sparse", "reuse")
@@ -136,7 +145,9 @@ class Context:
         nf = 9
         buf = (ctypes.c_double * (nf * max_records))()
         n = ctypes.c_int(0)
-        check(self.lib.wx_ctx_trace_read(self.h, buf, max_records, ctypes.byref(n)), self.h)
+        with self._lock:
+            self._follow_stream()
+            check(self.lib.wx_ctx_trace_read(self.h, buf, max_records, ctypes.byref(n)), self.h)
         out = []
         for i in range(n.value):
             r = buf[i * nf:(i + 1) * nf]
@@ -164,13 +175,18 @@ class Context:
 
 
 _contexts: dict[int, Context] = {}
+_contexts_lock = threading.Lock()
 
 
 def context(device: Optional[int] = None) -> Context:
     dev = torch.cuda.current_device() if device is None else device
-    if dev not in _contexts:
-        _contexts[dev] = Context(dev)
-    return _contexts[dev]
+    ctx = _contexts.get(dev)
+    if ctx is None:
+        with _contexts_lock:
+            ctx = _contexts.get(dev)
+            if ctx is None:
+                ctx = _contexts[dev] = Context(dev)
+    return ctx
 
 
 def _need_bf16_cuda(*ts: Optional[torch.Tensor]) -> None:
