@@ -48,7 +48,7 @@ struct OutsideCapture {
 
 void* workspace(wx_ctx* ctx, size_t bytes, int* status) {
   *status = WX_OK;
-  const bool capturing = stream_capturing(ctx);
+  const bool capturing = ctx->capturing = stream_capturing(ctx);
   wx_ctx::Scratch& own = capturing ? ctx->captured : ctx->direct;
   if (bytes <= own.ws_bytes) return own.ws;
   OutsideCapture outside;
@@ -163,7 +163,7 @@ static cudaError_t zero_now(int* p, int64_t n) {
 
 int* arrival_counters(wx_ctx* ctx, int64_t n, int* status) {
   *status = WX_OK;
-  const bool capturing = stream_capturing(ctx);
+  const bool capturing = ctx->capturing;
   wx_ctx::Scratch& own = capturing ? ctx->captured : ctx->direct;
   if (n <= own.n_arrivals) return own.arrivals;
   OutsideCapture outside;

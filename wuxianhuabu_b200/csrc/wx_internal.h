@@ -25,6 +25,7 @@ struct wx_ctx {
     int* arrivals = nullptr;
     int64_t n_arrivals = 0;
   } direct, captured;
+  bool capturing = false;  // which of them the call at hand uses (set by workspace)
   std::vector<void*> retired;
   size_t retired_bytes = 0;
   std::string last_error;
@@ -117,6 +118,7 @@ int make_tmap_bf16_3d(wx_ctx* ctx, CUtensorMap* map, const void* base, const uin
 
 // `n` counters on the device, zero between launches: a kernel that counts arrivals on them sets
 // each back to zero with the last arrival (every CTA arrives, whatever happened to its work).
+// To be called after workspace, which finds out whether the stream is being captured.
 int* arrival_counters(wx_ctx* ctx, int64_t n, int* status);
 
 // releases the NCCL communicator of a context (no-op without one)

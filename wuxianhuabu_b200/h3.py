@@ -90,8 +90,10 @@ class Context:
 
     def _follow_stream(self) -> None:
         raw = _current_raw_stream(self.device)
-        if raw == self._raw_stream:
-            return
+        if raw != self._raw_stream:
+            self._change_stream(raw)
+
+    def _change_stream(self, raw: int) -> None:
         s = torch.cuda.current_stream(self.device)
         # a stream that torch wraps for a caller has its handle as its id. The caller may destroy it
         # after a call, and may get the same handle again: what is kept of it is an event
@@ -123,7 +125,9 @@ class Context:
 
     def call(self, name: str, *args) -> None:
         with self._lock:
-            self._follow_stream()
+            raw = _current_raw_stream(self.device)
+            if raw != self._raw_stream:
+                self._change_stream(raw)
             st = getattr(self.lib, name)(self.h, *args)
             if self._record:
                 self._done = torch.cuda.Event()

@@ -240,15 +240,15 @@ def _batch_of(cu_seqlens: torch.Tensor) -> int:
     return batch
 
 
-def _int32(n: int) -> int:
-    """n, or the int32 nearest to it (a struct's field would keep the low bits)."""
-    return max(-1 << 31, min(n, (1 << 31) - 1))
+_INT32 = 1 << 31
 
 
 def _dims(n: int, batch: int, max_len: int, h: int, hk: int, d: int, causal: bool, window: int,
           scale: Optional[float]):
-    return C.byref(AttnDims(n, batch, _int32(max_len), h, hk, d, causal, _int32(window),
-                            d ** -0.5 if scale is None else scale))
+    if window >= _INT32 or window < 0 or max_len >= _INT32 or max_len < 0:
+        # (beyond 32 bits, the nearest int32: a struct's field would keep the low bits)
+        window, max_len = (max(-_INT32, min(x, _INT32 - 1)) for x in (window, max_len))
+    return C.byref(AttnDims(n, batch, max_len, h, hk, d, causal, window, d ** -0.5 if scale is None else scale))
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_len: int,
