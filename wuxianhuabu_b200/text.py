@@ -91,7 +91,25 @@ class RopeScaling:
     magnitude: float = 1.0
 
 
-class RopeTable:
+class _Described:
+    """An object whose tensors the library is told of in a struct, ``_desc``. It is made at the first call
+    that needs it, checked, and made again after an attribute was assigned; copies make their own."""
+
+    def __getattr__(self, name: str):  # (only where there is no such attribute)
+        if name != "_desc":
+            raise AttributeError(name)
+        self.__dict__["_desc"] = made = C.byref(self._describe())
+        return made
+
+    def __setattr__(self, name: str, value) -> None:
+        self.__dict__.pop("_desc", None)
+        object.__setattr__(self, name, value)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k != "_desc"}
+
+
+class RopeTable(_Described):
     """cos / sin of every position, fp32 [positions, rot / 2] (angles in 64 bits)."""
 
     def __init__(self, rot: int, positions: int, base: float = 10000.0, interleaved: bool = False,
@@ -110,26 +128,26 @@ class RopeTable:
         self.interleaved = interleaved
         self.cos = torch.empty((positions, rot // 2), dtype=torch.float32, device=dev)
         self.sin = torch.empty_like(self.cos)
-        self._desc = self._describe()
         ctx.call("wx_rope_table", inv.ctypes.data, rot // 2, positions, float(s.magnitude), _p(self.cos), _p(self.sin))
 
     @classmethod
     def from_tables(cls, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False) -> "RopeTable":
         """Over tables that exist already (not copied)."""
+        self = cls.__new__(cls)
+        self.cos, self.sin, self.interleaved, self.inv_freq = cos, sin, interleaved, None
+        self._desc  # (checked)
+        return self
+
+    def _describe(self) -> Rope:
+        cos, sin = self.cos, self.sin
         for t in (cos, sin):
             if not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 2:
                 raise _invalid("cos and sin must be contiguous CUDA fp32 [positions, rot / 2]")
         if cos.shape != sin.shape:
             raise _invalid("cos and sin must have one shape")
         _same_device(cos, sin)
-        self = cls.__new__(cls)
-        self.cos, self.sin, self.interleaved, self.inv_freq = cos, sin, interleaved, None
-        self._desc = self._describe()
-        return self
-
-    def _describe(self):
-        n, half = self.cos.shape
-        return C.byref(Rope(_p(self.cos), _p(self.sin), n, 2 * half, int(self.interleaved)))
+        n, half = cos.shape
+        return Rope(_p(cos), _p(sin), n, 2 * half, int(self.interleaved))
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [tokens, heads, head_dim] with token t turned by positions[t] (int32); ``out`` may be x."""
@@ -141,7 +159,7 @@ class RopeTable:
         return o
 
 
-class PagedKVCache:
+class PagedKVCache(_Described):
     """Pages of ``page_size`` tokens, [pages, kv_heads, page_size, head_dim] each for k and v in
     ``fmt`` ("bf16", "int8", "e4m3"); the 8-bit formats hold one fp32 scale per (token, head)
     row in [pages, kv_heads, page_size]. A slot is page * page_size + offset (int64)."""
@@ -152,42 +170,48 @@ class PagedKVCache:
             raise _invalid(f"unknown cache format {fmt!r}")
         dev = torch.device("cuda", context(device).device)
         shape = (pages, kv_heads, page_size, head_dim)
-        self.fmt = fmt
-        self.k = torch.zeros(shape, dtype=torch.uint8 if fmt != "bf16" else torch.bfloat16, device=dev)
-        self.v = torch.zeros_like(self.k)
-        if fmt != "bf16":
-            self.k, self.v = self.k.view(_FORMATS[fmt][1]), self.v.view(_FORMATS[fmt][1])
-        self.k_scale = self.v_scale = None
-        if fmt != "bf16":
-            self.k_scale = torch.zeros(shape[:3], dtype=torch.float32, device=dev)
-            self.v_scale = torch.zeros_like(self.k_scale)
-        self._describe()
+        kind = _FORMATS[fmt][1]
+        self.k, self.v = (torch.zeros(shape, dtype=kind if fmt == "bf16" else torch.uint8, device=dev).view(kind)
+                          for _ in range(2))
+        self.k_scale, self.v_scale = (None, None) if fmt == "bf16" else \
+            (torch.zeros(shape[:3], dtype=torch.float32, device=dev) for _ in range(2))
+        self._desc  # (checked)
 
     @classmethod
     def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                      v_scale: Optional[torch.Tensor] = None) -> "PagedKVCache":
         """Over buffers that exist already (not copied)."""
-        fmt = next((f for f, (_, d) in _FORMATS.items() if d == k.dtype), None)
-        if fmt is None or k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        self = cls.__new__(cls)
+        self.k, self.v = k, v
+        self.k_scale, self.v_scale = (k_scale, v_scale) if k.dtype != torch.bfloat16 else (None, None)
+        self._desc  # (checked)
+        return self
+
+    def __setattr__(self, name: str, value) -> None:
+        if name == "k":  # format and geometry are those of k
+            fmt = next((f for f, (_, d) in _FORMATS.items() if d == value.dtype), None)
+            if fmt is None or value.dim() != 4:
+                raise _invalid("k must be [pages, kv_heads, page_size, head_dim] of a cache format")
+            self.fmt = fmt
+            self.pages, self.kv_heads, self.page_size, self.head_dim = value.shape
+        super().__setattr__(name, value)
+
+    def _describe(self) -> KvCache:
+        k, v, scales = self.k, self.v, (self.k_scale, self.v_scale)
+        if k.shape != v.shape or k.dtype != v.dtype:
             raise _invalid("k and v must be [pages, kv_heads, page_size, head_dim] of one cache format")
         if not (k.is_cuda and k.is_contiguous() and v.is_contiguous()):
             raise _invalid("k and v must be contiguous CUDA tensors")
         _same_device(k, v)
-        if fmt != "bf16":
-            for s in (k_scale, v_scale):
+        if self.fmt == "bf16":
+            scales = None, None
+        else:
+            for s in scales:
                 if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or not s.is_contiguous():
                     raise _invalid("an 8-bit cache needs contiguous fp32 scales [pages, kv_heads, page_size]")
-            _same_device(k, k_scale, v_scale)
-        self = cls.__new__(cls)
-        self.fmt, self.k, self.v = fmt, k, v
-        self.k_scale, self.v_scale = (k_scale, v_scale) if fmt != "bf16" else (None, None)
-        self._describe()
-        return self
-
-    def _describe(self) -> None:
-        self.pages, self.kv_heads, self.page_size, self.head_dim = self.k.shape
-        self._desc = C.byref(KvCache(_p(self.k), _p(self.v), _p(self.k_scale), _p(self.v_scale), self.pages,
-                                     self.page_size, self.kv_heads, self.head_dim, _FORMATS[self.fmt][0]))
+            _same_device(k, *scales)
+        return KvCache(_p(k), _p(v), _p(scales[0]), _p(scales[1]), self.pages, self.page_size, self.kv_heads,
+                       self.head_dim, _FORMATS[self.fmt][0])
 
     def _kv(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor):
         n, h, d, ks = _rows(k, "k")
