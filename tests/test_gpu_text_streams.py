@@ -110,3 +110,26 @@ def test_threads_with_streams_of_their_own():
     _check_device()
     for g, w in zip(got, wants):
         assert all(_same(x, y) for x, y in zip(g, w))
+
+
+def test_tensors_on_another_device_than_the_current_one():
+    """The calls run where the tensors are: their scratch is allocated there, and the current device stays."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    want = []
+    for dev in (1, 0):
+        with torch.cuda.device(dev):
+            steps = Step("bf16", 9000, 1, 20), Step("int8", 6000, 100, 21)
+            if dev == 1:
+                there = steps
+            else:
+                want = [_clone(s.run()) for s in steps]
+    with torch.cuda.device(0):
+        got = [s.run() for s in there]
+        assert torch.cuda.current_device() == 0
+        for g, w in zip(got, want):
+            assert all(x.device.index == 1 for x in g)
+            assert _same([x.to("cuda:0") for x in g], w)
+    for dev in (0, 1):
+        with torch.cuda.device(dev):
+            _check_device()

@@ -86,6 +86,22 @@ int set_error(wx_ctx* ctx, int status, const char* fmt, ...);
     if (!(cond)) return ::wx::set_error((ctx), WX_ERR_INVALID, "invalid argument: %s", #cond); \
   } while (0)
 
+// Makes the context's device current for an entry point (its streams, buffers and launches belong there,
+// whatever device the caller has chosen), and the caller's current again at its end.
+struct DeviceScope {
+  int prev = -1;
+  explicit DeviceScope(const wx_ctx* ctx) {
+    int now = 0;
+    if (!ctx || cudaGetDevice(&now) != cudaSuccess || now == ctx->device) return;
+    if (cudaSetDevice(ctx->device) == cudaSuccess) prev = now;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // Returns a device buffer of at least `bytes` from the context arena (grown on
 // demand, during a stream capture too; contents undefined; valid until the next call that
 // grows it, and for the graph that a capture makes as long as the context).

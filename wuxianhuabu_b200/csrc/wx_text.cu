@@ -434,6 +434,7 @@ int wx_rope_inv_freq(int rot, double base, int scaling, double factor, double or
 
 int wx_rope_table(wx_ctx* ctx, const double* inv_freq, int nf, int64_t positions, double magnitude, float* cos_t,
                   float* sin_t) {
+  DeviceScope on_device(ctx);
   WX_CHECK_ARG(ctx, ctx && inv_freq && cos_t && sin_t && nf > 0 && nf <= kRopeMaxPairs && positions >= 0);
   WX_CHECK_ARG(ctx, positions < (int64_t)1 << 40);
   if (!positions) return WX_OK;
@@ -446,6 +447,7 @@ int wx_rope_table(wx_ctx* ctx, const double* inv_freq, int nf, int64_t positions
 
 int wx_rope_apply(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, const void* x, int64_t row_stride,
                   int64_t tokens, int heads, int head_dim, void* y, int64_t y_stride) {
+  DeviceScope on_device(ctx);
   WX_CHECK_ARG(ctx, ctx && tokens >= 0 && heads > 0);
   if (head_dim != 128 && head_dim != 64)
     return set_error(ctx, WX_ERR_UNSUPPORTED, "rope head_dim must be 128 or 64 (got %d)", head_dim);
@@ -466,6 +468,7 @@ int wx_rope_apply(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, co
 
 int wx_kv_append(wx_ctx* ctx, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
                  int64_t v_stride, int64_t tokens, const int64_t* slots) {
+  DeviceScope on_device(ctx);
   WX_CHECK_ARG(ctx, ctx && tokens >= 0);
   int st = check_kv_cache(ctx, cache);
   if (st || !tokens) return st;
@@ -484,6 +487,7 @@ int wx_kv_append(wx_ctx* ctx, const wx_kv_cache* cache, const void* k, int64_t k
 int wx_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, const void* q, int64_t q_stride,
                       int q_heads, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
                       int64_t v_stride, int64_t tokens, const int64_t* slots, void* q_out, int64_t q_out_stride) {
+  DeviceScope on_device(ctx);
   WX_CHECK_ARG(ctx, ctx && tokens >= 0 && q_heads > 0);
   int st = check_kv_cache(ctx, cache);
   if (st || !tokens) return st;
@@ -509,6 +513,7 @@ int wx_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions
 
 int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,
                int64_t out_stride) {
+  DeviceScope on_device(ctx);
   WX_CHECK_ARG(ctx, ctx && tokens >= 0);
   int st = check_kv_cache(ctx, cache);
   if (st || !tokens) return st;

@@ -795,6 +795,7 @@ extern "C" {
 int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride, int64_t total_k, const int32_t* cu_q,
                         const int32_t* cu_k, void* out, int64_t out_stride, float* lse) {
+  DeviceScope on_device(ctx);
   int st = check_dims(ctx, dims, q, q_stride, out, out_stride, cu_q);
   if (st || dims->total_q == 0 || dims->batch == 0) return st;
   const int64_t cols = (int64_t)dims->kv_heads * dims->head_dim;
@@ -815,6 +816,7 @@ int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int
                        const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
                        const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride,
                        float* lse) {
+  DeviceScope on_device(ctx);
   int st = check_dims(ctx, dims, q, q_stride, out, out_stride, cu_q);
   if (st) return st;
   if ((st = check_kv_cache(ctx, cache))) return st;
