@@ -701,7 +701,8 @@ int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int6
 typedef struct wx_attn_dims {
   int64_t total_q; /* query rows of all sequences */
   int32_t batch;   /* sequences */
-  int32_t max_q;   /* longest Lq: chooses the kernel; results do not depend on it */
+  int32_t max_q;   /* longest Lq: chooses the kernel; results do not depend on it (one far too
+                    * small may set the device error word: from some 2^32 units of 8 rows x 128 keys) */
   int32_t q_heads;
   int32_t kv_heads;
   int32_t head_dim;

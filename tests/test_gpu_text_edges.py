@@ -209,3 +209,37 @@ def test_every_e4m3_code_reads_as_itself():
         assert torch.equal(torch.nan_to_num(x, nan=1e9), torch.nan_to_num(want, nan=1e9))
 
 
+# ------------------------------------------------------------------------- lengths that mislead
+@pytest.mark.parametrize("lens", [[100, 7, 300], [1000]])
+def test_a_longest_length_that_is_too_small_changes_nothing(lens):
+    """It chooses the kernel: the one for few rows takes any number of them."""
+    text = _text()
+    g = _gen(sum(lens))
+    q, k, v = (_randn(g, sum(lens), h, 128) for h in (8, 2, 2))
+    for max_len in (0, 1, 2, -(-max(lens) // 2)):
+        out, lse = text.prompt_attention(q, k, v, _cu(lens), max_len, return_lse=True)
+        _check_device()
+        a = 0
+        for n in lens:
+            s = slice(a, a + n)
+            ref, rl, mag = ref_attention(q[s], k[s], v[s], 1 / math.sqrt(128), True, 0)
+            assert_same(out[s], lse[s], ref, rl, mag, f"len {n}, longest {max_len}")
+            a += n
+
+
+def test_more_work_than_the_kernel_for_few_rows_can_count_is_an_error():
+    """262,400 tokens that are announced as one: 64 heads of 32,800 tiles of 8 rows over 2,050 units of keys are
+    more than 2^32. Nothing is computed, and the error word says so."""
+    text = _text()
+    from wuxianhuabu_b200 import h3
+    n = 262400
+    assert 64 * (n // 8) * (n // 128) > 2 ** 32
+    q = torch.zeros((n, 64, 64), dtype=BF16, device="cuda")
+    text.prompt_attention(q, q, q, _cu([n]), 1)
+    with pytest.raises(h3.WxError):
+        _check_device()
+    small = _randn(_gen(1), 3, 64, 64)
+    out, lse = text.prompt_attention(small, small, small, _cu([3]), 3, return_lse=True)
+    _check_device()
+    ref, rl, mag = ref_attention(small, small, small, 1 / 8, True, 0)
+    assert_same(out, lse, ref, rl, mag)

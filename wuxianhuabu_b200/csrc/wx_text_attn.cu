@@ -71,6 +71,7 @@ __device__ __forceinline__ void copy_async_wait() {
 // (the expansion's instructions are the bound: issue slots 53 % busy, DRAM 34 %); a call with a few
 // keys 11 us, of which 7 on the device.
 constexpr int kUnit = 128;
+constexpr uint64_t kMaxUnits = 0xf0000000u;  // of a line: its end and one CTA's run more are below 2^32
 
 template <int FMT, int HD, int NT>
 struct RowsGeom {
@@ -121,12 +122,22 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     items = ((unsigned)(s.lq * p.group) + kRows - 1) / kRows * (unsigned)p.hkv;
     nu = (unsigned)max(1, (s.lk - k16 + kUnit - 1) / kUnit);
   };
-  unsigned my_items = 0, my_nu = 0, total = 0;  // of sequence loaded + lane
+  unsigned my_items = 0, my_nu = 0;  // of sequence loaded + lane
   int my_k16 = 0, loaded = -1;
+  uint64_t mine = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     line_of(b0 + lane, my_items, my_nu, my_k16);
     loaded = b0;
-    total += __reduce_add_sync(0xffffffffu, my_items * my_nu);
+    mine += (uint64_t)my_items * my_nu;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  // (a line beyond 32 bits takes sequences of many query rows, which this kernel is not chosen for unless
+  // the caller's longest length was far too small: an error, not rows left out)
+  unsigned total = (unsigned)mine;
+  if (mine > kMaxUnits) {
+    set_dev_error(p.err, kDevBadArgs);
+    total = 0;
   }
   const unsigned per = max((unsigned)min_units, (total + gridDim.x - 1) / gridDim.x);
   unsigned u = min(total, blockIdx.x * per);
