@@ -30,7 +30,8 @@ enum DevErr : int {
 // records kDevBounds in the error word and the access is skipped. In the normal build the
 // guard is `true` and its condition is not evaluated. Guarded: the GEMM epilogues' stores
 // (plain, q|k|v norm/RoPE with its peer rows, small-M), the attention output rows (local and
-// peer) and the reads of the kept-block lists.
+// peer), the reads of the kept-block lists, and on the text side the cache rows (read and written),
+// q and output rows and the partial sums. TMA boxes are held inside their tensors by the hardware.
 #ifndef WX_BOUNDS_CHECK
 #define WX_BOUNDS_CHECK 0
 #endif

@@ -221,6 +221,8 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
     if constexpr (FMT != kKvBf16) scale = quantise<FMT, 2 * W, kLanes>(x, qv);  // (all lanes: it shuffles)
     if (!live) continue;
     const int64_t row = ((((slot >> p.page_shift) * p.nkv + h) << p.page_shift) | (slot & ((1 << p.page_shift) - 1)));
+    if (!WX_IN_BOUNDS(p.err, is_q ? h >= 0 && h < p.nq : h >= 0 && h < p.nkv && (slot < 0 || row < p.n_slots * p.nkv)))
+      continue;
     if (is_q || FMT == kKvBf16) {
       __nv_bfloat16* o = is_q ? p.q_out + t * p.q_out_stride + (int64_t)h * HD
                               : reinterpret_cast<__nv_bfloat16*>(is_v ? p.vc : p.kc) + row * HD;
@@ -290,6 +292,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(ReadParams p) {
     if (r >= r1 || slot < 0) continue;
     const bool is_v = r >= p.nkv;
     const int64_t row = ((page * p.nkv + (is_v ? r - p.nkv : r)) << p.page_shift) | inside;
+    if (!WX_IN_BOUNDS(p.err, row >= 0 && row < p.n_slots * p.nkv)) continue;
     const uint4* src = reinterpret_cast<const uint4*>(is_v ? p.vc : p.kc) + (row * HD / 16 + j) * kVec;
 #pragma unroll
     for (int e = 0; e < kVec; ++e) x[g][e] = __ldg(src + e);

@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   // ---- loads: step i of this warp starts at key k_lo + (i * kWarps + warp) * 16; the pages of 32
   // consecutive steps are fetched at once, one per lane
   const bool paged = kW || p.block_table;
+  [[maybe_unused]] const int64_t kv_rows = paged ? (p.pages * p.hkv) << p.page_shift : p.total_k;
   int page_of = 0;
   auto first_key = [&](const Piece& c, int i) { return c.k_lo + (i * kWarps + warp) * 16; };
   // row of the step's first key: of the cache, or of the packed keys
@@ -235,11 +236,11 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   auto v_swz = [](int row) { return kRU == 4 ? (row >> 1) & 3 : row & 6; };
   const float* scale_at = kW ? (lane < 16 ? p.ks : p.vs) + (lane & 15) : nullptr;
   auto load_step = [&](const Piece& c, int i, uint32_t stage) {
-    if (i < c.steps) {
-      const int64_t row = step_row(c, i);
+    const int left = paged || i >= c.steps ? 15 : c.s.lk - 1 - first_key(c, i);
+    const int64_t row = i < c.steps ? step_row(c, i) : 0;
+    if (i < c.steps && WX_IN_BOUNDS(p.err, row >= 0 && left >= 0 && row + min(left, 15) < kv_rows)) {
       // (an 8-bit cache is paged: its 16 rows lie together)
       const int64_t kst = kW ? kRowBytes : k_stride, vst = kW ? kRowBytes : v_stride;
-      const int left = paged ? 15 : c.s.lk - 1 - first_key(c, i);
       const int64_t col = (paged ? 0 : (int64_t)c.h * kRowBytes) + lane % kRU * 16;
       const uint8_t* kb = k_base + row * kst + col;
       const uint8_t* vb = v_base + row * vst + col;
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = row0 + 8 * n + g;
-      const bool live = r < n_rows;
+      const bool live = r < n_rows && WX_IN_BOUNDS(p.err, cur.s.q0 >= 0 && cur.s.q0 + r / p.group < p.total_q);
       const int tok = live ? (int)((unsigned)r / (unsigned)p.group) : 0;
       const __nv_bfloat16* src = p.q + (cur.s.q0 + tok) * p.q_stride +
                                  (int64_t)(cur.h * p.group + (live ? r - tok * p.group : 0)) * HD;
@@ -601,6 +602,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
       const int tk = (int)((unsigned)r / (unsigned)p.group);
       const int64_t tok = done.s.q0 + tk;
       const int head = done.h * p.group + r - tk * p.group;
+      if (!WX_IN_BOUNDS(p.err, tok >= 0 && tok < p.total_q && head >= 0 && head < p.hq)) return;
       const float inv = L == 0.f ? 0.f : kByteUnit<FMT> / L;
       uint32_t w[kPer / 2];
 #pragma unroll
@@ -613,7 +615,8 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     };
     // partial sums of CTA c for this item: slot 0 if the item began in an earlier CTA, 1 if there
     auto slot_row = [&](unsigned c, int row) -> int64_t {
-      return (int64_t)(2 * c + (done.item_u0 >= c * per ? 1 : 0)) * kRows + row;
+      const int64_t at = (int64_t)(2 * c + (done.item_u0 >= c * per ? 1 : 0)) * kRows + row;
+      return WX_IN_BOUNDS(p.err, at >= 0 && at < 2 * (int64_t)gridDim.x * kRows) ? at : 0;
     };
     if (jg == 0) {
       clear();

@@ -355,7 +355,9 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         const int per_half = 64 / tp.box;
         const int page = page_of(t * boxes, lane % boxes);
         const int nb = min(boxes, (it.lk - t * 128 + tp.box - 1) / tp.box);
-        const int64_t row = cache_row(page, t * 128 + (lane % boxes) * tp.box);
+        int64_t row = cache_row(page, t * 128 + (lane % boxes) * tp.box);
+        // (the copy's bytes are waited for: it reads the first rows instead)
+        if (lane < nb && !WX_IN_BOUNDS(p.err, row >= 0 && row + tp.box <= (p.pages * p.hkv) << p.page_shift)) row = 0;
         if (is_k) {
           const uint32_t sc = nk % kTfScales, full = bar(kBTfScale + sc);
           const uint32_t dst = sbase + G::kScaleOff + sc * 1024 + (uint32_t)lane * tp.box * 4;
@@ -1091,7 +1093,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       const float inv = l == 0.f ? 0.f : __fdividef(kByteUnit<FMT>, l);
       const int bad = any ? *reinterpret_cast<const volatile int*>(&it.bad) : 0;
       const bool cut = it.pieces > 1;
-      const bool write = ok && live && WX_IN_BOUNDS(p.err, it.q0 + tok < p.total_q);
+      const bool write = ok && live && WX_IN_BOUNDS(p.err, it.q0 >= 0 && it.q0 + tok < p.total_q && it.h * p.group + my_g < p.hq &&
+                                                               it.piece >= 0 && it.piece < tp.splits);
       const int64_t at_row = ((int64_t)it.q0 + tok) * p.hq + it.h * p.group + my_g;
       const int64_t at_part = it.piece * (p.total_q * p.hq) + at_row;
       __nv_bfloat16* row = p.out + ((int64_t)it.q0 + tok) * p.out_stride + (int64_t)(it.h * p.group + my_g) * HD;
