@@ -243,3 +243,26 @@ def test_more_work_than_the_kernel_for_few_rows_can_count_is_an_error():
     _check_device()
     ref, rl, mag = ref_attention(small, small, small, 1 / 8, True, 0)
     assert_same(out, lse, ref, rl, mag)
+
+
+# -------------------------------------------------------------------------- alone and in a batch
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("q_lens", [[1, 1, 1, 1], [3, 2, 1, 4], [70, 5, 33, 1]])
+def test_a_sequence_alone_and_in_a_batch(fmt, q_lens):
+    """The batch deals the keys to other CTAs and joins other pieces: both are within the definition's
+    tolerance, and a sequence does not reach its neighbours' rows."""
+    text = _text()
+    g = _gen(sum(q_lens))
+    kv = [4000, 900, 2222, 17]
+    cache, table, q, ks, vs = _paged(g, fmt, q_lens, kv, 8, 2, 128, 64)
+    lens = torch.tensor(kv, dtype=torch.int32, device="cuda")
+    out, lse = text.paged_attention(q, cache, _cu(q_lens), lens, table, max(q_lens), return_lse=True)
+    a = 0
+    for i, n in enumerate(q_lens):
+        s = slice(a, a + n)
+        alone, lse1 = text.paged_attention(q[s], cache, _cu([n]), lens[i:i + 1], table[i:i + 1], n, return_lse=True)
+        _check_device()
+        ref, rl, mag = ref_attention(q[s], ks[i], vs[i], 1 / math.sqrt(128), True, 0)
+        assert_same(out[s], lse[s], ref, rl, mag, f"{i} in the batch")
+        assert_same(alone, lse1, ref, rl, mag, f"{i} alone")
+        a += n
