@@ -22,6 +22,8 @@ class World:
         monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: self.current())
         monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.current().touch().capturing is not None)
         monkeypatch.setattr(torch.cuda, "stream", self.on)
+        monkeypatch.setattr(torch.cuda, "set_stream", lambda s: setattr(self.local, "s", s))
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
         monkeypatch.setattr(torch.cuda, "Event", lambda *a, **k: FakeEvent(self))
         monkeypatch.setattr(_lib, "load", lambda: self.lib)
         self.stream = None  # of the library's context
@@ -59,6 +61,8 @@ class World:
 
 
 class FakeStream:
+    device_index = 0
+
     def __init__(self, world, handle, name, external=False):
         self.world, self.cuda_stream, self.name = world, handle, name
         self.stream_id = handle if external else (handle and 8 * handle + 3)  # (torch's own ids are no handles)

@@ -54,9 +54,18 @@ _current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _capturing(s: torch.cuda.Stream) -> bool:
-    with torch.cuda.stream(s):
+def _capturing(s: torch.cuda.Stream, current: torch.cuda.Stream) -> bool:
+    """Whether s is being captured (``current``: the current stream of its device)."""
+    if torch.cuda.current_device() != s.device_index:
+        with torch.cuda.stream(s):
+            return torch.cuda.is_current_stream_capturing()
+    if s is current:
         return torch.cuda.is_current_stream_capturing()
+    torch.cuda.set_stream(s)  # (a context manager around it takes 6 us)
+    try:
+        return torch.cuda.is_current_stream_capturing()
+    finally:
+        torch.cuda.set_stream(current)
 
 
 class Context:
@@ -98,15 +107,15 @@ class Context:
         # a stream that torch wraps for a caller has its handle as its id. The caller may destroy it
         # after a call, and may get the same handle again: what is kept of it is an event
         theirs = raw != 0 and s.stream_id == raw
-        if _capturing(s):
+        if _capturing(s, s):
             for last in (self._captured, self._direct):  # (a stream of direct calls may be captured since)
-                if last is not None and last.cuda_stream != raw and _capturing(last):
+                if last is not None and last.cuda_stream != raw and _capturing(last, s):
                     s.wait_stream(last)
             self._captured, self._record, again = None if theirs else s, False, True
         else:
             if self._done is not None:
                 s.wait_event(self._done)
-            elif self._direct is not None and self._direct.cuda_stream != raw and not _capturing(self._direct):
+            elif self._direct is not None and self._direct.cuda_stream != raw and not _capturing(self._direct, s):
                 s.wait_stream(self._direct)
             self._direct, self._done, self._record, again = (None, self._done, True, True) if theirs else \
                 (s, None, False, False)
