@@ -676,7 +676,7 @@ typedef struct wx_kv_cache {
   int32_t format;
 } wx_kv_cache;
 /* Writes k and v rows [tokens, kv_heads, head_dim] (bf16) to slots[t] = page * page_size +
- * offset (device; < 0 skips the token). 8-bit formats: scale = amax / 127 (int8) or
+ * offset (device; < 0 skips the token; the others of a call distinct). 8-bit formats: scale = amax / 127 (int8) or
  * amax / 448 (e4m3) of the row, value = x * (127 | 448) / amax to nearest even; a row with
  * infinity or NaN gets scale NaN (it reads back as NaN), one below 2^-100 throughout zeros.
  * A slot beyond the cache is skipped and sets the device error word. The writes store no e4m3 NaN
@@ -697,7 +697,9 @@ int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int6
  * Lk key rows stands at key i + Lk - Lq: causal lets it see keys up to there, window > 0 only
  * the last `window` keys up to there. out = softmax(scale q k^T) v; lse (optional, [total_q,
  * q_heads] fp32) = log of the softmax's denominator. A row that sees no key gets out 0 and
- * lse -inf. Keys that a row does not see do not influence it, whatever they hold. */
+ * lse -inf. Keys that a row does not see do not influence it, whatever they hold; NaN and
+ * infinities of those that it sees come out as the formula has them. Query rows that belong to no
+ * sequence are not written. */
 typedef struct wx_attn_dims {
   int64_t total_q; /* query rows of all sequences */
   int32_t batch;   /* sequences */

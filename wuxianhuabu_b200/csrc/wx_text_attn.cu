@@ -67,9 +67,9 @@ __device__ __forceinline__ void copy_async_wait() {
 // last to arrive joins them in key order (so the result does not depend on who is last).
 //
 // Measured, caches flushed from L2: 64 sequences, 32 / 8 heads of 128, 238,000 bf16 keys 191 us =
-// 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 48 us = 2.9 TB/s
-// (the expansion's instructions are the bound: issue slots 53 % busy, DRAM 34 %); a call with a few
-// keys 11 us, of which 7 on the device.
+// 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 42 us = 3.3 TB/s, e4m3
+// 41 (the expansion's instructions are the bound: issue slots 53 % busy, DRAM 34 %; the start and the
+// join are a third of it); a call with a few keys 11 us, of which 7 on the device.
 constexpr int kUnit = 128;
 constexpr uint64_t kMaxUnits = 0xf0000000u;  // of a line: its end and one CTA's run more are below 2^32
 
@@ -786,12 +786,21 @@ static int launch_rows_attn(wx_ctx* ctx, int head_dim, int64_t rows, const TextA
 
 // Few flattened rows a sequence (a decoding step, a few drafted tokens) go to the rows kernel, which
 // walks the keys once per 16 rows, more to the tcgen05 kernel, which does so once per 256. Rows : tcgen05
-// in us, 32 / 8 heads of 128:                 bf16        e4m3        int8
-//   32 sequences of 8,000 keys, 24 to 32 rows   326 : 253   294 : 388   244 : 376
-//                               48 rows                     431 : 392   358 : 382
-//                               64 rows         618 : 259   565 : 396   465 : 386
-//   1 sequence of 65,536 keys, 24 to 32 rows     92 : 87     91 : 116    80 : 114
-//                              48 rows          121 : 89    125 : 118   105 : 114
+// in us:                                                bf16        e4m3        int8
+//   32 sequences of 4,000 keys, 32 / 8 x 128, 24 rows   172 : 150   150 : 216   135 : 210
+//                                             40 rows   249 : 155   217 : 220   195 : 214
+//                                             56 rows   315 : 157   281 : 222   250 : 220
+//                               32 / 8 x 64,  24 rows   111 : 132   111 : 191   104 : 189
+//                                             40 rows   162 : 134   160 : 194   150 : 193
+//                                             56 rows   205 : 136   205 : 196   190 : 195
+//   1 sequence of 30,000 keys,  32 / 8 x 128, 24 rows    55 : 56     50 : 77     45 : 75
+//                                             40 rows    68 : 56     63 : 77     57 : 75
+//   8 sequences of 500 keys,    32 / 8 x 128, 24 rows    16 : 21     16 : 29     14 : 27
+//                                             56 rows    33 : 20     31 : 27     31 : 27
+//   16 of 8,000, window 700,    8 / 1 x 64,   64 rows    16 : 25     16 : 35     14 : 35
+// The bounds are set for many keys at head_dim 128. Where there is little work for the whole card (one
+// K/V head, short or windowed keys) the rows kernel stays ahead beyond them, by up to 2.4 times; a rule on
+// the amount of work, which is known on the device only, was not tried.
 static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParams& p, const KvSource& kv) {
   const int64_t rows = (int64_t)d->max_q * p.group;
   if (rows > (kv.format == kKvBf16 ? 16 : kv.format == kKvE4m3 ? 32 : 48)) return text_flash(ctx, p, d->head_dim, kv);
