@@ -468,7 +468,8 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
 #pragma unroll
             for (int rr = 0; rr < 4; ++rr) {
               uint4& x = vf.v[rr][0];
-              x = make_uint4(without_nan_codes(x.x), without_nan_codes(x.y), without_nan_codes(x.z), without_nan_codes(x.w));
+              x = make_uint4(without_nan_codes(x.x), without_nan_codes(x.y), without_nan_codes(x.z),
+                             without_nan_codes(x.w));
             }
 #pragma unroll 1
             for (int kk = 0; kk < 16; ++kk) {

@@ -93,9 +93,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // ------------------------------------------------------------------ 8-bit -> bf16
 // Two stored bytes -> a bf16 pair, exactly, in units of kByteUnit. int8: byte + 128 as the bits of a
 // bf16 is (byte + 128) * 2^-133 (subnormal or the first binade: one line), so one fused product with 2^120
-// and sum gives byte * 2^-13. e4m3: through f16 and fp32, four instructions a pair and half of them off the
-// integer pipe; shifting its bits into a bf16 took five and made numbers of the NaN codes (decoding over
-// 65,537 keys, 64 / 8 heads of 128: 41 us against 45).
+// and sum gives byte * 2^-13. e4m3: through f16 and fp32 in four conversions a pair, which keep NaN; shifting
+// the bits into a bf16 took five instructions and made numbers of the NaN codes (decoding over 65,537 keys,
+// 64 / 8 heads of 128: 41 us against 45).
 template <int FMT>
 constexpr float kByteUnit = FMT == kKvInt8 ? 8192.f : 1.f;
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
@@ -113,7 +113,9 @@ __device__ __forceinline__ uint32_t bytes_to_bf16x2(uint32_t a, uint32_t b, int 
                               : __byte_perm(a, b ^ 0x80808080u, (uint32_t)(lo | hi << 8)) & 0x00ff00ffu;
     return fma_bf16x2(w, 0x7b807b80u, 0xbc80bc80u);  // * 2^120 - 2^-6
   } else {
-    const uint32_t w = lo == 0 && hi == 1 ? a : lo == 2 && hi == 3 ? a >> 16 : __byte_perm(a, b, (uint32_t)(lo | hi << 4));
+    const uint32_t w = lo == 0 && hi == 1   ? a
+                       : lo == 2 && hi == 3 ? a >> 16
+                                            : __byte_perm(a, b, (uint32_t)(lo | hi << 4));
     const float2 x = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3)));
     return pack_bf16x2(x.x, x.y);
   }

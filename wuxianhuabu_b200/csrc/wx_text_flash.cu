@@ -198,7 +198,8 @@ __device__ __noinline__ void remember_codes(uint32_t raw, int tid, int key0, int
     const uint32_t bits =
         nan_code_mask(w.x) | nan_code_mask(w.y) << 4 | nan_code_mask(w.z) << 8 | nan_code_mask(w.w) << 12;
     if (!__any_sync(0xffffffffu, bits != 0)) continue;
-    sts128(at, make_uint4(without_nan_codes(w.x), without_nan_codes(w.y), without_nan_codes(w.z), without_nan_codes(w.w)));
+    sts128(at, make_uint4(without_nan_codes(w.x), without_nan_codes(w.y), without_nan_codes(w.z),
+                          without_nan_codes(w.w)));
     uint32_t mask[4], any = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -1093,8 +1094,9 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       const float inv = l == 0.f ? 0.f : __fdividef(kByteUnit<FMT>, l);
       const int bad = any ? *reinterpret_cast<const volatile int*>(&it.bad) : 0;
       const bool cut = it.pieces > 1;
-      const bool write = ok && live && WX_IN_BOUNDS(p.err, it.q0 >= 0 && it.q0 + tok < p.total_q && it.h * p.group + my_g < p.hq &&
-                                                               it.piece >= 0 && it.piece < tp.splits);
+      const bool write = ok && live &&
+                         WX_IN_BOUNDS(p.err, it.q0 >= 0 && it.q0 + tok < p.total_q && it.h * p.group + my_g < p.hq &&
+                                                 it.piece >= 0 && it.piece < tp.splits);
       const int64_t at_row = ((int64_t)it.q0 + tok) * p.hq + it.h * p.group + my_g;
       const int64_t at_part = it.piece * (p.total_q * p.hq) + at_row;
       __nv_bfloat16* row = p.out + ((int64_t)it.q0 + tok) * p.out_stride + (int64_t)(it.h * p.group + my_g) * HD;

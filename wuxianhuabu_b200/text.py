@@ -9,7 +9,8 @@ runs its text encoder once per generation, model/minimax h3/H3TextEncoder.swift)
 * ``paged_attention``  — new tokens (one per sequence or a chunk) over the cache
 
 Tensors are torch CUDA tensors used as device buffers; calls are ordered on torch's current
-stream and do not synchronise. q, k and v are [tokens, heads, head_dim] bf16 with contiguous
+stream, do not synchronise, and may be captured in CUDA graphs (whose replays must not overlap
+one another: they share the context's captured scratch). q, k and v are [tokens, heads, head_dim] bf16 with contiguous
 heads; the stride between tokens is free, so slices of a packed q|k|v projection need no copy.
 Errors raise ``WxError``; wrong values in device-side arguments (positions, slots, lengths,
 block entries) are caught by the kernels and raise at the next ``Context.check_device``.
