@@ -662,6 +662,21 @@ typedef struct wx_rope {
 int wx_rope_apply(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, const void* x, int64_t row_stride,
                   int64_t tokens, int heads, int head_dim, void* y, int64_t y_stride);
 
+/* Several positions a token (time, height and width of a picture's or clip's tokens): pair i turns by
+ * the position of axis axis_of_pair[i]. Positions are [n_axes][position_stride >= tokens] on the device. */
+typedef struct wx_rope_axes {
+  int32_t n_axes;           /* 1..4 */
+  uint8_t axis_of_pair[64]; /* of the rope's rot/2 pairs, each below n_axes */
+  int64_t position_stride;  /* entries between the axes' positions */
+} wx_rope_axes;
+/* q and k rows normalised head by head, y = x / sqrt(mean x^2 + eps) * norm (fp32, squares too; norm
+ * [head_dim] bf16, NULL: not normalised), and their first rot columns turned; one rounding to bf16.
+ * axes NULL: one position a token. k_heads may be 0; outputs may be the inputs. Positions as in wx_rope_apply. */
+int wx_norm_rope_apply(wx_ctx* ctx, const wx_rope* rope, const wx_rope_axes* axes, const int32_t* positions,
+                       const void* q, int64_t q_stride, int q_heads, const void* q_norm, const void* k,
+                       int64_t k_stride, int k_heads, const void* k_norm, float eps, int64_t tokens, int head_dim,
+                       void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride);
+
 /* ------------------------------------------- text side: paged K/V cache */
 enum wx_kv_format { WX_KV_BF16 = 0, WX_KV_INT8 = 1, WX_KV_E4M3 = 2 };
 typedef struct wx_kv_cache {
@@ -688,9 +703,41 @@ int wx_kv_append(wx_ctx* ctx, const wx_kv_cache* cache, const void* k, int64_t k
 int wx_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, const void* q, int64_t q_stride,
                       int q_heads, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
                       int64_t v_stride, int64_t tokens, const int64_t* slots, void* q_out, int64_t q_out_stride);
+/* The same with the norms and position axes of wx_norm_rope_apply (v is stored as it is). */
+int wx_norm_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const wx_rope_axes* axes, const int32_t* positions,
+                           const void* q, int64_t q_stride, int q_heads, const void* q_norm, const void* k_norm,
+                           float eps, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, int64_t tokens, const int64_t* slots, void* q_out,
+                           int64_t q_out_stride);
 /* k_out / v_out [tokens, kv_heads, head_dim] = bf16(value * scale) of the slots; < 0 reads zeros */
 int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,
                int64_t out_stride);
+
+/* Pages of a cache dealt out to the sequences of a batch, all on the device. The free list is a stack
+ * that grows downwards: free_pages[taken..pages) are free, those before may be anything. A sequence of
+ * lens[b] tokens holds the pages table[b][0 .. ceil(lens / page_size)). */
+typedef struct wx_page_pool {
+  int32_t* free_pages;  /* [pages] */
+  const int32_t* taken; /* [1] */
+  const int32_t* lens;  /* [batch] */
+  int32_t* table;       /* [batch][blocks_per_seq] */
+  int64_t pages;
+  int64_t blocks_per_seq;
+  int32_t batch;     /* at most 8192 */
+  int32_t page_size; /* 16, 32, 64, 128 or 256 */
+} wx_page_pool;
+/* One step: sequence b keeps its first keep[b] tokens (keep NULL: all) and gets add[b] more. Pages that it
+ * no longer needs go back onto the stack, in the order of the sequences; then those that others need come
+ * off it in that order. Writes the table's new entries, free_pages, and for the new tokens, sequence after
+ * sequence, positions (first_position + index in the sequence) and slots; the entries behind them
+ * up to `tokens` become position 0 and slot -1. cu [batch + 1] = offsets of the new tokens, kv_lens [batch] =
+ * keep + add (may be pool->lens: updated in place), taken_out [1] (may be pool->taken). With outputs apart from
+ * lens and taken the step can be planned again. A step that does not fit (more new tokens than `tokens`, no free
+ * page or table entry left, keep above the length, numbers below zero, a position beyond 32 bits) sets the device
+ * error word and changes nothing: kv_lens = lens, taken_out = taken, cu 0, no slots. */
+int wx_page_plan(wx_ctx* ctx, const wx_page_pool* pool, const int32_t* keep, const int32_t* add, int64_t tokens,
+                 int64_t first_position, int32_t* positions, int64_t* slots, int32_t* cu, int32_t* kv_lens,
+                 int32_t* taken_out);
 
 /* ------------------------------------------- text side: attention */
 /* Query head h reads K/V head h / (q_heads / kv_heads). Row i of a sequence with Lq query and

@@ -123,6 +123,15 @@ class KvCache(C.Structure):
                 ("format", C.c_int32)]
 
 
+class RopeAxes(C.Structure):
+    _fields_ = [("n_axes", C.c_int32), ("axis_of_pair", C.c_uint8 * 64), ("position_stride", C.c_int64)]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("free_pages", C.c_void_p), ("taken", C.c_void_p), ("lens", C.c_void_p), ("table", C.c_void_p),
+                ("pages", C.c_int64), ("blocks_per_seq", C.c_int64), ("batch", C.c_int32), ("page_size", C.c_int32)]
+
+
 class AttnDims(C.Structure):
     _fields_ = [("total_q", C.c_int64), ("batch", C.c_int32), ("max_q", C.c_int32), ("q_heads", C.c_int32),
                 ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32),
@@ -241,6 +250,11 @@ _SIGS = {
     "wx_kv_append": (_i32, [_vp, C.POINTER(KvCache), _vp, _i64, _vp, _i64, _i64, _vp]),
     "wx_rope_kv_append": (_i32, [_vp, C.POINTER(Rope), _vp, _vp, _i64, _i32, C.POINTER(KvCache), _vp, _i64, _vp, _i64,
                                  _i64, _vp, _vp, _i64]),
+    "wx_norm_rope_apply": (_i32, [_vp, C.POINTER(Rope), C.POINTER(RopeAxes), _vp, _vp, _i64, _i32, _vp, _vp, _i64, _i32,
+                                  _vp, _f32, _i64, _i32, _vp, _i64, _vp, _i64]),
+    "wx_norm_rope_kv_append": (_i32, [_vp, C.POINTER(Rope), C.POINTER(RopeAxes), _vp, _vp, _i64, _i32, _vp, _vp, _f32,
+                                      C.POINTER(KvCache), _vp, _i64, _vp, _i64, _i64, _vp, _vp, _i64]),
+    "wx_page_plan": (_i32, [_vp, C.POINTER(PagePool), _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "wx_kv_read": (_i32, [_vp, C.POINTER(KvCache), _vp, _i64, _vp, _vp, _i64]),
     "wx_prompt_attention": (_i32, [_vp, C.POINTER(AttnDims), _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp,
                                    _i64, _vp]),

@@ -47,12 +47,16 @@ __global__ void rope_table_kernel(RopeFreqs f, int nf, int64_t positions, double
 // = 5.45 TB/s with clean lines (three or two groups in flight 43 and 67, five 38); 4,096 tokens
 // with rope into an int8 cache and read back, 40 us for both (35.6). 300 tokens take 3 us on the
 // device, a third of the call.
+//
+// With HEADS, q and k rows are normalised first, y = x / sqrt(mean x^2 + eps) * w, the squares summed over
+// the row's lanes, and each pair may turn by a position of its own axis. All of it stays in fp32 until
+// the one rounding (or quantisation) at the end.
 constexpr int kRowGroups = 4;
 
 struct RowsParams {
   const __nv_bfloat16 *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;  // elements between tokens
-  int nq, nkv;                           // q rows, and k (= v) rows of a token (0 without a cache)
+  int nq, nkv, nv;                       // q, k and v rows of a token (no cache: v none)
   int64_t tokens;
   int rows_per_warp, chunks;             // a token's rows are dealt to `chunks` warps
   // rotation (rot = 0: none)
@@ -69,6 +73,15 @@ struct RowsParams {
   int64_t n_slots;
   int page_shift;
   int* err;
+  // HEADS: norm weights (nullptr: none), two bits for each pair's axis, where the axes' positions lie,
+  // and k rows that go here instead of into a cache
+  const __nv_bfloat16 *q_norm, *k_norm;
+  float eps;
+  int axes;
+  uint64_t axis_of[2];
+  int64_t pos_stride;
+  __nv_bfloat16* k_out;
+  int64_t k_out_stride;
 };
 
 template <int W>
@@ -131,13 +144,13 @@ __device__ __forceinline__ float quantise(const float (&x)[N], uint32_t (&w)[N /
   return finite ? (live ? __fdiv_rn(amax, kMax) : 0.f) : __int_as_float(0x7fc00000);
 }
 
-template <int FMT, int HD, int W, bool INTERLEAVED>
+template <int FMT, int HD, int W, bool INTERLEAVED, bool HEADS>
 __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
   constexpr int kLanes = HD / (2 * W);  // lanes of a row
   constexpr int kRows = 32 / kLanes;    // rows of a warp at a time
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes;
-  const int per_token = p.nq + 2 * p.nkv;
+  const int per_token = p.nq + p.nkv + p.nv;
   // a block: eight tokens, the same chunk of each
   const unsigned blk = blockIdx.x / (unsigned)p.chunks;
   const int64_t t = (int64_t)blk * 8 + (threadIdx.x >> 5);
@@ -164,23 +177,55 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
 
   float cs[W], sn[W];
   if (p.rot) {
-    const int64_t pos = p.pos[t];
-    if (pos < 0 || pos >= p.positions) {
+    int64_t pos = p.pos[t];
+    bool bad = pos < 0 || pos >= p.positions;
+    int64_t pos_of[4] = {pos, pos, pos, pos};
+    uint32_t codes = 0;  // axes of this lane's pairs, two bits each
+    if constexpr (HEADS) {
+      if (p.axes > 1) {
+        bool same = true;
+#pragma unroll
+        for (int a = 1; a < 4; ++a) {
+          if (a >= p.axes) break;
+          pos_of[a] = p.pos[a * p.pos_stride + t];
+          bad |= pos_of[a] < 0 || pos_of[a] >= p.positions;
+          same &= pos_of[a] == pos;
+        }
+        // (text: the axes run together, and one row of the table serves all pairs)
+        if (!same) codes = (uint32_t)(p.axis_of[j * W >= 32] >> (2 * (j * W & 31))) & ((1u << 2 * W) - 1u);
+      }
+    }
+    if (bad) {
       if (lane == 0) set_dev_error(p.err, kDevBadArgs);
       return;
     }
     if (turn) {
+      bool whole = true;
+      if constexpr (HEADS) {
+        whole = codes == (codes & 3u) * (0x5555u & ((1u << 2 * W) - 1u));
+        if (whole) pos = (codes & 3u) == 0 ? pos_of[0] : (codes & 3u) == 1 ? pos_of[1] : (codes & 3u) == 2 ? pos_of[2] : pos_of[3];
+      }
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < W; i += 4) {
-        const float4 c = *reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + W * j + i);
-        const float4 s = *reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + W * j + i);
-        cs[i] = c.x, cs[i + 1] = c.y, cs[i + 2] = c.z, cs[i + 3] = c.w;
-        sn[i] = s.x, sn[i + 1] = s.y, sn[i + 2] = s.z, sn[i + 3] = s.w;
+        for (int i = 0; i < W; i += 4) {
+          const float4 c = *reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + W * j + i);
+          const float4 s = *reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + W * j + i);
+          cs[i] = c.x, cs[i + 1] = c.y, cs[i + 2] = c.z, cs[i + 3] = c.w;
+          sn[i] = s.x, sn[i + 1] = s.y, sn[i + 2] = s.z, sn[i + 3] = s.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const uint32_t a = codes >> (2 * i) & 3u;
+          const int64_t at = (a == 0 ? pos_of[0] : a == 1 ? pos_of[1] : a == 2 ? pos_of[2] : pos_of[3]) * (p.rot / 2) + W * j + i;
+          cs[i] = p.cos_t[at];
+          sn[i] = p.sin_t[at];
+        }
       }
     }
   }
   int64_t slot = -1;
-  if (p.nkv) {
+  if (HEADS ? p.slots != nullptr : p.nkv) {
     slot = p.slots[t];
     if (slot >= p.n_slots) {
       if (lane == 0) set_dev_error(p.err, kDevBadArgs);
@@ -201,6 +246,25 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
       const uint32_t u = live ? a[g].w[i] : 0, v = live ? b[g].w[i] : 0;
       x[2 * i] = bf16_lo(u), x[2 * i + 1] = bf16_hi(u);
       x[W + 2 * i] = bf16_lo(v), x[W + 2 * i + 1] = bf16_hi(v);
+    }
+    if constexpr (HEADS) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2 * W; ++i) ss += x[i] * x[i];
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const __nv_bfloat16* weight = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
+      if (weight) {
+        const float rstd = rsqrtf(ss * (1.f / HD) + p.eps);
+        Cols<W> lo, hi;
+        lo.load(weight + c0);
+        hi.load(weight + c1);
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) {
+          x[2 * i] *= rstd * bf16_lo(lo.w[i]), x[2 * i + 1] *= rstd * bf16_hi(lo.w[i]);
+          x[W + 2 * i] *= rstd * bf16_lo(hi.w[i]), x[W + 2 * i + 1] *= rstd * bf16_hi(hi.w[i]);
+        }
+      }
     }
     if (turn && !is_v) {
       // (x1, x2) -> (x1 c - x2 s, x2 c + x1 s)
@@ -223,10 +287,12 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
     const int64_t row = ((((slot >> p.page_shift) * p.nkv + h) << p.page_shift) | (slot & ((1 << p.page_shift) - 1)));
     if (!WX_IN_BOUNDS(p.err, is_q ? h >= 0 && h < p.nq : h >= 0 && h < p.nkv && (slot < 0 || row < p.n_slots * p.nkv)))
       continue;
+    const bool plain_k = HEADS && !is_q && p.k_out;
     if (is_q || FMT == kKvBf16) {
-      __nv_bfloat16* o = is_q ? p.q_out + t * p.q_out_stride + (int64_t)h * HD
-                              : reinterpret_cast<__nv_bfloat16*>(is_v ? p.vc : p.kc) + row * HD;
-      if (!is_q && slot < 0) continue;
+      __nv_bfloat16* o = is_q      ? p.q_out + t * p.q_out_stride + (int64_t)h * HD
+                         : plain_k ? p.k_out + t * p.k_out_stride + (int64_t)h * HD
+                                   : reinterpret_cast<__nv_bfloat16*>(is_v ? p.vc : p.kc) + row * HD;
+      if (!is_q && !plain_k && slot < 0) continue;
       Cols<W> lo, hi;
 #pragma unroll
       for (int i = 0; i < W / 2; ++i) {
@@ -354,31 +420,36 @@ static int64_t deal_rows(wx_ctx* ctx, int64_t tokens, int per_token, int rows_at
 }
 
 template <int FMT, int HD, int W>
-static void start_rows(unsigned g, cudaStream_t s, const RowsParams& p) {
-  if (p.interleaved) text_rows_kernel<FMT, HD, W, true><<<g, 256, 0, s>>>(p);
-  else text_rows_kernel<FMT, HD, W, false><<<g, 256, 0, s>>>(p);
+static void start_rows(unsigned g, cudaStream_t s, const RowsParams& p, bool heads) {
+  if (heads) {
+    if (p.interleaved) text_rows_kernel<FMT, HD, W, true, true><<<g, 256, 0, s>>>(p);
+    else text_rows_kernel<FMT, HD, W, false, true><<<g, 256, 0, s>>>(p);
+  } else {
+    if (p.interleaved) text_rows_kernel<FMT, HD, W, true, false><<<g, 256, 0, s>>>(p);
+    else text_rows_kernel<FMT, HD, W, false, false><<<g, 256, 0, s>>>(p);
+  }
 }
 
 template <int HD, int W>
-static void start_rows(int fmt, unsigned g, cudaStream_t s, const RowsParams& p) {
-  if (fmt == kKvInt8) start_rows<kKvInt8, HD, W>(g, s, p);
-  else if (fmt == kKvE4m3) start_rows<kKvE4m3, HD, W>(g, s, p);
-  else start_rows<kKvBf16, HD, W>(g, s, p);
+static void start_rows(int fmt, unsigned g, cudaStream_t s, const RowsParams& p, bool heads) {
+  if (fmt == kKvInt8) start_rows<kKvInt8, HD, W>(g, s, p, heads);
+  else if (fmt == kKvE4m3) start_rows<kKvE4m3, HD, W>(g, s, p, heads);
+  else start_rows<kKvBf16, HD, W>(g, s, p, heads);
 }
 
-static int launch_rows(wx_ctx* ctx, RowsParams& p, int fmt, int head_dim) {
+static int launch_rows(wx_ctx* ctx, RowsParams& p, int fmt, int head_dim, bool heads = false) {
   if (p.tokens == 0) return WX_OK;
   const int W = p.rot % 16 == 0 ? 8 : 4;
   const int64_t blocks =
-      deal_rows(ctx, p.tokens, p.nq + 2 * p.nkv, 32 / (head_dim / (2 * W)), &p.rows_per_warp, &p.chunks);
+      deal_rows(ctx, p.tokens, p.nq + p.nkv + p.nv, 32 / (head_dim / (2 * W)), &p.rows_per_warp, &p.chunks);
   if (blocks > INT32_MAX) return set_error(ctx, WX_ERR_UNSUPPORTED, "too many tokens in one call");
   p.err = ctx->dev_err;
   ProfScope prof(ctx, kProfRow);
   const unsigned g = (unsigned)blocks;
   if (head_dim == 128)
-    W == 8 ? start_rows<128, 8>(fmt, g, ctx->stream, p) : start_rows<128, 4>(fmt, g, ctx->stream, p);
+    W == 8 ? start_rows<128, 8>(fmt, g, ctx->stream, p, heads) : start_rows<128, 4>(fmt, g, ctx->stream, p, heads);
   else
-    W == 8 ? start_rows<64, 8>(fmt, g, ctx->stream, p) : start_rows<64, 4>(fmt, g, ctx->stream, p);
+    W == 8 ? start_rows<64, 8>(fmt, g, ctx->stream, p, heads) : start_rows<64, 4>(fmt, g, ctx->stream, p, heads);
   return launch_status(ctx, "text_rows");
 }
 
@@ -396,7 +467,7 @@ static void set_rope(RowsParams& p, const wx_rope* r, const int32_t* pos) {
 }
 
 static void set_cache(RowsParams& p, const wx_kv_cache* c, const int64_t* slots) {
-  p.nkv = c->kv_heads;
+  p.nkv = p.nv = c->kv_heads;
   p.kc = static_cast<uint8_t*>(c->k);
   p.vc = static_cast<uint8_t*>(c->v);
   p.ks = c->k_scale;
@@ -404,6 +475,27 @@ static void set_cache(RowsParams& p, const wx_kv_cache* c, const int64_t* slots)
   p.slots = slots;
   p.n_slots = c->pages * c->page_size;
   p.page_shift = __builtin_ctz((unsigned)c->page_size);
+}
+
+// head norms and position axes of a call
+static int set_heads(wx_ctx* ctx, RowsParams& p, const wx_rope* rope, const wx_rope_axes* axes, const void* q_norm,
+                     const void* k_norm, float eps) {
+  WX_CHECK_ARG(ctx, aligned16(q_norm) && aligned16(k_norm));
+  WX_CHECK_ARG(ctx, (!q_norm && !k_norm) || (eps > 0.f && eps < INFINITY));
+  p.q_norm = static_cast<const __nv_bfloat16*>(q_norm);
+  p.k_norm = static_cast<const __nv_bfloat16*>(k_norm);
+  p.eps = eps;
+  p.axes = 1;
+  if (!axes) return WX_OK;
+  WX_CHECK_ARG(ctx, axes->n_axes >= 1 && axes->n_axes <= 4);
+  WX_CHECK_ARG(ctx, axes->n_axes == 1 || axes->position_stride >= p.tokens);
+  p.axes = axes->n_axes;
+  p.pos_stride = axes->position_stride;
+  for (int i = 0; i < rope->rot / 2; ++i) {
+    WX_CHECK_ARG(ctx, axes->axis_of_pair[i] < axes->n_axes);
+    p.axis_of[i / 32] |= (uint64_t)axes->axis_of_pair[i] << (2 * (i % 32));
+  }
+  return WX_OK;
 }
 
 }  // namespace wx
@@ -512,6 +604,67 @@ int wx_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions
   p.q_out = static_cast<__nv_bfloat16*>(q_out);
   p.q_out_stride = q_out_stride;
   return launch_rows(ctx, p, cache->format, hd);
+}
+
+int wx_norm_rope_apply(wx_ctx* ctx, const wx_rope* rope, const wx_rope_axes* axes, const int32_t* positions,
+                       const void* q, int64_t q_stride, int q_heads, const void* q_norm, const void* k,
+                       int64_t k_stride, int k_heads, const void* k_norm, float eps, int64_t tokens, int head_dim,
+                       void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride) {
+  DeviceScope on_device(ctx);
+  WX_CHECK_ARG(ctx, ctx && tokens >= 0 && q_heads > 0 && k_heads >= 0 && q_heads <= INT32_MAX - k_heads);
+  if (head_dim != 128 && head_dim != 64)
+    return set_error(ctx, WX_ERR_UNSUPPORTED, "rope head_dim must be 128 or 64 (got %d)", head_dim);
+  if (!tokens) return WX_OK;
+  int st = check_rope(ctx, rope, head_dim, positions);
+  if (st) return st;
+  WX_CHECK_ARG(ctx, row_ok(q, q_stride, q_heads, head_dim) && row_ok(q_out, q_out_stride, q_heads, head_dim));
+  WX_CHECK_ARG(ctx, k_heads == 0 ||
+                        (row_ok(k, k_stride, k_heads, head_dim) && row_ok(k_out, k_out_stride, k_heads, head_dim)));
+  RowsParams p{};
+  set_rope(p, rope, positions);
+  p.tokens = tokens;
+  if ((st = set_heads(ctx, p, rope, axes, q_norm, k_norm, eps))) return st;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.nq = q_heads;
+  p.nkv = k_heads;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.q_out_stride = q_out_stride;
+  p.k_out = static_cast<__nv_bfloat16*>(k_out);
+  p.k_out_stride = k_out_stride;
+  return launch_rows(ctx, p, kKvBf16, head_dim, true);
+}
+
+int wx_norm_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const wx_rope_axes* axes, const int32_t* positions,
+                           const void* q, int64_t q_stride, int q_heads, const void* q_norm, const void* k_norm,
+                           float eps, const wx_kv_cache* cache, const void* k, int64_t k_stride, const void* v,
+                           int64_t v_stride, int64_t tokens, const int64_t* slots, void* q_out,
+                           int64_t q_out_stride) {
+  DeviceScope on_device(ctx);
+  WX_CHECK_ARG(ctx, ctx && tokens >= 0 && q_heads > 0);
+  int st = check_kv_cache(ctx, cache);
+  if (st || !tokens) return st;
+  if ((st = check_rope(ctx, rope, cache->head_dim, positions))) return st;
+  const int hd = cache->head_dim;
+  WX_CHECK_ARG(ctx, slots && row_ok(q, q_stride, q_heads, hd) && row_ok(q_out, q_out_stride, q_heads, hd) &&
+                        row_ok(k, k_stride, cache->kv_heads, hd) && row_ok(v, v_stride, cache->kv_heads, hd));
+  RowsParams p{};
+  set_rope(p, rope, positions);
+  set_cache(p, cache, slots);
+  p.tokens = tokens;
+  if ((st = set_heads(ctx, p, rope, axes, q_norm, k_norm, eps))) return st;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const __nv_bfloat16*>(k);
+  p.v = static_cast<const __nv_bfloat16*>(v);
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.nq = q_heads;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.q_out_stride = q_out_stride;
+  return launch_rows(ctx, p, cache->format, hd, true);
 }
 
 int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,

@@ -3,7 +3,9 @@ linears to make the hidden states that ``H3TextRefiner`` and ``H3DiT.step`` take
 runs its text encoder once per generation, model/minimax h3/H3TextEncoder.swift).
 
 * ``RopeTable``        — rotary positions of a token stream (interleaved or half layout, part of
-  the head, scaled for long contexts)
+  the head, scaled for long contexts, one or several position axes), with norms of the q and k heads
+* ``PagePool``         — the pages of a cache dealt out to sequences, and a step's positions, slots
+  and lengths, made on the device
 * ``PagedKVCache``     — a paged K/V cache, quantised as it is written, read back on demand
 * ``prompt_attention`` — whole prompts: causal, grouped heads, packed sequences
 * ``paged_attention``  — new tokens (one per sequence or a chunk) over the cache
@@ -19,17 +21,18 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Sequence
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (KV_BF16, KV_E4M3, KV_INT8, ROPE_BY_PARTS, ROPE_LINEAR, ROPE_PLAIN, AttnDims, KvCache, Rope, WxError,
-                   check)
+from ._lib import (KV_BF16, KV_E4M3, KV_INT8, ROPE_BY_PARTS, ROPE_LINEAR, ROPE_PLAIN, AttnDims, KvCache, Rope, RopeAxes,
+                   WxError, check)
 from .h3 import _need_bf16_cuda, _p, context
 
-__all__ = ["RopeScaling", "RopeTable", "PagedKVCache", "prompt_attention", "paged_attention"]
+__all__ = ["RopeScaling", "RopeTable", "rope_axes", "PagePool", "StepPlan", "PagedKVCache", "prompt_attention",
+           "paged_attention"]
 
 _FORMATS = {"bf16": (KV_BF16, torch.bfloat16), "int8": (KV_INT8, torch.int8), "e4m3": (KV_E4M3, torch.float8_e4m3fn)}
 _SCALINGS = {"none": ROPE_PLAIN, "linear": ROPE_LINEAR, "by_parts": ROPE_BY_PARTS}
@@ -92,6 +95,17 @@ class RopeScaling:
     magnitude: float = 1.0
 
 
+def rope_axes(shares: Sequence[int], dealt: bool = False) -> tuple[int, ...]:
+    """The position axis of each pair, from the pairs that each axis has: in runs (axis 0's pairs first),
+    or ``dealt`` out in turn while an axis has pairs left."""
+    left = [int(n) for n in shares]
+    if not 1 <= len(left) <= 4 or min(left) < 0:
+        raise _invalid("shares must be the pairs of 1 to 4 axes")
+    if not dealt:
+        return tuple(a for a, n in enumerate(left) for _ in range(n))
+    return tuple(a for turn in range(max(left)) for a, n in enumerate(left) if turn < n)
+
+
 class _Described:
     """An object whose tensors the library is told of in a struct, ``_desc``. It is made at the first call
     that needs it, checked, and made again after an attribute was assigned; copies make their own."""
@@ -110,11 +124,25 @@ class _Described:
         return {k: v for k, v in self.__dict__.items() if k != "_desc"}
 
 
+def _head_norm(w: Optional[torch.Tensor], d: int, what: str) -> Optional[int]:
+    """The device pointer of a head norm's weight [head_dim]."""
+    if w is None:
+        return None
+    _need_bf16_cuda(w)
+    if w.numel() != d or not w.is_contiguous():
+        raise _invalid(f"{what} must be a contiguous [head_dim] tensor")
+    return w.data_ptr()
+
+
 class RopeTable(_Described):
-    """cos / sin of every position, fp32 [positions, rot / 2] (angles in 64 bits)."""
+    """cos / sin of every position, fp32 [positions, rot / 2] (angles in 64 bits). With ``axes`` (one
+    axis a pair, ``rope_axes``) a token has a position on each axis: positions are [axes, tokens]
+    then, instead of [tokens]."""
+    axes: Optional[tuple] = None
 
     def __init__(self, rot: int, positions: int, base: float = 10000.0, interleaved: bool = False,
-                 scaling: Optional[RopeScaling] = None, device: Optional[int] = None):
+                 scaling: Optional[RopeScaling] = None, device: Optional[int] = None,
+                 axes: Optional[Sequence[int]] = None):
         s = scaling or RopeScaling()
         if s.kind not in _SCALINGS:
             raise _invalid(f"unknown rope scaling {s.kind!r}")
@@ -127,15 +155,19 @@ class RopeTable(_Described):
         dev = torch.device("cuda", ctx.device)
         self.inv_freq = inv
         self.interleaved = interleaved
+        self.axes = axes
         self.cos = torch.empty((positions, rot // 2), dtype=torch.float32, device=dev)
         self.sin = torch.empty_like(self.cos)
+        self._desc  # (checked)
         ctx.call("wx_rope_table", inv.ctypes.data, rot // 2, positions, float(s.magnitude), _p(self.cos), _p(self.sin))
 
     @classmethod
-    def from_tables(cls, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False) -> "RopeTable":
+    def from_tables(cls, cos: torch.Tensor, sin: torch.Tensor, interleaved: bool = False,
+                    axes: Optional[Sequence[int]] = None) -> "RopeTable":
         """Over tables that exist already (not copied)."""
         self = cls.__new__(cls)
         self.cos, self.sin, self.interleaved, self.inv_freq = cos, sin, interleaved, None
+        self.axes = axes
         self._desc  # (checked)
         return self
 
@@ -148,16 +180,137 @@ class RopeTable(_Described):
             raise _invalid("cos and sin must have one shape")
         _same_device(cos, sin)
         n, half = cos.shape
+        if self.axes is not None and len(self.axes) != half:
+            raise _invalid(f"axes must have an entry for each of the {half} pairs, got {len(self.axes)}")
         return Rope(_p(cos), _p(sin), n, 2 * half, int(self.interleaved))
+
+    def __setattr__(self, name: str, value) -> None:
+        if name == "axes" and value is not None:
+            value = tuple(int(a) for a in value)
+            if not value or len(value) > 64 or min(value) < 0 or max(value) > 3:
+                raise _invalid("axes must name one of 4 axes for each pair")
+            # (as the library takes it, but for the positions' stride, which is the call's)
+            object.__setattr__(self, "_axes_as_bytes", bytes(RopeAxes(max(value) + 1, (C.c_uint8 * 64)(*value), 0)))
+        super().__setattr__(name, value)
+
+    def _at(self, positions: torch.Tensor, n: int):
+        """The device pointer of positions, and the axes of this call (None: one position a token)."""
+        if self.axes is None:
+            return _need_ints(torch.int32, n, "positions", positions), None
+        axes = RopeAxes.from_buffer_copy(self._axes_as_bytes)
+        if not positions.is_cuda or positions.dtype != torch.int32 or positions.dim() != 2 or \
+                positions.shape[0] < axes.n_axes or positions.shape[1] != n:
+            raise _invalid(f"positions must be a CUDA int32 [axes, tokens] tensor of {axes.n_axes} axes and {n} tokens")
+        axes.position_stride, inner = positions.stride()
+        if n > 1 and inner != 1:
+            raise _invalid("positions of an axis must be contiguous")
+        return positions.data_ptr(), C.byref(axes)
+
+    def apply_qk(self, q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_norm: Optional[torch.Tensor] = None,
+                 k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """q and k of the same tokens, each head normalised by its root mean square and q_norm / k_norm
+        [head_dim] where given, and turned, in one launch; outputs may be the inputs."""
+        n, hq, d, qs = _rows(q, "q")
+        nk, hk, dk, ks = _rows(k, "k")
+        if (nk, dk) != (n, d):
+            raise _invalid("k must have q's tokens and head_dim")
+        qw, kw = _head_norm(q_norm, d, "q_norm"), _head_norm(k_norm, d, "k_norm")
+        at, axes = self._at(positions, n)
+        qo, qos = _out_rows(q, n, hq, d, q_out, "q_out must have q's shape")
+        ko, kos = _out_rows(k, n, hk, d, k_out, "k_out must have k's shape")
+        dev = _same_device(q, k, positions, qo, ko, self.cos, *(w for w in (q_norm, k_norm) if w is not None))
+        context(dev).call("wx_norm_rope_apply", self._desc, axes, at, q.data_ptr(), qs, hq, qw, k.data_ptr(), ks, hk, kw,
+                          eps, n, d, qo.data_ptr(), qos, ko.data_ptr(), kos)
+        return qo, ko
 
     def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x [tokens, heads, head_dim] with token t turned by positions[t] (int32); ``out`` may be x."""
         n, h, d, stride = _rows(x, "x")
+        if self.axes is not None:
+            at, axes = self._at(positions, n)
+            o, ostride = _out_rows(x, n, h, d, out, "out must have x's shape")
+            context(_same_device(x, positions, o, self.cos)).call(
+                "wx_norm_rope_apply", self._desc, axes, at, x.data_ptr(), stride, h, None, None, 0, 0, None, 0.0, n, d,
+                o.data_ptr(), ostride, None, 0)
+            return o
         at = _need_ints(torch.int32, n, "positions", positions)
         o, ostride = _out_rows(x, n, h, d, out, "out must have x's shape")
         context(_same_device(x, positions, o, self.cos)).call(
             "wx_rope_apply", self._desc, at, x.data_ptr(), stride, n, h, d, o.data_ptr(), ostride)
         return o
+
+
+@dataclass
+class StepPlan:
+    """A step's arrays on the device: positions [tokens] int32, slots [tokens] int64 (-1: no token),
+    cu_seqlens [batch + 1], kv_lens [batch] and the free list's height [1] int32."""
+    positions: torch.Tensor
+    slots: torch.Tensor
+    cu_seqlens: torch.Tensor
+    kv_lens: torch.Tensor
+    taken: torch.Tensor
+
+
+class PagePool(_Described):
+    """The pages of a cache (or of several of one geometry) dealt out to the sequences of a batch, on the
+    device. ``free`` [pages] int32 is a stack that grows downwards: its entries from ``taken`` [1] on
+    are free. Sequence b has ``lens``[b] tokens in the pages ``table``[b] ([batch, blocks], the
+    ``block_table`` of ``paged_attention``)."""
+
+    def __init__(self, pages: int, page_size: int, batch: int, blocks: int, device: Optional[int] = None):
+        dev = torch.device("cuda", context(device).device)
+        if min(pages, blocks) <= 0 or batch < 0:
+            raise _invalid("pages and blocks must be positive, batch not negative")
+        self.page_size = page_size
+        self.free = torch.arange(pages, dtype=torch.int32, device=dev)
+        self.taken = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.table = torch.full((batch, blocks), -1, dtype=torch.int32, device=dev)
+        self._desc  # (checked)
+
+    @classmethod
+    def from_tensors(cls, page_size: int, free: torch.Tensor, taken: torch.Tensor, lens: torch.Tensor,
+                     table: torch.Tensor) -> "PagePool":
+        """Over arrays that exist already (not copied)."""
+        self = cls.__new__(cls)
+        self.page_size, self.free, self.taken, self.lens, self.table = page_size, free, taken, lens, table
+        self._desc  # (checked)
+        return self
+
+    def _describe(self) -> _lib.PagePool:
+        batch = self.lens.numel()
+        free = _need_ints(torch.int32, None, "free", self.free)
+        taken = _need_ints(torch.int32, 1, "taken", self.taken)
+        lens = _need_ints(torch.int32, None, "lens", self.lens)
+        table = _need_ints(torch.int32, None, "table", self.table)
+        if self.table.dim() != 2 or self.table.shape[0] != batch:
+            raise _invalid("table must be [batch, blocks]")
+        _same_device(self.free, self.taken, self.lens, self.table)
+        return _lib.PagePool(free, taken, lens, table, self.free.numel(), self.table.shape[1], batch, self.page_size)
+
+    def plan(self, new: torch.Tensor, tokens: int, keep: Optional[torch.Tensor] = None, first_position: int = 0,
+             commit: bool = True) -> StepPlan:
+        """One step: sequence b keeps its first keep[b] tokens (all without ``keep``) and gets new[b] more
+        (int32, on the device), pages being given back and taken as that needs: an ended sequence keeps 0,
+        rejected drafts are not kept. ``tokens``: entries of positions and slots, as many as the new tokens
+        or more. Positions count from ``first_position`` (tokens that stand before every sequence). With
+        ``commit`` lens and taken are brought up to date, and are the plan's kv_lens and taken; without, the
+        plan has its own and the step can be planned again. A step that does not fit raises at the next
+        ``check_device`` and changes nothing (no slots, no new tokens)."""
+        batch = self.lens.numel()
+        add = _need_ints(torch.int32, batch, "new", new)
+        kept = None if keep is None else _need_ints(torch.int32, batch, "keep", keep)
+        if not 0 <= tokens < _INT32 or not 0 <= first_position < _INT32:
+            raise _invalid("tokens and first_position must be in 0..2^31 - 1")
+        dev = _same_device(self.lens, new, new if keep is None else keep)
+        desc = self._desc
+        pos, slots = new.new_empty(tokens), new.new_empty(tokens, dtype=torch.int64)
+        cu = new.new_empty(batch + 1)
+        lens, taken = (self.lens, self.taken) if commit else (torch.empty_like(self.lens), torch.empty_like(self.taken))
+        context(dev).call("wx_page_plan", desc, kept, add, tokens, first_position, pos.data_ptr(), slots.data_ptr(),
+                          cu.data_ptr(), lens.data_ptr(), taken.data_ptr())
+        return StepPlan(pos, slots, cu, lens, taken)
 
 
 class PagedKVCache(_Described):
@@ -228,14 +381,25 @@ class PagedKVCache(_Described):
                                                         n, at)
 
     def append_roped(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, rope: RopeTable,
-                     positions: torch.Tensor, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """``rope.apply`` of q (returned) and k, and ``append`` of k and v, in one launch."""
+                     positions: torch.Tensor, q_out: Optional[torch.Tensor] = None,
+                     q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+                     eps: float = 1e-6) -> torch.Tensor:
+        """``rope.apply`` of q (returned) and k, and ``append`` of k and v, in one launch; with ``q_norm`` /
+        ``k_norm`` [head_dim] the heads are normalised first, as in ``rope.apply_qk``."""
         n, ks, vs, at = self._kv(k, v, slots)
         nq, hq, dq, qs = _rows(q, "q")
         if (nq, dq) != (n, self.head_dim):
             raise _invalid("q must be [tokens, q_heads, head_dim] of k's tokens")
-        pos = _need_ints(torch.int32, n, "positions", positions)
         o, ostride = _out_rows(q, n, hq, dq, q_out, "q_out must have q's shape")
+        if rope.axes is not None or q_norm is not None or k_norm is not None:
+            qw, kw = _head_norm(q_norm, dq, "q_norm"), _head_norm(k_norm, dq, "k_norm")
+            pos, axes = rope._at(positions, n)
+            dev = _same_device(self.k, q, k, v, slots, positions, o, rope.cos,
+                               *(w for w in (q_norm, k_norm) if w is not None))
+            context(dev).call("wx_norm_rope_kv_append", rope._desc, axes, pos, q.data_ptr(), qs, hq, qw, kw, eps,
+                              self._desc, k.data_ptr(), ks, v.data_ptr(), vs, n, at, o.data_ptr(), ostride)
+            return o
+        pos = _need_ints(torch.int32, n, "positions", positions)
         context(_same_device(self.k, q, k, v, slots, positions, o, rope.cos)).call(
             "wx_rope_kv_append", rope._desc, pos, q.data_ptr(), qs, hq, self._desc, k.data_ptr(), ks, v.data_ptr(), vs,
             n, at, o.data_ptr(), ostride)
