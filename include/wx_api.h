@@ -765,6 +765,12 @@ typedef struct wx_attn_dims {
 int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride, const void* k,
                         int64_t k_stride, const void* v, int64_t v_stride, int64_t total_k, const int32_t* cu_q,
                         const int32_t* cu_k, void* out, int64_t out_stride, float* lse);
+/* The same where, beside the window, the first `sinks` keys of a sequence stay visible (to rows that
+ * stand at or behind them): a row at key p sees j <= p with j > p - window or j < sinks. Without a window
+ * sinks change nothing. */
+int wx_prompt_attention_sinks(wx_ctx* ctx, const wx_attn_dims* dims, int32_t sinks, const void* q, int64_t q_stride,
+                              const void* k, int64_t k_stride, const void* v, int64_t v_stride, int64_t total_k,
+                              const int32_t* cu_q, const int32_t* cu_k, void* out, int64_t out_stride, float* lse);
 /* New tokens (1 per sequence when decoding, a chunk of a prompt otherwise) over the paged cache
  * that holds them already: sequence b has kv_lens[b] cached tokens in pages block_table[b,
  * 0..], its queries being the last ones. Block entries beyond the length are not read. Few query
@@ -772,6 +778,11 @@ int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, in
 int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
                        const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
                        const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride, float* lse);
+/* with first keys that stay visible beside the window, as in wx_prompt_attention_sinks */
+int wx_paged_attention_sinks(wx_ctx* ctx, const wx_attn_dims* dims, int32_t sinks, const void* q, int64_t q_stride,
+                             const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
+                             const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride,
+                             float* lse);
 
 #ifdef __cplusplus
 }

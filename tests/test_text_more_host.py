@@ -13,6 +13,10 @@ def test_calls_without_a_context_are_refused():
         == _lib.WX_ERR_INVALID
     assert lib.wx_norm_rope_kv_append(None, None, None, None, None, 0, 0, None, None, 0.0, None, None, 0, None, 0, 0, None,
                                       None, 0) == _lib.WX_ERR_INVALID
+    assert lib.wx_prompt_attention_sinks(None, None, 0, None, 0, None, 0, None, 0, 0, None, None, None, 0, None) \
+        == _lib.WX_ERR_INVALID
+    assert lib.wx_paged_attention_sinks(None, None, 0, None, 0, None, None, None, None, 0, None, 0, None) \
+        == _lib.WX_ERR_INVALID
     assert lib.wx_page_plan(None, None, None, None, 0, 0, None, None, None, None, None) == _lib.WX_ERR_INVALID
 
 

@@ -92,7 +92,7 @@ struct RowsGeom {
   static constexpr int kSmem = kWarps * kStages * kStep + kJoin;
 };
 
-template <int FMT, int HD, int NT>
+template <int FMT, int HD, int NT, int KEYS>
 __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     text_rows_attn_kernel(const uint8_t* __restrict__ k_base, const uint8_t* __restrict__ v_base, int64_t k_stride,
                           int64_t v_stride, TextAttnParams p, int min_units) {
@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
 
   // ---- the line of units, walked 32 sequences at a time by each warp for itself (32-bit
   // arithmetic: 64-bit divisions were most of a short call's start)
+  // (k16: first key; with first keys that stay visible, the 16-key steps before the window)
   auto line_of = [&](int b, unsigned& items, unsigned& nu, int& k16) {
     items = nu = 0;
     k16 = 0;
@@ -120,7 +121,8 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     const Seq s = load_seq(p, b);
     k16 = key_lo(p, s, 0) & ~15;
     items = ((unsigned)(s.lq * p.group) + kRows - 1) / kRows * (unsigned)p.hkv;
-    nu = (unsigned)max(1, (s.lk - k16 + kUnit - 1) / kUnit);
+    const int skip = KEYS == kSinkKeys ? key_gap<KEYS>(p, k16 >> 4, 16).gap << 4 : k16;
+    nu = (unsigned)max(1, (s.lk - skip + kUnit - 1) / kUnit);
   };
   unsigned my_items = 0, my_nu = 0;  // of sequence loaded + lane
   int my_k16 = 0, loaded = -1;
@@ -149,7 +151,8 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     Seq s;
     int b, h, rt;
     unsigned item, item_u0, nu;  // the item, its first unit and its units
-    int k_lo, k_hi;              // keys of this piece (k_lo a multiple of 16)
+    int k_lo, k_hi;              // keys of this piece (k_lo a multiple of 16), without those in the gap
+    KeyGap at16;                 // of 16-key steps
     int steps;                   // 16-key steps of this piece for this warp
   };
   // the sequence found last: its first unit and item, the end of its units, its row tiles and first key
@@ -194,8 +197,9 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     c.item = b_i0 + i;
     c.item_u0 = b_u0 + i * c.nu;
     const unsigned units = min(c.nu - u_in, u_end - at);
-    c.k_lo = k16 + (int)u_in * kUnit;
-    c.k_hi = min(c.s.lk, c.k_lo + (int)units * kUnit);
+    c.at16 = key_gap<KEYS>(p, k16 >> 4, 16);
+    c.k_lo = (KEYS == kSinkKeys ? 0 : k16) + (int)u_in * kUnit;
+    c.k_hi = min(c.s.lk - (c.at16.gap << 4), c.k_lo + (int)units * kUnit);
     const int n16 = max(0, (c.k_hi - c.k_lo + 15) / 16);
     c.steps = n16 > warp ? (n16 - warp + kWarps - 1) / kWarps : 0;
     return units;
@@ -206,7 +210,11 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   const bool paged = kW || p.block_table;
   [[maybe_unused]] const int64_t kv_rows = paged ? (p.pages * p.hkv) << p.page_shift : p.total_k;
   int page_of = 0;
-  auto first_key = [&](const Piece& c, int i) { return c.k_lo + (i * kWarps + warp) * 16; };
+  auto step_key = [&](const Piece& c, int i) { return c.k_lo + (i * kWarps + warp) * 16; };
+  auto first_key = [&](const Piece& c, int i) {
+    const int j = step_key(c, i);
+    return KEYS == kSinkKeys ? c.at16(j >> 4) << 4 : j;
+  };
   // row of the step's first key: of the cache, or of the packed keys
   auto step_row = [&](const Piece& c, int i) -> int64_t {
     const int j0 = first_key(c, i);
@@ -214,7 +222,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     if ((i & 31) == 0) {
       const int jl = first_key(c, i + lane);
       page_of = 0;
-      if (jl < c.k_hi) {
+      if (step_key(c, i + lane) < c.k_hi) {
         page_of = p.block_table[c.b * p.blocks_per_seq + (jl >> p.page_shift)];
         if (page_of < 0 || page_of >= p.pages) {
           set_dev_error(p.err, kDevBadArgs);
@@ -345,7 +353,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
       copy_async_wait<kD - 1>();
       __syncwarp();
       const int j0 = first_key(cur, i);
-      const bool masked = j0 + 16 > free_hi || j0 < free_lo;
+      const bool masked = j0 + 16 > free_hi || (j0 < free_lo && (KEYS != kSinkKeys || j0 + 16 > p.sinks));
       float sc[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int j = j0 + g + 8 * (q >> 1);
-            if (j >= lim_hi[n][q & 1] || j < lim_lo[n][q & 1]) sc[n][q] = -INFINITY;
+            if (!key_seen<KEYS>(p, j, lim_lo[n][q & 1], lim_hi[n][q & 1])) sc[n][q] = -INFINITY;
           }
         }
         // The maximum is moved only when it has grown by 2^8: most steps leave O^T alone and take no
@@ -482,7 +490,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                   for (int e = 0; e < 2; ++e)
-                    if ((x >> d & 1u) && j < lim_hi[n][e] && j >= lim_lo[n][e])
+                    if ((x >> d & 1u) && key_seen<KEYS>(p, j, lim_lo[n][e], lim_hi[n][e]))
                       acc[n][d >> 1][2 * (d & 1) + e] = __int_as_float(0x7fc00000);
             }
           }
@@ -529,7 +537,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
                   const float v = d & 1 ? bf16_hi(x) : bf16_lo(x);
 #pragma unroll
                   for (int e = 0; e < 2; ++e)
-                    if (j < lim_hi[n][e] && j >= lim_lo[n][e]) acc[n][d >> 1][2 * (d & 1) + e] += w[e] * v;
+                    if (key_seen<KEYS>(p, j, lim_lo[n][e], lim_hi[n][e])) acc[n][d >> 1][2 * (d & 1) + e] += w[e] * v;
                 }
               }
             }
@@ -751,7 +759,7 @@ static void fill_params(wx_ctx* ctx, const wx_attn_dims* d, const void* q, int64
   p.err = ctx->dev_err;
 }
 
-template <int FMT, int HD, int NT>
+template <int FMT, int HD, int NT, int KEYS>
 static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   using G = RowsGeom<FMT, HD, NT>;
   const int grid = std::min(ctx->num_sms, G::kWarps * (G::kPitch + 2) / 2);  // (an item's pieces: the join buffer)
@@ -769,7 +777,7 @@ static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   p.part_ml = reinterpret_cast<float*>(ws + o_ml);
   p.n_items = items;
   if (!(p.counters = arrival_counters(ctx, items, &st))) return st;
-  auto fn = text_rows_attn_kernel<FMT, HD, NT>;
+  auto fn = text_rows_attn_kernel<FMT, HD, NT, KEYS>;
   if ((st = ensure_smem_attr(ctx, (const void*)fn, G::kSmem, "text_rows_attn"))) return st;
   const int64_t bytes = G::kWide ? 1 : 2;
   ProfScope prof(ctx, kProfAttn);
@@ -778,11 +786,18 @@ static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   return launch_status(ctx, "text_rows_attn");
 }
 
-template <int FMT>
+template <int FMT, int KEYS>
 static int launch_rows_attn(wx_ctx* ctx, int head_dim, int64_t rows, const TextAttnParams& p, const KvSource& kv) {
   if (head_dim == 128)
-    return rows <= 8 ? launch_rows_attn<FMT, 128, 1>(ctx, p, kv) : launch_rows_attn<FMT, 128, 2>(ctx, p, kv);
-  return rows <= 8 ? launch_rows_attn<FMT, 64, 1>(ctx, p, kv) : launch_rows_attn<FMT, 64, 2>(ctx, p, kv);
+    return rows <= 8 ? launch_rows_attn<FMT, 128, 1, KEYS>(ctx, p, kv) : launch_rows_attn<FMT, 128, 2, KEYS>(ctx, p, kv);
+  return rows <= 8 ? launch_rows_attn<FMT, 64, 1, KEYS>(ctx, p, kv) : launch_rows_attn<FMT, 64, 2, KEYS>(ctx, p, kv);
+}
+
+template <int KEYS>
+static int launch_rows_attn(wx_ctx* ctx, int head_dim, int64_t rows, const TextAttnParams& p, const KvSource& kv) {
+  if (kv.format == kKvInt8) return launch_rows_attn<kKvInt8, KEYS>(ctx, head_dim, rows, p, kv);
+  if (kv.format == kKvE4m3) return launch_rows_attn<kKvE4m3, KEYS>(ctx, head_dim, rows, p, kv);
+  return launch_rows_attn<kKvBf16, KEYS>(ctx, head_dim, rows, p, kv);
 }
 
 // Few flattened rows a sequence (a decoding step, a few drafted tokens) go to the rows kernel, which
@@ -804,10 +819,10 @@ static int launch_rows_attn(wx_ctx* ctx, int head_dim, int64_t rows, const TextA
 // the amount of work, which is known on the device only, was not tried.
 static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParams& p, const KvSource& kv) {
   const int64_t rows = (int64_t)d->max_q * p.group;
-  if (rows > (kv.format == kKvBf16 ? 16 : kv.format == kKvE4m3 ? 32 : 48)) return text_flash(ctx, p, d->head_dim, kv);
-  if (kv.format == kKvInt8) return launch_rows_attn<kKvInt8>(ctx, d->head_dim, rows, p, kv);
-  if (kv.format == kKvE4m3) return launch_rows_attn<kKvE4m3>(ctx, d->head_dim, rows, p, kv);
-  return launch_rows_attn<kKvBf16>(ctx, d->head_dim, rows, p, kv);
+  const int keys = p.window && p.sinks ? kSinkKeys : kPlainKeys;
+  if (rows > (kv.format == kKvBf16 ? 16 : kv.format == kKvE4m3 ? 32 : 48)) return text_flash(ctx, p, d->head_dim, kv, keys);
+  return keys == kSinkKeys ? launch_rows_attn<kSinkKeys>(ctx, d->head_dim, rows, p, kv)
+                           : launch_rows_attn<kPlainKeys>(ctx, d->head_dim, rows, p, kv);
 }
 
 }  // namespace wx
@@ -816,10 +831,11 @@ using namespace wx;
 
 extern "C" {
 
-int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride, const void* k,
-                        int64_t k_stride, const void* v, int64_t v_stride, int64_t total_k, const int32_t* cu_q,
-                        const int32_t* cu_k, void* out, int64_t out_stride, float* lse) {
+int wx_prompt_attention_sinks(wx_ctx* ctx, const wx_attn_dims* dims, int32_t sinks, const void* q, int64_t q_stride,
+                              const void* k, int64_t k_stride, const void* v, int64_t v_stride, int64_t total_k,
+                              const int32_t* cu_q, const int32_t* cu_k, void* out, int64_t out_stride, float* lse) {
   DeviceScope on_device(ctx);
+  WX_CHECK_ARG(ctx, ctx && sinks >= 0);
   int st = check_dims(ctx, dims, q, q_stride, out, out_stride, cu_q);
   if (st || dims->total_q == 0 || dims->batch == 0) return st;
   const int64_t cols = (int64_t)dims->kv_heads * dims->head_dim;
@@ -828,6 +844,7 @@ int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, in
   WX_CHECK_ARG(ctx, total_k == 0 || (k && v && aligned16(k) && aligned16(v)));
   TextAttnParams p{};
   fill_params(ctx, dims, q, q_stride, cu_q, out, out_stride, lse, p);
+  p.sinks = sinks;
   p.cu_k = cu_k ? cu_k : cu_q;
   p.total_k = total_k;
   // (with no keys at all nothing is read: any valid address serves the tensor maps)
@@ -836,11 +853,19 @@ int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, in
   return dispatch_attn(ctx, dims, p, kv);
 }
 
-int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
-                       const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
-                       const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride,
-                       float* lse) {
+int wx_prompt_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, int64_t total_k, const int32_t* cu_q,
+                        const int32_t* cu_k, void* out, int64_t out_stride, float* lse) {
+  return wx_prompt_attention_sinks(ctx, dims, 0, q, q_stride, k, k_stride, v, v_stride, total_k, cu_q, cu_k, out,
+                                   out_stride, lse);
+}
+
+int wx_paged_attention_sinks(wx_ctx* ctx, const wx_attn_dims* dims, int32_t sinks, const void* q, int64_t q_stride,
+                             const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
+                             const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride,
+                             float* lse) {
   DeviceScope on_device(ctx);
+  WX_CHECK_ARG(ctx, ctx && sinks >= 0);
   int st = check_dims(ctx, dims, q, q_stride, out, out_stride, cu_q);
   if (st) return st;
   if ((st = check_kv_cache(ctx, cache))) return st;
@@ -851,6 +876,7 @@ int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int
   WX_CHECK_ARG(ctx, blocks_per_seq <= INT32_MAX / cache->page_size);
   TextAttnParams p{};
   fill_params(ctx, dims, q, q_stride, cu_q, out, out_stride, lse, p);
+  p.sinks = sinks;
   p.kv_lens = kv_lens;
   p.block_table = block_table;
   p.blocks_per_seq = blocks_per_seq;
@@ -861,6 +887,14 @@ int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int
   const KvSource kv{cache->k, cache->v, (uint64_t)cache->pages * cache->kv_heads * cache->page_size,
                     (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, cache->format};
   return dispatch_attn(ctx, dims, p, kv);
+}
+
+int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
+                       const wx_kv_cache* cache, const int32_t* cu_q, const int32_t* kv_lens,
+                       const int32_t* block_table, int64_t blocks_per_seq, void* out, int64_t out_stride,
+                       float* lse) {
+  return wx_paged_attention_sinks(ctx, dims, 0, q, q_stride, cache, cu_q, kv_lens, block_table, blocks_per_seq, out,
+                                  out_stride, lse);
 }
 
 }  // extern "C"

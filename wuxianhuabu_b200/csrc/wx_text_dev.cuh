@@ -9,6 +9,10 @@
 
 namespace wx {
 
+// Which keys a row sees: those up to its place within the window (kPlainKeys), or these and the
+// sequence's first `sinks` (kSinkKeys). The attention kernels are compiled for each.
+enum : int { kPlainKeys = 0, kSinkKeys = 1 };
+
 struct TextAttnParams {
   const __nv_bfloat16* q;
   int64_t q_stride;
@@ -26,6 +30,7 @@ struct TextAttnParams {
   int batch, hq, hkv, group;
   int64_t total_q, total_k;
   int causal, window;
+  int sinks;  // kSinkKeys: first keys that stay visible beside the window
   float sl2;  // scale * log2(e): scores and maxima are kept in base 2
   float* part;              // split items: [2 * gridDim][16][hd] sums, then [..][16] maxima and denominators
   float* part_ml;
@@ -42,7 +47,7 @@ struct KvSource {
 };
 
 // attention for many query rows (wx_text_flash.cu)
-int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv);
+int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv, int keys = kPlainKeys);
 
 // One sequence as the kernels see it; lengths and offsets from the device are clamped to the
 // buffers, so that wrong ones give wrong rows and an error word but no access outside.
@@ -82,6 +87,25 @@ __device__ __forceinline__ int key_hi(const TextAttnParams& p, const Seq& s, int
 }
 __device__ __forceinline__ int key_lo(const TextAttnParams& p, const Seq& s, int tok) {
   return p.window > 0 ? max(0, max(0, tok - s.lq + s.lk + 1) - p.window) : 0;
+}
+
+// whether a row with bounds [lo, hi) sees key j
+template <int KEYS>
+__device__ __forceinline__ bool key_seen(const TextAttnParams& p, int j, int lo, int hi) {
+  return j < hi && (j >= lo || (KEYS == kSinkKeys && j < p.sinks));
+}
+// Between the first keys and the window lie keys that no row of an item (of a call, in the rows kernel)
+// sees. Kernels walk a sequence's keys without them: of `first` units before the first row's window,
+// those that hold first keys stay, and unit u stands for u + gap from there on.
+struct KeyGap {
+  int first, gap;
+  __device__ __forceinline__ int operator()(int u) const { return u < first ? u : u + gap; }
+};
+template <int KEYS>
+__device__ __forceinline__ KeyGap key_gap(const TextAttnParams& p, int first, int unit) {
+  if constexpr (KEYS != kSinkKeys) return KeyGap{0, 0};
+  const int seen = (int)min64(first, ((int64_t)p.sinks + unit - 1) / unit);
+  return KeyGap{seen, first - seen};
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {

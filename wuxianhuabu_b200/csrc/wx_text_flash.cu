@@ -44,8 +44,8 @@ constexpr int kTfWaves = 3;          // pieces for each SM below which items are
 constexpr int kTfMinTiles = 8;       // tiles of a piece of an item: its start and end cost one or two
 constexpr int64_t kTfL2 = int64_t(48) << 20;
 // V rows with non-finite values remembered per item: every row of its masked tiles (an item's 256 tokens
-// end, and where a window cuts begin, in up to three tiles each)
-constexpr int kTfBadRows = 6 * 128;
+// end, and where a window cuts begin, in up to three tiles each; one more holds the last first key)
+constexpr int kTfBadRows = 7 * 128;
 constexpr int kTfBadWords = 9;       // key, columns with +infinity or NaN, columns with -infinity or NaN
 
 template <int FMT, int HD>
@@ -79,11 +79,21 @@ struct TfItem {
   int free_hi, free_lo;  // tiles inside [free_lo, free_hi) are unmasked for every row
   int bad;               // V rows with non-finite values (8-bit: NaN codes) found in masked tiles
   int piece, pieces;     // this part of the item's key tiles, and how many it was cut into
+  KeyGap at;             // which tile of the sequence a tile of the walk is
   __device__ int lo(int X) const { return X ? b0 : a0; }
   __device__ int hi(int X) const { return X ? b1 : a1; }
   __device__ int first() const { return a1 <= a0 ? b0 : b1 <= b0 ? a0 : min(a0, b0); }
   __device__ int last() const { return max(first(), max(a1 > a0 ? a1 : 0, b1 > b0 ? b1 : 0)); }
-  __device__ bool masked(int t) const { return t * 128 + 128 > free_hi || t * 128 < free_lo; }
+  // key tile t of the walk: its tile of the sequence, and whether some row does not see all of it
+  template <int KEYS>
+  __device__ int tile(int t) const {
+    return KEYS == kSinkKeys ? at(t) : t;
+  }
+  template <int KEYS>
+  __device__ bool masked(const TextAttnParams& p, int t) const {
+    const int j = tile<KEYS>(t) * 128;
+    return j + 128 > free_hi || (j < free_lo && (KEYS != kSinkKeys || j + 128 > p.sinks));
+  }
 };
 
 enum : int {
@@ -249,6 +259,18 @@ __device__ __forceinline__ int2 slot_tiles(const TextAttnParams& p, const Seq& s
   const int hi = key_hi(p, s, k1 - 1), lo = key_lo(p, s, k0);
   return hi > lo ? make_int2(lo >> 7, (hi + 127) >> 7) : make_int2(0, 0);
 }
+// The key tiles of both slots of the item from tok0 on, in its walk. With first keys that stay visible both walk
+// from those through the window of the item's first row.
+template <int KEYS>
+__device__ __forceinline__ KeyGap item_tiles(const TextAttnParams& p, const Seq& s, int tok0, int tt, int2& a, int2& b) {
+  a = slot_tiles(p, s, tok0, tt);
+  b = slot_tiles(p, s, tok0 + tt, tt);
+  if constexpr (KEYS != kSinkKeys) return KeyGap{0, 0};
+  const KeyGap at = key_gap<KEYS>(p, key_lo(p, s, tok0) >> 7, 128);
+  if (a.y > a.x) a = make_int2(0, a.y - at.gap);
+  if (b.y > b.x) b = make_int2(0, b.y - at.gap);
+  return at;
+}
 // The item's tiles [first, last) and the pieces that they are cut into, of at least kTfMinTiles
 __device__ __forceinline__ void cut_item(int2 a, int2 b, int splits, int& first, int& last, int& pieces) {
   first = a.y <= a.x ? b.x : b.y <= b.x ? a.x : min(a.x, b.x);
@@ -256,7 +278,7 @@ __device__ __forceinline__ void cut_item(int2 a, int2 b, int splits, int& first,
   pieces = min(splits, max(1, (last - first) / kTfMinTiles));
 }
 
-template <int FMT, int HD>
+template <int FMT, int HD, int KEYS>
 __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     text_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, TfParams tp) {
@@ -352,7 +374,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       };
       // 8-bit: a tile in two halves of 64 raw rows, its scales with the keys; rows past the
       // sequence's last key are not loaded (any byte expands to a finite value or, in K, NaN: masked)
-      auto load_raw = [&](bool is_k, int t) -> bool {
+      auto load_raw = [&](bool is_k, int walked) -> bool {
+        const int t = it.tile<KEYS>(walked);
         const int per_half = 64 / tp.box;
         const int page = page_of(t * boxes, lane % boxes);
         const int nb = min(boxes, (it.lk - t * 128 + tp.box - 1) / tp.box);
@@ -383,13 +406,14 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         }
         return true;
       };
-      auto load = [&](bool is_k, int t) -> bool {
-        if constexpr (kW) return load_raw(is_k, t);
+      auto load = [&](bool is_k, int walked) -> bool {
+        if constexpr (kW) return load_raw(is_k, walked);
+        const int t = it.tile<KEYS>(walked);
         const uint32_t cnt = is_k ? nk : nv;
         const int ns = is_k ? kKStages : kTfVStages;
         const uint32_t s = cnt % ns, par = ((cnt / ns) & 1) ^ 1u;
         if (!mbar_wait(bar((is_k ? kBTfKEmpty : kBTfVEmpty) + s), par, p.err, kDevTimeoutEmpty, abort_flag)) return false;
-        const bool mend = !is_k && it.masked(t);
+        const bool mend = !is_k && it.masked<KEYS>(p, walked);
         const uint32_t full = bar((is_k ? kBTfKFull : mend ? kBTfVRaw : kBTfVFull) + s);
         const uint32_t dst = is_k ? sK(s) : sV(s);
         const CUtensorMap* tm = is_k ? &tmK : &tmV;
@@ -573,7 +597,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
             dst->lk = s.lk;
             dst->q0 = (int)s.q0;
             dst->k0 = (int)s.k0;
-            int2 a = slot_tiles(p, s, tok0, tp.tt), b = slot_tiles(p, s, tok0 + tp.tt, tp.tt);
+            int2 a, b;
+            dst->at = item_tiles<KEYS>(p, s, tok0, tp.tt, a, b);
             int first, last, pieces;
             cut_item(a, b, tp.splits, first, last, pieces);
             const int piece = (int)(of_b - in_b * (unsigned)tp.splits), per = (last - first + pieces - 1) / pieces;
@@ -637,7 +662,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       const int t0 = cur.first(), t1 = cur.last();
       int bad = 0;
       for (int t = t0; t < t1 && ok; ++t) {
-        if (kW || !cur.masked(t)) continue;
+        if (kW || !cur.masked<KEYS>(p, t)) continue;
+        const int key0 = cur.tile<KEYS>(t) * 128;
         const uint32_t s = (nv + (uint32_t)(t - t0)) % kTfVStages;
         uint32_t& done = s == 0 ? raw[0] : raw[1];
         if (!mbar_wait(bar(kBTfVRaw + s), done & 1, p.err, kDevTimeoutFull, abort_flag)) {
@@ -650,7 +676,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 #pragma unroll 1
         for (int r = lane; r < 128; r += 32) {
           const uint32_t row = sV(s) + (uint32_t)r * 128;
-          const bool past = t * 128 + r >= cur.lk;
+          const bool past = key0 + r >= cur.lk;
           __nv_bfloat162 probe = __floats2bfloat162_rn(0.f, 0.f);
           const __nv_bfloat162 zero = probe;
 #pragma unroll 4
@@ -668,7 +694,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           const uint32_t who = __ballot_sync(0xffffffffu, odd);
           if (odd) {
             const int slot = bad + __popc(who & ((1u << lane) - 1u));
-            remember_row<HD>(row, r, t * 128 + r, slot < kTfBadRows ? list + slot * kTfBadWords : nullptr);
+            remember_row<HD>(row, r, key0 + r, slot < kTfBadRows ? list + slot * kTfBadWords : nullptr);
           }
           bad += __popc(who);
           __syncwarp();
@@ -712,7 +738,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         }
         const uint32_t dst = is_k ? sK(s) : sV(s);
         const int t = t0 + (int)(cnt - at_first);
-        const bool masked = at->masked(t);
+        const bool masked = at->masked<KEYS>(p, t);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half, ++nr) {
           const uint32_t rs = nr % kTfRaw;
@@ -721,7 +747,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           const uint32_t raw = sbase + G::kRawOff + rs * G::kRawBytes;
           // (NaN codes do what they should in a key and in a value that every row sees)
           if (FMT == kKvE4m3 && !is_k && masked)
-            remember_codes<HD>(raw, tid, t * 128 + half * 64, at->lk, items[n % kTfItems].bad, list);
+            remember_codes<HD>(raw, tid, at->tile<KEYS>(t) * 128 + half * 64, at->lk, items[n % kTfItems].bad, list);
 #pragma unroll
           for (int j = 0; j < 64 * HD / 16 / 128; ++j) {
             const int u = j * 128 + tid, row = half * 64 + u / (HD / 16), c = u % (HD / 16);
@@ -790,7 +816,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     // beside the conversion's. 1324 tokens over 26,383 cached e4m3 keys, 32 / 8 heads: 942 us with a
     // row per thread, 856 in fragments unrolled, 664 like this (bf16, a row per thread and unrolled:
     // 420, and rolled it loses a tenth).
-    auto frag_tile = [&](uint32_t g, int t, int a0, bool masked, int hi, int lo, float (&m)[4], float (&l)[4]) -> bool {
+    auto frag_tile = [&](uint32_t g, int t, bool starts, bool masked, int hi, int lo, float (&m)[4],
+                         float (&l)[4]) -> bool {
       const int tq = lane & 3;
       const uint32_t scales = sbase + G::kScaleOff + (g % kTfScales) * 1024 + tq * 8;
       if (!mbar_wait(bar(kBTfScale + g % kTfScales), (g / kTfScales) & 1, p.err, kDevTimeoutFull, abort_flag)) return false;
@@ -806,7 +833,9 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int from = (lane >> 2) + 8 * j;
-          keep[j] = below(__shfl_sync(0xffffffffu, hi, from)) & ~below(__shfl_sync(0xffffffffu, lo, from));
+          uint32_t hidden = below(__shfl_sync(0xffffffffu, lo, from));
+          if constexpr (KEYS == kSinkKeys) hidden &= ~below(p.sinks);
+          keep[j] = below(__shfl_sync(0xffffffffu, hi, from)) & ~hidden;
         }
       }
       // the row maxima, in base 2 and scaled
@@ -837,7 +866,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       };
       if (masked) maxima(std::true_type{});
       else maxima(std::false_type{});
-      bool grown = t == a0;
+      bool grown = starts;
 #pragma unroll
       for (int j = 0; j < 4; ++j) grown |= mx[j] - m[j] > 8.0f;
       // as for rows below; without growth by 2^8 the maxima need not even be gathered
@@ -849,7 +878,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 1));
           mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 2));
           alpha[j] = 1.f;
-          if (t == a0) {
+          if (starts) {
             m[j] = mx[j];
           } else if (mx[j] - m[j] > 8.0f) {
             alpha[j] = exp2_approx(m[j] - mx[j]);
@@ -974,20 +1003,26 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           if (c.valid) load_q(c);
           q_sent = true;
         }
-        const bool masked = it.masked(t);
+        const bool masked = it.masked<KEYS>(p, t);
+        const int key0 = it.tile<KEYS>(t) * 128;
         if constexpr (kW) {
           const uint32_t g = both + (uint32_t)(t - t0);
-          if (!frag_tile(g, t, a0, masked, hi, lo, m4, l4)) {
+          if (!frag_tile(g, key0 >> 7, t == a0, masked, hi, lo, m4, l4)) {
             ok = false;
             break;
           }
           continue;
         }
-        const int lim = hi - t * 128, from = lo - t * 128;
+        const int lim = hi - key0, from = lo - key0;
         // bits of the keys 32 c .. 32 c + 31 that this row sees
         auto keep_bits = [&](int c) -> uint32_t {
           const int a = min(32, max(0, lim - c * 32)), b = min(32, max(0, from - c * 32));
-          return (a == 32 ? ~0u : (1u << a) - 1u) & ~(b == 32 ? ~0u : (1u << b) - 1u);
+          uint32_t hidden = b == 32 ? ~0u : (1u << b) - 1u;
+          if constexpr (KEYS == kSinkKeys) {
+            const int n = min(32, max(0, p.sinks - key0 - c * 32));
+            hidden &= ~(n == 32 ? ~0u : (1u << n) - 1u);
+          }
+          return (a == 32 ? ~0u : (1u << a) - 1u) & ~hidden;
         };
         if (masked) {
           // a short loop over S in TMEM: few tiles are masked, and unrolled over 128 registers this
@@ -1125,7 +1160,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           for (int e = 0; e < min(bad, kTfBadRows); ++e) {
             const uint32_t* entry = list + e * kTfBadWords;
             const int key = (int)__ldcg(entry);
-            if (key >= lo && key < hi) {
+            if (key_seen<KEYS>(p, key, lo, hi)) {
               plus |= __ldcg(entry + 1 + (col >> 5)) >> (col & 31);
               minus |= __ldcg(entry + 5 + (col >> 5)) >> (col & 31);
             }
@@ -1182,7 +1217,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 }
 
 // Rows of items that were cut up: sums of the pieces, in order, brought to one maximum. A warp a row.
-template <int HD>
+template <int HD, int KEYS>
 __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   const TextAttnParams& p = tp.a;
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = p.total_q * p.hq;
@@ -1199,8 +1234,10 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   const int64_t tok = token - s.q0;
   if (tok < 0 || tok >= s.lq) return;
   const int tok0 = (int)tok / (2 * tp.tt) * (2 * tp.tt);
+  int2 a, e;
+  item_tiles<KEYS>(p, s, tok0, tp.tt, a, e);
   int first, last, pieces;
-  cut_item(slot_tiles(p, s, tok0, tp.tt), slot_tiles(p, s, tok0 + tp.tt, tp.tt), tp.splits, first, last, pieces);
+  cut_item(a, e, tp.splits, first, last, pieces);
   if (pieces < 2) return;
   constexpr int kPer = HD / 32;
   float o[kPer] = {};
@@ -1256,16 +1293,16 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
-template <int FMT, int HD>
+template <int FMT, int HD, int KEYS>
 static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, TfParams& tp) {
   using G = TfGeom<FMT, HD>;
-  auto fn = text_flash_kernel<FMT, HD>;
+  auto fn = text_flash_kernel<FMT, HD, KEYS>;
   int st = ensure_smem_attr(ctx, (const void*)fn, G::kSmem, "text_flash");
   if (st) return st;
   // setmaxnreg moves registers within what the launch reserved
   static const bool regs_ok = [] {
     cudaFuncAttributes fa{};
-    return cudaFuncGetAttributes(&fa, (const void*)text_flash_kernel<FMT, HD>) == cudaSuccess &&
+    return cudaFuncGetAttributes(&fa, (const void*)text_flash_kernel<FMT, HD, KEYS>) == cudaSuccess &&
            fa.numRegs * G::kThreads >= G::kRegsUsed;
   }();
   if (!regs_ok) return set_error(ctx, WX_ERR_CUDA, "text_flash: register split does not fit");
@@ -1274,7 +1311,7 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   // Too few items to level the SMs out are cut into pieces of their keys, as many as give kTfWaves
   // to an SM and as the longest range that a row can see allows.
   int64_t keys = p.block_table ? p.blocks_per_seq << p.page_shift : p.total_k;
-  if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 2 * tp.tt);
+  if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 2 * tp.tt + (KEYS == kSinkKeys ? p.sinks : 0));
   tp.splits = (int)std::max<int64_t>(1, std::min((kTfWaves * ctx->num_sms + items - 1) / items, keys / (128 * kTfMinTiles)));
   const int grid = (int)std::min<int64_t>(ctx->num_sms, items * tp.splits);
   const int64_t rows = tp.splits > 1 ? p.total_q * p.hq * tp.splits : 0;
@@ -1290,11 +1327,22 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   ProfScope prof(ctx, kProfAttn);
   fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(tq, tk, tv, tp);
   if (tp.splits == 1) return launch_status(ctx, "text_flash");
-  text_flash_join_kernel<HD><<<(unsigned)((p.total_q * p.hq + 7) / 8), 256, 0, ctx->stream>>>(tp);
+  text_flash_join_kernel<HD, KEYS><<<(unsigned)((p.total_q * p.hq + 7) / 8), 256, 0, ctx->stream>>>(tp);
   return launch_status(ctx, "text_flash", 2);
 }
 
-int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv) {
+template <int KEYS>
+static int launch_flash(wx_ctx* ctx, int format, int head_dim, const CUtensorMap& tq, const CUtensorMap& tk,
+                        const CUtensorMap& tv, TfParams& tp) {
+  const bool big = head_dim == 128;
+  if (format == kKvInt8)
+    return big ? launch_flash<kKvInt8, 128, KEYS>(ctx, tq, tk, tv, tp) : launch_flash<kKvInt8, 64, KEYS>(ctx, tq, tk, tv, tp);
+  if (format == kKvE4m3)
+    return big ? launch_flash<kKvE4m3, 128, KEYS>(ctx, tq, tk, tv, tp) : launch_flash<kKvE4m3, 64, KEYS>(ctx, tq, tk, tv, tp);
+  return big ? launch_flash<kKvBf16, 128, KEYS>(ctx, tq, tk, tv, tp) : launch_flash<kKvBf16, 64, KEYS>(ctx, tq, tk, tv, tp);
+}
+
+int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv, int keys) {
   TfParams tp{};
   tp.a = p;
   tp.box = p.block_table ? std::min(128, 1 << p.page_shift) : 128;
@@ -1305,18 +1353,17 @@ int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSourc
   const uint64_t ld[2] = {(uint64_t)head_dim, (uint64_t)p.q_stride};
   const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tp.tt};
   if ((st = make_tmap_bf16_3d(ctx, &tq, p.q, dims, ld, box))) return st;
-  const bool big = head_dim == 128;
   if (kv.format != kKvBf16) {  // raw rows by untiled copies: the maps of K and V are not used
     tp.box = std::min(64, 1 << p.page_shift);
     tp.k8 = static_cast<const uint8_t*>(kv.k);
     tp.v8 = static_cast<const uint8_t*>(kv.v);
-    if (kv.format == kKvInt8)
-      return big ? launch_flash<kKvInt8, 128>(ctx, tq, tq, tq, tp) : launch_flash<kKvInt8, 64>(ctx, tq, tq, tq, tp);
-    return big ? launch_flash<kKvE4m3, 128>(ctx, tq, tq, tq, tp) : launch_flash<kKvE4m3, 64>(ctx, tq, tq, tq, tp);
+    tk = tv = tq;
+  } else {
+    if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, tp.box))) return st;
+    if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, tp.box))) return st;
   }
-  if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, tp.box))) return st;
-  if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, tp.box))) return st;
-  return big ? launch_flash<kKvBf16, 128>(ctx, tq, tk, tv, tp) : launch_flash<kKvBf16, 64>(ctx, tq, tk, tv, tp);
+  return keys == kSinkKeys ? launch_flash<kSinkKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp)
+                           : launch_flash<kPlainKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp);
 }
 
 }  // namespace wx

@@ -440,15 +440,22 @@ def _dims(n: int, batch: int, max_len: int, h: int, hk: int, d: int, causal: boo
     return C.byref(AttnDims(n, batch, max_len, h, hk, d, causal, window, d ** -0.5 if scale is None else scale))
 
 
+def _first_keys(sinks: int) -> int:
+    if sinks < 0:
+        raise _invalid("sinks must not be negative")
+    return min(sinks, _INT32 - 1)  # (more than any sequence has)
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor, max_len: int,
                      scale: Optional[float] = None, causal: bool = True, window: int = 0,
                      cu_seqlens_k: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                     return_lse: bool = False):
+                     return_lse: bool = False, sinks: int = 0):
     """Packed prompts: sequence b is rows cu_seqlens[b]..cu_seqlens[b + 1] (int32, on the device)
     of q [total, q_heads, head_dim] and k, v [total, kv_heads, head_dim] (of cu_seqlens_k for k
     and v where they differ, the last query row standing at the last key). ``max_len``: the
-    longest query length. Returns out [total, q_heads, head_dim], with ``return_lse`` also the
-    log-sum-exp [total, q_heads] fp32."""
+    longest query length. A ``window`` leaves a row the last ``window`` keys up to its own, and with
+    ``sinks`` the sequence's first ``sinks`` keys too. Returns out [total, q_heads, head_dim], with
+    ``return_lse`` also the log-sum-exp [total, q_heads] fp32."""
     n, h, d, qs, o, os_, lse = _attn_out(q, out, return_lse)
     nk, hk, dk, ks = _rows(k, "k")
     nv, hv, dv, vs = _rows(v, "v")
@@ -458,17 +465,22 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     cu = _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
     cu_k = None if cu_seqlens_k is None else _need_ints(torch.int32, batch + 1, "cu_seqlens_k", cu_seqlens_k)
     dev = _same_device(q, k, v, cu_seqlens, o, cu_seqlens if cu_k is None else cu_seqlens_k)
-    context(dev).call("wx_prompt_attention", _dims(n, batch, max_len, h, hk, d, causal, window, scale), q.data_ptr(), qs,
-                      k.data_ptr(), ks, v.data_ptr(), vs, nk, cu, cu_k, o.data_ptr(), os_, _p(lse))
+    dims = _dims(n, batch, max_len, h, hk, d, causal, window, scale)
+    args = q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, nk, cu, cu_k, o.data_ptr(), os_, _p(lse)
+    if sinks:
+        context(dev).call("wx_prompt_attention_sinks", dims, _first_keys(sinks), *args)
+    else:
+        context(dev).call("wx_prompt_attention", dims, *args)
     return (o, lse) if return_lse else o
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tensor, kv_lens: torch.Tensor,
                     block_table: torch.Tensor, max_len: int, scale: Optional[float] = None, causal: bool = True,
-                    window: int = 0, out: Optional[torch.Tensor] = None, return_lse: bool = False):
+                    window: int = 0, out: Optional[torch.Tensor] = None, return_lse: bool = False, sinks: int = 0):
     """New tokens over the cache that already holds them: query rows cu_seqlens[b]..[b + 1] of q
     are the last of the kv_lens[b] tokens cached in pages block_table[b] (int32, [batch, blocks];
-    entries beyond the length are not read). ``max_len``: the longest query length."""
+    entries beyond the length are not read). ``max_len``: the longest query length; ``window`` and
+    ``sinks`` as in ``prompt_attention``."""
     n, h, d, qs, o, os_, lse = _attn_out(q, out, return_lse)
     batch = _batch_of(cu_seqlens)
     cu = _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
@@ -479,6 +491,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
     if d != cache.head_dim:
         raise _invalid("q must have the cache's head_dim")
     dev = _same_device(q, cache.k, cu_seqlens, kv_lens, block_table, o)
-    context(dev).call("wx_paged_attention", _dims(n, batch, max_len, h, cache.kv_heads, d, causal, window, scale),
-                      q.data_ptr(), qs, cache._desc, cu, lens, table, block_table.shape[1], o.data_ptr(), os_, _p(lse))
+    dims = _dims(n, batch, max_len, h, cache.kv_heads, d, causal, window, scale)
+    args = q.data_ptr(), qs, cache._desc, cu, lens, table, block_table.shape[1], o.data_ptr(), os_, _p(lse)
+    if sinks:
+        context(dev).call("wx_paged_attention_sinks", dims, _first_keys(sinks), *args)
+    else:
+        context(dev).call("wx_paged_attention", dims, *args)
     return (o, lse) if return_lse else o
