@@ -17,6 +17,8 @@ def test_calls_without_a_context_are_refused():
         == _lib.WX_ERR_INVALID
     assert lib.wx_paged_attention_sinks(None, None, 0, None, 0, None, None, None, None, 0, None, 0, None) \
         == _lib.WX_ERR_INVALID
+    assert lib.wx_prefix_attention(None, None, None, 0, None, None, 0, None, None, None, 0, 0, None, 0, None) \
+        == _lib.WX_ERR_INVALID
     assert lib.wx_page_plan(None, None, None, None, 0, 0, None, None, None, None, None) == _lib.WX_ERR_INVALID
 
 

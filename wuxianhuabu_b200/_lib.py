@@ -264,6 +264,8 @@ _SIGS = {
                                          _vp, _i64, _vp]),
     "wx_paged_attention_sinks": (_i32, [_vp, C.POINTER(AttnDims), _i32, _vp, _i64, C.POINTER(KvCache), _vp, _vp, _vp,
                                         _i64, _vp, _i64, _vp]),
+    "wx_prefix_attention": (_i32, [_vp, C.POINTER(AttnDims), _vp, _i64, C.POINTER(KvCache), _vp, _i64, _vp, _vp, _vp,
+                                   _i64, _i64, _vp, _i64, _vp]),
 }
 
 _lib = None

@@ -111,6 +111,20 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   const int g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)(warp * kD * G::kStep);
 
+  // kPrefixKeys: with a shared prefix, the rows of all sequences over its keys come first
+  const int front = KEYS == kPrefixKeys && p.shared ? 1 : 0;
+  auto seq_of = [&](int b) -> Seq {
+    if (KEYS == kPrefixKeys && b < front) return Seq{0, 0, (int)p.total_q, p.prefix};
+    return load_seq(p, KEYS == kPrefixKeys ? b - front : b);
+  };
+  auto hi_of = [&](int b, const Seq& s, int tok) -> int {
+    return KEYS == kPrefixKeys && b < front ? s.lk : key_hi(p, s, tok);
+  };
+  auto blocks_of = [&](int b) -> const int32_t* {
+    if constexpr (KEYS == kPrefixKeys) return b < front ? p.prefix_blocks : p.block_table + (b - front) * p.table_stride;
+    return p.block_table + b * p.blocks_per_seq;
+  };
+
   // ---- the line of units, walked 32 sequences at a time by each warp for itself (32-bit
   // arithmetic: 64-bit divisions were most of a short call's start)
   // (k16: first key; with first keys that stay visible, the 16-key steps before the window)
@@ -118,7 +132,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     items = nu = 0;
     k16 = 0;
     if (b >= p.batch) return;
-    const Seq s = load_seq(p, b);
+    const Seq s = seq_of(b);
     k16 = key_lo(p, s, 0) & ~15;
     items = ((unsigned)(s.lq * p.group) + kRows - 1) / kRows * (unsigned)p.hkv;
     const int skip = KEYS == kSinkKeys ? key_gap<KEYS>(p, k16 >> 4, 16).gap << 4 : k16;
@@ -181,7 +195,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
         b_u0 = wu + __shfl_sync(0xffffffffu, nc - n, src);
         b_end = wu + __shfl_sync(0xffffffffu, nc, src);
         b_i0 = wi + __shfl_sync(0xffffffffu, ic - my_items, src);
-        c.s = load_seq(p, c.b);
+        c.s = seq_of(c.b);
         rts = __shfl_sync(0xffffffffu, my_items, src) / (unsigned)p.hkv;
         c.nu = __shfl_sync(0xffffffffu, my_nu, src);
         k16 = __shfl_sync(0xffffffffu, my_k16, src);
@@ -223,7 +237,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
       const int jl = first_key(c, i + lane);
       page_of = 0;
       if (step_key(c, i + lane) < c.k_hi) {
-        page_of = p.block_table[c.b * p.blocks_per_seq + (jl >> p.page_shift)];
+        page_of = blocks_of(c.b)[jl >> p.page_shift];
         if (page_of < 0 || page_of >= p.pages) {
           set_dev_error(p.err, kDevBadArgs);
           page_of = 0;
@@ -323,13 +337,13 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
         const int rr = row0 + 8 * n + 2 * t + e;
         const bool here = rr < n_rows;
         const int tk = here ? (int)((unsigned)rr / (unsigned)p.group) : 0;
-        lim_hi[n][e] = here ? key_hi(p, cur.s, tk) : 0;
+        lim_hi[n][e] = here ? hi_of(cur.b, cur.s, tk) : 0;
         lim_lo[n][e] = here ? key_lo(p, cur.s, tk) : 0;
       }
     }
     // a step between these sees no mask in any row of the tile
     const int last_tok = (int)((unsigned)(min(n_rows, row0 + kRows) - 1) / (unsigned)p.group);
-    const int free_hi = key_hi(p, cur.s, (int)((unsigned)row0 / (unsigned)p.group));
+    const int free_hi = hi_of(cur.b, cur.s, (int)((unsigned)row0 / (unsigned)p.group));
     const int free_lo = key_lo(p, cur.s, last_tok);
 
     float acc[NT][kMT][4];
@@ -612,6 +626,15 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
       const int64_t tok = done.s.q0 + tk;
       const int head = done.h * p.group + r - tk * p.group;
       if (!WX_IN_BOUNDS(p.err, tok >= 0 && tok < p.total_q && head >= 0 && head < p.hq)) return;
+      if constexpr (KEYS == kPrefixKeys) {
+        const int64_t at = (done.b < front ? 0 : p.own_layer) * (p.total_q * p.hq) + tok * p.hq + head;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4)
+          *reinterpret_cast<float4*>(p.layer_o + at * HD + jc + i) =
+              make_float4(o[i] * kByteUnit<FMT>, o[i + 1] * kByteUnit<FMT>, o[i + 2] * kByteUnit<FMT>, o[i + 3] * kByteUnit<FMT>);
+        if ((threadIdx.x & 15) == 0) p.layer_ml[at] = make_float2(M, L);
+        return;
+      }
       const float inv = L == 0.f ? 0.f : kByteUnit<FMT> / L;
       uint32_t w[kPer / 2];
 #pragma unroll
@@ -763,13 +786,15 @@ template <int FMT, int HD, int NT, int KEYS>
 static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   using G = RowsGeom<FMT, HD, NT>;
   const int grid = std::min(ctx->num_sms, G::kWarps * (G::kPitch + 2) / 2);  // (an item's pieces: the join buffer)
-  const int64_t items = (int64_t)p.hkv * (p.total_q * p.group / G::kRows + p.batch);
+  const int64_t walks = KEYS == kPrefixKeys && p.shared ? 2 : 1;  // of each row
+  const int64_t items = (int64_t)p.hkv * (walks * (p.total_q * p.group / G::kRows) + p.batch);
   // the line of units is counted in 32 bits (only block tables that repeat pages get near)
-  if (p.block_table && items > UINT32_MAX / ((p.blocks_per_seq << p.page_shift) / kUnit + 1))
+  const int64_t most_keys = std::max<int64_t>(p.blocks_per_seq << p.page_shift, KEYS == kPrefixKeys ? p.prefix : 0);
+  if (p.block_table && items > UINT32_MAX / (most_keys / kUnit + 1))
     return set_error(ctx, WX_ERR_UNSUPPORTED, "batch * kv_heads * blocks_per_seq too large (2^32 units of 128 keys)");
   const size_t rows = (size_t)grid * 2 * G::kRows;
   int st;
-  Carve c;
+  Carve c{p.ws_reserved};
   const size_t o_part = c.take(rows * HD * 4), o_ml = c.take(rows * 8);
   uint8_t* ws = static_cast<uint8_t*>(workspace(ctx, c.off, &st));
   if (!ws) return st;
@@ -825,6 +850,135 @@ static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParam
                            : launch_rows_attn<kPlainKeys>(ctx, d->head_dim, rows, p, kv);
 }
 
+// ------------------------------------------------------------------ a prefix that all sequences share
+// softmax over the prefix P and the row's own keys S: with o = sum 2^(s - m) v, m and l of each part,
+//   M = max(m_P, m_S), out = (2^(m_P - M) o_P + 2^(m_S - M) o_S) / (2^(m_P - M) l_P + 2^(m_S - M) l_S).
+// The rows of all sequences walk the prefix together, so that its bytes are read once for up to 256 rows and
+// not once for each sequence; their own keys are walked as in any paged call. The parts' sums stay
+// in fp32 and are joined here, in the order of the keys. A warp a row.
+template <int HD>
+__global__ void __launch_bounds__(256) prefix_join_kernel(TextAttnParams p, int layers) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = p.total_q * p.hq;
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  const int64_t token = row / p.hq;
+  int b = 0;  // last sequence that begins at or before the token
+  for (int n = p.batch; n > 1;) {
+    const int half = n / 2;
+    if (p.cu_q[b + half] <= token) b += half;
+    n -= half;
+  }
+  if (token < p.cu_q[b] || token >= p.cu_q[b + 1]) return;
+  constexpr int kPer = HD / 32;
+  float o[kPer] = {};
+  float M = -INFINITY, L = 0.f;
+  for (int c = 0; c < layers; c += 32) {
+    const float2 ml = c + lane < layers ? p.layer_ml[(c + lane) * rows + row] : make_float2(-INFINITY, 0.f);
+    float m = ml.y != 0.f ? ml.x : -INFINITY;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    M = fmaxf(M, m);
+  }
+  for (int c = 0; c < layers; c += 4) {  // four layers' rows in flight
+    float x[4][kPer];
+    float2 ml[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t at = min(c + q, layers - 1) * rows + row;
+      ml[q] = p.layer_ml[at];
+      const float* src = p.layer_o + at * HD + lane * kPer;
+      if constexpr (kPer == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(src);
+        x[q][0] = y.x, x[q][1] = y.y, x[q][2] = y.z, x[q][3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(src);
+        x[q][0] = y.x, x[q][1] = y.y;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (c + q >= layers || ml[q].y == 0.f) continue;  // (nothing seen: its sums may be anything)
+      const float f = exp2_approx(ml[q].x - M);
+      L += ml[q].y * f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] += x[q][e] * f;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : __fdividef(1.0f, L);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + token * p.out_stride + (row - token * p.hq) * HD + lane * kPer);
+#pragma unroll
+  for (int e = 0; e < kPer; e += 2) dst[e / 2] = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
+}
+
+// Few rows a sequence: the prefix is walked for all rows together, by the kernel for few rows where they are few
+// in all, else by the tcgen05 kernel. Many rows a sequence (new prompts) fill an item by themselves: each walks
+// the prefix and its own keys in one go, and nothing is joined.
+static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p, const KvSource& kv) {
+  const int64_t few = kv.format == kKvBf16 ? 16 : kv.format == kKvE4m3 ? 32 : 48;
+  const int64_t own = (int64_t)d->max_q * p.group, all = p.total_q * p.group;
+  if (own > few) return text_flash(ctx, p, d->head_dim, kv, kPrefixKeys);
+  const bool flash = p.prefix && all > few;
+  const int layers = (flash ? text_flash_layers(ctx, p) : p.prefix ? 1 : 0) + 1;
+  const int64_t rows = p.total_q * p.hq;
+  Carve c;
+  const size_t o_o = c.take((size_t)(layers * rows) * d->head_dim * 4), o_ml = c.take((size_t)(layers * rows) * 8);
+  p.ws_reserved = c.off;
+  // what the kernels take for themselves is asked for now: a workspace that grew between them would lose the layers
+  const size_t rows_ws = (size_t)ctx->num_sms * 2 * 16 * (d->head_dim * 4 + 8) + 512;
+  int st;
+  uint8_t* ws = static_cast<uint8_t*>(workspace(ctx, c.off + std::max(rows_ws, text_flash_ws(ctx)), &st));
+  if (!ws) return st;
+  p.layer_o = reinterpret_cast<float*>(ws + o_o);
+  p.layer_ml = reinterpret_cast<float2*>(ws + o_ml);
+  p.own_layer = layers - 1;
+  if (flash) {
+    TextAttnParams f = p;
+    f.shared = 1;
+    f.batch = 1;
+    if ((st = text_flash(ctx, f, d->head_dim, kv, kPrefixKeys))) return st;
+  }
+  TextAttnParams r = p;
+  if (!flash && p.prefix) {
+    r.shared = 1;
+    ++r.batch;
+  }
+  if ((st = launch_rows_attn<kPrefixKeys>(ctx, d->head_dim, flash || !p.prefix ? own : all, r, kv))) return st;
+  ProfScope prof(ctx, kProfAttn);
+  const unsigned grid = (unsigned)((rows + 7) / 8);
+  if (d->head_dim == 128) prefix_join_kernel<128><<<grid, 256, 0, ctx->stream>>>(p, layers);
+  else prefix_join_kernel<64><<<grid, 256, 0, ctx->stream>>>(p, layers);
+  return launch_status(ctx, "prefix_join");
+}
+
+// checks of a call over the paged cache, and its parameters
+static int paged_params(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride, const wx_kv_cache* cache,
+                        const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
+                        int64_t blocks_per_seq, void* out, int64_t out_stride, float* lse, TextAttnParams& p,
+                        KvSource& kv, bool& empty) {
+  empty = true;
+  int st = check_dims(ctx, dims, q, q_stride, out, out_stride, cu_q);
+  if (st) return st;
+  if ((st = check_kv_cache(ctx, cache))) return st;
+  WX_CHECK_ARG(ctx, cache->kv_heads == dims->kv_heads && cache->head_dim == dims->head_dim);
+  WX_CHECK_ARG(ctx, cache->format != WX_KV_INT8 || dims->scale < 0x1p100f);  // (int8 scores are formed in units of 2^13)
+  if (dims->total_q == 0 || dims->batch == 0) return WX_OK;
+  WX_CHECK_ARG(ctx, kv_lens && block_table && blocks_per_seq > 0);
+  WX_CHECK_ARG(ctx, blocks_per_seq <= INT32_MAX / cache->page_size);
+  fill_params(ctx, dims, q, q_stride, cu_q, out, out_stride, lse, p);
+  p.kv_lens = kv_lens;
+  p.block_table = block_table;
+  p.blocks_per_seq = blocks_per_seq;
+  p.ks = cache->k_scale;
+  p.vs = cache->v_scale;
+  p.pages = cache->pages;
+  p.page_shift = __builtin_ctz((unsigned)cache->page_size);
+  kv = KvSource{cache->k, cache->v, (uint64_t)cache->pages * cache->kv_heads * cache->page_size,
+                (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, cache->format};
+  empty = false;
+  return WX_OK;
+}
+
 }  // namespace wx
 
 using namespace wx;
@@ -866,27 +1020,35 @@ int wx_paged_attention_sinks(wx_ctx* ctx, const wx_attn_dims* dims, int32_t sink
                              float* lse) {
   DeviceScope on_device(ctx);
   WX_CHECK_ARG(ctx, ctx && sinks >= 0);
-  int st = check_dims(ctx, dims, q, q_stride, out, out_stride, cu_q);
-  if (st) return st;
-  if ((st = check_kv_cache(ctx, cache))) return st;
-  WX_CHECK_ARG(ctx, cache->kv_heads == dims->kv_heads && cache->head_dim == dims->head_dim);
-  WX_CHECK_ARG(ctx, cache->format != WX_KV_INT8 || dims->scale < 0x1p100f);  // (int8 scores are formed in units of 2^13)
-  if (dims->total_q == 0 || dims->batch == 0) return WX_OK;
-  WX_CHECK_ARG(ctx, kv_lens && block_table && blocks_per_seq > 0);
-  WX_CHECK_ARG(ctx, blocks_per_seq <= INT32_MAX / cache->page_size);
   TextAttnParams p{};
-  fill_params(ctx, dims, q, q_stride, cu_q, out, out_stride, lse, p);
+  KvSource kv;
+  bool empty;
+  const int st = paged_params(ctx, dims, q, q_stride, cache, cu_q, kv_lens, block_table, blocks_per_seq, out, out_stride,
+                              lse, p, kv, empty);
+  if (st || empty) return st;
   p.sinks = sinks;
-  p.kv_lens = kv_lens;
-  p.block_table = block_table;
-  p.blocks_per_seq = blocks_per_seq;
-  p.ks = cache->k_scale;
-  p.vs = cache->v_scale;
-  p.pages = cache->pages;
-  p.page_shift = __builtin_ctz((unsigned)cache->page_size);
-  const KvSource kv{cache->k, cache->v, (uint64_t)cache->pages * cache->kv_heads * cache->page_size,
-                    (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, (uint64_t)cache->head_dim, cache->format};
   return dispatch_attn(ctx, dims, p, kv);
+}
+
+int wx_prefix_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
+                        const wx_kv_cache* cache, const int32_t* prefix_blocks, int64_t prefix_len,
+                        const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,
+                        int64_t blocks_per_seq, int64_t table_stride, void* out, int64_t out_stride, float* lse) {
+  DeviceScope on_device(ctx);
+  TextAttnParams p{};
+  KvSource kv;
+  bool empty;
+  WX_CHECK_ARG(ctx, ctx && dims && dims->window == 0);
+  const int st = paged_params(ctx, dims, q, q_stride, cache, cu_q, kv_lens, block_table, blocks_per_seq, out, out_stride,
+                              lse, p, kv, empty);
+  if (st || empty) return st;
+  WX_CHECK_ARG(ctx, prefix_len >= 0 && prefix_len <= INT32_MAX - 256 && (prefix_len == 0 || prefix_blocks));
+  WX_CHECK_ARG(ctx, table_stride >= blocks_per_seq);
+  p.prefix = (int)prefix_len;
+  p.front = (int)((prefix_len + 127) / 128);
+  p.prefix_blocks = prefix_blocks;
+  p.table_stride = table_stride;
+  return dispatch_prefix(ctx, dims, p, kv);
 }
 
 int wx_paged_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,

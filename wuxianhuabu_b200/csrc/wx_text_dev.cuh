@@ -9,9 +9,10 @@
 
 namespace wx {
 
-// Which keys a row sees: those up to its place within the window (kPlainKeys), or these and the
-// sequence's first `sinks` (kSinkKeys). The attention kernels are compiled for each.
-enum : int { kPlainKeys = 0, kSinkKeys = 1 };
+// Which keys a row sees: those up to its place within the window (kPlainKeys), these and the
+// sequence's first `sinks` (kSinkKeys), or a prefix common to all sequences and then its own
+// sequence's up to its place (kPrefixKeys). The attention kernels are compiled for each.
+enum : int { kPlainKeys = 0, kSinkKeys = 1, kPrefixKeys = 2 };
 
 struct TextAttnParams {
   const __nv_bfloat16* q;
@@ -31,6 +32,17 @@ struct TextAttnParams {
   int64_t total_q, total_k;
   int causal, window;
   int sinks;  // kSinkKeys: first keys that stay visible beside the window
+  // kPrefixKeys
+  int prefix;  // its keys,
+  int front;   // in tiles of 128
+  const int32_t* prefix_blocks;
+  int64_t table_stride;
+  int shared;  // text_flash: one walk over the prefix for the rows of all sequences (otherwise: each
+               // sequence's items walk the prefix, then its own keys). Rows kernel: sequence 0 is that walk
+  float* layer_o;     // sums of rows [layer][total_q * hq][hd], brought together by prefix_join_kernel
+  float2* layer_ml;   // their maxima (base 2) and denominators
+  int own_layer;      // rows kernel: of the sequences' own keys
+  size_t ws_reserved; // bytes of the workspace in use before the kernel's own
   float sl2;  // scale * log2(e): scores and maxima are kept in base 2
   float* part;              // split items: [2 * gridDim][16][hd] sums, then [..][16] maxima and denominators
   float* part_ml;
@@ -48,6 +60,9 @@ struct KvSource {
 
 // attention for many query rows (wx_text_flash.cu)
 int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv, int keys = kPlainKeys);
+// workspace that it takes beside layers, and the pieces (layers) of a shared walk over the prefix
+size_t text_flash_ws(wx_ctx* ctx);
+int text_flash_layers(wx_ctx* ctx, const TextAttnParams& p);
 
 // One sequence as the kernels see it; lengths and offsets from the device are clamped to the
 // buffers, so that wrong ones give wrong rows and an error word but no access outside.
@@ -90,8 +105,10 @@ __device__ __forceinline__ int key_lo(const TextAttnParams& p, const Seq& s, int
 }
 
 // whether a row with bounds [lo, hi) sees key j
+// (kPrefixKeys: of its own sequence; a key of the prefix goes by -1)
 template <int KEYS>
 __device__ __forceinline__ bool key_seen(const TextAttnParams& p, int j, int lo, int hi) {
+  if constexpr (KEYS == kPrefixKeys) return j < hi;
   return j < hi && (j >= lo || (KEYS == kSinkKeys && j < p.sinks));
 }
 // Between the first keys and the window lie keys that no row of an item (of a call, in the rows kernel)

@@ -84,14 +84,26 @@ struct TfItem {
   __device__ int hi(int X) const { return X ? b1 : a1; }
   __device__ int first() const { return a1 <= a0 ? b0 : b1 <= b0 ? a0 : min(a0, b0); }
   __device__ int last() const { return max(first(), max(a1 > a0 ? a1 : 0, b1 > b0 ? b1 : 0)); }
-  // key tile t of the walk: its tile of the sequence, and whether some row does not see all of it
+  // key tile t of the walk: its first key, the keys of what it belongs to (the sequence, or the prefix
+  // before it), and whether some row does not see all of it
   template <int KEYS>
-  __device__ int tile(int t) const {
-    return KEYS == kSinkKeys ? at(t) : t;
+  __device__ bool in_prefix(const TextAttnParams& p, int t) const {
+    return KEYS == kPrefixKeys && t < p.front;
+  }
+  template <int KEYS>
+  __device__ int key0(const TextAttnParams& p, int t) const {
+    if constexpr (KEYS == kSinkKeys) return at(t) * 128;
+    if constexpr (KEYS == kPrefixKeys) return (t < p.front ? t : t - p.front) * 128;
+    return t * 128;
+  }
+  template <int KEYS>
+  __device__ int keys(const TextAttnParams& p, int t) const {
+    return in_prefix<KEYS>(p, t) ? p.prefix : lk;
   }
   template <int KEYS>
   __device__ bool masked(const TextAttnParams& p, int t) const {
-    const int j = tile<KEYS>(t) * 128;
+    const int j = key0<KEYS>(p, t);
+    if (in_prefix<KEYS>(p, t)) return j + 128 > p.prefix;
     return j + 128 > free_hi || (j < free_lo && (KEYS != kSinkKeys || j + 128 > p.sinks));
   }
 };
@@ -198,7 +210,8 @@ __device__ __noinline__ void remember_row(uint32_t row, int r, int key, uint32_t
 // looks at the 16 bytes that it will expand itself (HD / 16 lanes a row), zeroes the codes there, and
 // their columns go to a new entry of the item's list, one a row. Behind the last key nobody sees them.
 template <int HD>
-__device__ __noinline__ void remember_codes(uint32_t raw, int tid, int key0, int lk, int& bad, uint32_t* list) {
+__device__ __noinline__ void remember_codes(uint32_t raw, int tid, int key0, int lk, bool prefix, int& bad,
+                                            uint32_t* list) {
   constexpr int kLanes = HD / 16;
   const int c = tid % kLanes;
 #pragma unroll 1
@@ -223,7 +236,7 @@ __device__ __noinline__ void remember_codes(uint32_t raw, int tid, int key0, int
       const int slot = atomicAdd(&bad, 1);
       if (slot < kTfBadRows) {
         uint32_t* entry = list + slot * kTfBadWords;
-        entry[0] = (uint32_t)key;
+        entry[0] = (uint32_t)(prefix ? -1 : key);
 #pragma unroll
         for (int e = 0; e < 4; ++e) entry[1 + e] = entry[5 + e] = mask[e];
       }
@@ -247,7 +260,7 @@ struct TfParams {
   int* next;           // [2] items handed out, CTAs that have finished (0, 0 between launches)
   uint32_t* bad_rows;  // [CTA][kTfItems][kTfBadRows][kTfBadWords]
   const uint8_t *k8, *v8;  // rows of an 8-bit cache
-  int splits;              // at most this many pieces of an item
+  int splits, min_tiles;   // at most this many pieces of an item, of so many tiles
   float* part;             // [splits][total_q * hq][HD] sums of the pieces' rows (items cut up only)
   float2* part_ml;         // [splits][total_q * hq] maximum (base 2) and denominator
 };
@@ -260,22 +273,32 @@ __device__ __forceinline__ int2 slot_tiles(const TextAttnParams& p, const Seq& s
   return hi > lo ? make_int2(lo >> 7, (hi + 127) >> 7) : make_int2(0, 0);
 }
 // The key tiles of both slots of the item from tok0 on, in its walk. With first keys that stay visible both walk
-// from those through the window of the item's first row.
+// from those through the window of the item's first row; with a prefix, from that through their own keys.
 template <int KEYS>
 __device__ __forceinline__ KeyGap item_tiles(const TextAttnParams& p, const Seq& s, int tok0, int tt, int2& a, int2& b) {
   a = slot_tiles(p, s, tok0, tt);
   b = slot_tiles(p, s, tok0 + tt, tt);
+  if constexpr (KEYS == kPrefixKeys) {
+    a = make_int2(0, tok0 < s.lq ? p.front + a.y : 0);
+    b = make_int2(0, tok0 + tt < s.lq ? p.front + b.y : 0);
+  }
   if constexpr (KEYS != kSinkKeys) return KeyGap{0, 0};
   const KeyGap at = key_gap<KEYS>(p, key_lo(p, s, tok0) >> 7, 128);
   if (a.y > a.x) a = make_int2(0, a.y - at.gap);
   if (b.y > b.x) b = make_int2(0, b.y - at.gap);
   return at;
 }
-// The item's tiles [first, last) and the pieces that they are cut into, of at least kTfMinTiles
-__device__ __forceinline__ void cut_item(int2 a, int2 b, int splits, int& first, int& last, int& pieces) {
+// kPrefixKeys, shared: the rows of all sequences as one, with no keys but the prefix's
+template <int KEYS>
+__device__ __forceinline__ Seq walk_seq(const TextAttnParams& p, int b) {
+  if (KEYS == kPrefixKeys && p.shared) return Seq{0, 0, (int)p.total_q, 0};
+  return load_seq(p, b);
+}
+// The item's tiles [first, last) and the pieces that they are cut into, of at least min_tiles
+__device__ __forceinline__ void cut_item(int2 a, int2 b, int splits, int min_tiles, int& first, int& last, int& pieces) {
   first = a.y <= a.x ? b.x : b.y <= b.x ? a.x : min(a.x, b.x);
   last = max(first, max(a.y > a.x ? a.y : 0, b.y > b.x ? b.y : 0));
-  pieces = min(splits, max(1, (last - first) / kTfMinTiles));
+  pieces = min(splits, max(1, (last - first) / min_tiles));
 }
 
 template <int FMT, int HD, int KEYS>
@@ -357,10 +380,18 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       auto page_of = [&](int b0, int bx) -> int {
         if (ids_from < 0 || b0 < ids_from || b0 + boxes > ids_from + 32) {
           ids_from = b0;
-          const int64_t j = (int64_t)(b0 + lane) * tp.box;
+          int64_t j = (int64_t)(b0 + lane) * tp.box;
           ids = 0;
-          if (j < it.lk) {
-            ids = p.block_table[it.b * p.blocks_per_seq + (j >> p.page_shift)];
+          bool here = j < it.lk;
+          const int32_t* table = p.block_table + it.b * p.blocks_per_seq;
+          if constexpr (KEYS == kPrefixKeys) {  // (boxes of the walk)
+            const int64_t front = (int64_t)p.front * 128;
+            table = j < front ? p.prefix_blocks : p.block_table + it.b * p.table_stride;
+            here = j < front ? j < p.prefix : j - front < it.lk;
+            if (j >= front) j -= front;
+          }
+          if (here) {
+            ids = table[j >> p.page_shift];
             if (ids < 0 || ids >= p.pages) {
               set_dev_error(p.err, kDevBadArgs);
               ids = 0;
@@ -374,12 +405,11 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       };
       // 8-bit: a tile in two halves of 64 raw rows, its scales with the keys; rows past the
       // sequence's last key are not loaded (any byte expands to a finite value or, in K, NaN: masked)
-      auto load_raw = [&](bool is_k, int walked) -> bool {
-        const int t = it.tile<KEYS>(walked);
-        const int per_half = 64 / tp.box;
-        const int page = page_of(t * boxes, lane % boxes);
-        const int nb = min(boxes, (it.lk - t * 128 + tp.box - 1) / tp.box);
-        int64_t row = cache_row(page, t * 128 + (lane % boxes) * tp.box);
+      auto load_raw = [&](bool is_k, int t) -> bool {
+        const int per_half = 64 / tp.box, key0 = it.key0<KEYS>(p, t);
+        const int page = page_of((KEYS == kPrefixKeys ? t : key0 >> 7) * boxes, lane % boxes);
+        const int nb = min(boxes, (it.keys<KEYS>(p, t) - key0 + tp.box - 1) / tp.box);
+        int64_t row = cache_row(page, key0 + (lane % boxes) * tp.box);
         // (the copy's bytes are waited for: it reads the first rows instead)
         if (lane < nb && !WX_IN_BOUNDS(p.err, row >= 0 && row + tp.box <= (p.pages * p.hkv) << p.page_shift)) row = 0;
         if (is_k) {
@@ -406,31 +436,31 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         }
         return true;
       };
-      auto load = [&](bool is_k, int walked) -> bool {
-        if constexpr (kW) return load_raw(is_k, walked);
-        const int t = it.tile<KEYS>(walked);
+      auto load = [&](bool is_k, int t) -> bool {
+        if constexpr (kW) return load_raw(is_k, t);
+        const int key0 = it.key0<KEYS>(p, t);
         const uint32_t cnt = is_k ? nk : nv;
         const int ns = is_k ? kKStages : kTfVStages;
         const uint32_t s = cnt % ns, par = ((cnt / ns) & 1) ^ 1u;
         if (!mbar_wait(bar((is_k ? kBTfKEmpty : kBTfVEmpty) + s), par, p.err, kDevTimeoutEmpty, abort_flag)) return false;
-        const bool mend = !is_k && it.masked<KEYS>(p, walked);
+        const bool mend = !is_k && it.masked<KEYS>(p, t);
         const uint32_t full = bar((is_k ? kBTfKFull : mend ? kBTfVRaw : kBTfVFull) + s);
         const uint32_t dst = is_k ? sK(s) : sV(s);
         const CUtensorMap* tm = is_k ? &tmK : &tmV;
         // boxes past the sequence's last key are not loaded (no page stands there)
-        const int nb = p.block_table ? min(boxes, (it.lk - t * 128 + tp.box - 1) / tp.box) : 1;
+        const int nb = p.block_table ? min(boxes, (it.keys<KEYS>(p, t) - key0 + tp.box - 1) / tp.box) : 1;
         if (lane == 0) {
           mbar_arrive_expect_tx(full, (uint32_t)(nb * tp.box * HD * 2));
           if (!is_k) mbar_arrive(bar(kBTfVFull + s));
         }
         __syncwarp();
         if (!p.block_table) {
-          if (lane < G::kChunks) tma_load_2d(dst + lane * kTfChunk, tm, full, it.h * HD + lane * 64, it.k0 + t * 128);
+          if (lane < G::kChunks) tma_load_2d(dst + lane * kTfChunk, tm, full, it.h * HD + lane * 64, it.k0 + key0);
         } else {
           const int bx = lane / G::kChunks, ch = lane % G::kChunks;
-          const int page = page_of(t * boxes, bx);
+          const int page = page_of((KEYS == kPrefixKeys ? t : key0 >> 7) * boxes, bx);
           if (bx < nb) {
-            const int row = (int)cache_row(page, t * 128 + bx * tp.box);
+            const int row = (int)cache_row(page, key0 + bx * tp.box);
             tma_load_2d(dst + ch * kTfChunk + bx * tp.box * 128, tm, full, ch * 64, row);
           }
         }
@@ -558,7 +588,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     // many heads as keep their keys and values (kTfL2 bytes) in L2 together.
     auto seq_items = [&](int b) -> int {
       if (b >= p.batch) return 0;
-      const Seq s = load_seq(p, b);
+      const Seq s = walk_seq<KEYS>(p, b);
       return (int)((unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt)) * p.hkv * tp.splits;
     };
     int wb = 0;
@@ -581,9 +611,9 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           const unsigned in_b = of_b / (unsigned)tp.splits;
           int found = 1;
           if (lane == 0) {
-            const Seq s = load_seq(p, wb + src);
+            const Seq s = walk_seq<KEYS>(p, wb + src);
             const unsigned tiles = (unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt);
-            const unsigned fit = (unsigned)(kTfL2 / (HD * 4)) / (unsigned)max(1, s.lk);
+            const unsigned fit = (unsigned)(kTfL2 / (HD * 4)) / (unsigned)max(1, KEYS == kPrefixKeys ? max(s.lk, p.prefix) : s.lk);
             const unsigned heads = max(1u, min((unsigned)p.hkv, fit));
             const unsigned chunk = in_b / (tiles * heads), rest = in_b - chunk * tiles * heads;
             const unsigned mine = min(heads, p.hkv - chunk * heads);
@@ -600,7 +630,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
             int2 a, b;
             dst->at = item_tiles<KEYS>(p, s, tok0, tp.tt, a, b);
             int first, last, pieces;
-            cut_item(a, b, tp.splits, first, last, pieces);
+            cut_item(a, b, tp.splits, tp.min_tiles, first, last, pieces);
             const int piece = (int)(of_b - in_b * (unsigned)tp.splits), per = (last - first + pieces - 1) / pieces;
             first += piece * per;
             last = min(last, first + per);
@@ -663,7 +693,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       int bad = 0;
       for (int t = t0; t < t1 && ok; ++t) {
         if (kW || !cur.masked<KEYS>(p, t)) continue;
-        const int key0 = cur.tile<KEYS>(t) * 128;
+        const int key0 = cur.key0<KEYS>(p, t), keys = cur.keys<KEYS>(p, t);
         const uint32_t s = (nv + (uint32_t)(t - t0)) % kTfVStages;
         uint32_t& done = s == 0 ? raw[0] : raw[1];
         if (!mbar_wait(bar(kBTfVRaw + s), done & 1, p.err, kDevTimeoutFull, abort_flag)) {
@@ -676,7 +706,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 #pragma unroll 1
         for (int r = lane; r < 128; r += 32) {
           const uint32_t row = sV(s) + (uint32_t)r * 128;
-          const bool past = key0 + r >= cur.lk;
+          const bool past = key0 + r >= keys;
           __nv_bfloat162 probe = __floats2bfloat162_rn(0.f, 0.f);
           const __nv_bfloat162 zero = probe;
 #pragma unroll 4
@@ -694,7 +724,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           const uint32_t who = __ballot_sync(0xffffffffu, odd);
           if (odd) {
             const int slot = bad + __popc(who & ((1u << lane) - 1u));
-            remember_row<HD>(row, r, key0 + r, slot < kTfBadRows ? list + slot * kTfBadWords : nullptr);
+            remember_row<HD>(row, r, cur.in_prefix<KEYS>(p, t) ? -1 : key0 + r, slot < kTfBadRows ? list + slot * kTfBadWords : nullptr);
           }
           bad += __popc(who);
           __syncwarp();
@@ -747,7 +777,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           const uint32_t raw = sbase + G::kRawOff + rs * G::kRawBytes;
           // (NaN codes do what they should in a key and in a value that every row sees)
           if (FMT == kKvE4m3 && !is_k && masked)
-            remember_codes<HD>(raw, tid, at->tile<KEYS>(t) * 128 + half * 64, at->lk, items[n % kTfItems].bad, list);
+            remember_codes<HD>(raw, tid, at->key0<KEYS>(p, t) + half * 64, at->keys<KEYS>(p, t), at->in_prefix<KEYS>(p, t),
+                               items[n % kTfItems].bad, list);
 #pragma unroll
           for (int j = 0; j < 64 * HD / 16 / 128; ++j) {
             const int u = j * 128 + tid, row = half * 64 + u / (HD / 16), c = u % (HD / 16);
@@ -971,10 +1002,10 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       const int a0 = any ? it.lo(X) : t1, a1 = any ? it.hi(X) : t1;
       const int tok = it.tok0 + X * tp.tt + my_tok;
       const bool live = r < tp.tt * p.group && tok < it.lq;
-      int hi = 0, lo = 0;
+      int own_hi = 0, lo = 0;
       if (live) {
         const Seq s{it.q0, it.k0, it.lq, it.lk};
-        hi = key_hi(p, s, tok);
+        own_hi = key_hi(p, s, tok);
         lo = key_lo(p, s, tok);
       }
       bool q_sent = false;
@@ -1004,7 +1035,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           q_sent = true;
         }
         const bool masked = it.masked<KEYS>(p, t);
-        const int key0 = it.tile<KEYS>(t) * 128;
+        const int key0 = it.key0<KEYS>(p, t);
+        const int hi = it.in_prefix<KEYS>(p, t) ? p.prefix : own_hi;
         if constexpr (kW) {
           const uint32_t g = both + (uint32_t)(t - t0);
           if (!frag_tile(g, key0 >> 7, t == a0, masked, hi, lo, m4, l4)) {
@@ -1128,7 +1160,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       tc_fence_after();
       const float inv = l == 0.f ? 0.f : __fdividef(kByteUnit<FMT>, l);
       const int bad = any ? *reinterpret_cast<const volatile int*>(&it.bad) : 0;
-      const bool cut = it.pieces > 1;
+      const bool cut = it.pieces > 1 || (KEYS == kPrefixKeys && p.shared);
       const bool write = ok && live &&
                          WX_IN_BOUNDS(p.err, it.q0 >= 0 && it.q0 + tok < p.total_q && it.h * p.group + my_g < p.hq &&
                                                  it.piece >= 0 && it.piece < tp.splits);
@@ -1160,7 +1192,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           for (int e = 0; e < min(bad, kTfBadRows); ++e) {
             const uint32_t* entry = list + e * kTfBadWords;
             const int key = (int)__ldcg(entry);
-            if (key_seen<KEYS>(p, key, lo, hi)) {
+            if (key_seen<KEYS>(p, key, lo, own_hi)) {
               plus |= __ldcg(entry + 1 + (col >> 5)) >> (col & 31);
               minus |= __ldcg(entry + 5 + (col >> 5)) >> (col & 31);
             }
@@ -1237,7 +1269,7 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   int2 a, e;
   item_tiles<KEYS>(p, s, tok0, tp.tt, a, e);
   int first, last, pieces;
-  cut_item(a, e, tp.splits, first, last, pieces);
+  cut_item(a, e, tp.splits, tp.min_tiles, first, last, pieces);
   if (pieces < 2) return;
   constexpr int kPer = HD / 32;
   float o[kPer] = {};
@@ -1293,6 +1325,23 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
 }
 
+size_t text_flash_ws(wx_ctx* ctx) { return (size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4; }
+
+// Pieces of the shared walk: the fewest rounds over the SMs, of which each takes a piece's tiles and a
+// start and end worth some three; a layer that is written and read again costs what a tile does.
+int text_flash_layers(wx_ctx* ctx, const TextAttnParams& p) {
+  const int64_t tt = 128 / p.group, items = p.hkv * ((p.total_q + 2 * tt - 1) / (2 * tt));
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int n = 1; n <= std::min(p.front, 64); ++n) {
+    const int per = (p.front + n - 1) / n;
+    if ((p.front + per - 1) / per != n) continue;  // (a piece would be empty)
+    const int64_t cost = (items * n + ctx->num_sms - 1) / ctx->num_sms * (per + 3) + n;
+    if (cost < least) least = cost, best = n;
+  }
+  return best;
+}
+
 template <int FMT, int HD, int KEYS>
 static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, TfParams& tp) {
   using G = TfGeom<FMT, HD>;
@@ -1312,21 +1361,27 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   // to an SM and as the longest range that a row can see allows.
   int64_t keys = p.block_table ? p.blocks_per_seq << p.page_shift : p.total_k;
   if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 2 * tp.tt + (KEYS == kSinkKeys ? p.sinks : 0));
+  if (KEYS == kPrefixKeys) keys += p.front * 128;
+  tp.min_tiles = kTfMinTiles;
   tp.splits = (int)std::max<int64_t>(1, std::min((kTfWaves * ctx->num_sms + items - 1) / items, keys / (128 * kTfMinTiles)));
+  if (KEYS == kPrefixKeys && p.shared) {
+    tp.splits = text_flash_layers(ctx, p);
+    tp.min_tiles = 1;
+  }
   const int grid = (int)std::min<int64_t>(ctx->num_sms, items * tp.splits);
   const int64_t rows = tp.splits > 1 ? p.total_q * p.hq * tp.splits : 0;
-  Carve c;
-  const size_t o_bad = c.take((size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4);
-  const size_t o_part = c.take((size_t)rows * HD * 4), o_ml = c.take((size_t)rows * 8);
+  Carve c{p.ws_reserved};
+  const size_t o_bad = c.take(text_flash_ws(ctx));
+  const size_t o_part = p.shared ? 0 : c.take((size_t)rows * HD * 4), o_ml = p.shared ? 0 : c.take((size_t)rows * 8);
   uint8_t* ws = static_cast<uint8_t*>(workspace(ctx, c.off, &st));
   if (!ws) return st;
   tp.bad_rows = reinterpret_cast<uint32_t*>(ws + o_bad);
-  tp.part = reinterpret_cast<float*>(ws + o_part);
-  tp.part_ml = reinterpret_cast<float2*>(ws + o_ml);
+  tp.part = p.shared ? p.layer_o : reinterpret_cast<float*>(ws + o_part);
+  tp.part_ml = p.shared ? p.layer_ml : reinterpret_cast<float2*>(ws + o_ml);
   if (!(tp.next = arrival_counters(ctx, 2, &st))) return st;
   ProfScope prof(ctx, kProfAttn);
   fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(tq, tk, tv, tp);
-  if (tp.splits == 1) return launch_status(ctx, "text_flash");
+  if (tp.splits == 1 || p.shared) return launch_status(ctx, "text_flash");
   text_flash_join_kernel<HD, KEYS><<<(unsigned)((p.total_q * p.hq + 7) / 8), 256, 0, ctx->stream>>>(tp);
   return launch_status(ctx, "text_flash", 2);
 }
@@ -1362,6 +1417,7 @@ int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSourc
     if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, tp.box))) return st;
     if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, tp.box))) return st;
   }
+  if (keys == kPrefixKeys) return launch_flash<kPrefixKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp);
   return keys == kSinkKeys ? launch_flash<kSinkKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp)
                            : launch_flash<kPlainKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp);
 }

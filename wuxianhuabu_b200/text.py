@@ -9,6 +9,7 @@ runs its text encoder once per generation, model/minimax h3/H3TextEncoder.swift)
 * ``PagedKVCache``     — a paged K/V cache, quantised as it is written, read back on demand
 * ``prompt_attention`` — whole prompts: causal, grouped heads, packed sequences
 * ``paged_attention``  — new tokens (one per sequence or a chunk) over the cache
+* ``prefix_attention`` — the same where all sequences stand behind one cached prefix
 
 Tensors are torch CUDA tensors used as device buffers; calls are ordered on torch's current
 stream, do not synchronise, and may be captured in CUDA graphs (whose replays must not overlap
@@ -32,7 +33,7 @@ from ._lib import (KV_BF16, KV_E4M3, KV_INT8, ROPE_BY_PARTS, ROPE_LINEAR, ROPE_P
 from .h3 import _need_bf16_cuda, _p, context
 
 __all__ = ["RopeScaling", "RopeTable", "rope_axes", "PagePool", "StepPlan", "PagedKVCache", "prompt_attention",
-           "paged_attention"]
+           "paged_attention", "prefix_attention"]
 
 _FORMATS = {"bf16": (KV_BF16, torch.bfloat16), "int8": (KV_INT8, torch.int8), "e4m3": (KV_E4M3, torch.float8_e4m3fn)}
 _SCALINGS = {"none": ROPE_PLAIN, "linear": ROPE_LINEAR, "by_parts": ROPE_BY_PARTS}
@@ -497,4 +498,35 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, cu_seqlens: torch.Tens
         context(dev).call("wx_paged_attention_sinks", dims, _first_keys(sinks), *args)
     else:
         context(dev).call("wx_paged_attention", dims, *args)
+    return (o, lse) if return_lse else o
+
+
+def prefix_attention(q: torch.Tensor, cache: PagedKVCache, prefix_blocks: torch.Tensor, prefix_len: int,
+                     cu_seqlens: torch.Tensor, kv_lens: torch.Tensor, block_table: torch.Tensor, max_len: int,
+                     scale: Optional[float] = None, causal: bool = True, out: Optional[torch.Tensor] = None,
+                     return_lse: bool = False):
+    """``paged_attention`` where every sequence stands behind the same ``prefix_len`` cached tokens, in pages
+    prefix_blocks (int32): these are walked once for the whole batch and seen by every row. kv_lens and
+    block_table are of each sequence's own tokens behind them; block_table may be columns of a larger table
+    (``prefix_attention(q, cache, table[0, :n], n * page_size, cu, lens - n * page_size, table[:, n:], ...)``)."""
+    n, h, d, qs, o, os_, lse = _attn_out(q, out, return_lse)
+    batch = _batch_of(cu_seqlens)
+    cu = _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
+    lens = _need_ints(torch.int32, batch, "kv_lens", kv_lens)
+    prefix = _need_ints(torch.int32, None, "prefix_blocks", prefix_blocks)
+    if not 0 <= prefix_len <= prefix_blocks.numel() * cache.page_size:
+        raise _invalid(f"prefix_len must be in 0..{prefix_blocks.numel() * cache.page_size} (prefix_blocks' tokens)")
+    if block_table.dim() != 2 or block_table.shape[0] != batch or not block_table.is_cuda or \
+            block_table.dtype != torch.int32:
+        raise _invalid("block_table must be a CUDA int32 [batch, blocks] tensor")
+    blocks = block_table.shape[1]
+    stride, inner = block_table.stride()
+    if (blocks > 1 and inner != 1) or (batch > 1 and stride < blocks):
+        raise _invalid("block_table must have contiguous rows")
+    if d != cache.head_dim:
+        raise _invalid("q must have the cache's head_dim")
+    dev = _same_device(q, cache.k, cu_seqlens, kv_lens, block_table, prefix_blocks, o)
+    context(dev).call("wx_prefix_attention", _dims(n, batch, max_len, h, cache.kv_heads, d, causal, 0, scale),
+                      q.data_ptr(), qs, cache._desc, prefix, prefix_len, cu, lens, block_table.data_ptr(), blocks,
+                      max(stride, blocks), o.data_ptr(), os_, _p(lse))
     return (o, lse) if return_lse else o
