@@ -46,6 +46,16 @@ CASES = [  # tokens, q heads, k heads, head_dim, rot, interleaved, shares of the
     (2100, 8, 2, 64, 32, False, None, False, "qk"),
     (65, 40, 8, 128, 128, False, (64,), False, ""),
     (19, 3, 3, 128, 104, False, (20, 16, 16), True, ""),
+    # many tokens: persistent warps
+    (1800, 32, 8, 128, 128, False, (24, 20, 20), True, "qk"),
+    (2001, 13, 7, 128, 128, True, (24, 20, 20), False, "qk"),
+    (1777, 29, 15, 64, 64, False, (12, 10, 10), True, "qk"),
+    (3700, 14, 5, 128, 64, False, (16, 16), True, "q"),
+    (2900, 31, 9, 64, 24, True, (3, 3, 3, 3), True, "k"),
+    (1850, 40, 33, 64, 40, False, (10, 5, 5), False, "qk"),
+    (4000, 11, 5, 128, 8, False, None, False, "qk"),
+    (1776, 33, 17, 128, 120, False, None, False, ""),
+    (5000, 3, 1, 128, 128, False, None, False, "qk"),  # (not for them: few heads)
 ]
 
 
@@ -145,6 +155,41 @@ def test_rows_of_zeros_infinities_and_nan():
     same = torch.ones(5, 3, dtype=torch.bool, device="cuda")
     same[2, 1] = same[3, 0] = False
     assert torch.equal(a[same], c[same])
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+def test_many_tokens_with_wrong_positions_and_slots(fmt):
+    """Tokens that are skipped or wrong, among thousands that are not: the others as without them."""
+    text = _text()
+    from wuxianhuabu_b200 import h3
+    g = _gen(9)
+    n = 2500
+    tab = text.RopeTable(128, 500, axes=text.rope_axes((24, 20, 20), True))
+    q, k, v = _randn(g, n, 14, 128), _randn(g, n, 7, 128), _randn(g, n, 7, 128)
+    w = torch.ones(128, dtype=BF16, device="cuda")
+    pos = torch.randint(0, 500, (3, n), generator=g, device="cuda", dtype=torch.int32)
+    slots = torch.randperm(n + 12, generator=g, device="cuda")[:n]
+    caches = [text.PagedKVCache((n + 31) // 16, 16, 7, 128, fmt) for _ in range(2)]
+    want = caches[0].append_roped(q, k, v, slots, tab, pos, q_norm=w, k_norm=w)
+    _check_device()
+    some, skipped, wrong, far = (torch.arange(i, n, 97, device="cuda") for i in range(4))
+    slots2, pos2 = slots.clone(), pos.clone()
+    slots2[skipped] = -5
+    slots2[far] = (n + 31) // 16 * 16
+    pos2[2, wrong] = 500
+    pos2[0, some[:3]] = -1
+    out = torch.full_like(q, 9.0)
+    caches[1].append_roped(q, k, v, slots2, tab, pos2, q_out=out, q_norm=w, k_norm=w)
+    with pytest.raises(h3.WxError):
+        _check_device()
+    lost = torch.zeros(n, dtype=torch.bool, device="cuda")
+    lost[wrong] = lost[some[:3]] = True
+    assert (out[lost] == 9.0).all() and torch.equal(out[~lost], want[~lost])
+    unwritten = lost.clone()
+    unwritten[skipped] = unwritten[far] = True
+    for a, b in zip(caches[0].read(slots), caches[1].read(slots)):
+        assert not b[unwritten].any() and torch.equal(a[~unwritten], b[~unwritten])
+    _check_device()
 
 
 def test_positions_outside_the_table_and_skipped_slots():

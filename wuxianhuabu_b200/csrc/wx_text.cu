@@ -10,6 +10,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "wx_internal.h"
 #include "wx_text_dev.cuh"
@@ -47,16 +48,13 @@ __global__ void rope_table_kernel(RopeFreqs f, int nf, int64_t positions, double
 // = 5.45 TB/s with clean lines (three or two groups in flight 43 and 67, five 38); 4,096 tokens
 // with rope into an int8 cache and read back, 40 us for both (35.6). 300 tokens take 3 us on the
 // device, a third of the call.
-//
-// With HEADS, q and k rows are normalised first, y = x / sqrt(mean x^2 + eps) * w, the squares summed over
-// the row's lanes, and each pair may turn by a position of its own axis. All of it stays in fp32 until
-// the one rounding (or quantisation) at the end.
 constexpr int kRowGroups = 4;
 
 struct RowsParams {
   const __nv_bfloat16 *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;  // elements between tokens
-  int nq, nkv, nv;                       // q, k and v rows of a token (no cache: v none)
+  int nq, nkv;                           // q rows, and k (= v) rows of a token (0 without a cache)
+  int nv;                                // head_rows_kernel: v rows
   int64_t tokens;
   int rows_per_warp, chunks;             // a token's rows are dealt to `chunks` warps
   // rotation (rot = 0: none)
@@ -73,15 +71,6 @@ struct RowsParams {
   int64_t n_slots;
   int page_shift;
   int* err;
-  // HEADS: norm weights (nullptr: none), two bits for each pair's axis, where the axes' positions lie,
-  // and k rows that go here instead of into a cache
-  const __nv_bfloat16 *q_norm, *k_norm;
-  float eps;
-  int axes;
-  uint64_t axis_of[2];
-  int64_t pos_stride;
-  __nv_bfloat16* k_out;
-  int64_t k_out_stride;
 };
 
 template <int W>
@@ -95,6 +84,24 @@ struct Cols {  // W bf16 columns in memory
       const uint2 x = *reinterpret_cast<const uint2*>(p);
       w[0] = x.x, w[1] = x.y;
     }
+  }
+  __device__ __forceinline__ void lds(uint32_t at) {
+    if constexpr (W == 8) {
+      const uint4 x = lds128(at);
+      w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+      const uint2 x = lds64(at);
+      w[0] = x.x, w[1] = x.y;
+    }
+  }
+  __device__ __forceinline__ void sts(uint32_t at) const {
+    if constexpr (W == 8)
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    else asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(at), "r"(w[0]), "r"(w[1]) : "memory");
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) w[i] = 0;
   }
   __device__ __forceinline__ void store(__nv_bfloat16* p) const {
     if constexpr (W == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -144,13 +151,13 @@ __device__ __forceinline__ float quantise(const float (&x)[N], uint32_t (&w)[N /
   return finite ? (live ? __fdiv_rn(amax, kMax) : 0.f) : __int_as_float(0x7fc00000);
 }
 
-template <int FMT, int HD, int W, bool INTERLEAVED, bool HEADS>
+template <int FMT, int HD, int W, bool INTERLEAVED>
 __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
   constexpr int kLanes = HD / (2 * W);  // lanes of a row
   constexpr int kRows = 32 / kLanes;    // rows of a warp at a time
   const int lane = threadIdx.x & 31;
   const int j = lane % kLanes;
-  const int per_token = p.nq + p.nkv + p.nv;
+  const int per_token = p.nq + 2 * p.nkv;
   // a block: eight tokens, the same chunk of each
   const unsigned blk = blockIdx.x / (unsigned)p.chunks;
   const int64_t t = (int64_t)blk * 8 + (threadIdx.x >> 5);
@@ -177,55 +184,23 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
 
   float cs[W], sn[W];
   if (p.rot) {
-    int64_t pos = p.pos[t];
-    bool bad = pos < 0 || pos >= p.positions;
-    int64_t pos_of[4] = {pos, pos, pos, pos};
-    uint32_t codes = 0;  // axes of this lane's pairs, two bits each
-    if constexpr (HEADS) {
-      if (p.axes > 1) {
-        bool same = true;
-#pragma unroll
-        for (int a = 1; a < 4; ++a) {
-          if (a >= p.axes) break;
-          pos_of[a] = p.pos[a * p.pos_stride + t];
-          bad |= pos_of[a] < 0 || pos_of[a] >= p.positions;
-          same &= pos_of[a] == pos;
-        }
-        // (text: the axes run together, and one row of the table serves all pairs)
-        if (!same) codes = (uint32_t)(p.axis_of[j * W >= 32] >> (2 * (j * W & 31))) & ((1u << 2 * W) - 1u);
-      }
-    }
-    if (bad) {
+    const int64_t pos = p.pos[t];
+    if (pos < 0 || pos >= p.positions) {
       if (lane == 0) set_dev_error(p.err, kDevBadArgs);
       return;
     }
     if (turn) {
-      bool whole = true;
-      if constexpr (HEADS) {
-        whole = codes == (codes & 3u) * (0x5555u & ((1u << 2 * W) - 1u));
-        if (whole) pos = (codes & 3u) == 0 ? pos_of[0] : (codes & 3u) == 1 ? pos_of[1] : (codes & 3u) == 2 ? pos_of[2] : pos_of[3];
-      }
-      if (whole) {
 #pragma unroll
-        for (int i = 0; i < W; i += 4) {
-          const float4 c = *reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + W * j + i);
-          const float4 s = *reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + W * j + i);
-          cs[i] = c.x, cs[i + 1] = c.y, cs[i + 2] = c.z, cs[i + 3] = c.w;
-          sn[i] = s.x, sn[i + 1] = s.y, sn[i + 2] = s.z, sn[i + 3] = s.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const uint32_t a = codes >> (2 * i) & 3u;
-          const int64_t at = (a == 0 ? pos_of[0] : a == 1 ? pos_of[1] : a == 2 ? pos_of[2] : pos_of[3]) * (p.rot / 2) + W * j + i;
-          cs[i] = p.cos_t[at];
-          sn[i] = p.sin_t[at];
-        }
+      for (int i = 0; i < W; i += 4) {
+        const float4 c = *reinterpret_cast<const float4*>(p.cos_t + pos * (p.rot / 2) + W * j + i);
+        const float4 s = *reinterpret_cast<const float4*>(p.sin_t + pos * (p.rot / 2) + W * j + i);
+        cs[i] = c.x, cs[i + 1] = c.y, cs[i + 2] = c.z, cs[i + 3] = c.w;
+        sn[i] = s.x, sn[i + 1] = s.y, sn[i + 2] = s.z, sn[i + 3] = s.w;
       }
     }
   }
   int64_t slot = -1;
-  if (HEADS ? p.slots != nullptr : p.nkv) {
+  if (p.nkv) {
     slot = p.slots[t];
     if (slot >= p.n_slots) {
       if (lane == 0) set_dev_error(p.err, kDevBadArgs);
@@ -246,25 +221,6 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
       const uint32_t u = live ? a[g].w[i] : 0, v = live ? b[g].w[i] : 0;
       x[2 * i] = bf16_lo(u), x[2 * i + 1] = bf16_hi(u);
       x[W + 2 * i] = bf16_lo(v), x[W + 2 * i + 1] = bf16_hi(v);
-    }
-    if constexpr (HEADS) {
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 2 * W; ++i) ss += x[i] * x[i];
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const __nv_bfloat16* weight = is_q ? p.q_norm : is_v ? nullptr : p.k_norm;
-      if (weight) {
-        const float rstd = rsqrtf(ss * (1.f / HD) + p.eps);
-        Cols<W> lo, hi;
-        lo.load(weight + c0);
-        hi.load(weight + c1);
-#pragma unroll
-        for (int i = 0; i < W / 2; ++i) {
-          x[2 * i] *= rstd * bf16_lo(lo.w[i]), x[2 * i + 1] *= rstd * bf16_hi(lo.w[i]);
-          x[W + 2 * i] *= rstd * bf16_lo(hi.w[i]), x[W + 2 * i + 1] *= rstd * bf16_hi(hi.w[i]);
-        }
-      }
     }
     if (turn && !is_v) {
       // (x1, x2) -> (x1 c - x2 s, x2 c + x1 s)
@@ -287,12 +243,10 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
     const int64_t row = ((((slot >> p.page_shift) * p.nkv + h) << p.page_shift) | (slot & ((1 << p.page_shift) - 1)));
     if (!WX_IN_BOUNDS(p.err, is_q ? h >= 0 && h < p.nq : h >= 0 && h < p.nkv && (slot < 0 || row < p.n_slots * p.nkv)))
       continue;
-    const bool plain_k = HEADS && !is_q && p.k_out;
     if (is_q || FMT == kKvBf16) {
-      __nv_bfloat16* o = is_q      ? p.q_out + t * p.q_out_stride + (int64_t)h * HD
-                         : plain_k ? p.k_out + t * p.k_out_stride + (int64_t)h * HD
-                                   : reinterpret_cast<__nv_bfloat16*>(is_v ? p.vc : p.kc) + row * HD;
-      if (!is_q && !plain_k && slot < 0) continue;
+      __nv_bfloat16* o = is_q ? p.q_out + t * p.q_out_stride + (int64_t)h * HD
+                              : reinterpret_cast<__nv_bfloat16*>(is_v ? p.vc : p.kc) + row * HD;
+      if (!is_q && slot < 0) continue;
       Cols<W> lo, hi;
 #pragma unroll
       for (int i = 0; i < W / 2; ++i) {
@@ -312,6 +266,533 @@ __global__ void __launch_bounds__(256, 3) text_rows_kernel(RowsParams p) {
       }
       if (j == 0) (is_v ? p.vs : p.ks)[row] = scale;
     }
+  }
+}
+
+// ---------------------------------------------------------------- head norms and position axes
+// q and k rows normalised, y = x / sqrt(mean x^2 + eps) * w, and turned, each pair by the position of its own axis;
+// k and v into a cache, or k beside q. All of it in fp32 until the one rounding (or quantisation) at the end.
+//
+// Lanes, columns and loads as above. There is more to do for the same bytes, and issue slots run out before HBM
+// does (366 instructions for the four rows that a warp works on at a time: 43 us for a clip's 8,064 tokens, 32 + 8
+// heads of 128; rope alone takes 162 and 28 us), hence:
+// - a warp's rows are of one norm, q or k (and v), and the weight goes into the rotation's factors:
+//   u = x1 (w1 c) - x2 (w2 s), v = x2 (w2 c) + x1 (w1 s). A warp makes them for its token, a lane a pair or two,
+//   while its rows are on their way, and reads them from shared memory as it needs them (in registers
+//   they would cost an SM a block of its three);
+// - q rows lie side by side: one address and constant offsets. Squares, scaling, rotation in packed pairs.
+// Measured with kernels as below, in us beside their rule (launch_heads).
+struct HeadParams {
+  RowsParams r;
+  int nk;  // k rows (of a cache, or to k_out)
+  const __nv_bfloat16 *q_norm, *k_norm;  // nullptr: not normalised
+  float eps;
+  int axes;
+  uint64_t axis_of[2];  // two bits for each pair
+  int64_t pos_stride;   // between the axes' positions
+  __nv_bfloat16* k_out;
+  int64_t k_out_stride;
+  int q_chunks;  // of the `chunks` warps of a token
+};
+
+// W floats of shared memory as pairs
+template <int W>
+__device__ __forceinline__ void lds_pairs(uint32_t at, float2 (&f)[W / 2]) {
+#pragma unroll
+  for (int i = 0; i < W; i += 4) {
+    const uint4 x = lds128(at + i * 4);
+    f[i / 2] = make_float2(__uint_as_float(x.x), __uint_as_float(x.y));
+    f[i / 2 + 1] = make_float2(__uint_as_float(x.z), __uint_as_float(x.w));
+  }
+}
+
+// a lane's first, second, third and fourth factors, and where it reads them
+template <int W>
+struct Factors {
+  float2 a[W / 2], b[W / 2], c[W / 2], d[W / 2];
+};
+struct FactorsAt {
+  uint32_t a, b, c, d;
+  template <int W>
+  __device__ __forceinline__ void load(Factors<W>& f) const {
+    lds_pairs<W>(a, f.a);
+    lds_pairs<W>(b, f.b);
+    lds_pairs<W>(c, f.c);
+    lds_pairs<W>(d, f.d);
+  }
+};
+template <int HD, int W, bool INTERLEAVED>
+__device__ __forceinline__ FactorsAt factors_at(const float* table, int j) {
+  constexpr int kPairs = HD / 2;
+  FactorsAt f;
+  f.a = smem_u32(table) + (INTERLEAVED ? 2 : 1) * W * j * 4;
+  f.b = f.a + (INTERLEAVED ? 2 : 1) * kPairs * 4;
+  f.c = f.a + (INTERLEAVED ? W : 2 * kPairs) * 4;
+  f.d = f.b + (INTERLEAVED ? W : 2 * kPairs) * 4;
+  return f;
+}
+// one pair's factors, of columns cA and cB: w_A c, -w_B s, w_B c, w_A s (columns that do not turn: c 1, s 0). Half
+// layout: an array of each; interleaved: the first and third side by side, then the others
+template <int HD, int W, bool INTERLEAVED>
+__device__ __forceinline__ void put_factors(float* f, int pair, float c, float s, float wa, float wb) {
+  constexpr int kPairs = HD / 2;
+  if constexpr (INTERLEAVED) {
+    *reinterpret_cast<float2*>(f + 2 * pair) = make_float2(wa * c, wb * c);
+    *reinterpret_cast<float2*>(f + 2 * kPairs + 2 * pair) = make_float2(-wb * s, wa * s);
+  } else {
+    f[pair] = wa * c;
+    f[kPairs + pair] = -wb * s;
+    f[2 * kPairs + pair] = wb * c;
+    f[3 * kPairs + pair] = wa * s;
+  }
+}
+template <int W, bool INTERLEAVED>
+__device__ __forceinline__ int2 columns_of(int pair, int rot) {
+  if (INTERLEAVED) return make_int2(2 * pair, 2 * pair + 1);
+  if (pair < rot / 2) return make_int2(pair, rot / 2 + pair);
+  return make_int2(2 * pair - pair % W, 2 * pair - pair % W + W);
+}
+
+// A lane's columns c0.. (x1) and c1.. (x2) of a row
+template <int W>
+__device__ __forceinline__ void unpack(const Cols<W>& lo, const Cols<W>& hi, float2 (&x1)[W / 2], float2 (&x2)[W / 2]) {
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    x1[i] = make_float2(bf16_lo(lo.w[i]), bf16_hi(lo.w[i]));
+    x2[i] = make_float2(bf16_lo(hi.w[i]), bf16_hi(hi.w[i]));
+  }
+}
+template <int W>
+__device__ __forceinline__ float square_sum(const float2 (&x1)[W / 2], const float2 (&x2)[W / 2]) {
+  float2 s1 = make_float2(0.f, 0.f), s2 = s1;
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    s1 = __ffma2_rn(x1[i], x1[i], s1);
+    s2 = __ffma2_rn(x2[i], x2[i], s2);
+  }
+  return (s1.x + s1.y) + (s2.x + s2.y);
+}
+// scaled, weighted and turned
+template <int W, bool INTERLEAVED>
+__device__ __forceinline__ void turn_row(float2 (&x1)[W / 2], float2 (&x2)[W / 2], float rstd, bool turn, const Factors<W>& f) {
+  const float2 rr = make_float2(rstd, rstd);
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    x1[i] = __fmul2_rn(x1[i], rr);
+    x2[i] = __fmul2_rn(x2[i], rr);
+  }
+  if (turn) {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      if (INTERLEAVED) {  // a pair's columns times (w_A c, w_B c), their swap times (-w_B s, w_A s)
+        x1[i] = __ffma2_rn(x1[i], f.a[i], __fmul2_rn(make_float2(x1[i].y, x1[i].x), f.b[i]));
+        x2[i] = __ffma2_rn(x2[i], f.c[i], __fmul2_rn(make_float2(x2[i].y, x2[i].x), f.d[i]));
+      } else {
+        const float2 u = __ffma2_rn(x1[i], f.a[i], __fmul2_rn(x2[i], f.b[i]));
+        x2[i] = __ffma2_rn(x2[i], f.c[i], __fmul2_rn(x1[i], f.d[i]));
+        x1[i] = u;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      x1[i] = __fmul2_rn(x1[i], f.a[i]);
+      x2[i] = __fmul2_rn(x2[i], f.c[i]);
+    }
+  }
+}
+template <int W>
+__device__ __forceinline__ void pack(const float2 (&x1)[W / 2], const float2 (&x2)[W / 2], Cols<W>& lo, Cols<W>& hi) {
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    lo.w[i] = pack_bf16x2(x1[i].x, x1[i].y);
+    hi.w[i] = pack_bf16x2(x2[i].x, x2[i].y);
+  }
+}
+// quantised to row `row` of the cache, head column c0.. and to_c1 behind it. All lanes of the warp call
+template <int FMT, int HD, int W>
+__device__ __forceinline__ void store_quantised(const RowsParams& p, const float2 (&x1)[W / 2], const float2 (&x2)[W / 2],
+                                                bool write, bool is_v, int64_t row, int c0, int to_c1, bool first_lane) {
+  float x[2 * W];
+#pragma unroll
+  for (int i = 0; i < W / 2; ++i) {
+    x[2 * i] = x1[i].x, x[2 * i + 1] = x1[i].y;
+    x[W + 2 * i] = x2[i].x, x[W + 2 * i + 1] = x2[i].y;
+  }
+  uint32_t q[W / 2];
+  const float scale = quantise<FMT, 2 * W, HD / (2 * W)>(x, q);
+  if (!write) return;
+  uint8_t* o = (is_v ? p.vc : p.kc) + row * HD + c0;
+  if constexpr (W == 8) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(q[0], q[1]);
+    *reinterpret_cast<uint2*>(o + to_c1) = make_uint2(q[2], q[3]);
+  } else {
+    *reinterpret_cast<uint32_t*>(o) = q[0];
+    *reinterpret_cast<uint32_t*>(o + to_c1) = q[1];
+  }
+  if (first_lane) (is_v ? p.vs : p.ks)[row] = scale;
+}
+
+template <int FMT, int HD, int W, bool INTERLEAVED>
+__global__ void __launch_bounds__(256, 3) head_rows_kernel(HeadParams hp) {
+  const RowsParams& p = hp.r;
+  constexpr int kLanes = HD / (2 * W);  // lanes of a row
+  constexpr int kRows = 32 / kLanes;    // rows of a warp at a time
+  constexpr int kPairs = HD / 2;
+  // of the warp's token
+  __shared__ __align__(16) float factors[8][4 * kPairs];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int j = lane % kLanes, sub = lane / kLanes;
+  const unsigned blk = blockIdx.x / (unsigned)p.chunks;
+  const int64_t t = (int64_t)blk * 8 + warp;
+  if (t >= p.tokens) return;
+  const int chunk = (int)(blockIdx.x - blk * (unsigned)p.chunks);
+  const bool is_q = chunk < hp.q_chunks;
+  // rows of this warp: r0.. of q, or of k and then v (from n0 on)
+  const int r0 = (is_q ? chunk : chunk - hp.q_chunks) * p.rows_per_warp;
+  const int n0 = is_q ? p.nq : hp.nk;
+  const int r1 = min(is_q ? p.nq : hp.nk + p.nv, r0 + p.rows_per_warp);
+
+  const bool turn = j < p.rot / (2 * W);
+  const bool apart = turn && !INTERLEAVED;  // pairs (i, i + rot / 2)
+  const int c0 = apart ? W * j : 2 * W * j;
+  const int c1 = apart ? p.rot / 2 + W * j : 2 * W * j + W;
+
+  // row 0's columns c0.. of q or k, and of v nk rows before its first
+  const __nv_bfloat16* src0 = (is_q ? p.q + t * p.q_stride : p.k + t * p.k_stride) + c0;
+  const __nv_bfloat16* src1 = is_q ? src0 : p.v + t * p.v_stride - (int64_t)hp.nk * HD + c0;
+  const int to_c1 = c1 - c0;
+  Cols<W> a[kRowGroups], b[kRowGroups];
+  const __nv_bfloat16* q_from = src0 + (r0 + sub) * HD;
+#pragma unroll
+  for (int g = 0; g < kRowGroups; ++g) {
+    const int r = r0 + g * kRows + sub;
+    if (r < r1) {
+      const __nv_bfloat16* src = is_q ? q_from + g * (kRows * HD) : (r < n0 ? src0 : src1) + r * HD;
+      a[g].load(src);
+      b[g].load(src + to_c1);
+    } else {  // (its lanes are a row of their own)
+      a[g].clear();
+      b[g].clear();
+    }
+  }
+
+  // ---- the factors, with the rows on their way
+  const __nv_bfloat16* weight = is_q ? hp.q_norm : hp.k_norm;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kPairs / 32; ++i) {
+    const int pair = i * 32 + lane;
+    const int2 cols = columns_of<W, INTERLEAVED>(pair, p.rot);
+    float c = 1.f, s = 0.f;
+    if (pair < p.rot / 2) {
+      const int axis = (int)(hp.axis_of[i] >> (2 * lane)) & 3;
+      const int64_t pos = p.pos[axis * hp.pos_stride + t];
+      if (pos < 0 || pos >= p.positions) {
+        bad = true;
+      } else {
+        const int64_t at = pos * (p.rot / 2) + pair;
+        c = __ldg(p.cos_t + at);
+        s = __ldg(p.sin_t + at);
+      }
+    }
+    float wa = 1.f, wb = 1.f;
+    if (weight) wa = __bfloat162float(weight[cols.x]), wb = __bfloat162float(weight[cols.y]);
+    put_factors<HD, W, INTERLEAVED>(factors[warp], pair, c, s, wa, wb);
+  }
+  if (__any_sync(0xffffffffu, bad)) {
+    if (lane == 0) set_dev_error(p.err, kDevBadArgs);
+    return;
+  }
+  __syncwarp();
+  const FactorsAt factor = factors_at<HD, W, INTERLEAVED>(factors[warp], j);
+
+  // ---- where the rows go
+  const bool cached = !is_q && !hp.k_out;
+  // (rows of a bf16 cache and plain ones by address, those of an 8-bit cache by their number)
+  __nv_bfloat16 *dst0 = is_q ? p.q_out + t * p.q_out_stride : hp.k_out + t * hp.k_out_stride, *dst1 = dst0;
+  int64_t row0 = 0;  // cache row of head 0
+  if (cached) {
+    const int64_t slot = p.slots[t];
+    if (slot >= p.n_slots && lane == 0) set_dev_error(p.err, kDevBadArgs);
+    if (slot < 0 || slot >= p.n_slots) return;
+    row0 = ((slot >> p.page_shift) * hp.nk << p.page_shift) | (slot & ((1 << p.page_shift) - 1));
+    if (FMT == kKvBf16) {
+      dst0 = reinterpret_cast<__nv_bfloat16*>(p.kc) + row0 * HD;
+      dst1 = reinterpret_cast<__nv_bfloat16*>(p.vc) + row0 * HD - ((int64_t)hp.nk * HD << p.page_shift);
+    }
+  }
+  dst0 += c0;
+  dst1 += c0;
+  const int64_t stride = cached ? (int64_t)HD << p.page_shift : HD;
+
+  __nv_bfloat16* q_to = dst0 + (r0 + sub) * HD;
+#pragma unroll
+  for (int g = 0; g < kRowGroups; ++g) {
+    if (r0 + g * kRows >= r1) break;  // (the warp as a whole)
+    const int r = r0 + g * kRows + sub;
+    const bool live = r < r1, is_v = r >= n0;
+    float2 x1[W / 2], x2[W / 2];
+    unpack<W>(a[g], b[g], x1, x2);
+    float rstd = 1.f;
+    if (weight) {  // (all lanes: it shuffles)
+      float ss = square_sum<W>(x1, x2);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      rstd = rsqrtf(ss * (1.f / HD) + hp.eps);
+    }
+    if (!is_v) {
+      Factors<W> f;
+      factor.load(f);
+      turn_row<W, INTERLEAVED>(x1, x2, rstd, turn, f);
+    }
+    if (FMT == kKvBf16 || !cached) {
+      if (!live) continue;
+      if (!WX_IN_BOUNDS(p.err, r >= 0 && r < (is_q ? p.nq : hp.nk + p.nv) && (is_q || !is_v || cached))) continue;
+      __nv_bfloat16* o = is_q ? q_to + g * (kRows * HD) : (is_v ? dst1 : dst0) + r * stride;
+      Cols<W> lo, hi;
+      pack<W>(x1, x2, lo, hi);
+      lo.store(o);
+      hi.store(o + to_c1);
+    } else {
+      const int64_t row = row0 + ((int64_t)(is_v ? r - hp.nk : r) << p.page_shift);
+      const bool write = live && WX_IN_BOUNDS(p.err, row >= 0 && row < p.n_slots * hp.nk);
+      store_quantised<FMT, HD, W>(p, x1, x2, write, is_v, row, c0, to_c1, j == 0);
+    }
+  }
+}
+
+// The same for many tokens: persistent warps, each with a ring of its own in shared memory, through which the
+// rows of its tokens pass in chunks of 4 KB. Bulk copies bring them (a token's heads lie side by side) and
+// take them away, so that loads stay in flight while the warp computes; in the kernel above a warp's life is a load,
+// then its arithmetic, and neither keeps HBM busy. Positions run two tokens ahead, table rows one. A chunk's row
+// groups are worked on side by side: one after the other (12 warps, 4 stages) their latency made it 42 us.
+// Measured: q and k of 8,064 tokens, 32 + 8 heads of 128, three axes, 31.9 us = 5.3 TB/s (rows kernel 41); 4,277 tokens
+// into an int8 cache 21 us (30). Issue slots 53 % busy, four warps to a scheduler.
+constexpr int kStreamWarps = 16, kStreamStages = 3, kStreamChunk = 4096;
+template <int HD>
+struct StreamGeom {
+  static constexpr int kRing = kStreamWarps * kStreamStages * kStreamChunk;
+  static constexpr int kFactors = kStreamWarps * 2 * 2 * HD * 4;  // of q's and of k's norm
+  static constexpr int kSmem = kRing + kFactors + kStreamWarps * kStreamStages * 8 + 16;
+};
+
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// waits until at most N of the thread's groups still read shared memory
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+template <int FMT, int HD, int W, bool INTERLEAVED>
+__global__ void __launch_bounds__(32 * kStreamWarps, 1) head_stream_kernel(HeadParams hp) {
+  const RowsParams& p = hp.r;
+  using G = StreamGeom<HD>;
+  constexpr int kLanes = HD / (2 * W), kRows = 32 / kLanes, kPairs = HD / 2;
+  constexpr int kChunkRows = kStreamChunk / (2 * HD), kGroups = kChunkRows / kRows;
+  extern __shared__ uint4 smem_raw[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int j = lane % kLanes, sub = lane / kLanes;
+  uint8_t* smem = reinterpret_cast<uint8_t*>(smem_raw);
+  const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * kStreamStages * kStreamChunk);
+  float* table_q = reinterpret_cast<float*>(smem + G::kRing) + warp * 2 * 4 * kPairs;
+  float* table_k = table_q + 4 * kPairs;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + G::kRing + G::kFactors) + warp * kStreamStages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + G::kRing + G::kFactors + kStreamWarps * kStreamStages * 8);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  if (lane == 0) {
+    for (int i = 0; i < kStreamStages; ++i) mbar_init(smem_u32(bars + i), 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  const int q_chunks = (p.nq + kChunkRows - 1) / kChunkRows, chunks = q_chunks + (hp.nk + p.nv + kChunkRows - 1) / kChunkRows;
+  const int64_t step = (int64_t)gridDim.x * kStreamWarps, first = (int64_t)warp * gridDim.x + blockIdx.x;
+
+  // ---- loads, by lane 0: chunk after chunk of the warp's tokens
+  int64_t load_t = first;
+  int load_c = 0;
+  auto issue = [&](uint32_t stage) {
+    if (load_t >= p.tokens) return;
+    const uint32_t dst = ring + stage * kStreamChunk, bar = smem_u32(bars + stage);
+    if (load_c < q_chunks) {
+      const int a = load_c * kChunkRows, n = min(p.nq - a, kChunkRows);
+      mbar_arrive_expect_tx(bar, (uint32_t)(n * HD * 2));
+      bulk_load(dst, p.q + load_t * p.q_stride + a * HD, (uint32_t)(n * HD * 2), bar);
+    } else {
+      const int a = (load_c - q_chunks) * kChunkRows, e = min(hp.nk + p.nv, a + kChunkRows);
+      const int nk = max(0, min(e, hp.nk) - a), nv = e - a - nk;
+      mbar_arrive_expect_tx(bar, (uint32_t)((nk + nv) * HD * 2));
+      if (nk) bulk_load(dst, p.k + load_t * p.k_stride + a * HD, (uint32_t)(nk * HD * 2), bar);
+      if (nv)
+        bulk_load(dst + nk * HD * 2, p.v + load_t * p.v_stride + (a + nk - hp.nk) * HD, (uint32_t)(nv * HD * 2), bar);
+    }
+    if (++load_c == chunks) load_c = 0, load_t += step;
+  };
+  if (lane == 0)
+    for (int i = 0; i < kStreamStages - 1; ++i) issue(i);
+
+  // ---- positions and table rows, ahead of their tokens; a lane has pairs lane, lane + 32
+  constexpr int kMine = kPairs / 32;
+  int64_t pos[kMine];
+  float cs[kMine], sn[kMine], qa[kMine], qb[kMine], ka[kMine], kb[kMine];
+  bool bad = false;
+  auto fetch_pos = [&](int64_t t) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int axis = (int)(hp.axis_of[i] >> (2 * lane)) & 3;
+      pos[i] = t < p.tokens && i * 32 + lane < p.rot / 2 ? p.pos[axis * hp.pos_stride + t] : -1;
+    }
+  };
+  auto fetch_rows = [&](int64_t t) {
+    bad = false;
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      cs[i] = 1.f, sn[i] = 0.f;
+      if (t >= p.tokens || i * 32 + lane >= p.rot / 2) continue;
+      if (pos[i] < 0 || pos[i] >= p.positions) {
+        bad = true;
+        continue;
+      }
+      const int64_t at = pos[i] * (p.rot / 2) + i * 32 + lane;
+      cs[i] = __ldg(p.cos_t + at);
+      sn[i] = __ldg(p.sin_t + at);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kMine; ++i) {
+    const int2 c = columns_of<W, INTERLEAVED>(i * 32 + lane, p.rot);
+    qa[i] = hp.q_norm ? __bfloat162float(hp.q_norm[c.x]) : 1.f;
+    qb[i] = hp.q_norm ? __bfloat162float(hp.q_norm[c.y]) : 1.f;
+    ka[i] = hp.k_norm ? __bfloat162float(hp.k_norm[c.x]) : 1.f;
+    kb[i] = hp.k_norm ? __bfloat162float(hp.k_norm[c.y]) : 1.f;
+  }
+  const bool cached = !hp.k_out && hp.nk > 0;
+  fetch_pos(first);
+  int64_t slot = cached && first < p.tokens ? p.slots[first] : -1, next_slot = -1;
+  fetch_rows(first);
+  fetch_pos(first + step);
+
+  const bool turn = j < p.rot / (2 * W);
+  const bool apart = turn && !INTERLEAVED;  // pairs (i, i + rot / 2)
+  const int c0 = apart ? W * j : 2 * W * j;
+  const int to_c1 = apart ? p.rot / 2 : W;
+  const FactorsAt fq = factors_at<HD, W, INTERLEAVED>(table_q, j), fk = factors_at<HD, W, INTERLEAVED>(table_k, j);
+
+  uint32_t task = 0;
+  bool ok = true;
+  for (int64_t t = first; t < p.tokens && ok; t += step) {
+    // ---- this token's factors; the next one's table row, the one's after it positions
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      put_factors<HD, W, INTERLEAVED>(table_q, i * 32 + lane, cs[i], sn[i], qa[i], qb[i]);
+      put_factors<HD, W, INTERLEAVED>(table_k, i * 32 + lane, cs[i], sn[i], ka[i], kb[i]);
+    }
+    const bool skip = __any_sync(0xffffffffu, bad);
+    if (skip && lane == 0) set_dev_error(p.err, kDevBadArgs);
+    fetch_rows(t + step);
+    fetch_pos(t + 2 * step);
+    next_slot = cached && t + step < p.tokens ? p.slots[t + step] : -1;
+    if (slot >= p.n_slots && cached) {
+      if (lane == 0) set_dev_error(p.err, kDevBadArgs);
+      slot = -1;
+    }
+    // cache row of head 0
+    const int64_t row0 = ((slot >> p.page_shift) * hp.nk << p.page_shift) | (slot & ((1 << p.page_shift) - 1));
+    __syncwarp();
+
+    for (int c = 0; c < chunks; ++c, ++task) {
+      const uint32_t stage = task % kStreamStages, at = ring + stage * kStreamChunk;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(bars + stage), (task / kStreamStages) & 1, p.err, kDevTimeoutFull,
+                                             abort_flag))) {
+        ok = false;
+        break;
+      }
+      const bool is_q = c < q_chunks;
+      const int r0 = (is_q ? c : c - q_chunks) * kChunkRows;
+      const int n0 = is_q ? p.nq : hp.nk;
+      const int r1 = min(is_q ? p.nq : hp.nk + p.nv, r0 + kChunkRows);
+      const bool to_cache = !is_q && cached;
+      const bool norm = (is_q ? hp.q_norm : hp.k_norm) != nullptr;
+      if (!skip && !(to_cache && slot < 0)) {
+        // (all groups' reads, sums and joins over the lanes together: one after the other, their latency was
+        // most of a chunk's time)
+        Cols<W> lo[kGroups], hi[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          const uint32_t x_at = at + (uint32_t)((g * kRows + sub) * HD + c0) * 2;
+          lo[g].lds(x_at);
+          hi[g].lds(x_at + to_c1 * 2);
+        }
+        float rstd[kGroups];
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          float2 x1[W / 2], x2[W / 2];
+          unpack<W>(lo[g], hi[g], x1, x2);
+          rstd[g] = norm ? square_sum<W>(x1, x2) : 1.f;
+        }
+        if (norm) {
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) rstd[g] += __shfl_xor_sync(0xffffffffu, rstd[g], o);
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) rstd[g] = rsqrtf(rstd[g] * (1.f / HD) + hp.eps);
+        }
+        Factors<W> f;
+        (is_q ? fq : fk).load(f);
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+          if (r0 + g * kRows >= (FMT == kKvBf16 ? min(n0, r1) : r1)) break;  // (the warp as a whole; bf16 v goes as it came)
+          const int r = r0 + g * kRows + sub;
+          const bool live = r < r1, is_v = r >= n0;
+          float2 x1[W / 2], x2[W / 2];
+          unpack<W>(lo[g], hi[g], x1, x2);
+          if (!is_v) turn_row<W, INTERLEAVED>(x1, x2, rstd[g], turn, f);
+          if (FMT == kKvBf16 || !to_cache) {
+            const uint32_t x_at = at + (uint32_t)((g * kRows + sub) * HD + c0) * 2;
+            Cols<W> y, z;
+            pack<W>(x1, x2, y, z);
+            if (live && !is_v) {
+              y.sts(x_at);
+              z.sts(x_at + to_c1 * 2);
+            }
+          } else {
+            const int64_t row = row0 + ((int64_t)(is_v ? r - hp.nk : r) << p.page_shift);
+            const bool write = live && WX_IN_BOUNDS(p.err, row >= 0 && row < p.n_slots * hp.nk);
+            store_quantised<FMT, HD, W>(p, x1, x2, write, is_v, row, c0, to_c1, j == 0);
+          }
+        }
+        // ---- away with them: rows of one output as a whole, those of a cache one by one
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (!to_cache) {
+          __nv_bfloat16* o = is_q ? p.q_out + t * p.q_out_stride : hp.k_out + t * hp.k_out_stride;
+          if (lane == 0 && WX_IN_BOUNDS(p.err, r0 >= 0 && r1 <= n0)) bulk_store(o + r0 * HD, at, (uint32_t)((r1 - r0) * HD * 2));
+        } else if (FMT == kKvBf16) {
+          for (int r = r0 + lane; r < r1; r += 32) {
+            const int64_t row = row0 + ((int64_t)(r >= n0 ? r - hp.nk : r) << p.page_shift);
+            if (WX_IN_BOUNDS(p.err, row >= 0 && row < p.n_slots * hp.nk))
+              bulk_store((r >= n0 ? p.vc : p.kc) + row * HD * 2, at + (uint32_t)((r - r0) * HD * 2), HD * 2);
+          }
+        }
+      }
+      bulk_commit();
+      bulk_wait_read<1>();  // the chunk before this one has left its stage:
+      __syncwarp();         // that is the one to fill next
+      if (lane == 0) issue((task + kStreamStages - 1) % kStreamStages);
+    }
+    slot = next_slot;
+  }
+  bulk_wait_all();
+  if (!ok) {  // copies still in flight must land before the CTA ends: the time of one more bounded wait
+    const uint64_t from = globaltimer_ns();
+    while (globaltimer_ns() - from < 2000000ull) {}
   }
 }
 
@@ -420,36 +901,31 @@ static int64_t deal_rows(wx_ctx* ctx, int64_t tokens, int per_token, int rows_at
 }
 
 template <int FMT, int HD, int W>
-static void start_rows(unsigned g, cudaStream_t s, const RowsParams& p, bool heads) {
-  if (heads) {
-    if (p.interleaved) text_rows_kernel<FMT, HD, W, true, true><<<g, 256, 0, s>>>(p);
-    else text_rows_kernel<FMT, HD, W, false, true><<<g, 256, 0, s>>>(p);
-  } else {
-    if (p.interleaved) text_rows_kernel<FMT, HD, W, true, false><<<g, 256, 0, s>>>(p);
-    else text_rows_kernel<FMT, HD, W, false, false><<<g, 256, 0, s>>>(p);
-  }
+static void start_rows(unsigned g, cudaStream_t s, const RowsParams& p) {
+  if (p.interleaved) text_rows_kernel<FMT, HD, W, true><<<g, 256, 0, s>>>(p);
+  else text_rows_kernel<FMT, HD, W, false><<<g, 256, 0, s>>>(p);
 }
 
 template <int HD, int W>
-static void start_rows(int fmt, unsigned g, cudaStream_t s, const RowsParams& p, bool heads) {
-  if (fmt == kKvInt8) start_rows<kKvInt8, HD, W>(g, s, p, heads);
-  else if (fmt == kKvE4m3) start_rows<kKvE4m3, HD, W>(g, s, p, heads);
-  else start_rows<kKvBf16, HD, W>(g, s, p, heads);
+static void start_rows(int fmt, unsigned g, cudaStream_t s, const RowsParams& p) {
+  if (fmt == kKvInt8) start_rows<kKvInt8, HD, W>(g, s, p);
+  else if (fmt == kKvE4m3) start_rows<kKvE4m3, HD, W>(g, s, p);
+  else start_rows<kKvBf16, HD, W>(g, s, p);
 }
 
-static int launch_rows(wx_ctx* ctx, RowsParams& p, int fmt, int head_dim, bool heads = false) {
+static int launch_rows(wx_ctx* ctx, RowsParams& p, int fmt, int head_dim) {
   if (p.tokens == 0) return WX_OK;
   const int W = p.rot % 16 == 0 ? 8 : 4;
   const int64_t blocks =
-      deal_rows(ctx, p.tokens, p.nq + p.nkv + p.nv, 32 / (head_dim / (2 * W)), &p.rows_per_warp, &p.chunks);
+      deal_rows(ctx, p.tokens, p.nq + 2 * p.nkv, 32 / (head_dim / (2 * W)), &p.rows_per_warp, &p.chunks);
   if (blocks > INT32_MAX) return set_error(ctx, WX_ERR_UNSUPPORTED, "too many tokens in one call");
   p.err = ctx->dev_err;
   ProfScope prof(ctx, kProfRow);
   const unsigned g = (unsigned)blocks;
   if (head_dim == 128)
-    W == 8 ? start_rows<128, 8>(fmt, g, ctx->stream, p, heads) : start_rows<128, 4>(fmt, g, ctx->stream, p, heads);
+    W == 8 ? start_rows<128, 8>(fmt, g, ctx->stream, p) : start_rows<128, 4>(fmt, g, ctx->stream, p);
   else
-    W == 8 ? start_rows<64, 8>(fmt, g, ctx->stream, p, heads) : start_rows<64, 4>(fmt, g, ctx->stream, p, heads);
+    W == 8 ? start_rows<64, 8>(fmt, g, ctx->stream, p) : start_rows<64, 4>(fmt, g, ctx->stream, p);
   return launch_status(ctx, "text_rows");
 }
 
@@ -467,7 +943,7 @@ static void set_rope(RowsParams& p, const wx_rope* r, const int32_t* pos) {
 }
 
 static void set_cache(RowsParams& p, const wx_kv_cache* c, const int64_t* slots) {
-  p.nkv = p.nv = c->kv_heads;
+  p.nkv = c->kv_heads;
   p.kc = static_cast<uint8_t*>(c->k);
   p.vc = static_cast<uint8_t*>(c->v);
   p.ks = c->k_scale;
@@ -478,7 +954,7 @@ static void set_cache(RowsParams& p, const wx_kv_cache* c, const int64_t* slots)
 }
 
 // head norms and position axes of a call
-static int set_heads(wx_ctx* ctx, RowsParams& p, const wx_rope* rope, const wx_rope_axes* axes, const void* q_norm,
+static int set_heads(wx_ctx* ctx, HeadParams& p, const wx_rope* rope, const wx_rope_axes* axes, const void* q_norm,
                      const void* k_norm, float eps) {
   WX_CHECK_ARG(ctx, aligned16(q_norm) && aligned16(k_norm));
   WX_CHECK_ARG(ctx, (!q_norm && !k_norm) || (eps > 0.f && eps < INFINITY));
@@ -488,7 +964,7 @@ static int set_heads(wx_ctx* ctx, RowsParams& p, const wx_rope* rope, const wx_r
   p.axes = 1;
   if (!axes) return WX_OK;
   WX_CHECK_ARG(ctx, axes->n_axes >= 1 && axes->n_axes <= 4);
-  WX_CHECK_ARG(ctx, axes->n_axes == 1 || axes->position_stride >= p.tokens);
+  WX_CHECK_ARG(ctx, axes->n_axes == 1 || axes->position_stride >= p.r.tokens);
   p.axes = axes->n_axes;
   p.pos_stride = axes->position_stride;
   for (int i = 0; i < rope->rot / 2; ++i) {
@@ -496,6 +972,61 @@ static int set_heads(wx_ctx* ctx, RowsParams& p, const wx_rope* rope, const wx_r
     p.axis_of[i / 32] |= (uint64_t)axes->axis_of_pair[i] << (2 * (i % 32));
   }
   return WX_OK;
+}
+
+template <int FMT, int HD, int W, bool INTERLEAVED>
+static int start_heads(wx_ctx* ctx, const HeadParams& p, unsigned grid, bool stream) {
+  if (!stream) {
+    head_rows_kernel<FMT, HD, W, INTERLEAVED><<<grid, 256, 0, ctx->stream>>>(p);
+    return launch_status(ctx, "head_rows");
+  }
+  auto fn = head_stream_kernel<FMT, HD, W, INTERLEAVED>;
+  const int st = ensure_smem_attr(ctx, (const void*)fn, StreamGeom<HD>::kSmem, "head_stream");
+  if (st) return st;
+  fn<<<grid, 32 * kStreamWarps, StreamGeom<HD>::kSmem, ctx->stream>>>(p);
+  return launch_status(ctx, "head_stream");
+}
+template <int FMT, int HD>
+static int start_heads(wx_ctx* ctx, const HeadParams& p, unsigned g, bool wide, bool stream) {
+  if (wide)
+    return p.r.interleaved ? start_heads<FMT, HD, 8, true>(ctx, p, g, stream) : start_heads<FMT, HD, 8, false>(ctx, p, g, stream);
+  return p.r.interleaved ? start_heads<FMT, HD, 4, true>(ctx, p, g, stream) : start_heads<FMT, HD, 4, false>(ctx, p, g, stream);
+}
+template <int HD>
+static int start_heads(wx_ctx* ctx, int fmt, const HeadParams& p, unsigned g, bool wide, bool stream) {
+  if (fmt == kKvInt8) return start_heads<kKvInt8, HD>(ctx, p, g, wide, stream);
+  if (fmt == kKvE4m3) return start_heads<kKvE4m3, HD>(ctx, p, g, wide, stream);
+  return start_heads<kKvBf16, HD>(ctx, p, g, wide, stream);
+}
+static int launch_heads(wx_ctx* ctx, HeadParams& p, int fmt, int head_dim) {
+  const bool wide = p.r.rot % 16 == 0;
+  p.r.err = ctx->dev_err;
+  ProfScope prof(ctx, kProfRow);
+  // The persistent kernel takes chunks of 4 KB: it wants one and a half for each of its warps at least, and rows
+  // that fill them. Rows kernel : persistent, us a call, 32 + 8 heads of 128 (48 rows in 3 chunks) 600 tokens
+  // 12.3 : 12.3, 1,500 18.5 : 14.3, 8,000 45 : 39 (into int8 55 : 47); 8 + 1 heads (10 rows in 2 chunks)
+  // 8,000 22.5 : 24.5; 16 + 16 heads of 64 (48 of 64 rows) 4,000 18.4 : 16.4, 8,000 into int8 31 : 35.
+  const int per = kStreamChunk / (2 * head_dim), per_token = p.r.nq + p.nk + p.r.nv;
+  const int64_t filled = (p.r.nq + per - 1) / per + (p.nk + p.r.nv + per - 1) / per;
+  const bool stream = 2 * p.r.tokens * filled >= 3 * (int64_t)ctx->num_sms * kStreamWarps && 5 * per_token >= 3 * filled * per;
+  unsigned grid;
+  if (stream) {
+    grid = (unsigned)ctx->num_sms;
+  } else {
+    // as deal_rows, but for q rows and k and v rows apart
+    const int at_once = 32 / (head_dim / (wide ? 16 : 8));
+    int rows = at_once * kRowGroups;
+    auto chunks = [&] { return (p.r.nq + rows - 1) / rows + (p.nk + p.r.nv + rows - 1) / rows; };
+    while (rows > at_once && p.r.tokens * chunks() < (int64_t)ctx->num_sms * 64) rows /= 2;
+    p.r.rows_per_warp = rows;
+    p.q_chunks = (p.r.nq + rows - 1) / rows;
+    p.r.chunks = chunks();
+    const int64_t blocks = (p.r.tokens + 7) / 8 * p.r.chunks;
+    if (blocks > INT32_MAX) return set_error(ctx, WX_ERR_UNSUPPORTED, "too many tokens in one call");
+    grid = (unsigned)blocks;
+  }
+  return head_dim == 128 ? start_heads<128>(ctx, fmt, p, grid, wide, stream)
+                         : start_heads<64>(ctx, fmt, p, grid, wide, stream);
 }
 
 }  // namespace wx
@@ -620,21 +1151,21 @@ int wx_norm_rope_apply(wx_ctx* ctx, const wx_rope* rope, const wx_rope_axes* axe
   WX_CHECK_ARG(ctx, row_ok(q, q_stride, q_heads, head_dim) && row_ok(q_out, q_out_stride, q_heads, head_dim));
   WX_CHECK_ARG(ctx, k_heads == 0 ||
                         (row_ok(k, k_stride, k_heads, head_dim) && row_ok(k_out, k_out_stride, k_heads, head_dim)));
-  RowsParams p{};
-  set_rope(p, rope, positions);
-  p.tokens = tokens;
+  HeadParams p{};
+  set_rope(p.r, rope, positions);
+  p.r.tokens = tokens;
   if ((st = set_heads(ctx, p, rope, axes, q_norm, k_norm, eps))) return st;
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
-  p.q_stride = q_stride;
-  p.k_stride = k_stride;
-  p.nq = q_heads;
-  p.nkv = k_heads;
-  p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  p.q_out_stride = q_out_stride;
+  p.r.q = static_cast<const __nv_bfloat16*>(q);
+  p.r.k = static_cast<const __nv_bfloat16*>(k);
+  p.r.q_stride = q_stride;
+  p.r.k_stride = k_stride;
+  p.r.nq = q_heads;
+  p.nk = k_heads;
+  p.r.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.r.q_out_stride = q_out_stride;
   p.k_out = static_cast<__nv_bfloat16*>(k_out);
   p.k_out_stride = k_out_stride;
-  return launch_rows(ctx, p, kKvBf16, head_dim, true);
+  return launch_heads(ctx, p, kKvBf16, head_dim);
 }
 
 int wx_norm_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const wx_rope_axes* axes, const int32_t* positions,
@@ -650,21 +1181,22 @@ int wx_norm_rope_kv_append(wx_ctx* ctx, const wx_rope* rope, const wx_rope_axes*
   const int hd = cache->head_dim;
   WX_CHECK_ARG(ctx, slots && row_ok(q, q_stride, q_heads, hd) && row_ok(q_out, q_out_stride, q_heads, hd) &&
                         row_ok(k, k_stride, cache->kv_heads, hd) && row_ok(v, v_stride, cache->kv_heads, hd));
-  RowsParams p{};
-  set_rope(p, rope, positions);
-  set_cache(p, cache, slots);
-  p.tokens = tokens;
+  HeadParams p{};
+  set_rope(p.r, rope, positions);
+  set_cache(p.r, cache, slots);
+  p.r.tokens = tokens;
   if ((st = set_heads(ctx, p, rope, axes, q_norm, k_norm, eps))) return st;
-  p.q = static_cast<const __nv_bfloat16*>(q);
-  p.k = static_cast<const __nv_bfloat16*>(k);
-  p.v = static_cast<const __nv_bfloat16*>(v);
-  p.q_stride = q_stride;
-  p.k_stride = k_stride;
-  p.v_stride = v_stride;
-  p.nq = q_heads;
-  p.q_out = static_cast<__nv_bfloat16*>(q_out);
-  p.q_out_stride = q_out_stride;
-  return launch_rows(ctx, p, cache->format, hd, true);
+  p.r.q = static_cast<const __nv_bfloat16*>(q);
+  p.r.k = static_cast<const __nv_bfloat16*>(k);
+  p.r.v = static_cast<const __nv_bfloat16*>(v);
+  p.r.q_stride = q_stride;
+  p.r.k_stride = k_stride;
+  p.r.v_stride = v_stride;
+  p.r.nq = q_heads;
+  p.nk = p.r.nv = cache->kv_heads;
+  p.r.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.r.q_out_stride = q_out_stride;
+  return launch_heads(ctx, p, cache->format, hd);
 }
 
 int wx_kv_read(wx_ctx* ctx, const wx_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k_out, void* v_out,

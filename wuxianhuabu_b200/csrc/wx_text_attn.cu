@@ -66,6 +66,10 @@ __device__ __forceinline__ void copy_async_wait() {
 // into equal runs, one per CTA. A CTA whose run covers part of an item leaves its partial sums; the
 // last to arrive joins them in key order (so the result does not depend on who is last).
 //
+// kChunkKeys (own keys behind a shared prefix, many short sequences): units of `chunk` keys go to single
+// warps, on demand, and each leaves its sums as a layer for prefix_join_kernel. No warp waits for another, where
+// a piece per CTA costs its search, loads and join in turn: 64 sequences of 1 to 701 bf16 keys 43 -> CHUNK_US us.
+//
 // Measured, caches flushed from L2: 64 sequences, 32 / 8 heads of 128, 238,000 bf16 keys 191 us =
 // 5.4 TB/s (6.2 TB/s a further key); one sequence, 64 / 8 heads, 65,537 int8 keys 42 us = 3.3 TB/s, e4m3
 // 41 (the expansion's instructions are the bound: issue slots 53 % busy, DRAM 34 %; the start and the
@@ -98,6 +102,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
                           int64_t v_stride, TextAttnParams p, int min_units) {
   using G = RowsGeom<FMT, HD, NT>;
   constexpr bool kW = G::kWide;
+  constexpr bool kSolo = KEYS == kChunkKeys;  // a unit is one warp's
   constexpr int kWarps = G::kWarps, kRows = G::kRows, kU = G::kUnits16;
   constexpr int kMT = HD / 16;                 // 16-column tiles of O^T
   constexpr int kRowBytes = kW ? HD : HD * 2;
@@ -111,17 +116,16 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   const int g = lane >> 2, t = lane & 3;
   const uint32_t ring = smem_u32(smem_raw) + (uint32_t)(warp * kD * G::kStep);
 
-  // kPrefixKeys: with a shared prefix, the rows of all sequences over its keys come first
-  const int front = KEYS == kPrefixKeys && p.shared ? 1 : 0;
+  // behind a prefix: where it is shared, the rows of all sequences over its keys come first
+  constexpr bool kBehind = KEYS >= kPrefixKeys;
+  const int front = kBehind && p.shared ? 1 : 0;
   auto seq_of = [&](int b) -> Seq {
-    if (KEYS == kPrefixKeys && b < front) return Seq{0, 0, (int)p.total_q, p.prefix};
-    return load_seq(p, KEYS == kPrefixKeys ? b - front : b);
+    if (kBehind && b < front) return Seq{0, 0, (int)p.total_q, p.prefix};
+    return load_seq(p, kBehind ? b - front : b);
   };
-  auto hi_of = [&](int b, const Seq& s, int tok) -> int {
-    return KEYS == kPrefixKeys && b < front ? s.lk : key_hi(p, s, tok);
-  };
+  auto hi_of = [&](int b, const Seq& s, int tok) -> int { return kBehind && b < front ? s.lk : key_hi(p, s, tok); };
   auto blocks_of = [&](int b) -> const int32_t* {
-    if constexpr (KEYS == kPrefixKeys) return b < front ? p.prefix_blocks : p.block_table + (b - front) * p.table_stride;
+    if constexpr (kBehind) return b < front ? p.prefix_blocks : p.block_table + (b - front) * p.table_stride;
     return p.block_table + b * p.blocks_per_seq;
   };
 
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     k16 = key_lo(p, s, 0) & ~15;
     items = ((unsigned)(s.lq * p.group) + kRows - 1) / kRows * (unsigned)p.hkv;
     const int skip = KEYS == kSinkKeys ? key_gap<KEYS>(p, k16 >> 4, 16).gap << 4 : k16;
-    nu = (unsigned)max(1, (s.lk - skip + kUnit - 1) / kUnit);
+    nu = kSolo ? (unsigned)max(1, (s.lk - 1) / p.chunk + 1) : (unsigned)max(1, (s.lk - skip + kUnit - 1) / kUnit);
   };
   unsigned my_items = 0, my_nu = 0;  // of sequence loaded + lane
   int my_k16 = 0, loaded = -1;
@@ -156,8 +160,13 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     total = 0;
   }
   const unsigned per = max((unsigned)min_units, (total + gridDim.x - 1) / gridDim.x);
-  unsigned u = min(total, blockIdx.x * per);
-  const unsigned u_end = min(total, u + per);
+  // (kSolo: units are handed out on demand. Beside the shared walk CTAs begin late: nothing is set apart for them)
+  const unsigned apart = kSolo && !p.after_walk ? gridDim.x * kWarps : 0;
+  auto take_unit = [&]() -> unsigned { return lane == 0 ? apart + (unsigned)atomicAdd(p.counters, 1) : 0u; };
+  unsigned u = !kSolo ? min(total, blockIdx.x * per)
+               : apart ? blockIdx.x + gridDim.x * warp
+                       : __shfl_sync(0xffffffffu, take_unit(), 0);
+  const unsigned u_end = kSolo ? total : min(total, u + per);
 
   int wb = 0;               // sequences before wb hold
   unsigned wu = 0, wi = 0;  // this many units and items
@@ -165,6 +174,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     Seq s;
     int b, h, rt;
     unsigned item, item_u0, nu;  // the item, its first unit and its units
+    unsigned u_in;               // its first unit of the item
     int k_lo, k_hi;              // keys of this piece (k_lo a multiple of 16), without those in the gap
     KeyGap at16;                 // of 16-key steps
     int steps;                   // 16-key steps of this piece for this warp
@@ -210,12 +220,14 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     c.rt = (int)(i % rts);
     c.item = b_i0 + i;
     c.item_u0 = b_u0 + i * c.nu;
-    const unsigned units = min(c.nu - u_in, u_end - at);
+    const unsigned units = kSolo ? 1 : min(c.nu - u_in, u_end - at);
+    c.u_in = u_in;
     c.at16 = key_gap<KEYS>(p, k16 >> 4, 16);
-    c.k_lo = (KEYS == kSinkKeys ? 0 : k16) + (int)u_in * kUnit;
-    c.k_hi = min(c.s.lk - (c.at16.gap << 4), c.k_lo + (int)units * kUnit);
+    const int unit = kSolo ? p.chunk : kUnit;
+    c.k_lo = (KEYS == kSinkKeys ? 0 : k16) + (int)u_in * unit;
+    c.k_hi = min(c.s.lk - (c.at16.gap << 4), c.k_lo + (int)units * unit);
     const int n16 = max(0, (c.k_hi - c.k_lo + 15) / 16);
-    c.steps = n16 > warp ? (n16 - warp + kWarps - 1) / kWarps : 0;
+    c.steps = kSolo ? n16 : n16 > warp ? (n16 - warp + kWarps - 1) / kWarps : 0;
     return units;
   };
 
@@ -224,7 +236,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   const bool paged = kW || p.block_table;
   [[maybe_unused]] const int64_t kv_rows = paged ? (p.pages * p.hkv) << p.page_shift : p.total_k;
   int page_of = 0;
-  auto step_key = [&](const Piece& c, int i) { return c.k_lo + (i * kWarps + warp) * 16; };
+  auto step_key = [&](const Piece& c, int i) { return c.k_lo + (kSolo ? i : i * kWarps + warp) * 16; };
   auto first_key = [&](const Piece& c, int i) {
     const int j = step_key(c, i);
     return KEYS == kSinkKeys ? c.at16(j >> 4) << 4 : j;
@@ -310,6 +322,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     first_loads(cur);
   }
   while (have) {
+    [[maybe_unused]] const unsigned next_u = kSolo ? take_unit() : 0;
     const int n_rows = cur.s.lq * p.group;
     const int row0 = cur.rt * kRows;
     // ---- q fragments: row 8 n + g, columns in the order of the K reads; the limits of rows 2t, 2t+1
@@ -574,13 +587,40 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     // ---- the next piece's first loads go out before this one is joined
     const Piece done = cur;
     const unsigned u_done = u;
-    u += units;
+    u = kSolo ? __shfl_sync(0xffffffffu, next_u, 0) : u + units;
     have = u < u_end;
     if (have) {
       units = piece_at(u, cur);
       first_loads(cur);
     }
 
+    if constexpr (kSolo) {
+      const int64_t layer = (done.b < front ? 0 : p.own_layer) + (int64_t)done.u_in;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = l[n][e];
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+          const int r = row0 + 8 * n + 2 * t + e;
+          if (r >= n_rows) continue;
+          const int tk = (int)((unsigned)r / (unsigned)p.group);
+          const int64_t tok = done.s.q0 + tk;
+          const int head = done.h * p.group + r - tk * p.group;
+          if (!WX_IN_BOUNDS(p.err, tok >= 0 && tok < p.total_q && head >= 0 && head < p.hq && layer < p.layers)) continue;
+          const int64_t at = layer * (p.total_q * p.hq) + tok * p.hq + head;
+          if (g == 0) p.layer_ml[at] = make_float2(m[n][e], x);
+          if (done.steps == 0) continue;  // (nothing seen: the sums are not looked at)
+          float* dst = p.layer_o + at * HD;
+          constexpr float kB = kByteUnit<FMT>;
+#pragma unroll
+          for (int d = 0; d < HD / 8; d += 4)
+            *reinterpret_cast<float4*>(dst + column(d)) = make_float4(
+                acc[n][d >> 1][e] * kB, acc[n][d >> 1][2 + e] * kB, acc[n][(d >> 1) + 1][e] * kB, acc[n][(d >> 1) + 1][2 + e] * kB);
+        }
+      continue;
+    }
     // ---- join the warps
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -626,7 +666,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
       const int64_t tok = done.s.q0 + tk;
       const int head = done.h * p.group + r - tk * p.group;
       if (!WX_IN_BOUNDS(p.err, tok >= 0 && tok < p.total_q && head >= 0 && head < p.hq)) return;
-      if constexpr (KEYS == kPrefixKeys) {
+      if constexpr (kBehind) {
         const int64_t at = (done.b < front ? 0 : p.own_layer) * (p.total_q * p.hq) + tok * p.hq + head;
 #pragma unroll
         for (int i = 0; i < kPer; i += 4)
@@ -740,9 +780,35 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     }
     __syncthreads();  // the join buffer is free again
   }
+  if constexpr (kSolo) {
+    let_next_begin();
+    __syncwarp();
+    if (lane == 0 && atomicAdd(p.counters + 1, 1) == (int)gridDim.x * kWarps - 1) {
+      p.counters[0] = 0;  // nobody asks any more: ready for the next launch
+      p.counters[1] = 0;
+    }
+    wait_for_last();  // (the join is told of this kernel's end alone, and needs the shared walk's too)
+  }
 }
 
 // --------------------------------------------------------------------- host side
+// a launch that may begin before the kernel before it has ended (as soon as that lets it)
+template <class... P, class... A>
+static int launch_dependent(wx_ctx* ctx, void (*fn)(P...), unsigned grid, unsigned threads, size_t smem, A... args) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  WX_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...));
+  return WX_OK;
+}
+
 static int check_dims(wx_ctx* ctx, const wx_attn_dims* d, const void* q, int64_t q_stride, const void* out,
                       int64_t out_stride, const int32_t* cu_q) {
   WX_CHECK_ARG(ctx, ctx && d && d->total_q >= 0 && d->batch >= 0 && d->q_heads > 0 && d->kv_heads > 0);
@@ -785,15 +851,33 @@ static void fill_params(wx_ctx* ctx, const wx_attn_dims* d, const void* q, int64
 template <int FMT, int HD, int NT, int KEYS>
 static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   using G = RowsGeom<FMT, HD, NT>;
+  constexpr bool kSolo = KEYS == kChunkKeys, kBehind = KEYS >= kPrefixKeys;
   const int grid = std::min(ctx->num_sms, G::kWarps * (G::kPitch + 2) / 2);  // (an item's pieces: the join buffer)
-  const int64_t walks = KEYS == kPrefixKeys && p.shared ? 2 : 1;  // of each row
+  const int64_t walks = kBehind && p.shared ? 2 : 1;  // of each row
   const int64_t items = (int64_t)p.hkv * (walks * (p.total_q * p.group / G::kRows) + p.batch);
   // the line of units is counted in 32 bits (only block tables that repeat pages get near)
-  const int64_t most_keys = std::max<int64_t>(p.blocks_per_seq << p.page_shift, KEYS == kPrefixKeys ? p.prefix : 0);
-  if (p.block_table && items > UINT32_MAX / (most_keys / kUnit + 1))
-    return set_error(ctx, WX_ERR_UNSUPPORTED, "batch * kv_heads * blocks_per_seq too large (2^32 units of 128 keys)");
-  const size_t rows = (size_t)grid * 2 * G::kRows;
+  const int64_t most_keys = std::max<int64_t>(p.blocks_per_seq << p.page_shift, kBehind ? p.prefix : 0);
+  if (p.block_table && items > UINT32_MAX / (most_keys / (kSolo ? p.chunk : kUnit) + 1))
+    return set_error(ctx, WX_ERR_UNSUPPORTED, "batch * kv_heads * blocks_per_seq too large (2^32 units of %d keys)",
+                     kSolo ? p.chunk : kUnit);
   int st;
+  auto fn = text_rows_attn_kernel<FMT, HD, NT, KEYS>;
+  const int64_t bytes = G::kWide ? 1 : 2;
+  const auto *k = static_cast<const uint8_t*>(kv.k), *v = static_cast<const uint8_t*>(kv.v);
+  if constexpr (kSolo) {
+    // It may begin while the shared walk is at work, on the SMs that this leaves free: what it reads was there before.
+    // (counters of its own, beside the walk's)
+    if (!(p.counters = arrival_counters(ctx, 16, &st))) return st;
+    p.counters += 8;
+    constexpr int smem = G::kWarps * G::kStages * G::kStep;
+    if ((st = ensure_smem_attr(ctx, (const void*)fn, smem, "text_rows_attn"))) return st;
+    ProfScope prof(ctx, kProfAttn);
+    const int64_t ks = (int64_t)kv.k_stride * bytes, vs = (int64_t)kv.v_stride * bytes;
+    if (p.after_walk) st = launch_dependent(ctx, fn, grid, G::kThreads, smem, k, v, ks, vs, p, 1);
+    else fn<<<grid, G::kThreads, smem, ctx->stream>>>(k, v, ks, vs, p, 1);
+    return st ? st : launch_status(ctx, "text_rows_attn");
+  }
+  const size_t rows = (size_t)grid * 2 * G::kRows;
   Carve c{p.ws_reserved};
   const size_t o_part = c.take(rows * HD * 4), o_ml = c.take(rows * 8);
   uint8_t* ws = static_cast<uint8_t*>(workspace(ctx, c.off, &st));
@@ -802,12 +886,9 @@ static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   p.part_ml = reinterpret_cast<float*>(ws + o_ml);
   p.n_items = items;
   if (!(p.counters = arrival_counters(ctx, items, &st))) return st;
-  auto fn = text_rows_attn_kernel<FMT, HD, NT, KEYS>;
   if ((st = ensure_smem_attr(ctx, (const void*)fn, G::kSmem, "text_rows_attn"))) return st;
-  const int64_t bytes = G::kWide ? 1 : 2;
   ProfScope prof(ctx, kProfAttn);
-  fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(static_cast<const uint8_t*>(kv.k), static_cast<const uint8_t*>(kv.v),
-                                                   (int64_t)kv.k_stride * bytes, (int64_t)kv.v_stride * bytes, p, 2);
+  fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(k, v, (int64_t)kv.k_stride * bytes, (int64_t)kv.v_stride * bytes, p, 2);
   return launch_status(ctx, "text_rows_attn");
 }
 
@@ -855,74 +936,44 @@ static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParam
 //   M = max(m_P, m_S), out = (2^(m_P - M) o_P + 2^(m_S - M) o_S) / (2^(m_P - M) l_P + 2^(m_S - M) l_S).
 // The rows of all sequences walk the prefix together, so that its bytes are read once for up to 256 rows and
 // not once for each sequence; their own keys are walked as in any paged call. The parts' sums stay
-// in fp32 and are joined here, in the order of the keys. A warp a row.
+// in fp32 and are joined here, in the order of the keys.
 template <int HD>
-__global__ void __launch_bounds__(256) prefix_join_kernel(TextAttnParams p, int layers) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = p.total_q * p.hq;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t token = row / p.hq;
-  int b = 0;  // last sequence that begins at or before the token
-  for (int n = p.batch; n > 1;) {
-    const int half = n / 2;
-    if (p.cu_q[b + half] <= token) b += half;
-    n -= half;
-  }
-  if (token < p.cu_q[b] || token >= p.cu_q[b + 1]) return;
-  constexpr int kPer = HD / 32;
-  float o[kPer] = {};
-  float M = -INFINITY, L = 0.f;
-  for (int c = 0; c < layers; c += 32) {
-    const float2 ml = c + lane < layers ? p.layer_ml[(c + lane) * rows + row] : make_float2(-INFINITY, 0.f);
-    float m = ml.y != 0.f ? ml.x : -INFINITY;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    M = fmaxf(M, m);
-  }
-  for (int c = 0; c < layers; c += 4) {  // four layers' rows in flight
-    float x[4][kPer];
-    float2 ml[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int64_t at = min(c + q, layers - 1) * rows + row;
-      ml[q] = p.layer_ml[at];
-      const float* src = p.layer_o + at * HD + lane * kPer;
-      if constexpr (kPer == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(src);
-        x[q][0] = y.x, x[q][1] = y.y, x[q][2] = y.z, x[q][3] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(src);
-        x[q][0] = y.x, x[q][1] = y.y;
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (c + q >= layers || ml[q].y == 0.f) continue;  // (nothing seen: its sums may be anything)
-      const float f = exp2_approx(ml[q].x - M);
-      L += ml[q].y * f;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) o[e] += x[q][e] * f;
-    }
-  }
-  const float inv = L == 0.f ? 0.f : __fdividef(1.0f, L);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + token * p.out_stride + (row - token * p.hq) * HD + lane * kPer);
-#pragma unroll
-  for (int e = 0; e < kPer; e += 2) dst[e / 2] = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
-  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
+__global__ void __launch_bounds__(256) prefix_join_kernel(TextAttnParams p) {
+  int head;
+  const int64_t token = join_token(p, head);
+  const int b = seq_of_token(p, token);
+  const bool live = token < p.total_q && token >= p.cu_q[b] && token < p.cu_q[b + 1];
+  const int layers = p.own_layer + (p.chunk ? max(1, (load_seq(p, b).lk - 1) / p.chunk + 1) : 1);
+  wait_for_last();
+  if (!live) return;
+  const int64_t row0 = token * p.hq + head;
+  join_rows<HD>(p.layer_o, p.layer_ml, p.total_q * p.hq, row0, min(kJoinRows, p.hq - head), layers,
+                p.out + token * p.out_stride + (int64_t)head * HD, p.lse ? p.lse + row0 : nullptr);
 }
 
 // Few rows a sequence: the prefix is walked for all rows together, by the kernel for few rows where they are few
 // in all, else by the tcgen05 kernel. Many rows a sequence (new prompts) fill an item by themselves: each walks
 // the prefix and its own keys in one go, and nothing is joined.
+constexpr int kChunkLayers = 32, kChunkMost = 512;  // layers of own keys at most, keys of a chunk at most
 static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p, const KvSource& kv) {
   const int64_t few = kv.format == kKvBf16 ? 16 : kv.format == kKvE4m3 ? 32 : 48;
   const int64_t own = (int64_t)d->max_q * p.group, all = p.total_q * p.group;
   if (own > few) return text_flash(ctx, p, d->head_dim, kv, kPrefixKeys);
   const bool flash = p.prefix && all > few;
-  const int layers = (flash ? text_flash_layers(ctx, p) : p.prefix ? 1 : 0) + 1;
+  const bool both = p.prefix && !flash;  // the rows kernel walks the prefix too
+  // Own keys in chunks, of as many as give each warp two units (12 warps an SM) within kChunkLayers
+  // layers; where that takes long chunks (few long sequences) a piece per CTA divides them more evenly
+  const int64_t most = std::max<int64_t>(p.blocks_per_seq << p.page_shift, both ? p.prefix : 0);
+  const int64_t items = std::max<int64_t>(1, (int64_t)p.hkv * p.batch * ((own + 7) / 8));
+  const int64_t want = std::min<int64_t>(kChunkLayers, (24 * ctx->num_sms + items - 1) / items);
+  const int64_t chunk = std::max<int64_t>(64, ((most + want - 1) / want + 15) / 16 * 16);
+  p.chunk = chunk <= kChunkMost ? (int)chunk : 0;
+  auto parts = [&](int64_t keys) { return p.chunk ? (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk) : 1; };
+  p.own_layer = flash ? text_flash_layers(ctx, p) : both ? parts(p.prefix) : 0;
+  p.layers = p.own_layer + parts(p.blocks_per_seq << p.page_shift);
   const int64_t rows = p.total_q * p.hq;
   Carve c;
-  const size_t o_o = c.take((size_t)(layers * rows) * d->head_dim * 4), o_ml = c.take((size_t)(layers * rows) * 8);
+  const size_t o_o = c.take((size_t)(p.layers * rows) * d->head_dim * 4), o_ml = c.take((size_t)(p.layers * rows) * 8);
   p.ws_reserved = c.off;
   // what the kernels take for themselves is asked for now: a workspace that grew between them would lose the layers
   const size_t rows_ws = (size_t)ctx->num_sms * 2 * 16 * (d->head_dim * 4 + 8) + 512;
@@ -931,7 +982,6 @@ static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p
   if (!ws) return st;
   p.layer_o = reinterpret_cast<float*>(ws + o_o);
   p.layer_ml = reinterpret_cast<float2*>(ws + o_ml);
-  p.own_layer = layers - 1;
   if (flash) {
     TextAttnParams f = p;
     f.shared = 1;
@@ -939,16 +989,19 @@ static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p
     if ((st = text_flash(ctx, f, d->head_dim, kv, kPrefixKeys))) return st;
   }
   TextAttnParams r = p;
-  if (!flash && p.prefix) {
+  r.after_walk = flash;
+  if (both) {
     r.shared = 1;
     ++r.batch;
   }
-  if ((st = launch_rows_attn<kPrefixKeys>(ctx, d->head_dim, flash || !p.prefix ? own : all, r, kv))) return st;
+  st = p.chunk ? launch_rows_attn<kChunkKeys>(ctx, d->head_dim, both ? all : own, r, kv)
+               : launch_rows_attn<kPrefixKeys>(ctx, d->head_dim, both ? all : own, r, kv);
+  if (st) return st;
   ProfScope prof(ctx, kProfAttn);
-  const unsigned grid = (unsigned)((rows + 7) / 8);
-  if (d->head_dim == 128) prefix_join_kernel<128><<<grid, 256, 0, ctx->stream>>>(p, layers);
-  else prefix_join_kernel<64><<<grid, 256, 0, ctx->stream>>>(p, layers);
-  return launch_status(ctx, "prefix_join");
+  const unsigned grid = join_blocks(p);
+  st = d->head_dim == 128 ? launch_dependent(ctx, prefix_join_kernel<128>, grid, 256, 0, p)
+                          : launch_dependent(ctx, prefix_join_kernel<64>, grid, 256, 0, p);
+  return st ? st : launch_status(ctx, "prefix_join");
 }
 
 // checks of a call over the paged cache, and its parameters

@@ -11,8 +11,9 @@ namespace wx {
 
 // Which keys a row sees: those up to its place within the window (kPlainKeys), these and the
 // sequence's first `sinks` (kSinkKeys), or a prefix common to all sequences and then its own
-// sequence's up to its place (kPrefixKeys). The attention kernels are compiled for each.
-enum : int { kPlainKeys = 0, kSinkKeys = 1, kPrefixKeys = 2 };
+// sequence's up to its place (kPrefixKeys; kChunkKeys: the same in the rows kernel's form for short
+// sequences). The attention kernels are compiled for each.
+enum : int { kPlainKeys = 0, kSinkKeys = 1, kPrefixKeys = 2, kChunkKeys = 3 };
 
 struct TextAttnParams {
   const __nv_bfloat16* q;
@@ -40,8 +41,11 @@ struct TextAttnParams {
   int shared;  // text_flash: one walk over the prefix for the rows of all sequences (otherwise: each
                // sequence's items walk the prefix, then its own keys). Rows kernel: sequence 0 is that walk
   float* layer_o;     // sums of rows [layer][total_q * hq][hd], brought together by prefix_join_kernel
+  int layers;
   float2* layer_ml;   // their maxima (base 2) and denominators
-  int own_layer;      // rows kernel: of the sequences' own keys
+  int own_layer;      // rows kernel: of the sequences' own keys (kChunkKeys: of the first `chunk` of them)
+  int chunk;          // kChunkKeys: keys of a unit, a layer each; 0: one layer
+  int after_walk;     // kChunkKeys, host: launched right behind the shared walk by text_flash
   size_t ws_reserved; // bytes of the workspace in use before the kernel's own
   float sl2;  // scale * log2(e): scores and maxima are kept in base 2
   float* part;              // split items: [2 * gridDim][16][hd] sums, then [..][16] maxima and denominators
@@ -108,7 +112,7 @@ __device__ __forceinline__ int key_lo(const TextAttnParams& p, const Seq& s, int
 // (kPrefixKeys: of its own sequence; a key of the prefix goes by -1)
 template <int KEYS>
 __device__ __forceinline__ bool key_seen(const TextAttnParams& p, int j, int lo, int hi) {
-  if constexpr (KEYS == kPrefixKeys) return j < hi;
+  if constexpr (KEYS >= kPrefixKeys) return j < hi;
   return j < hi && (j >= lo || (KEYS == kSinkKeys && j < p.sinks));
 }
 // Between the first keys and the window lie keys that no row of an item (of a call, in the rows kernel)
@@ -211,10 +215,110 @@ __device__ __forceinline__ uint32_t lds_u16(uint32_t a) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
   return v;
 }
+// Dependent launches: a kernel lets the next one on its stream begin (where that was launched for it), and
+// waits for the one before to be complete and its memory visible.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+
+// ------------------------------------------------------------------ partial sums of rows, joined
+// Layer i of row r holds o = sum 2^(s - m) v at (i * rows + r), and (m, l) beside it (base 2; l 0: the layer's
+// keys are not seen, its sums may be anything). A warp joins kJoinRows neighbouring rows, in the order of the layers:
+//   M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
+// Bound by the layers' bytes, if enough of them are in flight: the rows of a warp belong to one token, so that
+// what is found out about its sequence serves them all, and eight rows' loads go out at once (a row a warp,
+// four in flight: 31 us for 33,852 rows of 3 layers; now JOIN_US).
+constexpr int kJoinRows = 4;
+template <int HD>
+__device__ __forceinline__ void join_rows(const float* o_base, const float2* ml_base, int64_t rows, int64_t row0, int n,
+                                          int layers, __nv_bfloat16* out, float* lse) {
+  constexpr int kPer = HD / 32;
+  const int lane = threadIdx.x & 31, mine = lane % kJoinRows;  // lane: layer c + lane / 4 of row row0 + mine
+  auto ml_of = [&](int c) {
+    const int i = c + lane / kJoinRows;
+    return i < layers && mine < n ? __ldcg(ml_base + i * rows + row0 + mine) : make_float2(-INFINITY, 0.f);
+  };
+  float M = -INFINITY, L = 0.f;
+  for (int c = 0; c < layers; c += 32 / kJoinRows) {
+    const float2 ml = ml_of(c);
+    M = fmaxf(M, ml.y != 0.f ? ml.x : -INFINITY);
+  }
+#pragma unroll
+  for (int d = kJoinRows; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  float o[kJoinRows][kPer] = {};
+  for (int c = 0; c < layers; c += 32 / kJoinRows) {
+    const float2 ml = ml_of(c);
+    const float f = ml.y != 0.f ? exp2_approx(ml.x - M) : 0.f;
+    const uint32_t seen = __ballot_sync(0xffffffffu, ml.y != 0.f);
+    if (ml.y != 0.f) L += ml.y * f;
+#pragma unroll 1
+    for (int i = 0; i < 32 / kJoinRows && c + i < layers; i += 2) {
+      float x[2][kJoinRows][kPer];
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int r = 0; r < kJoinRows; ++r) {
+          const float* src = o_base + (min(c + i + q, layers - 1) * rows + row0 + min(r, n - 1)) * HD + lane * kPer;
+          if constexpr (kPer == 4) {
+            const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+            x[q][r][0] = y.x, x[q][r][1] = y.y, x[q][r][2] = y.z, x[q][r][3] = y.w;
+          } else {
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+            x[q][r][0] = y.x, x[q][r][1] = y.y;
+          }
+        }
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int r = 0; r < kJoinRows; ++r) {
+          const int from = (i + q) * kJoinRows + r;
+          const float w = __shfl_sync(0xffffffffu, f, from);
+          if (seen >> from & 1u)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) o[r][e] += x[q][r][e] * w;
+        }
+    }
+  }
+#pragma unroll
+  for (int d = kJoinRows; d < 32; d <<= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+#pragma unroll
+  for (int r = 0; r < kJoinRows; ++r) {
+    const float l = __shfl_sync(0xffffffffu, L, r);
+    if (r >= n) break;
+    const float inv = l == 0.f ? 0.f : __fdividef(1.0f, l);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(out + r * HD + lane * kPer);
+    if constexpr (kPer == 4)
+      *reinterpret_cast<uint2*>(dst) =
+          make_uint2(pack_bf16x2(o[r][0] * inv, o[r][1] * inv), pack_bf16x2(o[r][2] * inv, o[r][3] * inv));
+    else dst[0] = pack_bf16x2(o[r][0] * inv, o[r][1] * inv);
+  }
+  if (lse && lane < n) lse[lane] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
+}
+// the warp's token and first head: a token's heads in groups of kJoinRows
+__device__ __forceinline__ int64_t join_token(const TextAttnParams& p, int& head) {
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int groups = (p.hq + kJoinRows - 1) / kJoinRows;
+  const int64_t token = at / groups;
+  head = (int)(at - token * groups) * kJoinRows;
+  return token;
+}
+inline unsigned join_blocks(const TextAttnParams& p) {
+  return (unsigned)((p.total_q * ((p.hq + kJoinRows - 1) / kJoinRows) + 7) / 8);
+}
+// last sequence that begins at or before a token
+__device__ __forceinline__ int seq_of_token(const TextAttnParams& p, int64_t token) {
+  int b = 0;
+  for (int n = p.batch; n > 1;) {
+    const int half = n / 2;
+    if (p.cu_q[b + half] <= token) b += half;
+    n -= half;
+  }
+  return b;
 }
 
 }  // namespace wx

@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
   TfItem* items = reinterpret_cast<TfItem*>(smem + G::kItemOff);
   static_assert(sizeof(TfItem) <= 128, "item slots");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (KEYS == kPrefixKeys && p.shared) let_next_begin();  // the walk over the sequences' own keys
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBTfCount; ++i) {
@@ -1173,46 +1174,55 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       const auto other = reinterpret_cast<__nv_bfloat16*>(
           __shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), 1));
       __nv_bfloat16 *even = lane & 1 ? other : row, *odd = lane & 1 ? row : other;
-#pragma unroll 1
-      for (int c = 0; c < HD / 16; ++c) {
-        float o[16];
+      // columns col.. of this row's sums, N of them. Non-finite values of V that the row does see are put
+      // back: infinities add up, both signs to NaN
+      auto sums = [&](int col, auto& o) {
+        constexpr int N = sizeof(o) / sizeof(float);
         if (any) {
-          tmem_ld16(tO + c * 16, o);
+          if constexpr (N == 32) tmem_ld32(tO + col, o);
+          else tmem_ld16(tO + col, o);
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = 0.f;
+          for (int i = 0; i < N; ++i) o[i] = 0.f;
         }
-        if (bad) {  // non-finite values of V that this row does see: infinities add up, both signs to NaN
-          const int col = c * 16;
-          uint32_t plus = 0u, minus = 0u;
-          const uint32_t* list =
-              tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
+        if (!bad) return;
+        uint32_t plus = 0u, minus = 0u;
+        const uint32_t* list =
+            tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
 #pragma unroll 1
-          for (int e = 0; e < min(bad, kTfBadRows); ++e) {
-            const uint32_t* entry = list + e * kTfBadWords;
-            const int key = (int)__ldcg(entry);
-            if (key_seen<KEYS>(p, key, lo, own_hi)) {
-              plus |= __ldcg(entry + 1 + (col >> 5)) >> (col & 31);
-              minus |= __ldcg(entry + 5 + (col >> 5)) >> (col & 31);
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (plus >> i & 1u) o[i] += INFINITY;
-            if (minus >> i & 1u) o[i] -= INFINITY;
+        for (int e = 0; e < min(bad, kTfBadRows); ++e) {
+          const uint32_t* entry = list + e * kTfBadWords;
+          const int key = (int)__ldcg(entry);
+          if (key_seen<KEYS>(p, key, lo, own_hi)) {
+            plus |= __ldcg(entry + 1 + (col >> 5)) >> (col & 31);
+            minus |= __ldcg(entry + 5 + (col >> 5)) >> (col & 31);
           }
         }
-        if (cut) {
-          if (write) {
-            float* dst = tp.part + at_part * HD + c * 16;
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
+        for (int i = 0; i < N; ++i) {
+          if (plus >> i & 1u) o[i] += INFINITY;
+          if (minus >> i & 1u) o[i] -= INFINITY;
+        }
+      };
+      if (cut) {  // whole lines of a row at a time
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          float o[32];
+          sums(c, o);
+          if (write) {
+            float* dst = tp.part + at_part * HD + c;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
               *reinterpret_cast<float4*>(dst + i) =
                   make_float4(o[i] * kByteUnit<FMT>, o[i + 1] * kByteUnit<FMT>, o[i + 2] * kByteUnit<FMT>, o[i + 3] * kByteUnit<FMT>);
           }
-          continue;
         }
+      }
+#pragma unroll 1
+      for (int c = 0; c < (cut ? 0 : HD / 16); ++c) {
+        float o[16];
+        sums(c * 16, o);
         uint4 w0 = make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
                               pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
         uint4 w1 = make_uint4(pack_bf16x2(o[8] * inv, o[9] * inv), pack_bf16x2(o[10] * inv, o[11] * inv),
@@ -1248,21 +1258,14 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
   }
 }
 
-// Rows of items that were cut up: sums of the pieces, in order, brought to one maximum. A warp a row.
+// Rows of items that were cut up: sums of the pieces, in order, brought to one maximum.
 template <int HD, int KEYS>
 __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   const TextAttnParams& p = tp.a;
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = p.total_q * p.hq;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t token = row / p.hq;
-  int b = 0;  // last sequence that begins at or before the token
-  for (int n = p.batch; n > 1;) {
-    const int half = n / 2;
-    if (p.cu_q[b + half] <= token) b += half;
-    n -= half;
-  }
-  const Seq s = load_seq(p, b);
+  int head;
+  const int64_t token = join_token(p, head);
+  if (token >= p.total_q) return;
+  const Seq s = load_seq(p, seq_of_token(p, token));
   const int64_t tok = token - s.q0;
   if (tok < 0 || tok >= s.lq) return;
   const int tok0 = (int)tok / (2 * tp.tt) * (2 * tp.tt);
@@ -1271,72 +1274,27 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   int first, last, pieces;
   cut_item(a, e, tp.splits, tp.min_tiles, first, last, pieces);
   if (pieces < 2) return;
-  constexpr int kPer = HD / 32;
-  float o[kPer] = {};
-  float M = -INFINITY, L = 0.f;
-  auto piece = [&](int i) { return i < pieces ? tp.part_ml[i * rows + row] : make_float2(-INFINITY, 0.f); };
-  for (int c = 0; c < pieces; c += 32) {
-    const float2 ml = piece(c + lane);
-    float m = ml.y != 0.f ? ml.x : -INFINITY;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    M = fmaxf(M, m);
-  }
-  for (int c = 0; c < pieces; c += 32) {
-    const float2 ml = piece(c + lane);
-    const float f = ml.y != 0.f ? exp2_approx(ml.x - M) : 0.f;
-    const uint32_t seen = __ballot_sync(0xffffffffu, ml.y != 0.f);
-    float l = ml.y != 0.f ? ml.y * f : 0.f;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-    L += l;
-    const int n = min(32, pieces - c);
-#pragma unroll 1
-    for (int i = 0; i < n; i += 8) {  // eight pieces' rows in flight
-      float x[8][kPer];
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float* src = tp.part + (min(c + i + q, pieces - 1) * rows + row) * HD + lane * kPer;
-        if constexpr (kPer == 4) {
-          const float4 y = *reinterpret_cast<const float4*>(src);
-          x[q][0] = y.x;
-          x[q][1] = y.y;
-          x[q][2] = y.z;
-          x[q][3] = y.w;
-        } else {
-          const float2 y = *reinterpret_cast<const float2*>(src);
-          x[q][0] = y.x;
-          x[q][1] = y.y;
-        }
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float w = __shfl_sync(0xffffffffu, f, (i + q) & 31);
-        if (i + q < n && (seen >> (i + q) & 1u))  // (nothing seen: its sums may be anything)
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) o[e] += x[q][e] * w;
-      }
-    }
-  }
-  const float inv = L == 0.f ? 0.f : __fdividef(1.0f, L);
-  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + token * p.out_stride + (row - token * p.hq) * HD + lane * kPer);
-#pragma unroll
-  for (int e = 0; e < kPer; e += 2) dst[e / 2] = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
-  if (p.lse && lane == 0) p.lse[row] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
+  const int64_t row0 = token * p.hq + head;
+  join_rows<HD>(tp.part, tp.part_ml, p.total_q * p.hq, row0, min(kJoinRows, p.hq - head), pieces,
+                p.out + token * p.out_stride + (int64_t)head * HD, p.lse ? p.lse + row0 : nullptr);
 }
 
 size_t text_flash_ws(wx_ctx* ctx) { return (size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4; }
 
-// Pieces of the shared walk: the fewest rounds over the SMs, of which each takes a piece's tiles and a
-// start and end worth some three; a layer that is written and read again costs what a tile does.
+// Pieces of the shared walk. A piece takes its tiles and a start and end worth some twelve (17 us, and 2 us a tile
+// at bf16, 3.3 on 8-bit caches); counted are its rounds over the SMs and, since the walk over the sequences' own
+// keys runs beside it on the SMs that it leaves, its share of all SMs' time. 64 rows x 4 over 8,011 bf16 keys (8
+// heads, own keys too): 3 pieces 67, 5: 50, 7: 45, 9: 43, 12: 46, 16: 52 us; 128 x 8 over 40,000 e4m3 keys: 3: 363,
+// 4: 298, 6: 374, 8: 300, 16: 318 us.
 int text_flash_layers(wx_ctx* ctx, const TextAttnParams& p) {
   const int64_t tt = 128 / p.group, items = p.hkv * ((p.total_q + 2 * tt - 1) / (2 * tt));
   int best = 1;
-  int64_t least = INT64_MAX;
+  double least = INFINITY;
   for (int n = 1; n <= std::min(p.front, 64); ++n) {
     const int per = (p.front + n - 1) / n;
     if ((p.front + per - 1) / per != n) continue;  // (a piece would be empty)
-    const int64_t cost = (items * n + ctx->num_sms - 1) / ctx->num_sms * (per + 3) + n;
+    const int64_t rounds = (items * n + ctx->num_sms - 1) / ctx->num_sms;
+    const double cost = (per + 12) * (rounds + (double)(items * n) / ctx->num_sms);
     if (cost < least) least = cost, best = n;
   }
   return best;
@@ -1382,7 +1340,7 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   ProfScope prof(ctx, kProfAttn);
   fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(tq, tk, tv, tp);
   if (tp.splits == 1 || p.shared) return launch_status(ctx, "text_flash");
-  text_flash_join_kernel<HD, KEYS><<<(unsigned)((p.total_q * p.hq + 7) / 8), 256, 0, ctx->stream>>>(tp);
+  text_flash_join_kernel<HD, KEYS><<<join_blocks(p), 256, 0, ctx->stream>>>(tp);
   return launch_status(ctx, "text_flash", 2);
 }
 

@@ -306,9 +306,13 @@ class PagePool(_Described):
             raise _invalid("tokens and first_position must be in 0..2^31 - 1")
         dev = _same_device(self.lens, new, new if keep is None else keep)
         desc = self._desc
-        pos, slots = new.new_empty(tokens), new.new_empty(tokens, dtype=torch.int64)
-        cu = new.new_empty(batch + 1)
-        lens, taken = (self.lens, self.taken) if commit else (torch.empty_like(self.lens), torch.empty_like(self.taken))
+        slots = new.new_empty(tokens, dtype=torch.int64)
+        # (one allocation, cut up: each is a microsecond and more)
+        if commit:
+            pos, cu = new.new_empty(tokens + batch + 1).split_with_sizes((tokens, batch + 1))
+            lens, taken = self.lens, self.taken
+        else:
+            pos, cu, lens, taken = new.new_empty(tokens + 2 * batch + 2).split_with_sizes((tokens, batch + 1, batch, 1))
         context(dev).call("wx_page_plan", desc, kept, add, tokens, first_position, pos.data_ptr(), slots.data_ptr(),
                           cu.data_ptr(), lens.data_ptr(), taken.data_ptr())
         return StepPlan(pos, slots, cu, lens, taken)
