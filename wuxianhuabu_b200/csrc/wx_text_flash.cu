@@ -29,6 +29,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "wx_text_dev.cuh"
@@ -679,31 +680,23 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       __syncwarp();
       return more;
     };
-    // Item n is announced while item n - 1 is at work (as soon as the slot of the one before is
-    // free), so that its loads and first products follow on without a gap; then the masked V
-    // tiles of item n - 1 are mended as they land.
-    bool more = true;
-    for (int next = 0; more; ++next) {
-      more = announce(next);
-      const int n = next - 1;
-      if (n < 0) continue;
+    // A masked weight is 0, but 0 * NaN is not: keys past the end are zeroed, and non-finite
+    // values elsewhere are zeroed and remembered for the rows that do see them.
+    int bad = 0;
+    auto mend = [&](int n, int from, int to) {
       const TfItem& cur = items[n % kTfItems];
       uint32_t* list =
           tp.bad_rows + ((int64_t)blockIdx.x * kTfItems + n % kTfItems) * (int64_t)kTfBadRows * kTfBadWords;
-      const int t0 = cur.first(), t1 = cur.last();
-      int bad = 0;
-      for (int t = t0; t < t1 && ok; ++t) {
+      for (int t = from; t < to && ok; ++t) {
         if (kW || !cur.masked<KEYS>(p, t)) continue;
         const int key0 = cur.key0<KEYS>(p, t), keys = cur.keys<KEYS>(p, t);
-        const uint32_t s = (nv + (uint32_t)(t - t0)) % kTfVStages;
+        const uint32_t s = (nv + (uint32_t)(t - cur.first())) % kTfVStages;
         uint32_t& done = s == 0 ? raw[0] : raw[1];
         if (!mbar_wait(bar(kBTfVRaw + s), done & 1, p.err, kDevTimeoutFull, abort_flag)) {
           ok = false;
           break;
         }
         ++done;
-        // A masked weight is 0, but 0 * NaN is not: keys past the end are zeroed, and non-finite
-        // values elsewhere are zeroed and remembered for the rows that do see them.
 #pragma unroll 1
         for (int r = lane; r < 128; r += 32) {
           const uint32_t row = sV(s) + (uint32_t)r * 128;
@@ -735,6 +728,21 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBTfVFull + s));
+      }
+    };
+    // Item n + 1 is announced while item n is at work (as soon as the slot of the one before is free), so
+    // that its loads and first products follow on without a gap. The masked V tiles of item n are mended as they
+    // land; the first ones, which land while the item before it ends, before the next item is looked for: behind that
+    // they held up a windowed item's second tile by 3 us (9001 + 1 + 5003 tokens, window 1024: WINDOW_US).
+    bool more = announce(0);
+    for (int n = 0; more; ++n) {
+      const TfItem& cur = items[n % kTfItems];
+      const int t0 = cur.first(), t1 = cur.last(), early = min(t1, t0 + kTfVStages);
+      bad = 0;
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {  // (one copy of the code: a second one cost long prompts 2 %)
+        mend(n, part ? early : t0, part ? t1 : early);
+        if (part == 0) more = announce(n + 1);
       }
       nv += (uint32_t)(t1 - t0);
     }
@@ -1325,6 +1333,16 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   if (KEYS == kPrefixKeys && p.shared) {
     tp.splits = text_flash_layers(ctx, p);
     tp.min_tiles = 1;
+  } else if (KEYS == kPrefixKeys) {
+    // Behind a prefix all items are long and much alike, so that whole rounds count: of the pieces, each with a
+    // start and end worth two tiles, and a join worth three. (148 items of 50 int8 tiles: whole 181 us, in 2, 3, 5
+    // pieces 208, 222, 247)
+    const double some = p.hkv * (p.total_q / (2.0 * tp.tt) + 0.5 * p.batch), tiles = p.front + (keys - p.front * 128) / 256.0;
+    double least = INFINITY;
+    for (int n = 1; n == 1 || (n <= 64 && n * kTfMinTiles <= tiles); ++n) {
+      const double cost = std::ceil(some * n / ctx->num_sms) * (tiles / n + 2) + (n > 1 ? 3 : 0);
+      if (cost < least) least = cost, tp.splits = n;
+    }
   }
   const int grid = (int)std::min<int64_t>(ctx->num_sms, items * tp.splits);
   const int64_t rows = tp.splits > 1 ? p.total_q * p.hq * tp.splits : 0;
