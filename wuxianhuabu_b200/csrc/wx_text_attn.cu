@@ -852,7 +852,8 @@ template <int FMT, int HD, int NT, int KEYS>
 static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   using G = RowsGeom<FMT, HD, NT>;
   constexpr bool kSolo = KEYS == kChunkKeys, kBehind = KEYS >= kPrefixKeys;
-  const int grid = std::min(ctx->num_sms, G::kWarps * (G::kPitch + 2) / 2);  // (an item's pieces: the join buffer)
+  // (an item's pieces: the join buffer)
+  const int grid = kSolo ? p.ctas : std::min(ctx->num_sms, G::kWarps * (G::kPitch + 2) / 2);
   const int64_t walks = kBehind && p.shared ? 2 : 1;  // of each row
   const int64_t items = (int64_t)p.hkv * (walks * (p.total_q * p.group / G::kRows) + p.batch);
   // the line of units is counted in 32 bits (only block tables that repeat pages get near)
@@ -937,18 +938,18 @@ static int dispatch_attn(wx_ctx* ctx, const wx_attn_dims* d, const TextAttnParam
 // The rows of all sequences walk the prefix together, so that its bytes are read once for up to 256 rows and
 // not once for each sequence; their own keys are walked as in any paged call. The parts' sums stay
 // in fp32 and are joined here, in the order of the keys.
-template <int HD>
+template <int HD, int R>
 __global__ void __launch_bounds__(256) prefix_join_kernel(TextAttnParams p) {
   int head;
-  const int64_t token = join_token(p, head);
+  const int64_t token = join_token<R>(p, head);
   const int b = seq_of_token(p, token);
   const bool live = token < p.total_q && token >= p.cu_q[b] && token < p.cu_q[b + 1];
   const int layers = p.own_layer + (p.chunk ? max(1, (load_seq(p, b).lk - 1) / p.chunk + 1) : 1);
   wait_for_last();
   if (!live) return;
   const int64_t row0 = token * p.hq + head;
-  join_rows<HD>(p.layer_o, p.layer_ml, p.total_q * p.hq, row0, min(kJoinRows, p.hq - head), layers,
-                p.out + token * p.out_stride + (int64_t)head * HD, p.lse ? p.lse + row0 : nullptr);
+  join_rows<HD, R>(p.layer_o, p.layer_ml, p.total_q * p.hq, row0, min(R, p.hq - head), layers,
+                   p.out + token * p.out_stride + (int64_t)head * HD, p.lse ? p.lse + row0 : nullptr);
 }
 
 // Few rows a sequence: the prefix is walked for all rows together, by the kernel for few rows where they are few
@@ -990,6 +991,13 @@ static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p
   }
   TextAttnParams r = p;
   r.after_walk = flash;
+  // Beside the shared walk there is a CTA for each SM that it leaves free, if those are a third: CTAs
+  // that begin behind it would find the work done, and hold the join up by their own start (3 us)
+  r.ctas = ctx->num_sms;
+  if (flash) {
+    const int64_t left = ctx->num_sms - text_flash_walk_ctas(p, p.own_layer);
+    if (3 * left >= ctx->num_sms) r.ctas = (int)left;
+  }
   if (both) {
     r.shared = 1;
     ++r.batch;
@@ -998,9 +1006,12 @@ static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p
                : launch_rows_attn<kPrefixKeys>(ctx, d->head_dim, both ? all : own, r, kv);
   if (st) return st;
   ProfScope prof(ctx, kProfAttn);
-  const unsigned grid = join_blocks(p);
-  st = d->head_dim == 128 ? launch_dependent(ctx, prefix_join_kernel<128>, grid, 256, 0, p)
-                          : launch_dependent(ctx, prefix_join_kernel<64>, grid, 256, 0, p);
+  if (join_by_fours(ctx, p))
+    st = d->head_dim == 128 ? launch_dependent(ctx, prefix_join_kernel<128, 4>, join_blocks(p, 4), 256, 0, p)
+                            : launch_dependent(ctx, prefix_join_kernel<64, 4>, join_blocks(p, 4), 256, 0, p);
+  else
+    st = d->head_dim == 128 ? launch_dependent(ctx, prefix_join_kernel<128, 1>, join_blocks(p, 1), 256, 0, p)
+                            : launch_dependent(ctx, prefix_join_kernel<64, 1>, join_blocks(p, 1), 256, 0, p);
   return st ? st : launch_status(ctx, "prefix_join");
 }
 

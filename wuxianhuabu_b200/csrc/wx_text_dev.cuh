@@ -45,6 +45,7 @@ struct TextAttnParams {
   float2* layer_ml;   // their maxima (base 2) and denominators
   int own_layer;      // rows kernel: of the sequences' own keys (kChunkKeys: of the first `chunk` of them)
   int chunk;          // kChunkKeys: keys of a unit, a layer each; 0: one layer
+  int ctas;           // kChunkKeys, host
   int after_walk;     // kChunkKeys, host: launched right behind the shared walk by text_flash
   size_t ws_reserved; // bytes of the workspace in use before the kernel's own
   float sl2;  // scale * log2(e): scores and maxima are kept in base 2
@@ -67,6 +68,7 @@ int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSourc
 // workspace that it takes beside layers, and the pieces (layers) of a shared walk over the prefix
 size_t text_flash_ws(wx_ctx* ctx);
 int text_flash_layers(wx_ctx* ctx, const TextAttnParams& p);
+int64_t text_flash_walk_ctas(const TextAttnParams& p, int layers);
 
 // One sequence as the kernels see it; lengths and offsets from the device are clamped to the
 // buffers, so that wrong ones give wrong rows and an error word but no access outside.
@@ -228,41 +230,41 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 // ------------------------------------------------------------------ partial sums of rows, joined
 // Layer i of row r holds o = sum 2^(s - m) v at (i * rows + r), and (m, l) beside it (base 2; l 0: the layer's
-// keys are not seen, its sums may be anything). A warp joins kJoinRows neighbouring rows, in the order of the layers:
+// keys are not seen, its sums may be anything). A warp joins R neighbouring rows, in the order of the layers:
 //   M = max m, out = sum 2^(m - M) o / sum 2^(m - M) l.
-// Bound by the layers' bytes, if enough of them are in flight: the rows of a warp belong to one token, so that
-// what is found out about its sequence serves them all, and eight rows' loads go out at once (a row a warp,
-// four in flight: 31 us for 33,852 rows of 3 layers; now JOIN_US).
-constexpr int kJoinRows = 4;
-template <int HD>
+// Bound by the layers' bytes, if enough of them are in flight: eight rows' loads go out at once, of eight layers where
+// rows are few (a row a warp; 2,048 rows of 13 layers 7 us with four rows, 3 with one) and of two layers where
+// there are many: the rows of a warp belong to one token, so that what is found out about its sequence serves
+// them all (a row a warp, four loads in flight: 31 us for 33,852 rows of 3 layers, 14 with four rows).
+template <int HD, int R>
 __device__ __forceinline__ void join_rows(const float* o_base, const float2* ml_base, int64_t rows, int64_t row0, int n,
                                           int layers, __nv_bfloat16* out, float* lse) {
-  constexpr int kPer = HD / 32;
-  const int lane = threadIdx.x & 31, mine = lane % kJoinRows;  // lane: layer c + lane / 4 of row row0 + mine
+  constexpr int kPer = HD / 32, kLayers = 8 / R;
+  const int lane = threadIdx.x & 31, mine = lane % R;  // lane: layer c + lane / R of row row0 + mine
   auto ml_of = [&](int c) {
-    const int i = c + lane / kJoinRows;
+    const int i = c + lane / R;
     return i < layers && mine < n ? __ldcg(ml_base + i * rows + row0 + mine) : make_float2(-INFINITY, 0.f);
   };
   float M = -INFINITY, L = 0.f;
-  for (int c = 0; c < layers; c += 32 / kJoinRows) {
+  for (int c = 0; c < layers; c += 32 / R) {
     const float2 ml = ml_of(c);
     M = fmaxf(M, ml.y != 0.f ? ml.x : -INFINITY);
   }
 #pragma unroll
-  for (int d = kJoinRows; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-  float o[kJoinRows][kPer] = {};
-  for (int c = 0; c < layers; c += 32 / kJoinRows) {
+  for (int d = R; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  float o[R][kPer] = {};
+  for (int c = 0; c < layers; c += 32 / R) {
     const float2 ml = ml_of(c);
     const float f = ml.y != 0.f ? exp2_approx(ml.x - M) : 0.f;
     const uint32_t seen = __ballot_sync(0xffffffffu, ml.y != 0.f);
     if (ml.y != 0.f) L += ml.y * f;
 #pragma unroll 1
-    for (int i = 0; i < 32 / kJoinRows && c + i < layers; i += 2) {
-      float x[2][kJoinRows][kPer];
+    for (int i = 0; i < 32 / R && c + i < layers; i += kLayers) {
+      float x[kLayers][R][kPer];
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
+      for (int q = 0; q < kLayers; ++q)
 #pragma unroll
-        for (int r = 0; r < kJoinRows; ++r) {
+        for (int r = 0; r < R; ++r) {
           const float* src = o_base + (min(c + i + q, layers - 1) * rows + row0 + min(r, n - 1)) * HD + lane * kPer;
           if constexpr (kPer == 4) {
             const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
@@ -273,10 +275,10 @@ __device__ __forceinline__ void join_rows(const float* o_base, const float2* ml_
           }
         }
 #pragma unroll
-      for (int q = 0; q < 2; ++q)
+      for (int q = 0; q < kLayers; ++q)
 #pragma unroll
-        for (int r = 0; r < kJoinRows; ++r) {
-          const int from = (i + q) * kJoinRows + r;
+        for (int r = 0; r < R; ++r) {
+          const int from = (i + q) * R + r;
           const float w = __shfl_sync(0xffffffffu, f, from);
           if (seen >> from & 1u)
 #pragma unroll
@@ -285,9 +287,9 @@ __device__ __forceinline__ void join_rows(const float* o_base, const float2* ml_
     }
   }
 #pragma unroll
-  for (int d = kJoinRows; d < 32; d <<= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+  for (int d = R; d < 32; d <<= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
 #pragma unroll
-  for (int r = 0; r < kJoinRows; ++r) {
+  for (int r = 0; r < R; ++r) {
     const float l = __shfl_sync(0xffffffffu, L, r);
     if (r >= n) break;
     const float inv = l == 0.f ? 0.f : __fdividef(1.0f, l);
@@ -299,17 +301,20 @@ __device__ __forceinline__ void join_rows(const float* o_base, const float2* ml_
   }
   if (lse && lane < n) lse[lane] = L == 0.f ? -INFINITY : (M + __log2f(L)) * 0.69314718055994531f;
 }
-// the warp's token and first head: a token's heads in groups of kJoinRows
+// the warp's token and first head: a token's heads in groups of R
+template <int R>
 __device__ __forceinline__ int64_t join_token(const TextAttnParams& p, int& head) {
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int groups = (p.hq + kJoinRows - 1) / kJoinRows;
+  const int groups = (p.hq + R - 1) / R;
   const int64_t token = at / groups;
-  head = (int)(at - token * groups) * kJoinRows;
+  head = (int)(at - token * groups) * R;
   return token;
 }
-inline unsigned join_blocks(const TextAttnParams& p) {
-  return (unsigned)((p.total_q * ((p.hq + kJoinRows - 1) / kJoinRows) + 7) / 8);
+inline unsigned join_blocks(const TextAttnParams& p, int R) {
+  return (unsigned)((p.total_q * ((p.hq + R - 1) / R) + 7) / 8);
 }
+// rows of a warp: four, where that leaves every SM sixteen warps
+inline bool join_by_fours(const wx_ctx* ctx, const TextAttnParams& p) { return p.total_q * p.hq >= (int64_t)ctx->num_sms * 64; }
 // last sequence that begins at or before a token
 __device__ __forceinline__ int seq_of_token(const TextAttnParams& p, int64_t token) {
   int b = 0;

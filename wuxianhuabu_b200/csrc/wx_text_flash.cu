@@ -1267,11 +1267,11 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 }
 
 // Rows of items that were cut up: sums of the pieces, in order, brought to one maximum.
-template <int HD, int KEYS>
+template <int HD, int KEYS, int R>
 __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   const TextAttnParams& p = tp.a;
   int head;
-  const int64_t token = join_token(p, head);
+  const int64_t token = join_token<R>(p, head);
   if (token >= p.total_q) return;
   const Seq s = load_seq(p, seq_of_token(p, token));
   const int64_t tok = token - s.q0;
@@ -1283,11 +1283,17 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   cut_item(a, e, tp.splits, tp.min_tiles, first, last, pieces);
   if (pieces < 2) return;
   const int64_t row0 = token * p.hq + head;
-  join_rows<HD>(tp.part, tp.part_ml, p.total_q * p.hq, row0, min(kJoinRows, p.hq - head), pieces,
-                p.out + token * p.out_stride + (int64_t)head * HD, p.lse ? p.lse + row0 : nullptr);
+  join_rows<HD, R>(tp.part, tp.part_ml, p.total_q * p.hq, row0, min(R, p.hq - head), pieces,
+                   p.out + token * p.out_stride + (int64_t)head * HD, p.lse ? p.lse + row0 : nullptr);
 }
 
 size_t text_flash_ws(wx_ctx* ctx) { return (size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4; }
+
+static int64_t walk_items(const TextAttnParams& p) {
+  const int64_t rows = 2 * (128 / p.group);
+  return p.hkv * ((p.total_q + rows - 1) / rows);
+}
+int64_t text_flash_walk_ctas(const TextAttnParams& p, int layers) { return walk_items(p) * layers; }
 
 // Pieces of the shared walk. A piece takes its tiles and a start and end worth some twelve (17 us, and 2 us a tile
 // at bf16, 3.3 on 8-bit caches); counted are its rounds over the SMs and, since the walk over the sequences' own
@@ -1295,7 +1301,7 @@ size_t text_flash_ws(wx_ctx* ctx) { return (size_t)ctx->num_sms * kTfItems * kTf
 // heads, own keys too): 3 pieces 67, 5: 50, 7: 45, 9: 43, 12: 46, 16: 52 us; 128 x 8 over 40,000 e4m3 keys: 3: 363,
 // 4: 298, 6: 374, 8: 300, 16: 318 us.
 int text_flash_layers(wx_ctx* ctx, const TextAttnParams& p) {
-  const int64_t tt = 128 / p.group, items = p.hkv * ((p.total_q + 2 * tt - 1) / (2 * tt));
+  const int64_t items = walk_items(p);
   int best = 1;
   double least = INFINITY;
   for (int n = 1; n <= std::min(p.front, 64); ++n) {
@@ -1322,7 +1328,8 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   }();
   if (!regs_ok) return set_error(ctx, WX_ERR_CUDA, "text_flash: register split does not fit");
   const TextAttnParams& p = tp.a;
-  const int64_t items = (int64_t)p.hkv * (p.total_q / (2 * tp.tt) + p.batch);
+  // (at most: each sequence's last item may be a part of one; the shared walk has one sequence)
+  const int64_t items = KEYS == kPrefixKeys && p.shared ? walk_items(p) : (int64_t)p.hkv * (p.total_q / (2 * tp.tt) + p.batch);
   // Too few items to level the SMs out are cut into pieces of their keys, as many as give kTfWaves
   // to an SM and as the longest range that a row can see allows.
   int64_t keys = p.block_table ? p.blocks_per_seq << p.page_shift : p.total_k;
@@ -1358,7 +1365,8 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   ProfScope prof(ctx, kProfAttn);
   fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(tq, tk, tv, tp);
   if (tp.splits == 1 || p.shared) return launch_status(ctx, "text_flash");
-  text_flash_join_kernel<HD, KEYS><<<join_blocks(p), 256, 0, ctx->stream>>>(tp);
+  if (join_by_fours(ctx, p)) text_flash_join_kernel<HD, KEYS, 4><<<join_blocks(p, 4), 256, 0, ctx->stream>>>(tp);
+  else text_flash_join_kernel<HD, KEYS, 1><<<join_blocks(p, 1), 256, 0, ctx->stream>>>(tp);
   return launch_status(ctx, "text_flash", 2);
 }
 
