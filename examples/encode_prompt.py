@@ -3,12 +3,15 @@ text model built from the quantised linears and the text-side operators, then th
 
     python examples/encode_prompt.py [--cache bf16|int8|e4m3] [--layers N] [--new N]
 
-1. Two prompts of different lengths go through the model packed into one batch: rope + cache write
-   in one launch, causal attention with grouped heads over the packed rows.
-2. Both are continued token by token (greedy), all sequences in one call: rope + cache write, then
+1. Two prompts of different lengths go through the model packed into one batch: a step's pages, slots and
+   positions are planned on the device, head norms + rope + cache write are one launch, and the rows attend
+   to one another, causal, with grouped heads.
+2. Both are continued token by token (greedy), all sequences in one call: the same, with
    attention over the paged cache. A prompt may also arrive in pieces (``chunks``): the same call
    with several tokens a sequence.
-3. The hidden states of a sequence, one row per token, are what ``H3TextRefiner`` takes.
+3. Prompts that begin with the same text stand behind one cached copy of it, which is walked once for
+   all of them.
+4. The hidden states of a sequence, one row per token, are what ``H3TextRefiner`` takes.
 """
 from __future__ import annotations
 
@@ -16,6 +19,7 @@ import argparse
 from dataclasses import dataclass
 from pathlib import Path
 import sys
+from typing import Optional
 
 import torch
 
@@ -53,6 +57,7 @@ class TextModel:
                             fc1=linear(2 * cfg.ffn, cfg.hidden), fc2=linear(cfg.hidden, cfg.ffn))
                        for _ in range(cfg.layers)]
         self.norm = ones
+        self.head_norm = torch.ones(cfg.head_dim, dtype=torch.bfloat16, device="cuda")  # (of q's and of k's heads)
         self.rope = text.RopeTable(cfg.head_dim, positions, base=10000.0)
 
     def forward(self, ids, positions, slots, caches, attend):
@@ -68,7 +73,8 @@ class TextModel:
             q = qkv[:, :inner].unflatten(1, (c.heads, c.head_dim))  # slices: no copies are made
             k = qkv[:, inner:inner + kv].unflatten(1, (c.kv_heads, c.head_dim))
             v = qkv[:, inner + kv:].unflatten(1, (c.kv_heads, c.head_dim))
-            q = caches[i].append_roped(q, k, v, slots, self.rope, positions)
+            q = caches[i].append_roped(q, k, v, slots, self.rope, positions, q_norm=self.head_norm,
+                                       k_norm=self.head_norm, eps=c.eps)
             o = attend(i, q, k, v)
             x = w["out"](o.flatten(1), h3.EPI_GATE_RESID, gate=gate, resid=x, rowmap=row0)
             y = w["fc1"](h3.rms_norm(x, self.norm, c.eps), h3.EPI_SWIGLU)
@@ -77,49 +83,53 @@ class TextModel:
 
 
 class Sequences:
-    """The cached state of a batch: pages of every layer, dealt out as the sequences grow."""
+    """The cached state of a batch: pages of every layer, dealt out as the sequences grow. ``common``: tokens
+    that every sequence begins with, cached once, before them."""
 
-    def __init__(self, model: TextModel, batch: int, max_tokens: int, page: int = 16, fmt: str = "bf16"):
+    def __init__(self, model: TextModel, batch: int, max_tokens: int, page: int = 16, fmt: str = "bf16",
+                 common: Optional[list[int]] = None):
         c = model.cfg
-        self.model, self.page, self.lens = model, page, [0] * batch
-        blocks = -(-max_tokens // page)
-        self.caches = [text.PagedKVCache(batch * blocks, page, c.kv_heads, c.head_dim, fmt) for _ in range(c.layers)]
-        # pages of the sequences interleave, as they would after some traffic
-        self.table = torch.arange(batch * blocks, dtype=torch.int32).view(blocks, batch).t().contiguous()
-        self.table_gpu = self.table.cuda()
+        self.model, self.common = model, len(common or ())
+        front, blocks = -(-self.common // page), -(-max_tokens // page)
+        pages = front + batch * blocks
+        self.caches = [text.PagedKVCache(pages, page, c.kv_heads, c.head_dim, fmt) for _ in range(c.layers)]
+        self.pool = text.PagePool(pages, page, batch, blocks)
+        if common:  # a sequence of its own, whose pages stay taken
+            first = Sequences.__new__(Sequences)
+            first.model, first.common, first.caches = model, 0, self.caches
+            first.pool = text.PagePool.from_tensors(page, self.pool.free, self.pool.taken, self.pool.lens.new_zeros(1),
+                                                    self.pool.table.new_zeros(1, front))
+            first.extend([common])
+            self.front = first.pool.table[0]
 
-    def _advance(self, ids: list[list[int]]):
-        pos, slots, cu = [], [], [0]
-        for b, seq in enumerate(ids):
-            for t in range(self.lens[b], self.lens[b] + len(seq)):
-                pos.append(t)
-                slots.append(int(self.table[b, t // self.page]) * self.page + t % self.page)
-            self.lens[b] += len(seq)
-            cu.append(cu[-1] + len(seq))
-        flat = [i for seq in ids for i in seq]
-        return (torch.tensor(flat, device="cuda"), torch.tensor(pos, dtype=torch.int32, device="cuda"),
-                torch.tensor(slots, dtype=torch.int64, device="cuda"), torch.tensor(cu, dtype=torch.int32, device="cuda"),
-                max(len(seq) for seq in ids))
+    def _step(self, ids: list[list[int]]):
+        new = torch.tensor([len(seq) for seq in ids], dtype=torch.int32, device="cuda")
+        flat = torch.tensor([i for seq in ids for i in seq], device="cuda")
+        return flat, self.pool.plan(new, flat.numel(), first_position=self.common), max(len(seq) for seq in ids)
 
     def prompts(self, ids: list[list[int]]) -> torch.Tensor:
         """Whole prompts, packed, into empty caches."""
-        tok, pos, slots, cu, longest = self._advance(ids)
+        tok, plan, longest = self._step(ids)
+        norm, eps = self.model.head_norm, self.model.cfg.eps
 
         def attend(i, q, k, v):
             # (the prompt attends to its own bf16 rows; only later tokens read the cache)
-            return text.prompt_attention(q, self.model.rope.apply(k, pos), v, cu, longest)
+            k = self.model.rope.apply(k, plan.positions, norm=norm, eps=eps)
+            return text.prompt_attention(q, k, v, plan.cu_seqlens, longest)
 
-        return self.model.forward(tok, pos, slots, self.caches, attend)
+        return self.model.forward(tok, plan.positions, plan.slots, self.caches, attend)
 
     def extend(self, ids: list[list[int]]) -> torch.Tensor:
         """Some more tokens of every sequence, attending to all that is cached."""
-        tok, pos, slots, cu, longest = self._advance(ids)
-        lens = torch.tensor(self.lens, dtype=torch.int32, device="cuda")
+        tok, plan, longest = self._step(ids)
 
         def attend(i, q, k, v):
-            return text.paged_attention(q, self.caches[i], cu, lens, self.table_gpu, longest)
+            if self.common:
+                return text.prefix_attention(q, self.caches[i], self.front, self.common, plan.cu_seqlens, plan.kv_lens,
+                                             self.pool.table, longest)
+            return text.paged_attention(q, self.caches[i], plan.cu_seqlens, plan.kv_lens, self.pool.table, longest)
 
-        return self.model.forward(tok, pos, slots, self.caches, attend)
+        return self.model.forward(tok, plan.positions, plan.slots, self.caches, attend)
 
 
 def refiner(cfg: TextConfig, seed: int = 2) -> h3.H3TextRefiner:
@@ -171,6 +181,13 @@ def main(argv=None) -> dict:
              for at in range(0, max(map(len, ids)), 32)]
     chunks = [torch.cat([p[b] for p in parts]) for b in range(len(ids))]
 
+    # the first 40 tokens of one prompt as the common beginning of three
+    common = prompts[0][:40]
+    ends = [prompts[0][40:], prompts[1], prompts[1][:5]]
+    behind = Sequences(model, 3, 128, fmt=a.cache, common=common)
+    shared = list(behind.extend(ends).split([len(e) for e in ends]))
+    apart = Sequences(model, 3, 128, fmt=a.cache).prompts([common + e for e in ends]).split([40 + len(e) for e in ends])
+
     def differ(x, y) -> float:
         return max(float((p.float() - q.float()).norm() / q.float().norm()) for p, q in zip(x, y))
 
@@ -178,10 +195,12 @@ def main(argv=None) -> dict:
     conditions = [refine(s) for s in grown]
     h3.context().check_device()
     result = dict(tokens=[len(i) for i in ids], stepwise=differ(grown, whole), chunked=differ(chunks, whole),
+                  shared=differ(shared, [x[40:] for x in apart]),
                   conditions=[tuple(c.shape) for c in conditions],
                   finite=all(bool(torch.isfinite(c.float()).all()) for c in conditions))
     print(f"cache {a.cache}: sequences of {result['tokens']} tokens; states token by token against one pass: "
-          f"{result['stepwise']:.4f}, in chunks: {result['chunked']:.4f}; conditions {result['conditions']}")
+          f"{result['stepwise']:.4f}, in chunks: {result['chunked']:.4f}, behind a common beginning: "
+          f"{result['shared']:.4f}; conditions {result['conditions']}")
     return result
 
 

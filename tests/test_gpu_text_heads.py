@@ -90,8 +90,8 @@ def test_apply_qk(i):
     both = torch.cat([q, k], 1)
     tab.apply_qk(both[:, :hq], both[:, hq:], pos, q_norm=qw, k_norm=kw, eps=eps, q_out=both[:, :hq], k_out=both[:, hq:])
     assert torch.equal(both[:, :hq], got[0]) and torch.equal(both[:, hq:], got[1])
-    if not norms:
-        assert torch.equal(tab.apply(q, pos), got[0])
+    assert torch.equal(tab.apply(q, pos, norm=qw, eps=eps), got[0])
+    assert torch.equal(tab.apply(k, pos, norm=kw, eps=eps, out=torch.empty_like(k)), got[1])
     _check_device()
 
 
@@ -251,6 +251,7 @@ def test_refusals():
                  lambda: tab.apply_qk(q, k, pos, q_norm=w[:32]), lambda: tab.apply_qk(q, k, pos, k_norm=w.float()),
                  lambda: tab.apply_qk(q, k, pos, q_norm=w, eps=0.0), lambda: tab.apply_qk(q, k, pos, q_norm=w, eps=math.nan),
                  lambda: tab.apply_qk(q, k, pos, q_norm=w.repeat(2)[4:68]),  # (not on a 16-byte boundary)
+                 lambda: tab.apply(q, pos, norm=w[:8]), lambda: tab.apply(q, pos, norm=w, eps=-1.0),
                  lambda: tab.apply_qk(q, k, pos, q_out=q[:4]), lambda: tab.apply_qk(q.cpu(), k, pos),
                  lambda: text.RopeTable(64, 30, axes=(0, 1)), lambda: text.RopeTable(64, 30, axes=[4] * 32),
                  lambda: text.RopeTable(64, 30, axes=[-1] * 32), lambda: text.RopeTable(64, 30, axes=())):

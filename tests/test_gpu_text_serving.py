@@ -280,6 +280,18 @@ def test_many_tokens_write_only_their_rows():
             assert torch.equal(a[other], b[other])
 
 
+def test_the_example_shares_a_beginning():
+    """Prompts behind one cached beginning give the states of the whole prompts, up to the roundings of bf16 between
+    the layers, which are made at the same places in both."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("encode_prompt_shared", ROOT / "examples" / "encode_prompt.py")
+    module = importlib.util.module_from_spec(spec)
+    sys.modules["encode_prompt_shared"] = module
+    spec.loader.exec_module(module)
+    r = module.main(["--new", "2"])
+    assert r["finite"] and r["shared"] < 0.02, r
+
+
 CHILD = r'''
 import sys
 import numpy as np

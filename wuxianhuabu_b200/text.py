@@ -225,14 +225,17 @@ class RopeTable(_Described):
                           eps, n, d, qo.data_ptr(), qos, ko.data_ptr(), kos)
         return qo, ko
 
-    def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """x [tokens, heads, head_dim] with token t turned by positions[t] (int32); ``out`` may be x."""
+    def apply(self, x: torch.Tensor, positions: torch.Tensor, out: Optional[torch.Tensor] = None,
+              norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+        """x [tokens, heads, head_dim] with token t turned by positions[t] (int32); ``out`` may be x. With
+        ``norm`` [head_dim] each head is normalised first, as in ``apply_qk``."""
         n, h, d, stride = _rows(x, "x")
-        if self.axes is not None:
+        if self.axes is not None or norm is not None:
+            weight = _head_norm(norm, d, "norm")
             at, axes = self._at(positions, n)
             o, ostride = _out_rows(x, n, h, d, out, "out must have x's shape")
-            context(_same_device(x, positions, o, self.cos)).call(
-                "wx_norm_rope_apply", self._desc, axes, at, x.data_ptr(), stride, h, None, None, 0, 0, None, 0.0, n, d,
+            context(_same_device(x, positions, o, self.cos, x if norm is None else norm)).call(
+                "wx_norm_rope_apply", self._desc, axes, at, x.data_ptr(), stride, h, weight, None, 0, 0, None, eps, n, d,
                 o.data_ptr(), ostride, None, 0)
             return o
         at = _need_ints(torch.int32, n, "positions", positions)
