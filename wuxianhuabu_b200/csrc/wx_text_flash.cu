@@ -80,7 +80,7 @@ struct TfItem {
   int free_hi, free_lo;  // tiles inside [free_lo, free_hi) are unmasked for every row
   int bad;               // V rows with non-finite values (8-bit: NaN codes) found in masked tiles
   int piece, pieces;     // this part of the item's key tiles, and how many it was cut into
-  KeyGap at;             // which tile of the sequence a tile of the walk is
+  KeyGap at;             // kSinkKeys: which key of the sequence a key of the walk is
   __device__ int lo(int X) const { return X ? b0 : a0; }
   __device__ int hi(int X) const { return X ? b1 : a1; }
   __device__ int first() const { return a1 <= a0 ? b0 : b1 <= b0 ? a0 : min(a0, b0); }
@@ -93,7 +93,7 @@ struct TfItem {
   }
   template <int KEYS>
   __device__ int key0(const TextAttnParams& p, int t) const {
-    if constexpr (KEYS == kSinkKeys) return at(t) * 128;
+    if constexpr (KEYS == kSinkKeys) return at(t * 128);
     if constexpr (KEYS == kPrefixKeys) return (t < p.front ? t : t - p.front) * 128;
     return t * 128;
   }
@@ -101,9 +101,15 @@ struct TfItem {
   __device__ int keys(const TextAttnParams& p, int t) const {
     return in_prefix<KEYS>(p, t) ? p.prefix : lk;
   }
+  // first keys in front, keys of the window behind them
+  template <int KEYS>
+  __device__ bool two_parts(int t) const {
+    return KEYS == kSinkKeys && t * 128 < at.first && t * 128 + 128 > at.first;
+  }
   template <int KEYS>
   __device__ bool masked(const TextAttnParams& p, int t) const {
     const int j = key0<KEYS>(p, t);
+    if (two_parts<KEYS>(t)) return true;
     if (in_prefix<KEYS>(p, t)) return j + 128 > p.prefix;
     return j + 128 > free_hi || (j < free_lo && (KEYS != kSinkKeys || j + 128 > p.sinks));
   }
@@ -274,20 +280,45 @@ __device__ __forceinline__ int2 slot_tiles(const TextAttnParams& p, const Seq& s
   return hi > lo ? make_int2(lo >> 7, (hi + 127) >> 7) : make_int2(0, 0);
 }
 // The key tiles of both slots of the item from tok0 on, in its walk. With first keys that stay visible both walk
-// from those through the window of the item's first row; with a prefix, from that through their own keys.
+// from those through the window of the item's first row. That is in whole tiles of the sequence, or, over packed
+// keys where it saves a tile, to 16 keys, the first keys sharing theirs with the window's first (32 / 8 heads of 128, 4
+// first keys, window 1024: 10 or 11 tiles become 9, 287 us 274; window 256: 80, 72). Where it saves none, a window
+// and items that are whole tiles would lose their edges' alignment. With a prefix, from that through their own keys.
 template <int KEYS>
 __device__ __forceinline__ KeyGap item_tiles(const TextAttnParams& p, const Seq& s, int tok0, int tt, int2& a, int2& b) {
+  if constexpr (KEYS == kSinkKeys) {
+    const int lo = key_lo(p, s, tok0);
+    auto gap_by = [&](int unit) {
+      const KeyGap u = key_gap<KEYS>(p, lo / unit, unit);
+      return KeyGap{u.first * unit, u.gap * unit};
+    };
+    KeyGap at = gap_by(128);
+    auto tiles = [&](int k0) {
+      const int k1 = min(s.lq, k0 + tt), hi = k0 < k1 ? key_hi(p, s, k1 - 1) : 0;
+      return make_int2(0, hi > 0 ? (hi - at.gap + 127) >> 7 : 0);
+    };
+    a = tiles(tok0);
+    b = tiles(tok0 + tt);
+    if (!p.block_table) {
+      const KeyGap whole = at;
+      const int2 a0 = a, b0 = b;
+      at = gap_by(16);
+      a = tiles(tok0);
+      b = tiles(tok0 + tt);
+      if (max(a.y, b.y) < max(a0.y, b0.y)) return at;
+      at = whole;
+      a = a0;
+      b = b0;
+    }
+    return at;
+  }
   a = slot_tiles(p, s, tok0, tt);
   b = slot_tiles(p, s, tok0 + tt, tt);
   if constexpr (KEYS == kPrefixKeys) {
     a = make_int2(0, tok0 < s.lq ? p.front + a.y : 0);
     b = make_int2(0, tok0 + tt < s.lq ? p.front + b.y : 0);
   }
-  if constexpr (KEYS != kSinkKeys) return KeyGap{0, 0};
-  const KeyGap at = key_gap<KEYS>(p, key_lo(p, s, tok0) >> 7, 128);
-  if (a.y > a.x) a = make_int2(0, a.y - at.gap);
-  if (b.y > b.x) b = make_int2(0, b.y - at.gap);
-  return at;
+  return KeyGap{0, 0};
 }
 // kPrefixKeys, shared: the rows of all sequences as one, with no keys but the prefix's
 template <int KEYS>
@@ -305,7 +336,8 @@ __device__ __forceinline__ void cut_item(int2 a, int2 b, int splits, int min_til
 template <int FMT, int HD, int KEYS>
 __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     text_flash_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, TfParams tp) {
+                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmK16,
+                      const __grid_constant__ CUtensorMap tmV16, TfParams tp) {
   using G = TfGeom<FMT, HD>;
   constexpr bool kW = G::kWide;
   constexpr int kTile = G::kTile, kKStages = G::kKStages;
@@ -456,7 +488,12 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           if (!is_k) mbar_arrive(bar(kBTfVFull + s));
         }
         __syncwarp();
-        if (!p.block_table) {
+        if (!p.block_table && it.two_parts<KEYS>(t)) {  // in boxes of 16 rows
+          const int bx = lane / G::kChunks, ch = lane % G::kChunks;
+          if (bx < 8)
+            tma_load_2d(dst + ch * kTfChunk + bx * 2048, is_k ? &tmK16 : &tmV16, full, it.h * HD + ch * 64,
+                        it.k0 + it.at(t * 128 + bx * 16));
+        } else if (!p.block_table) {
           if (lane < G::kChunks) tma_load_2d(dst + lane * kTfChunk, tm, full, it.h * HD + lane * 64, it.k0 + key0);
         } else {
           const int bx = lane / G::kChunks, ch = lane % G::kChunks;
@@ -690,6 +727,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
       for (int t = from; t < to && ok; ++t) {
         if (kW || !cur.masked<KEYS>(p, t)) continue;
         const int key0 = cur.key0<KEYS>(p, t), keys = cur.keys<KEYS>(p, t);
+        auto key_of = [&](int r) { return KEYS == kSinkKeys ? cur.at(t * 128 + r) : key0 + r; };
         const uint32_t s = (nv + (uint32_t)(t - cur.first())) % kTfVStages;
         uint32_t& done = s == 0 ? raw[0] : raw[1];
         if (!mbar_wait(bar(kBTfVRaw + s), done & 1, p.err, kDevTimeoutFull, abort_flag)) {
@@ -700,7 +738,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
 #pragma unroll 1
         for (int r = lane; r < 128; r += 32) {
           const uint32_t row = sV(s) + (uint32_t)r * 128;
-          const bool past = key0 + r >= keys;
+          const bool past = key_of(r) >= keys;
           __nv_bfloat162 probe = __floats2bfloat162_rn(0.f, 0.f);
           const __nv_bfloat162 zero = probe;
 #pragma unroll 4
@@ -718,7 +756,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           const uint32_t who = __ballot_sync(0xffffffffu, odd);
           if (odd) {
             const int slot = bad + __popc(who & ((1u << lane) - 1u));
-            remember_row<HD>(row, r, cur.in_prefix<KEYS>(p, t) ? -1 : key0 + r, slot < kTfBadRows ? list + slot * kTfBadWords : nullptr);
+            remember_row<HD>(row, r, cur.in_prefix<KEYS>(p, t) ? -1 : key_of(r), slot < kTfBadRows ? list + slot * kTfBadWords : nullptr);
           }
           bad += __popc(who);
           __syncwarp();
@@ -1033,6 +1071,10 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           pass_turn();
           continue;
         }
+        // (looked up before S is there, not between it and its maxima)
+        const bool masked = it.masked<KEYS>(p, t), split = it.two_parts<KEYS>(t);
+        const int key0 = it.key0<KEYS>(p, t);
+        const int hi = it.in_prefix<KEYS>(p, t) ? p.prefix : own_hi;
         if (!mbar_wait(bar(kBTfSFull + X), (mine + (uint32_t)(t - a0)) & 1, p.err, kDevTimeoutSoftmax, abort_flag)) {
           ok = false;
           break;
@@ -1044,9 +1086,6 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           if (c.valid) load_q(c);
           q_sent = true;
         }
-        const bool masked = it.masked<KEYS>(p, t);
-        const int key0 = it.key0<KEYS>(p, t);
-        const int hi = it.in_prefix<KEYS>(p, t) ? p.prefix : own_hi;
         if constexpr (kW) {
           const uint32_t g = both + (uint32_t)(t - t0);
           if (!frag_tile(g, key0 >> 7, t == a0, masked, hi, lo, m4, l4)) {
@@ -1055,16 +1094,23 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
           }
           continue;
         }
-        const int lim = hi - key0, from = lo - key0;
-        // bits of the keys 32 c .. 32 c + 31 that this row sees
-        auto keep_bits = [&](int c) -> uint32_t {
-          const int a = min(32, max(0, lim - c * 32)), b = min(32, max(0, from - c * 32));
+        // bits of the keys 32 c .. 32 c + 31 that this row sees, the tile's first key being key0
+        auto bits_from = [&](int key0, int c) -> uint32_t {
+          const int a = min(32, max(0, hi - key0 - c * 32)), b = min(32, max(0, lo - key0 - c * 32));
           uint32_t hidden = b == 32 ? ~0u : (1u << b) - 1u;
           if constexpr (KEYS == kSinkKeys) {
             const int n = min(32, max(0, p.sinks - key0 - c * 32));
             hidden &= ~(n == 32 ? ~0u : (1u << n) - 1u);
           }
           return (a == 32 ? ~0u : (1u << a) - 1u) & ~hidden;
+        };
+        auto keep_bits = [&](int c) -> uint32_t {
+          if (split) {
+            const int n = it.at.first - t * 128 - c * 32;  // first keys among them
+            const uint32_t front = n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u;
+            return (bits_from(t * 128, c) & front) | (bits_from(t * 128 + it.at.gap, c) & ~front);
+          }
+          return bits_from(key0, c);
         };
         if (masked) {
           // a short loop over S in TMEM: few tiles are masked, and unrolled over 128 registers this
@@ -1288,6 +1334,10 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
                    p.out + token * p.out_stride + (int64_t)head * HD, p.lse ? p.lse + row0 : nullptr);
 }
 
+struct TfMaps {
+  CUtensorMap q, k, v, k16, v16;  // (k16, v16: boxes of 16 rows, for first keys beside a window over packed keys)
+};
+
 size_t text_flash_ws(wx_ctx* ctx) { return (size_t)ctx->num_sms * kTfItems * kTfBadRows * kTfBadWords * 4; }
 
 static int64_t walk_items(const TextAttnParams& p) {
@@ -1316,7 +1366,7 @@ int text_flash_layers(wx_ctx* ctx, const TextAttnParams& p) {
 }
 
 template <int FMT, int HD, int KEYS>
-static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, TfParams& tp) {
+static int launch_flash(wx_ctx* ctx, const TfMaps& maps, TfParams& tp) {
   using G = TfGeom<FMT, HD>;
   auto fn = text_flash_kernel<FMT, HD, KEYS>;
   int st = ensure_smem_attr(ctx, (const void*)fn, G::kSmem, "text_flash");
@@ -1364,7 +1414,7 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
   tp.part_ml = p.shared ? p.layer_ml : reinterpret_cast<float2*>(ws + o_ml);
   if (!(tp.next = arrival_counters(ctx, 2, &st))) return st;
   ProfScope prof(ctx, kProfAttn);
-  fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(tq, tk, tv, tp);
+  fn<<<grid, G::kThreads, G::kSmem, ctx->stream>>>(maps.q, maps.k, maps.v, maps.k16, maps.v16, tp);
   if (tp.splits == 1 || p.shared) return launch_status(ctx, "text_flash");
   if (join_by_fours(ctx, p)) text_flash_join_kernel<HD, KEYS, 4><<<join_blocks(p, 4), 256, 0, ctx->stream>>>(tp);
   else text_flash_join_kernel<HD, KEYS, 1><<<join_blocks(p, 1), 256, 0, ctx->stream>>>(tp);
@@ -1372,14 +1422,13 @@ static int launch_flash(wx_ctx* ctx, const CUtensorMap& tq, const CUtensorMap& t
 }
 
 template <int KEYS>
-static int launch_flash(wx_ctx* ctx, int format, int head_dim, const CUtensorMap& tq, const CUtensorMap& tk,
-                        const CUtensorMap& tv, TfParams& tp) {
+static int launch_flash(wx_ctx* ctx, int format, int head_dim, const TfMaps& maps, TfParams& tp) {
   const bool big = head_dim == 128;
   if (format == kKvInt8)
-    return big ? launch_flash<kKvInt8, 128, KEYS>(ctx, tq, tk, tv, tp) : launch_flash<kKvInt8, 64, KEYS>(ctx, tq, tk, tv, tp);
+    return big ? launch_flash<kKvInt8, 128, KEYS>(ctx, maps, tp) : launch_flash<kKvInt8, 64, KEYS>(ctx, maps, tp);
   if (format == kKvE4m3)
-    return big ? launch_flash<kKvE4m3, 128, KEYS>(ctx, tq, tk, tv, tp) : launch_flash<kKvE4m3, 64, KEYS>(ctx, tq, tk, tv, tp);
-  return big ? launch_flash<kKvBf16, 128, KEYS>(ctx, tq, tk, tv, tp) : launch_flash<kKvBf16, 64, KEYS>(ctx, tq, tk, tv, tp);
+    return big ? launch_flash<kKvE4m3, 128, KEYS>(ctx, maps, tp) : launch_flash<kKvE4m3, 64, KEYS>(ctx, maps, tp);
+  return big ? launch_flash<kKvBf16, 128, KEYS>(ctx, maps, tp) : launch_flash<kKvBf16, 64, KEYS>(ctx, maps, tp);
 }
 
 int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSource& kv, int keys) {
@@ -1387,24 +1436,30 @@ int text_flash(wx_ctx* ctx, const TextAttnParams& p, int head_dim, const KvSourc
   tp.a = p;
   tp.box = p.block_table ? std::min(128, 1 << p.page_shift) : 128;
   tp.tt = 128 / p.group;
-  CUtensorMap tq, tk, tv;
+  TfMaps maps;
   int st;
   const uint64_t dims[3] = {(uint64_t)head_dim, (uint64_t)p.hq, (uint64_t)p.total_q};
   const uint64_t ld[2] = {(uint64_t)head_dim, (uint64_t)p.q_stride};
   const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)tp.tt};
-  if ((st = make_tmap_bf16_3d(ctx, &tq, p.q, dims, ld, box))) return st;
+  if ((st = make_tmap_bf16_3d(ctx, &maps.q, p.q, dims, ld, box))) return st;
   if (kv.format != kKvBf16) {  // raw rows by untiled copies: the maps of K and V are not used
     tp.box = std::min(64, 1 << p.page_shift);
     tp.k8 = static_cast<const uint8_t*>(kv.k);
     tp.v8 = static_cast<const uint8_t*>(kv.v);
-    tk = tv = tq;
+    maps.k = maps.v = maps.q;
   } else {
-    if ((st = make_tmap_bf16_2d(ctx, &tk, kv.k, kv.rows, kv.cols, kv.k_stride, 64, tp.box))) return st;
-    if ((st = make_tmap_bf16_2d(ctx, &tv, kv.v, kv.rows, kv.cols, kv.v_stride, 64, tp.box))) return st;
+    if ((st = make_tmap_bf16_2d(ctx, &maps.k, kv.k, kv.rows, kv.cols, kv.k_stride, 64, tp.box))) return st;
+    if ((st = make_tmap_bf16_2d(ctx, &maps.v, kv.v, kv.rows, kv.cols, kv.v_stride, 64, tp.box))) return st;
   }
-  if (keys == kPrefixKeys) return launch_flash<kPrefixKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp);
-  return keys == kSinkKeys ? launch_flash<kSinkKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp)
-                           : launch_flash<kPlainKeys>(ctx, kv.format, head_dim, tq, tk, tv, tp);
+  maps.k16 = maps.k;
+  maps.v16 = maps.v;
+  if (keys == kSinkKeys && !p.block_table) {
+    if ((st = make_tmap_bf16_2d(ctx, &maps.k16, kv.k, kv.rows, kv.cols, kv.k_stride, 64, 16))) return st;
+    if ((st = make_tmap_bf16_2d(ctx, &maps.v16, kv.v, kv.rows, kv.cols, kv.v_stride, 64, 16))) return st;
+  }
+  if (keys == kPrefixKeys) return launch_flash<kPrefixKeys>(ctx, kv.format, head_dim, maps, tp);
+  return keys == kSinkKeys ? launch_flash<kSinkKeys>(ctx, kv.format, head_dim, maps, tp)
+                           : launch_flash<kPlainKeys>(ctx, kv.format, head_dim, maps, tp);
 }
 
 }  // namespace wx
