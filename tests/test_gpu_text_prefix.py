@@ -56,6 +56,10 @@ CASES = [  # prefix, q_lens, kv_lens, q heads, kv heads, head_dim, page
     (9000, [70], [70], 4, 1, 128, 64),                      # few items: pieces
     (5000, [2] * 3, [1000, 2, 30], 40, 2, 64, 64),
     (300, [1] * 9, [20] * 9, 64, 1, 128, 32),
+    (200, [1] * 5, [1, 90, 17, 0, 300], 128, 1, 64, 64),                # as many query heads to a K/V head as there may be
+    (513, [1] * 70, [5000 if i == 33 else 3 for i in range(70)], 8, 4, 128, 64),  # one long among short: longer chunks
+    (900, [1] * 300, [1 + 7 * i % 200 for i in range(300)], 4, 4, 64, 16),       # fewer, longer chunks
+    (3000, [1, 1], [40, 3000], 4, 1, 128, 16),                          # few items, long: a piece per CTA
 ]
 
 
@@ -142,6 +146,19 @@ def test_what_stands_behind_the_prefix_s_end_is_not_seen(q_lens, fmt):
     assert torch.isnan(again[:, 2:][..., hurt]).all() and torch.equal(again[:, :2], out[:, :2])
     again[:, 2:] = torch.where(hurt, out[:, 2:], again[:, 2:])  # (the other columns, summed another way, stand)
     _check(again, lse2, q, q_lens, ks, vs)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8"])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1] * 40, [1 + 9 * i for i in range(40)]), ([1, 2], [30, 5]),
+                                            ([100, 7], [100, 90])])
+def test_tables_far_wider_than_the_lengths(q_lens, kv_lens, fmt):
+    text = _text()
+    cache, front, table, q, ks, vs = _behind(_gen(77), fmt, 800, q_lens, kv_lens, 8, 2, 128, 16)
+    wide = torch.full((len(q_lens), 9000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    out, lse = text.prefix_attention(q, cache, front, 800, _cu(q_lens), _i32(kv_lens), wide, max(q_lens), return_lse=True)
+    _check_device()
+    _check(out, lse, q, q_lens, ks, vs)
 
 
 def test_rows_behind_the_last_sequence_are_left():

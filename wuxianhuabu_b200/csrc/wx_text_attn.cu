@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     k16 = key_lo(p, s, 0) & ~15;
     items = ((unsigned)(s.lq * p.group) + kRows - 1) / kRows * (unsigned)p.hkv;
     const int skip = KEYS == kSinkKeys ? key_gap<KEYS>(p, k16 >> 4, 16).gap << 4 : k16;
-    nu = kSolo ? (unsigned)max(1, (s.lk - 1) / p.chunk + 1) : (unsigned)max(1, (s.lk - skip + kUnit - 1) / kUnit);
+    nu = kSolo ? (unsigned)chunks_of(p.chunk, p.chunks, s.lk) : (unsigned)max(1, (s.lk - skip + kUnit - 1) / kUnit);
   };
   unsigned my_items = 0, my_nu = 0;  // of sequence loaded + lane
   int my_k16 = 0, loaded = -1;
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     const unsigned units = kSolo ? 1 : min(c.nu - u_in, u_end - at);
     c.u_in = u_in;
     c.at16 = key_gap<KEYS>(p, k16 >> 4, 16);
-    const int unit = kSolo ? p.chunk : kUnit;
+    const int unit = kSolo ? chunk_of(p.chunk, p.chunks, c.s.lk) : kUnit;
     c.k_lo = (KEYS == kSinkKeys ? 0 : k16) + (int)u_in * unit;
     c.k_hi = min(c.s.lk - (c.at16.gap << 4), c.k_lo + (int)units * unit);
     const int n16 = max(0, (c.k_hi - c.k_lo + 15) / 16);
@@ -237,7 +237,10 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
   const bool paged = kW || p.block_table;
   [[maybe_unused]] const int64_t kv_rows = paged ? (p.pages * p.hkv) << p.page_shift : p.total_k;
   int page_of = 0;
-  auto step_key = [&](const Piece& c, int i) { return c.k_lo + (kSolo ? i : i * kWarps + warp) * 16; };
+  // (without a sign: steps that a piece near 2^31 keys does not have may lie beyond)
+  auto step_key = [&](const Piece& c, int i) {
+    return (int)((unsigned)c.k_lo + (unsigned)(kSolo ? i : i * kWarps + warp) * 16u);
+  };
   auto first_key = [&](const Piece& c, int i) {
     const int j = step_key(c, i);
     return KEYS == kSinkKeys ? c.at16(j >> 4) << 4 : j;
@@ -249,7 +252,7 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
     if ((i & 31) == 0) {
       const int jl = first_key(c, i + lane);
       page_of = 0;
-      if (step_key(c, i + lane) < c.k_hi) {
+      if ((unsigned)step_key(c, i + lane) < (unsigned)c.k_hi) {
         page_of = blocks_of(c.b)[jl >> p.page_shift];
         if (page_of < 0 || page_of >= p.pages) {
           set_dev_error(p.err, kDevBadArgs);
@@ -846,6 +849,7 @@ static void fill_params(wx_ctx* ctx, const wx_attn_dims* d, const void* q, int64
   p.causal = d->causal != 0;
   p.window = d->window;
   p.sl2 = (float)((double)d->scale * 1.4426950408889634);
+  p.max_q = d->max_q;
   p.err = ctx->dev_err;
 }
 
@@ -859,9 +863,8 @@ static int launch_rows_attn(wx_ctx* ctx, TextAttnParams p, const KvSource& kv) {
   const int64_t items = (int64_t)p.hkv * (walks * (p.total_q * p.group / G::kRows) + p.batch);
   // the line of units is counted in 32 bits (only block tables that repeat pages get near)
   const int64_t most_keys = std::max<int64_t>(p.blocks_per_seq << p.page_shift, kBehind ? p.prefix : 0);
-  if (p.block_table && items > UINT32_MAX / (most_keys / (kSolo ? p.chunk : kUnit) + 1))
-    return set_error(ctx, WX_ERR_UNSUPPORTED, "batch * kv_heads * blocks_per_seq too large (2^32 units of %d keys)",
-                     kSolo ? p.chunk : kUnit);
+  if (p.block_table && items > UINT32_MAX / (kSolo ? p.chunks : most_keys / kUnit + 1))
+    return set_error(ctx, WX_ERR_UNSUPPORTED, "batch * kv_heads * blocks_per_seq too large (2^32 units of 128 keys)");
   int st;
   auto fn = text_rows_attn_kernel<FMT, HD, NT, KEYS>;
   const int64_t bytes = G::kWide ? 1 : 2;
@@ -945,7 +948,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(TextAttnParams p) {
   const int64_t token = join_token<R>(p, head);
   const int b = seq_of_token(p, token);
   const bool live = token < p.total_q && token >= p.cu_q[b] && token < p.cu_q[b + 1];
-  const int layers = p.own_layer + (p.chunk ? max(1, (load_seq(p, b).lk - 1) / p.chunk + 1) : 1);
+  const int layers = p.own_layer + (p.chunk ? chunks_of(p.chunk, p.chunks, load_seq(p, b).lk) : 1);
   wait_for_last();
   if (!live) return;
   const int64_t row0 = token * p.hq + head;
@@ -957,21 +960,27 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(TextAttnParams p) {
 // in all or the prefix is short, else by the tcgen05 kernel (64 rows over 2,000 bf16 keys, 8 heads, 17.2 us against
 // 20.7, over 20,000 80 against 45; 100 rows over 1,000 e4m3 keys, 16 heads of 64, 33 against 26). Many rows a sequence
 // (new prompts) fill an item by themselves: each walks the prefix and its own keys in one go.
-constexpr int kChunkLayers = 32, kChunkMost = 512;  // layers of own keys at most, keys of a chunk at most
 static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p, const KvSource& kv) {
   const int64_t few = kv.format == kKvBf16 ? 16 : kv.format == kKvE4m3 ? 32 : 48;
   const int64_t own = (int64_t)d->max_q * p.group, all = p.total_q * p.group;
   if (own > few) return text_flash(ctx, p, d->head_dim, kv, kPrefixKeys);
   const bool flash = p.prefix && all > few && (all + 15) / 16 * p.prefix * p.hkv > 65536;
   const bool both = p.prefix && !flash;  // the rows kernel walks the prefix too
-  // Own keys in chunks, of as many as give each warp two units (12 warps an SM) within kChunkLayers
-  // layers; where that takes long chunks (few long sequences) a piece per CTA divides them more evenly
+  // Own keys in chunks for single warps: of 128 keys, or 64 where there are few items (64 sequences of 1 to 701 bf16
+  // keys: 64 43, 128 41, 256 48 us in all; three sequences behind 333 keys, 16 heads of 64: 64 9.2, 128 10.5), and of
+  // more where that would be more than so many chunks a sequence: each is a layer, for which room is set aside, and
+  // the more items there are, the fewer chunks give each warp its share. What lengths there are is known on
+  // the device only, the tables' width being their bound; items that are too few to give every warp a unit
+  // although their keys may be many are left to a piece per CTA, which divides them evenly.
   const int64_t most = std::max<int64_t>(p.blocks_per_seq << p.page_shift, both ? p.prefix : 0);
-  const int64_t items = std::max<int64_t>(1, (int64_t)p.hkv * p.batch * ((own + 7) / 8));
-  const int64_t want = std::min<int64_t>(kChunkLayers, (24 * ctx->num_sms + items - 1) / items);
-  const int64_t chunk = std::max<int64_t>(64, ((most + want - 1) / want + 15) / 16 * 16);
-  p.chunk = chunk <= kChunkMost ? (int)chunk : 0;
-  auto parts = [&](int64_t keys) { return p.chunk ? (int)std::max<int64_t>(1, (keys + p.chunk - 1) / p.chunk) : 1; };
+  const int64_t items = (int64_t)p.hkv * (both ? p.batch * ((own + 7) / 8) + (all + 7) / 8 : p.batch * ((own + 7) / 8));
+  p.chunk = items >= 256 ? 128 : 64;
+  p.chunks = items < 1024 ? 32 : items < 4096 ? 16 : items < 16384 ? 8 : 4;
+  if (items * p.chunks < 12 * (int64_t)ctx->num_sms && most > p.chunks * p.chunk) p.chunk = 0;
+  // the most chunks that any length up to `keys` has
+  auto parts = [&](int64_t keys) {
+    return !p.chunk ? 1 : keys >= (int64_t)p.chunks * p.chunk ? p.chunks : chunks_of(p.chunk, p.chunks, (int)keys);
+  };
   p.own_layer = flash ? text_flash_layers(ctx, p) : both ? parts(p.prefix) : 0;
   p.layers = p.own_layer + parts(p.blocks_per_seq << p.page_shift);
   const int64_t rows = p.total_q * p.hq;
@@ -1108,7 +1117,9 @@ int wx_prefix_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, in
   const int st = paged_params(ctx, dims, q, q_stride, cache, cu_q, kv_lens, block_table, blocks_per_seq, out, out_stride,
                               lse, p, kv, empty);
   if (st || empty) return st;
-  WX_CHECK_ARG(ctx, prefix_len >= 0 && prefix_len <= INT32_MAX - 256 && (prefix_len == 0 || prefix_blocks));
+  WX_CHECK_ARG(ctx, prefix_len >= 0 && (prefix_len == 0 || prefix_blocks));
+  if (prefix_len > INT32_MAX - 8192)  // (tiles and steps behind the last key are counted in 32 bits too)
+    return set_error(ctx, WX_ERR_UNSUPPORTED, "prefix_len must be below 2^31 - 8192");
   WX_CHECK_ARG(ctx, table_stride >= blocks_per_seq);
   p.prefix = (int)prefix_len;
   p.front = (int)((prefix_len + 127) / 128);

@@ -43,8 +43,9 @@ struct TextAttnParams {
   float* layer_o;     // sums of rows [layer][total_q * hq][hd], brought together by prefix_join_kernel
   int layers;
   float2* layer_ml;   // their maxima (base 2) and denominators
-  int own_layer;      // rows kernel: of the sequences' own keys (kChunkKeys: of the first `chunk` of them)
-  int chunk;          // kChunkKeys: keys of a unit, a layer each; 0: one layer
+  int own_layer;      // rows kernel: of the sequences' own keys (kChunkKeys: of their first chunk)
+  int chunk, chunks;  // kChunkKeys: keys of a unit, a layer each, at least, and units at most; 0: one layer
+  int max_q;          // host: the caller's longest query length
   int ctas;           // kChunkKeys, host
   int after_walk;     // kChunkKeys, host: launched right behind the shared walk by text_flash
   size_t ws_reserved; // bytes of the workspace in use before the kernel's own
@@ -57,6 +58,15 @@ struct TextAttnParams {
 };
 
 // where K and V rows lie: `rows` rows of `cols` elements (strides in elements)
+// kChunkKeys: a sequence's keys go to `most` units at most, of whole steps of 16 and `chunk` keys at least.
+__host__ __device__ inline int chunk_of(int chunk, int most, int lk) {
+  const int even = (lk / most + 16) & ~15;  // (more than lk / most)
+  return even > chunk ? even : chunk;
+}
+__host__ __device__ inline int chunks_of(int chunk, int most, int lk) {
+  return lk > 0 ? (lk - 1) / chunk_of(chunk, most, lk) + 1 : 1;
+}
+
 struct KvSource {
   const void *k, *v;
   uint64_t rows, cols, k_stride, v_stride;

@@ -1385,7 +1385,7 @@ static int launch_flash(wx_ctx* ctx, const TfMaps& maps, TfParams& tp) {
   // to an SM and as the longest range that a row can see allows.
   int64_t keys = p.block_table ? p.blocks_per_seq << p.page_shift : p.total_k;
   if (p.window) keys = std::min<int64_t>(keys, (int64_t)p.window + 2 * tp.tt + (KEYS == kSinkKeys ? p.sinks : 0));
-  if (KEYS == kPrefixKeys) keys += p.front * 128;
+  if (KEYS == kPrefixKeys) keys += (int64_t)p.front * 128;
   tp.min_tiles = kTfMinTiles;
   tp.splits = (int)std::max<int64_t>(1, std::min((kTfWaves * ctx->num_sms + items - 1) / items, keys / (128 * kTfMinTiles)));
   if (KEYS == kPrefixKeys && p.shared) {
@@ -1395,7 +1395,9 @@ static int launch_flash(wx_ctx* ctx, const TfMaps& maps, TfParams& tp) {
     // Behind a prefix all items are long and much alike, so that whole rounds count: of the pieces, each with a
     // start and end worth two tiles, and a join worth three. (148 items of 50 int8 tiles: whole 181 us, in 2, 3, 5
     // pieces 208, 222, 247)
-    const double some = p.hkv * (p.total_q / (2.0 * tp.tt) + 0.5 * p.batch), tiles = p.front + (keys - p.front * 128) / 256.0;
+    // Own keys are taken to be the new tokens' and half of them to be seen: the tables may be far wider.
+    const double some = p.hkv * (p.total_q / (2.0 * tp.tt) + 0.5 * p.batch);
+    const double tiles = p.front + std::min<int64_t>(p.blocks_per_seq << p.page_shift, p.max_q) / 256.0;
     double least = INFINITY;
     for (int n = 1; n == 1 || (n <= 64 && n * kTfMinTiles <= tiles); ++n) {
       const double cost = std::ceil(some * n / ctx->num_sms) * (tiles / n + 2) + (n > 1 ? 3 : 0);
