@@ -966,15 +966,17 @@ static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p
   if (own > few) return text_flash(ctx, p, d->head_dim, kv, kPrefixKeys);
   const bool flash = p.prefix && all > few && (all + 15) / 16 * p.prefix * p.hkv > 65536;
   const bool both = p.prefix && !flash;  // the rows kernel walks the prefix too
-  // Own keys in chunks for single warps: of 128 keys, or 64 where there are few items (64 sequences of 1 to 701 bf16
-  // keys: 64 43, 128 41, 256 48 us in all; three sequences behind 333 keys, 16 heads of 64: 64 9.2, 128 10.5), and of
+  // Own keys in chunks for single warps, the longer the more items there are (keys a chunk: us in all. 3 sequences
+  // behind 333 keys, 16 heads of 64, 64 items: 64: 9.4, 128: 10.8; 8 of 900 bf16 keys behind 4,000, 96 items: 64: 27, 96: 22,
+  // 128: 24; 64 of 1 to 701 behind 8,011, 512 items: 64: 41, 128: 42, 256: 49; 128 of 20 to 1,520 e4m3 keys behind 40,000,
+  // 1,024 items: 128: 294, 384: 278; 100 of 1,200 behind 5,000, 1,600 items: 128: 180, 384: 156), and of
   // more where that would be more than so many chunks a sequence: each is a layer, for which room is set aside, and
   // the more items there are, the fewer chunks give each warp its share. What lengths there are is known on
   // the device only, the tables' width being their bound; items that are too few to give every warp a unit
   // although their keys may be many are left to a piece per CTA, which divides them evenly.
   const int64_t most = std::max<int64_t>(p.blocks_per_seq << p.page_shift, both ? p.prefix : 0);
   const int64_t items = (int64_t)p.hkv * (both ? p.batch * ((own + 7) / 8) + (all + 7) / 8 : p.batch * ((own + 7) / 8));
-  p.chunk = items >= 256 ? 128 : 64;
+  p.chunk = items < 80 ? 64 : items < 256 ? 96 : items < 1024 ? 128 : 384;
   p.chunks = items < 1024 ? 32 : items < 4096 ? 16 : items < 16384 ? 8 : 4;
   if (items * p.chunks < 12 * (int64_t)ctx->num_sms && most > p.chunks * p.chunk) p.chunk = 0;
   // the most chunks that any length up to `keys` has
