@@ -21,7 +21,7 @@
 // Measured (caches flushed from L2): packed causal prompts of 9001 + 1 + 5003 + 2380 tokens, 32 / 8
 // heads of 128: 785 us in single calls (1.17 PFLOP/s of useful work), 920 in a row under the power
 // cap; 4096 + 1117 tokens, 16 heads of 64, window 1024: 64 us; 1024 + 300 tokens over 16,384 + 9,999
-// cached keys, 32 / 8 heads of 128: 360 us at bf16, 550 at e4m3. Tensor pipe 51 % busy on a prompt
+// cached keys, 32 / 8 heads of 128: 360 us at bf16, 540 at e4m3. Tensor pipe 51 % busy on a prompt
 // of 4096 tokens, 28 % on an e4m3 cache. What bounds it is a slot's chain from one S to the next (S,
 // its maxima, the exponentials in their turn, the issue of P V and S): some 3,700 cycles at bf16 against 2,048
 // tensor cycles for both slots; on 8-bit caches 5,400, the four conversion warps being nearly as long.
