@@ -191,6 +191,81 @@ def test_two_streams_and_branches_of_a_capture():
     _check_device()
 
 
+def _call(server, n=1, seed=1):
+    """A prefix call of n new rows a sequence over what the server holds, and the same rows as a slice."""
+    s = server
+    q = _randn(_gen(seed), n * s.batch, s.hq + 3, s.hd)[:, 1:1 + s.hq]
+    cu = _cu([n] * s.batch)
+    return lambda **how: s.text.prefix_attention(how.pop("q", q), s.cache, s.front, s.prefix, cu, s.pool.lens, s.pool.table,
+                                                 n, **how), q
+
+
+def _served(fmt, batch, prefix, seed):
+    s = Server(fmt, batch, prefix, seed=seed)
+    n = [5 + 3 * i % 40 for i in range(batch)]
+    s.step(_i32(n), sum(n), max(n), *s.rows(sum(n)))
+    return s
+
+
+@pytest.mark.parametrize("batch,n", [(40, 1), (3, 1), (5, 40)])
+def test_rows_of_a_packed_projection_in_and_out(batch, n):
+    call, q = _call(_served("bf16", batch, 700, 11), n)
+    want = call(q=q.contiguous())
+    whole, out = _framed(n * batch, 8, 128)
+    assert torch.equal(call(), want) and torch.equal(call(out=out), want)
+    _check_device()
+    assert torch.equal(out, want) and _frame_kept(whole, n * batch, 8)
+
+
+def test_a_profiled_call_and_two_threads():
+    """Events between the kernels of a call, and calls of two threads on streams of their own."""
+    import ctypes
+    import threading
+    from wuxianhuabu_b200 import h3
+    calls = [_call(_served("bf16", 40, 900, 12))[0], _call(_served("int8", 33, 1500, 13))[0]]
+    wants = [c() for c in calls]
+    ctx = h3.context()
+    assert ctx.lib.wx_ctx_profile_enable(ctx.h, 1) == 0
+    try:
+        got = [c() for c in calls]
+        ms, counts = (ctypes.c_double * 16)(), (ctypes.c_int64 * 16)()
+        torch.cuda.synchronize()
+        ctx.lib.wx_ctx_profile_read(ctx.h, ms, counts, 16)
+    finally:
+        assert ctx.lib.wx_ctx_profile_enable(ctx.h, 0) == 0
+    assert all(torch.equal(a, b) for a, b in zip(got, wants))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [calls[i]() for _ in range(30)]
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(o for o in outs if not torch.equal(o, wants[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    _check_device()
+
+
+def test_sequences_that_begin_behind_the_first_row():
+    s = _served("e4m3", 20, 400, 14)
+    q = _randn(_gen(3), 25, 8, 128)
+    out = torch.full_like(q, 3.0)
+    cu = torch.arange(21, dtype=torch.int32, device="cuda") + 4
+    s.text.prefix_attention(q, s.cache, s.front, s.prefix, cu, s.pool.lens, s.pool.table, 1, out=out)
+    _check_device()
+    assert (out[:4] == 3.0).all() and (out[24:] == 3.0).all()
+    for b, n in enumerate(s.pool.lens.tolist()):
+        k, v = (torch.cat(x) for x in zip(s.front_kv, s.stored(s.pool.table[b], n)))
+        ref, _, mag = ref_seen(q[4 + b:5 + b], k, v, 128 ** -0.5, torch.ones(1, 400 + n, dtype=torch.bool, device="cuda"))
+        assert_attention(out[4 + b:5 + b], None, ref, None, mag, f"sequence {b}")
+
+
 @pytest.mark.parametrize("fmt,pages", [("bf16", 9000), ("int8", 18000)])
 @pytest.mark.parametrize("q_lens", [[1, 1], [1] * 40, [70, 3]])
 def test_a_cache_beyond_32_bit_offsets(fmt, pages, q_lens):
