@@ -948,7 +948,7 @@ __global__ void __launch_bounds__(256) prefix_join_kernel(TextAttnParams p) {
   const int64_t token = join_token<R>(p, head);
   const int b = seq_of_token(p, token);
   const bool live = token < p.total_q && token >= p.cu_q[b] && token < p.cu_q[b + 1];
-  const int layers = p.own_layer + (p.chunk ? chunks_of(p.chunk, p.chunks, load_seq(p, b).lk) : 1);
+  const int layers = p.own_layer + layers_of(p.chunk, p.chunks, load_seq(p, b).lk);
   wait_for_last();
   if (!live) return;
   const int64_t row0 = token * p.hq + head;
@@ -979,12 +979,9 @@ static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p
   p.chunk = items < 80 ? 64 : items < 256 ? 96 : items < 1024 ? 128 : 384;
   p.chunks = items < 1024 ? 32 : items < 4096 ? 16 : items < 16384 ? 8 : 4;
   if (items * p.chunks < 12 * (int64_t)ctx->num_sms && most > p.chunks * p.chunk) p.chunk = 0;
-  // the most chunks that any length up to `keys` has
-  auto parts = [&](int64_t keys) {
-    return !p.chunk ? 1 : keys >= (int64_t)p.chunks * p.chunk ? p.chunks : chunks_of(p.chunk, p.chunks, (int)keys);
-  };
-  p.own_layer = flash ? text_flash_layers(ctx, p) : both ? parts(p.prefix) : 0;
-  p.layers = p.own_layer + parts(p.blocks_per_seq << p.page_shift);
+  // (the prefix's layers are all joined, so they are those that its walk writes; own lengths are known on the device)
+  p.own_layer = flash ? text_flash_layers(ctx, p) : both ? layers_of(p.chunk, p.chunks, p.prefix) : 0;
+  p.layers = p.own_layer + most_layers(p.chunk, p.chunks, p.blocks_per_seq << p.page_shift);
   const int64_t rows = p.total_q * p.hq;
   Carve c;
   const size_t o_o = c.take((size_t)(p.layers * rows) * d->head_dim * 4), o_ml = c.take((size_t)(p.layers * rows) * 8);

@@ -66,6 +66,12 @@ __host__ __device__ inline int chunk_of(int chunk, int most, int lk) {
 __host__ __device__ inline int chunks_of(int chunk, int most, int lk) {
   return lk > 0 ? (lk - 1) / chunk_of(chunk, most, lk) + 1 : 1;
 }
+// Layers that a walk over lk keys writes (chunk 0: a single one): what is joined is this many, no more. Room is made
+// for those of every length up to `keys`: of some longer ones there are fewer, their chunks being rounded up to 16 keys.
+__host__ __device__ inline int layers_of(int chunk, int most, int lk) { return chunk ? chunks_of(chunk, most, lk) : 1; }
+__host__ __device__ inline int most_layers(int chunk, int most, int64_t keys) {
+  return chunk && keys >= (int64_t)most * chunk ? most : layers_of(chunk, most, (int)keys);
+}
 
 struct KvSource {
   const void *k, *v;
