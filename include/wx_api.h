@@ -663,11 +663,12 @@ int wx_rope_apply(wx_ctx* ctx, const wx_rope* rope, const int32_t* positions, co
                   int64_t tokens, int heads, int head_dim, void* y, int64_t y_stride);
 
 /* Several positions a token (time, height and width of a picture's or clip's tokens): pair i turns by
- * the position of axis axis_of_pair[i]. Positions are [n_axes][position_stride >= tokens] on the device. */
+ * the position of axis axis_of_pair[i]. Positions are [n_axes][position_stride >= tokens] on the device, or
+ * [tokens] with position_stride 0: one position of a token on every axis, as text has. */
 typedef struct wx_rope_axes {
   int32_t n_axes;           /* 1..4 */
   uint8_t axis_of_pair[64]; /* of the rope's rot/2 pairs, each below n_axes */
-  int64_t position_stride;  /* entries between the axes' positions */
+  int64_t position_stride;  /* entries between the axes' positions, 0 where all axes share them */
 } wx_rope_axes;
 /* q and k rows normalised head by head, y = x / sqrt(mean x^2 + eps) * norm (fp32, squares too; norm
  * [head_dim] bf16, NULL: not normalised), and their first rot columns turned; one rounding to bf16.

@@ -964,7 +964,8 @@ static int set_heads(wx_ctx* ctx, HeadParams& p, const wx_rope* rope, const wx_r
   p.axes = 1;
   if (!axes) return WX_OK;
   WX_CHECK_ARG(ctx, axes->n_axes >= 1 && axes->n_axes <= 4);
-  WX_CHECK_ARG(ctx, axes->n_axes == 1 || axes->position_stride >= p.r.tokens);
+  // (0: positions that all axes share, as text's are)
+  WX_CHECK_ARG(ctx, axes->n_axes == 1 || axes->position_stride == 0 || axes->position_stride >= p.r.tokens);
   p.axes = axes->n_axes;
   p.pos_stride = axes->position_stride;
   for (int i = 0; i < rope->rot / 2; ++i) {

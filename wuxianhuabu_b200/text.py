@@ -138,7 +138,7 @@ def _head_norm(w: Optional[torch.Tensor], d: int, what: str) -> Optional[int]:
 class RopeTable(_Described):
     """cos / sin of every position, fp32 [positions, rot / 2] (angles in 64 bits). With ``axes`` (one
     axis a pair, ``rope_axes``) a token has a position on each axis: positions are [axes, tokens]
-    then, instead of [tokens]."""
+    then, instead of [tokens]; text's, the same on every axis, may be an expanded row."""
     axes: Optional[tuple] = None
 
     def __init__(self, rot: int, positions: int, base: float = 10000.0, interleaved: bool = False,
