@@ -786,9 +786,9 @@ int wx_paged_attention_sinks(wx_ctx* ctx, const wx_attn_dims* dims, int32_t sink
                              float* lse);
 /* A batch behind one cached prefix, read once for all of it: each sequence's keys are the prefix_len tokens in
  * pages prefix_blocks (device, ceil(prefix_len / page_size) entries), seen by every query row, and then its own
- * kv_lens[b] cached tokens in pages block_table[b * table_stride ..] (blocks_per_seq entries; table_stride >= that, so
- * that the columns behind a prefix's in a larger table serve), of which row i sees those up to i + Lk - Lq with
- * causal. No window. prefix_len may be 0. */
+ * kv_lens[b] cached tokens in pages block_table[b * table_stride ..] (blocks_per_seq entries, at least 1; table_stride >=
+ * that, so that the columns behind a prefix's in a larger table serve, or 0: one row of pages for all sequences), of
+ * which row i sees those up to i + Lk - Lq with causal. No window. prefix_len may be 0. */
 int wx_prefix_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, int64_t q_stride,
                         const wx_kv_cache* cache, const int32_t* prefix_blocks, int64_t prefix_len,
                         const int32_t* cu_q, const int32_t* kv_lens, const int32_t* block_table,

@@ -3,7 +3,8 @@ same values laid out in full, bit for bit."""
 import pytest
 import torch
 
-from tests.test_gpu_text import BF16, _check_device, _gen, _randn, _slots, _text
+from tests.test_gpu_text import BF16, _check_device, _cu, _gen, _randn, _slots, _text
+from tests.test_gpu_text_prefix import _behind, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -57,4 +58,30 @@ def test_overlapping_axes_are_refused():
     for stride in (1, 4):
         with pytest.raises(h3.WxError):
             rope.apply(q, pos.as_strided((3, 5), (stride, 1)))
+    _check_device()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("q_lens", [[1] * 3, [1] * 40, [60, 3], [1]])
+def test_own_pages_that_all_sequences_share(q_lens, fmt):
+    """Sequences over the same own pages, to lengths of their own: one row of the table for all of them."""
+    text = _text()
+    prefix, kv_lens = 300, [60 + 3 * i for i in range(len(q_lens))]
+    cache, front, table, q, _, _ = _behind(_gen(len(q_lens)), fmt, prefix, q_lens, kv_lens, 8, 2, 128, 16)
+    row = table[-1]
+    shared, full = row.expand(len(q_lens), -1), row.expand(len(q_lens), -1).contiguous()
+    got = [text.prefix_attention(q, cache, front, prefix, _cu(q_lens), _i32(kv_lens), t, max(q_lens), return_lse=True)
+           for t in (shared, full)]
+    _check_device()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_block_tables_whose_rows_overlap_are_refused():
+    text = _text()
+    from wuxianhuabu_b200 import h3
+    cache, front, table, q, _, _ = _behind(_gen(2), "bf16", 100, [1, 1], [5, 40], 4, 2, 128, 16)
+    for stride in (1, 2):
+        with pytest.raises(h3.WxError):
+            text.prefix_attention(q, cache, front, 100, _cu([1, 1]), _i32([5, 40]),
+                                  table.as_strided((2, 3), (stride, 1)), 1)
     _check_device()

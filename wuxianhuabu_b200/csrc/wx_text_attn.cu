@@ -1119,7 +1119,7 @@ int wx_prefix_attention(wx_ctx* ctx, const wx_attn_dims* dims, const void* q, in
   WX_CHECK_ARG(ctx, prefix_len >= 0 && (prefix_len == 0 || prefix_blocks));
   if (prefix_len > INT32_MAX - 8192)  // (tiles and steps behind the last key are counted in 32 bits too)
     return set_error(ctx, WX_ERR_UNSUPPORTED, "prefix_len must be below 2^31 - 8192");
-  WX_CHECK_ARG(ctx, table_stride >= blocks_per_seq);
+  WX_CHECK_ARG(ctx, table_stride >= blocks_per_seq || table_stride == 0);
   p.prefix = (int)prefix_len;
   p.front = (int)((prefix_len + 127) / 128);
   p.prefix_blocks = prefix_blocks;

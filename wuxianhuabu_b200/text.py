@@ -514,8 +514,9 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, prefix_blocks: torch.
                      return_lse: bool = False):
     """``paged_attention`` where every sequence stands behind the same ``prefix_len`` cached tokens, in pages
     prefix_blocks (int32): these are walked once for the whole batch and seen by every row. kv_lens and
-    block_table are of each sequence's own tokens behind them; block_table may be columns of a larger table
-    (``prefix_attention(q, cache, table[0, :n], n * page_size, cu, lens - n * page_size, table[:, n:], ...)``)."""
+    block_table are of each sequence's own tokens behind them; block_table (one column at least) may be columns
+    of a larger table (``prefix_attention(q, cache, table[0, :n], n * page_size, cu, lens - n * page_size,
+    table[:, n:], ...)``) or one row expanded to all sequences."""
     n, h, d, qs, o, os_, lse = _attn_out(q, out, return_lse)
     batch = _batch_of(cu_seqlens)
     cu = _need_ints(torch.int32, None, "cu_seqlens", cu_seqlens)
@@ -528,12 +529,13 @@ def prefix_attention(q: torch.Tensor, cache: PagedKVCache, prefix_blocks: torch.
         raise _invalid("block_table must be a CUDA int32 [batch, blocks] tensor")
     blocks = block_table.shape[1]
     stride, inner = block_table.stride()
-    if (blocks > 1 and inner != 1) or (batch > 1 and stride < blocks):
-        raise _invalid("block_table must have contiguous rows")
+    if (blocks > 1 and inner != 1) or (batch > 1 and 0 < stride < blocks):
+        raise _invalid("block_table must have contiguous rows, apart or one for all sequences")
+    stride = stride if batch > 1 else blocks
     if d != cache.head_dim:
         raise _invalid("q must have the cache's head_dim")
     dev = _same_device(q, cache.k, cu_seqlens, kv_lens, block_table, prefix_blocks, o)
     context(dev).call("wx_prefix_attention", _dims(n, batch, max_len, h, cache.kv_heads, d, causal, 0, scale),
                       q.data_ptr(), qs, cache._desc, prefix, prefix_len, cu, lens, block_table.data_ptr(), blocks,
-                      max(stride, blocks), o.data_ptr(), os_, _p(lse))
+                      stride, o.data_ptr(), os_, _p(lse))
     return (o, lse) if return_lse else o
