@@ -44,6 +44,7 @@ constexpr int kTfChunk = 128 * 128;  // one 64-column SW128 chunk of a 128-row t
 constexpr int kTfWaves = 3;          // pieces for each SM below which items are cut up
 constexpr int kTfMinTiles = 8;       // tiles of a piece of an item: its start and end cost one or two
 constexpr int64_t kTfL2 = int64_t(48) << 20;
+constexpr int64_t kTfPartBytes = int64_t(256) << 20;  // partial sums of items cut up behind a prefix, at most
 // V rows with non-finite values remembered per item: every row of its masked tiles (an item's 256 tokens
 // end, and where a window cuts begin, in up to three tiles each; one more holds the last first key)
 constexpr int kTfBadRows = 7 * 128;
@@ -1365,6 +1366,23 @@ int text_flash_layers(wx_ctx* ctx, const TextAttnParams& p) {
   return best;
 }
 
+// Pieces of the items of new prompts behind a prefix, `some` items of so many key tiles. They are long and much alike,
+// so that whole rounds over the SMs count (2.05 us a tile at bf16, 3.25 on 8-bit caches): a piece's start and end are
+// worth four tiles, a join three and the bytes of the pieces' sums, written and read once each, which also have to
+// fit into kTfPartBytes. us in 1, 2, 3, 4, 6 pieces, 32 / 8 heads of 128: sequences of 64 tokens behind 8,000, 160 items at
+// bf16 264, 238, 227, 231, 242 and at e4m3 436, 375, 342, 342, 344; 240 items 272, 320, 295, 324, 338; 64 items of 200 tokens
+// behind 6,016 107, 74, 96, 84, 98; 148 items of 28 / 4 heads behind 6,000 int8 keys 180, 209, 223, 233, 260. Two rounds of
+// items and more are left whole: 320 items 385, 401, 399, 414, 444, 480 items 506, 555, 563, 602, 641.
+inline int prefix_pieces(int num_sms, double some, double tiles, int64_t rows, int head_dim, bool wide) {
+  const double join = (double)rows * (head_dim * 8 + 16) / (wide ? 21e6 : 13.3e6);  // of a piece of every row, in tiles
+  auto cost = [&](int n) { return std::ceil(some * n / num_sms) * (tiles / n + 4) + (n > 1 ? 3 + n * join : 0); };
+  int best = 1;
+  if (some >= 2 * num_sms) return best;
+  for (int n = 2; n <= 64 && n * kTfMinTiles <= tiles && n * rows * (head_dim * 4 + 8) <= kTfPartBytes; ++n)
+    if (cost(n) < 0.99 * cost(best)) best = n;
+  return best;
+}
+
 template <int FMT, int HD, int KEYS>
 static int launch_flash(wx_ctx* ctx, const TfMaps& maps, TfParams& tp) {
   using G = TfGeom<FMT, HD>;
@@ -1392,17 +1410,14 @@ static int launch_flash(wx_ctx* ctx, const TfMaps& maps, TfParams& tp) {
     tp.splits = text_flash_layers(ctx, p);
     tp.min_tiles = 1;
   } else if (KEYS == kPrefixKeys) {
-    // Behind a prefix all items are long and much alike, so that whole rounds count: of the pieces, each with a
-    // start and end worth two tiles, and a join worth three. (148 items of 50 int8 tiles: whole 181 us, in 2, 3, 5
-    // pieces 208, 222, 247)
+    // items: the longest sequence's, and of the others as many; or half of one more than whole ones, if lengths differ
+    const double item = 2.0 * tp.tt, longest = std::ceil(p.max_q / item), others = longest * (p.batch - 1);
+    const double rest = (double)std::max<int64_t>(0, p.total_q - p.max_q) / item + 0.5 * (p.batch - 1);
+    const bool even = p.total_q == (int64_t)p.max_q * p.batch;
+    const double some = p.hkv * (longest + (even ? others : std::min(others, rest)));
     // Own keys are taken to be the new tokens' and half of them to be seen: the tables may be far wider.
-    const double some = p.hkv * (p.total_q / (2.0 * tp.tt) + 0.5 * p.batch);
     const double tiles = p.front + std::min<int64_t>(p.blocks_per_seq << p.page_shift, p.max_q) / 256.0;
-    double least = INFINITY;
-    for (int n = 1; n == 1 || (n <= 64 && n * kTfMinTiles <= tiles); ++n) {
-      const double cost = std::ceil(some * n / ctx->num_sms) * (tiles / n + 2) + (n > 1 ? 3 : 0);
-      if (cost < least) least = cost, tp.splits = n;
-    }
+    tp.splits = prefix_pieces(ctx->num_sms, some, tiles, p.total_q * p.hq, HD, G::kWide);
   }
   const int grid = (int)std::min<int64_t>(ctx->num_sms, items * tp.splits);
   const int64_t rows = tp.splits > 1 ? p.total_q * p.hq * tp.splits : 0;
