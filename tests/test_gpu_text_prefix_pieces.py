@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.test_gpu_text import _check_device, _cu, _gen, _paged, _text, assert_attention
-from tests.test_gpu_text_prefix import _i32
+from tests.test_gpu_text_prefix import _behind, _check, _i32
 from tests.test_gpu_text_sinks import ref_seen
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +47,38 @@ def test_many_rows_take_little_room(lens, prefix):
     assert held <= 64 << 20, held
     last = len(lens) - 1
     _some_rows(got, q, lens, ks, vs, [(0, 0), (0, lens[0] - 1), (4, 500), (last, 1), (last, lens[0] - 1)])
+
+
+def test_few_items_over_many_own_keys_are_cut():
+    """40 new tokens, 30,000 own keys, a short prefix: 8 items, whose keys the SMs share."""
+    text = _text()
+    cache, front, table, q, ks, vs = _behind(_gen(5), "bf16", 128, [40], [30000], 32, 8, 128, 64)
+    run = lambda: text.prefix_attention(q, cache, front, 128, _cu([40]), _i32([30000]), table, 40,  # noqa: E731
+                                        return_lse=True)
+    got, held = _with_new_context(run)
+    _, one = _with_new_context(lambda: text.prefix_attention(q, cache, front, 128, _cu([40]), _i32([40]),
+                                                                 table[:, :1], 40))
+    assert held - one >= 8 * 40 * 32 * 128 * 4, (held, one)  # eight pieces' sums at least
+    _check_device()
+    _check(*got, q, [40], ks, vs)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "e4m3"])
+@pytest.mark.parametrize("wide", [0, 3000])
+@pytest.mark.parametrize("prefix,q_lens,kv_lens,hq,hkv,hd,page", [
+    (300, [40, 33, 70, 1], [9000, 40, 70, 2500], 8, 2, 128, 64),      # the longest first
+    (300, [65, 3, 0, 40], [65, 3, 0, 20001], 28, 4, 128, 32),         # an empty sequence, the longest last
+    (2500, [200, 64], [200, 12000], 16, 4, 64, 16),                   # whole rounds of one, pieces of the other
+    (0, [90, 50], [7000, 50], 4, 1, 128, 128)])
+def test_long_and_short_sequences_in_one_call(prefix, q_lens, kv_lens, hq, hkv, hd, page, wide, fmt):
+    text = _text()
+    cache, front, table, q, ks, vs = _behind(_gen(prefix), fmt, prefix, q_lens, kv_lens, hq, hkv, hd, page)
+    if wide:
+        far = torch.full((len(q_lens), wide), -1, dtype=torch.int32, device="cuda")
+        far[:, :table.shape[1]] = table
+        table = far
+    out = torch.full_like(q, float("nan"))
+    got = text.prefix_attention(q, cache, front, prefix, _cu(q_lens), _i32(kv_lens), table, max(q_lens), out=out,
+                                return_lse=True)
+    _check_device()
+    _check(*got, q, q_lens, ks, vs)

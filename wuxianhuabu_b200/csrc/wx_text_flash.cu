@@ -269,6 +269,7 @@ struct TfParams {
   uint32_t* bad_rows;  // [CTA][kTfItems][kTfBadRows][kTfBadWords]
   const uint8_t *k8, *v8;  // rows of an 8-bit cache
   int splits, min_tiles;   // at most this many pieces of an item, of so many tiles
+  int usual, long_tiles;   // kPrefixKeys: `usual` pieces in sequences of fewer tiles than this
   float* part;             // [splits][total_q * hq][HD] sums of the pieces' rows (items cut up only)
   float2* part_ml;         // [splits][total_q * hq] maximum (base 2) and denominator
 };
@@ -327,11 +328,18 @@ __device__ __forceinline__ Seq walk_seq(const TextAttnParams& p, int b) {
   if (KEYS == kPrefixKeys && p.shared) return Seq{0, 0, (int)p.total_q, 0};
   return load_seq(p, b);
 }
+// At most so many pieces of an item of the sequence. As many numbers stand for them, so that there are no more than are
+// likely to be used: a CTA looks for its next item ahead of time, and those that come upon no piece go on to one that
+// another would have had time for (4 x 200 tokens behind 6,016 in a wide table, one piece of three used: 207 us, not 111).
+template <int KEYS>
+__device__ __forceinline__ int most_pieces(const TfParams& tp, const Seq& s) {
+  return KEYS == kPrefixKeys && tp.a.front + (s.lk >> 7) < tp.long_tiles ? tp.usual : tp.splits;
+}
 // The item's tiles [first, last) and the pieces that they are cut into, of at least min_tiles
-__device__ __forceinline__ void cut_item(int2 a, int2 b, int splits, int min_tiles, int& first, int& last, int& pieces) {
+__device__ __forceinline__ void cut_item(int2 a, int2 b, int most, int min_tiles, int& first, int& last, int& pieces) {
   first = a.y <= a.x ? b.x : b.y <= b.x ? a.x : min(a.x, b.x);
   last = max(first, max(a.y > a.x ? a.y : 0, b.y > b.x ? b.y : 0));
-  pieces = min(splits, max(1, (last - first) / min_tiles));
+  pieces = min(most, max(1, (last - first) / min_tiles));
 }
 
 template <int FMT, int HD, int KEYS>
@@ -629,7 +637,7 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
     auto seq_items = [&](int b) -> int {
       if (b >= p.batch) return 0;
       const Seq s = walk_seq<KEYS>(p, b);
-      return (int)((unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt)) * p.hkv * tp.splits;
+      return (int)((unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt)) * p.hkv * most_pieces<KEYS>(tp, s);
     };
     int wb = 0;
     int wi = 0;  // items of the sequences before wb
@@ -648,10 +656,11 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
         if (at < wi + all) {
           const int src = __ffs(__ballot_sync(0xffffffffu, at < wi + nc)) - 1;
           const unsigned of_b = (unsigned)(at - wi - __shfl_sync(0xffffffffu, nc - n, src));
-          const unsigned in_b = of_b / (unsigned)tp.splits;
           int found = 1;
           if (lane == 0) {
             const Seq s = walk_seq<KEYS>(p, wb + src);
+            const int most = most_pieces<KEYS>(tp, s);
+            const unsigned in_b = of_b / (unsigned)most;
             const unsigned tiles = (unsigned)(s.lq + 2 * tp.tt - 1) / (unsigned)(2 * tp.tt);
             const unsigned fit = (unsigned)(kTfL2 / (HD * 4)) / (unsigned)max(1, KEYS == kPrefixKeys ? max(s.lk, p.prefix) : s.lk);
             const unsigned heads = max(1u, min((unsigned)p.hkv, fit));
@@ -670,8 +679,8 @@ __global__ void __launch_bounds__(TfGeom<FMT, HD>::kThreads, 1)
             int2 a, b;
             dst->at = item_tiles<KEYS>(p, s, tok0, tp.tt, a, b);
             int first, last, pieces;
-            cut_item(a, b, tp.splits, tp.min_tiles, first, last, pieces);
-            const int piece = (int)(of_b - in_b * (unsigned)tp.splits), per = (last - first + pieces - 1) / pieces;
+            cut_item(a, b, most, tp.min_tiles, first, last, pieces);
+            const int piece = (int)(of_b - in_b * (unsigned)most), per = (last - first + pieces - 1) / pieces;
             first += piece * per;
             last = min(last, first + per);
             a = make_int2(max(a.x, first), min(a.y, last));
@@ -1328,7 +1337,7 @@ __global__ void __launch_bounds__(256) text_flash_join_kernel(TfParams tp) {
   int2 a, e;
   item_tiles<KEYS>(p, s, tok0, tp.tt, a, e);
   int first, last, pieces;
-  cut_item(a, e, tp.splits, tp.min_tiles, first, last, pieces);
+  cut_item(a, e, most_pieces<KEYS>(tp, s), tp.min_tiles, first, last, pieces);
   if (pieces < 2) return;
   const int64_t row0 = token * p.hq + head;
   join_rows<HD, R>(tp.part, tp.part_ml, p.total_q * p.hq, row0, min(R, p.hq - head), pieces,
@@ -1415,9 +1424,15 @@ static int launch_flash(wx_ctx* ctx, const TfMaps& maps, TfParams& tp) {
     const double rest = (double)std::max<int64_t>(0, p.total_q - p.max_q) / item + 0.5 * (p.batch - 1);
     const bool even = p.total_q == (int64_t)p.max_q * p.batch;
     const double some = p.hkv * (longest + (even ? others : std::min(others, rest)));
-    // Own keys are taken to be the new tokens' and half of them to be seen: the tables may be far wider.
+    // Own keys are taken to be the new tokens' and half of them to be seen. There may be far more, by the tables' bound
+    // (how many is known on the device): sequences of twice the tiles and more are cut as those of other calls. 40 tokens
+    // over 30,000 own keys behind 128 whole : cut, us, one sequence 434 : 64, 12 of them 457 : 352, four of 200 behind 3,008, one
+    // of which has 30,000, 490 : 207. Where no sequence of a wide table is that long, the join that finds nothing to do costs 4 to
+    // 12 us: 3 x 60 tokens behind 512 25 : 31, 8 x 200 behind 6,016 209 : 221.
     const double tiles = p.front + std::min<int64_t>(p.blocks_per_seq << p.page_shift, p.max_q) / 256.0;
-    tp.splits = prefix_pieces(ctx->num_sms, some, tiles, p.total_q * p.hq, HD, G::kWide);
+    tp.usual = prefix_pieces(ctx->num_sms, some, tiles, p.total_q * p.hq, HD, G::kWide);
+    tp.long_tiles = 2 * (int)std::ceil(tiles);
+    tp.splits = keys / 128 < tp.long_tiles ? tp.usual : std::max(tp.splits, tp.usual);
   }
   const int grid = (int)std::min<int64_t>(ctx->num_sms, items * tp.splits);
   const int64_t rows = tp.splits > 1 ? p.total_q * p.hq * tp.splits : 0;
