@@ -287,7 +287,6 @@ struct HeadParams {
   int nk;  // k rows (of a cache, or to k_out)
   const __nv_bfloat16 *q_norm, *k_norm;  // nullptr: not normalised
   float eps;
-  int axes;
   uint64_t axis_of[2];  // two bits for each pair
   int64_t pos_stride;   // between the axes' positions
   __nv_bfloat16* k_out;
@@ -961,12 +960,10 @@ static int set_heads(wx_ctx* ctx, HeadParams& p, const wx_rope* rope, const wx_r
   p.q_norm = static_cast<const __nv_bfloat16*>(q_norm);
   p.k_norm = static_cast<const __nv_bfloat16*>(k_norm);
   p.eps = eps;
-  p.axes = 1;
   if (!axes) return WX_OK;
   WX_CHECK_ARG(ctx, axes->n_axes >= 1 && axes->n_axes <= 4);
   // (0: positions that all axes share, as text's are)
   WX_CHECK_ARG(ctx, axes->n_axes == 1 || axes->position_stride == 0 || axes->position_stride >= p.r.tokens);
-  p.axes = axes->n_axes;
   p.pos_stride = axes->position_stride;
   for (int i = 0; i < rope->rot / 2; ++i) {
     WX_CHECK_ARG(ctx, axes->axis_of_pair[i] < axes->n_axes);

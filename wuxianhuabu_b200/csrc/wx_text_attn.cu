@@ -472,7 +472,9 @@ __global__ void __launch_bounds__(RowsGeom<FMT, HD, NT>::kThreads, 1)
           sc[n][e] = w0;
           sc[n][2 + e] = w1;
         }
-        // P rounded to bf16 for the tensor product (the denominator sums the unrounded values)
+        // P rounded to bf16 for the tensor product, which takes both operands in V's type (the denominator sums the
+        // unrounded values): up to 2^-8 of each weight, which partly cancels over the keys. Relative to 64 bits a row is
+        // off by 0.0019 to 0.0024, where weights kept in fp32 leave 0.0016, the output's own rounding.
         pb[n][0] = transpose_8x8(pack_bf16x2(sc[n][0], sc[n][1]));
         pb[n][1] = transpose_8x8(pack_bf16x2(sc[n][2], sc[n][3]));
       }

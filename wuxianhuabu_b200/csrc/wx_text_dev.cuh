@@ -57,7 +57,6 @@ struct TextAttnParams {
   int* err;
 };
 
-// where K and V rows lie: `rows` rows of `cols` elements (strides in elements)
 // kChunkKeys: a sequence's keys go to `most` units at most, of whole steps of 16 and `chunk` keys at least.
 __host__ __device__ inline int chunk_of(int chunk, int most, int lk) {
   const int even = (lk / most + 16) & ~15;  // (more than lk / most)
@@ -73,6 +72,7 @@ __host__ __device__ inline int most_layers(int chunk, int most, int64_t keys) {
   return chunk && keys >= (int64_t)most * chunk ? most : layers_of(chunk, most, (int)keys);
 }
 
+// where K and V rows lie: `rows` rows of `cols` elements (strides in elements)
 struct KvSource {
   const void *k, *v;
   uint64_t rows, cols, k_stride, v_stride;
