@@ -15,7 +15,7 @@ SRC = r'''
 #define __device__
 %s
 int main() {
-  const int chunks[] = {0, 64, 96, 128, 384}, mosts[] = {4, 8, 16, 32};
+  const int chunks[] = {0, 64, 96, 128, 256}, mosts[] = {4, 8, 16, 32};
   for (int chunk : chunks)
     for (int most : mosts) {
       int seen = 0;  // of all lengths up to lk
