@@ -31,7 +31,8 @@ int main() {
                         most_layers(chunk, most, lk)), 1;
       }
       for (int64_t keys : {int64_t(1) << 30, (int64_t(1) << 31) - 1, int64_t(1) << 34})
-        if (most_layers(chunk, most, keys) != (chunk ? most : 1)) return printf("%%d of %%d: %%lld\n", chunk, most, (long long)keys), 1;
+        if (most_layers(chunk, most, keys) != (chunk ? most : 1))
+          return printf("%%d of %%d: %%lld\n", chunk, most, (long long)keys), 1;
     }
   return 0;
 }

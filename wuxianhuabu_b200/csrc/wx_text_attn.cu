@@ -970,17 +970,18 @@ static int dispatch_prefix(wx_ctx* ctx, const wx_attn_dims* d, TextAttnParams& p
   const bool both = p.prefix && !flash;  // the rows kernel walks the prefix too
   // Own keys in chunks for single warps, the longer the more items there are (keys a chunk: us in all. 3 sequences
   // behind 333 keys, 16 heads of 64, 64 items: 64: 9.4, 128: 10.8; 8 of 900 bf16 keys behind 4,000, 96 items: 64: 27, 96: 22,
-  // 128: 24; 64 of 1 to 701 behind 8,011, 512 items: 64: 41, 128: 42, 256: 49). With many items the lengths decide, which only
-  // the device knows: 128 : 256 : 384 keys a chunk, 32 / 8 heads, sequences of 1 to 700 keys behind 8,000, 640 items at
-  // bf16 66 : 76 : 80, 1,024 items 82 : 86 : 100 and at e4m3 84 : 96 : 102; of 20 to 3,000 640 items 137 : 135 : 133 and 117 : 111
-  // : 121, 1,024 items 182 : 182 : 182 and 148 : 141 : 143; 100 of 1,200 behind 5,000, 16 / 16 heads, 1,600 items 250 : 229 : 234;
-  // 128 of 20 to 1,520 e4m3 keys behind 40,000, 64 / 8 heads, 1,024 items 303 : 293 : 287. Chunks are longer where there would be
-  // more than so many of a sequence: each is a layer, for which room is set aside, and the more items there are, the
-  // fewer chunks give each warp its share.
+  // 128: 24; 64 of 1 to 701 behind 8,011, 512 items: 64: 41, 128: 42, 256: 49). With many items the lengths decide, which
+  // only the device knows: 128 : 256 : 384 keys a chunk, 32 / 8 heads, sequences of 1 to 700 keys behind 8,000, 640 items
+  // at bf16 66 : 76 : 80, 1,024 items 82 : 86 : 100 and at e4m3 84 : 96 : 102; of 20 to 3,000, 640 items 137 : 135 : 133 and
+  // 117 : 111 : 121, 1,024 items 182 : 182 : 182 and 148 : 141 : 143; 100 of 1,200 behind 5,000, 16 / 16 heads, 1,600 items
+  // 250 : 229 : 234; 128 of 20 to 1,520 e4m3 keys behind 40,000, 64 / 8 heads, 1,024 items 303 : 293 : 287. Chunks are
+  // longer where there would be more than so many of a sequence: each is a layer, for which room is set aside, and the
+  // more items there are, the fewer chunks give each warp its share.
   // Items that are too few to give every warp a unit although their keys may be many, which the tables' width bounds,
-  // are left to a piece per CTA, which divides them evenly. A piece per CTA : chunks of 64, us in tables of 131,072 keys: 1 x 30,000
-  // own keys 47 : 66, 5 x 100,000 338 : 471, 20 of which one has 100,000 66 : 180, 6 of up to 300 behind 333 22.5 : 16.4, 5 of 100 to
-  // 500 behind 8,000 45 : 35: the most that a wide table costs short sequences.
+  // are left to a piece per CTA, which divides them evenly. A piece per CTA : chunks of 64, us in tables of 131,072
+  // keys, 32 / 8 heads: 1 x 30,000 own keys 47 : 66, 5 x 100,000 338 : 471, 6 of up to 300 behind 333 22.5 : 16.4, 5 of
+  // 100 to 500 behind 8,000 45 : 35, the most that a wide table costs short sequences; 8 / 2 heads, 20 of which one has
+  // 100,000, 66 : 180.
   const int64_t most = std::max<int64_t>(p.blocks_per_seq << p.page_shift, both ? p.prefix : 0);
   const int64_t items = (int64_t)p.hkv * (both ? p.batch * ((own + 7) / 8) + (all + 7) / 8 : p.batch * ((own + 7) / 8));
   p.chunk = items < 80 ? 64 : items < 256 ? 96 : items < 1024 ? 128 : 256;

@@ -1425,10 +1425,10 @@ static int launch_flash(wx_ctx* ctx, const TfMaps& maps, TfParams& tp) {
     const bool even = p.total_q == (int64_t)p.max_q * p.batch;
     const double some = p.hkv * (longest + (even ? others : std::min(others, rest)));
     // Own keys are taken to be the new tokens' and half of them to be seen. There may be far more, by the tables' bound
-    // (how many is known on the device): sequences of twice the tiles and more are cut as those of other calls. 40 tokens
-    // over 30,000 own keys behind 128 whole : cut, us, one sequence 434 : 64, 12 of them 457 : 352, four of 200 behind 3,008, one
-    // of which has 30,000, 490 : 207. Where no sequence of a wide table is that long, the join that finds nothing to do costs 4 to
-    // 12 us: 3 x 60 tokens behind 512 25 : 31, 8 x 200 behind 6,016 209 : 221.
+    // (how many is known on the device): sequences of twice the tiles and more are cut as those of other calls. 40
+    // tokens over 30,000 own keys behind 128 whole : cut, us, one sequence 434 : 64, 12 of them 457 : 352, four of 200
+    // behind 3,008, one of which has 30,000, 490 : 207. Where no sequence of a wide table is that long, the join that
+    // finds nothing to do costs 4 to 12 us: 3 x 60 tokens behind 512 25 : 31, 8 x 200 behind 6,016 209 : 221.
     const double tiles = p.front + std::min<int64_t>(p.blocks_per_seq << p.page_shift, p.max_q) / 256.0;
     tp.usual = prefix_pieces(ctx->num_sms, some, tiles, p.total_q * p.hq, HD, G::kWide);
     tp.long_tiles = 2 * (int)std::ceil(tiles);
